@@ -50,6 +50,25 @@ class Qwen3ConfigT(C.Structure):
                 ("kv_int8", C.c_uint32), ("kv_block_size", C.c_uint32), ("kv_num_blocks", C.c_uint32)]
 
 
+class Kv8T(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k_pool", "v_pool", "k_scales", "v_scales")] + \
+               [("pool_words", C.c_uint64), ("n_scales", C.c_uint64), ("block_tables", C.c_void_p)] + \
+               [(n, C.c_uint32) for n in ("max_blocks", "block_size", "n_kv_heads", "head_dim")]
+
+
+class Kv8BatchT(C.Structure):
+    _fields_ = [("row_start", C.c_void_p), ("seq_lens", C.c_void_p)] + \
+               [(n, C.c_uint32) for n in ("batch", "rows", "max_rows", "max_len")]
+
+
+class QkRowsT(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v")] + \
+               [(n, C.c_uint64) for n in ("q_stride", "k_stride", "v_stride")] + [("dtype", C.c_int)] + \
+               [(n, C.c_uint32) for n in ("rows", "n_heads", "n_kv_heads", "head_dim")] + \
+               [("positions", C.c_void_p), ("inv_freq", C.c_void_p), ("rotary_dim", C.c_uint32),
+                ("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("eps", C.c_float)]
+
+
 class CostT(C.Structure):
     _fields_ = [("flops", C.c_uint64), ("int_ops", C.c_uint64), ("bytes", C.c_uint64)]
 
@@ -72,6 +91,12 @@ SIGNATURES = {
     "bh_paged_kv_append_i8": (i32, [vp, vp, vp, vp, vp, vp, u64, vp, u64, u32, u32, u32, u32]),
     "bh_paged_decode_scores_i8": (i32, [vp, vp, vp, u64, vp, vp, vp, u64, vp] + [u32] * 8 + [f32]),
     "bh_paged_decode_apply_i8": (i32, [vp, vp, vp, u64, vp, vp, vp, u64, vp] + [u32] * 8),
+    "bh_qk_norm_rope": (i32, [vp, P(QkRowsT), vp, u64, vp, u64]),
+    "bh_qk_norm_rope_append_i8": (i32, [vp, P(QkRowsT), P(Kv8T), P(Kv8BatchT), vp, vp, vp, u64]),
+    "bh_paged_attention_i8_workspace": (i32, [P(Kv8T), P(Kv8BatchT), u32, P(u64)]),
+    "bh_paged_attention_i8": (i32, [vp, vp, u64, i32, u32, P(Kv8T), P(Kv8BatchT), f32, vp, vp, vp, u64]),
+    "bh_paged_weight_sums_i8": (i32, [vp, vp, u64, i32, u32, vp, P(Kv8T), P(Kv8BatchT), f32, vp, u32]),
+    "bh_paged_kv_evict_i8": (i32, [vp, P(Kv8T), vp, u32, vp, u32, u32, u32, u32, vp, u32, vp, u32, vp, vp]),
     "bh_reserve_workspace": (i32, [vp, u32, u32, u32]),
     "bh_matmul_i8_static": (i32, [vp, vp, vp, f32, f32, vp, u32, u32, u32]),
     "bh_linear_i8": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, i32, u32, u32, u32]),

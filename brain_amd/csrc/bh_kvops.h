@@ -1,0 +1,104 @@
+// What the operators of the int8 paged KV cache share (bh_rope.hip,
+// bh_pattn.hip, bh_evict.hip): the cache and the batch as the kernels take
+// them, and their checks.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "../../include/brain_hip.h"
+#include "bh_common.h"
+
+namespace bh {
+
+constexpr uint32_t NO_SLOT = 0xffffffffu;
+
+// A bh_kv8 whose geometry has been checked. Slots from `nslots` on lie outside
+// the pool or the scales: a table entry that names one is skipped.
+struct Kv8 {
+    uint32_t* pool[2];  // codes of keys, values
+    float* scales[2];
+    const uint32_t* bt;
+    uint32_t max_bt, bs, nkv, hd, nslots;
+    int bs_shift;  // log2(bs), or -1
+
+    __device__ __forceinline__ uint32_t block_of(uint32_t j) const { return bs_shift >= 0 ? j >> bs_shift : j / bs; }
+    // Slot of position j of sequence b in a table of `cols` entries a row.
+    __device__ __forceinline__ uint32_t slot_in(const uint32_t* tables, uint32_t cols, uint32_t b, uint32_t j) const {
+        const uint32_t blk = block_of(j);
+        if (blk >= cols) return NO_SLOT;
+        const uint64_t s = (uint64_t)tables[(uint64_t)b * cols + blk] * bs + (j - blk * bs);
+        return s < nslots ? (uint32_t)s : NO_SLOT;
+    }
+    __device__ __forceinline__ uint32_t slot(uint32_t b, uint32_t j) const { return slot_in(bt, max_bt, b, j); }
+    __device__ __forceinline__ size_t row(uint32_t slot) const { return (size_t)slot * (nkv * hd); }  // bytes
+};
+
+// The rows of a ragged batch: sequence b has rows [start[b], start[b + 1]),
+// the last ones of its len[b] cached positions.
+struct Kv8Rows {
+    const uint32_t* start;  // null: one row for each sequence
+    const uint32_t* lens;
+    uint32_t batch, rows;
+
+    __device__ __forceinline__ uint32_t first(uint32_t b) const { return start ? min(start[b], rows) : min(b, rows); }
+    __device__ __forceinline__ uint32_t end(uint32_t b) const { return start ? min(start[b + 1], rows) : min(b + 1, rows); }
+};
+
+// The last b < n for which below(b), a condition that holds up to some b and
+// not behind it; NO_SLOT if there is none. For a whole wave; one load of the
+// conditions' data for each factor of 64 in n. (Where the condition is not of
+// that kind the answer is still below n.)
+template <class F>
+__device__ __forceinline__ uint32_t wave_last(uint32_t n, uint32_t lane, F below) {
+    uint32_t lo = 0;
+    while (n) {
+        const uint32_t step = (n + 63) / 64, i = lane * step;
+        const bool yes = i < n && below(lo + min(i, n - 1));
+        const unsigned long long m = __ballot(yes);
+        if (!m) return NO_SLOT;
+        const uint32_t c = (63u - (uint32_t)__builtin_clzll(m)) * step;
+        if (step == 1) return lo + c;
+        lo += c;
+        n = min(step, n - c);
+    }
+    return NO_SLOT;
+}
+
+// Host checks: BH_OK, or the error of `who`.
+int check_kv8(const char* who, const bh_kv8* kv, Kv8* out);
+int check_kv8_batch(const char* who, const bh_kv8_batch* bt, Kv8Rows* out);
+
+inline bool aligned_to(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// Element types of activations.
+struct F32 {
+    typedef float elem;
+    static __device__ __forceinline__ float get(const float* p) { return *p; }
+    static __device__ __forceinline__ void get4(const float* p, float (&x)[4]) {
+        const float4 v = *reinterpret_cast<const float4*>(p);
+        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+    }
+    static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
+    static __device__ __forceinline__ void put4(float* p, const float (&x)[4]) {
+        *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    }
+};
+struct Bf16 {
+    typedef uint16_t elem;
+    static __device__ __forceinline__ float get(const uint16_t* p) {
+        return __builtin_bit_cast(float, (uint32_t)*p << 16);
+    }
+    static __device__ __forceinline__ void get4(const uint16_t* p, float (&x)[4]) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        x[0] = __builtin_bit_cast(float, v.x << 16), x[1] = __builtin_bit_cast(float, v.x & 0xffff0000u);
+        x[2] = __builtin_bit_cast(float, v.y << 16), x[3] = __builtin_bit_cast(float, v.y & 0xffff0000u);
+    }
+    static __device__ __forceinline__ void put(uint16_t* p, float v) { *p = f32_to_bf16_rne(v); }
+    static __device__ __forceinline__ void put4(uint16_t* p, const float (&x)[4]) {
+        *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
+    }
+};
+
+}  // namespace bh

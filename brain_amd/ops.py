@@ -4,9 +4,11 @@ torch only supplies device memory and the current HIP stream; all arithmetic
 runs in the library's gfx950 kernels. Packed int8 tensors are torch.int32
 tensors holding the u32 words (4 int8 per word, little-endian along K).
 """
+import ctypes as C
+
 import torch
 
-from ._lib import BH_OUT_BF16, BH_OUT_F32, BH_OUT_I32, check, load
+from ._lib import BH_OUT_BF16, BH_OUT_F32, BH_OUT_I32, Kv8BatchT, Kv8T, QkRowsT, check, load
 
 _CODES = {torch.float32: BH_OUT_F32, torch.bfloat16: BH_OUT_BF16, torch.int32: BH_OUT_I32}
 
@@ -251,3 +253,251 @@ def moe_linear_gated_i8(xq, wq, sx, sw, gate, e_idx, out=None):
     check(load().bh_moe_linear_gated_i8(_stream(), _ptr(xq), _ptr(wq), _ptr(sx), _ptr(sw), _ptr(gate), n_experts,
                                         e_idx, _ptr(out), m, kg, n))
     return out
+
+
+class PagedKV8:
+    """An int8 paged KV cache (bh_kv8): pools of int32 words (4 codes each,
+    n_kv * head_dim bytes a slot) and f32 scales [slots, n_kv] for keys and
+    values, block_tables [batch, max_blocks] int32. Position j of sequence b is
+    slot block_tables[b, j // block_size] * block_size + j % block_size. Holds
+    the tensors; make it once for a cache."""
+
+    def __init__(self, k_pool, v_pool, k_scales, v_scales, block_tables, block_size, head_dim):
+        _dev(k_pool, v_pool, k_scales, v_scales, block_tables)
+        if head_dim <= 0 or head_dim % 4 or head_dim > 256:
+            raise ValueError(f"PagedKV8: head_dim {head_dim}, a multiple of 4 up to 256")
+        if block_size <= 0:
+            raise ValueError(f"PagedKV8: block_size {block_size}")
+        if k_scales.dim() != 2 or block_tables.dim() != 2:
+            raise ValueError("PagedKV8: scales [slots, n_kv] and block_tables [batch, max_blocks] expected")
+        slots, n_kv = k_scales.shape
+        for name, t, dtype, numel in (("k_pool", k_pool, torch.int32, slots * n_kv * head_dim // 4),
+                                      ("v_pool", v_pool, torch.int32, slots * n_kv * head_dim // 4),
+                                      ("k_scales", k_scales, torch.float32, slots * n_kv),
+                                      ("v_scales", v_scales, torch.float32, slots * n_kv),
+                                      ("block_tables", block_tables, torch.int32, 0)):
+            _need(t, dtype, numel, name)
+            if t.device != k_pool.device:
+                raise ValueError(f"PagedKV8: {name} is on {t.device}, k_pool on {k_pool.device}")
+        self.k_pool, self.v_pool, self.k_scales, self.v_scales = k_pool, v_pool, k_scales, v_scales
+        self.block_tables, self.block_size, self.head_dim, self.n_kv = block_tables, block_size, head_dim, n_kv
+        self.device = k_pool.device
+        self.desc = Kv8T(_ptr(k_pool), _ptr(v_pool), _ptr(k_scales), _ptr(v_scales), slots * n_kv * head_dim // 4,
+                         slots * n_kv, _ptr(block_tables), block_tables.shape[1], block_size, n_kv, head_dim)
+
+
+def _heads(t, dtype, hd, name):
+    """Row stride (elements) of [rows, heads, hd] `t`, whose heads lie side by side."""
+    if t.dtype != dtype:
+        raise ValueError(f"{name}: dtype {t.dtype}, expected {dtype}")
+    if not t.is_cuda:
+        raise ValueError("brain_amd.ops: tensors must live on the GPU")
+    if t.dim() != 3 or t.shape[2] != hd:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected [rows, heads, {hd}]")
+    rs, hs, es = t.stride()
+    rows, heads = t.shape[0], t.shape[1]
+    if (hd > 1 and es != 1) or (heads > 1 and hs != hd) or (rows > 1 and rs < heads * hd):
+        raise ValueError(f"{name}: strides {t.stride()}; the heads of a row must lie side by side")
+    return rs if rows > 1 else heads * hd
+
+
+def _same_device(device, **ts):
+    # The launches go to the current device's current stream.
+    if device.index is not None and device.index != torch.cuda.current_device():
+        raise ValueError(f"brain_amd.ops: the tensors are on {device}, the current device is "
+                         f"{torch.cuda.current_device()}")
+    for name, t in ts.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, expected {device}")
+
+
+def _kv_batch(cache, rows, seq_lens, row_start, max_rows, max_len):
+    batch = seq_lens.numel()
+    _dev(seq_lens, row_start)
+    _need(seq_lens, torch.int32, batch, "seq_lens")
+    if batch > cache.block_tables.shape[0]:
+        raise ValueError(f"seq_lens: {batch} sequences, block_tables has {cache.block_tables.shape[0]}")
+    if row_start is None:
+        if rows != batch:
+            raise ValueError(f"row_start: {rows} rows of {batch} sequences need one")
+    else:
+        _need(row_start, torch.int32, batch + 1, "row_start")
+        if row_start.numel() != batch + 1:
+            raise ValueError(f"row_start: {row_start.numel()} entries for {batch} sequences")
+    return Kv8BatchT(_ptr(row_start), _ptr(seq_lens), batch, rows, max_rows or 0, max_len or 0)
+
+
+_ACT = {torch.float32: BH_OUT_F32, torch.bfloat16: BH_OUT_BF16}
+
+
+def _qk_rows(q, k, v, positions, inv_freq, q_weight, k_weight, eps):
+    if q.dtype not in _ACT:
+        raise ValueError(f"q: dtype {q.dtype}, expected float32 or bfloat16")
+    if q.dim() != 3 or k.dim() != 3:
+        raise ValueError("q, k: [rows, heads, head_dim] expected")
+    rows, nh, hd = q.shape
+    nkv = k.shape[1]
+    strides = [_heads(q, q.dtype, hd, "q"), _heads(k, q.dtype, hd, "k"), 0]
+    if k.shape[0] != rows:
+        raise ValueError(f"k: {k.shape[0]} rows, q has {rows}")
+    if v is not None:
+        strides[2] = _heads(v, q.dtype, hd, "v")
+        if v.shape != k.shape:
+            raise ValueError(f"v: shape {tuple(v.shape)}, k has {tuple(k.shape)}")
+    _dev(positions, inv_freq, q_weight, k_weight)
+    _need(positions, torch.int32, rows, "positions")
+    _need(inv_freq, torch.float64, 0, "inv_freq")
+    if 2 * inv_freq.numel() > hd:
+        raise ValueError(f"inv_freq: {inv_freq.numel()} pairs, head_dim {hd}")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None:
+            _need(w, torch.float32, hd, name)
+    _same_device(q.device, k=k, v=v, positions=positions, inv_freq=inv_freq, q_weight=q_weight, k_weight=k_weight)
+    return QkRowsT(q.data_ptr(), k.data_ptr(), _ptr(v), *strides, _ACT[q.dtype], rows, nh, nkv, hd, _ptr(positions),
+                   _ptr(inv_freq), 2 * inv_freq.numel(), _ptr(q_weight), _ptr(k_weight), eps)
+
+
+def rope_frequencies(rotary_dim, theta, device="cuda"):
+    """inv_freq of plain RoPE: theta^(-2i / rotary_dim), f64 [rotary_dim / 2]."""
+    return theta ** (-torch.arange(0, rotary_dim, 2, device=device, dtype=torch.float64) / rotary_dim)
+
+
+def _out_like(out, t, name):
+    if out is None:
+        return torch.empty(t.shape, device=t.device, dtype=t.dtype), t.shape[1] * t.shape[2]
+    stride = _heads(out, t.dtype, t.shape[2], name)
+    if out.shape != t.shape:
+        raise ValueError(f"{name}: shape {tuple(out.shape)}, expected {tuple(t.shape)}")
+    _same_device(t.device, **{name: out})
+    return out, stride
+
+
+def qk_norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e-6, q_out=None, k_out=None):
+    """Per-head RMSNorm (where a weight is given) and rotation of q [rows,
+    n_heads, hd] and k [rows, n_kv, hd], f32 or bf16, views of a joined
+    projection included: pair (i, i + rotary_dim/2) is turned by
+    positions[row] * inv_freq[i], rotary_dim = 2 * inv_freq.numel(). Returns
+    (q_out, k_out), which may be q and k themselves."""
+    rows = _qk_rows(q, k, None, positions, inv_freq, q_weight, k_weight, eps)
+    q_out, qs = _out_like(q_out, q, "q_out")
+    k_out, ks = _out_like(k_out, k, "k_out")
+    check(load().bh_qk_norm_rope(_stream(), C.byref(rows), q_out.data_ptr(), qs, k_out.data_ptr(), ks))
+    return q_out, k_out
+
+
+def qk_norm_rope_append_i8(q, k, v, positions, inv_freq, cache, seq_lens, row_start=None, q_weight=None, k_weight=None,
+                           eps=1e-6, k_clip=None, v_clip=None, q_out=None):
+    """qk_norm_rope, with the turned keys and the values quantised into the
+    cache (PagedKV8): the rows row_start[b] .. row_start[b + 1] become the last
+    positions of sequence b's seq_lens[b] (row_start None: one row each).
+    Returns q_out."""
+    rows = _qk_rows(q, k, v, positions, inv_freq, q_weight, k_weight, eps)
+    if (k.shape[1], k.shape[2]) != (cache.n_kv, cache.head_dim):
+        raise ValueError(f"k: heads {tuple(k.shape[1:])}, the cache has {(cache.n_kv, cache.head_dim)}")
+    batch = _kv_batch(cache, q.shape[0], seq_lens, row_start, 0, 0)
+    _dev(k_clip, v_clip)
+    for name, t in (("k_clip", k_clip), ("v_clip", v_clip)):
+        if t is not None:
+            _need(t, torch.float32, cache.n_kv, name)
+    _same_device(q.device, cache=cache, seq_lens=seq_lens, row_start=row_start, k_clip=k_clip, v_clip=v_clip)
+    q_out, qs = _out_like(q_out, q, "q_out")
+    check(load().bh_qk_norm_rope_append_i8(_stream(), C.byref(rows), C.byref(cache.desc), C.byref(batch), _ptr(k_clip),
+                                           _ptr(v_clip), q_out.data_ptr(), qs))
+    return q_out
+
+
+def _queries(q, cache, seq_lens, row_start, max_rows, max_len):
+    if q.dtype not in _ACT:
+        raise ValueError(f"q: dtype {q.dtype}, expected float32 or bfloat16")
+    stride = _heads(q, q.dtype, cache.head_dim, "q")
+    if q.shape[1] == 0 or q.shape[1] % cache.n_kv:
+        raise ValueError(f"q: {q.shape[1]} heads over {cache.n_kv} kv heads")
+    batch = _kv_batch(cache, q.shape[0], seq_lens, row_start, max_rows, max_len)
+    _same_device(q.device, cache=cache, seq_lens=seq_lens, row_start=row_start)
+    return stride, batch
+
+
+def paged_attention_i8(q, cache, seq_lens, row_start=None, scale=None, max_rows=None, max_len=None, out=None, lse=None):
+    """Causal attention of q [rows, n_heads, hd] (f32 or bf16) over the cache
+    (PagedKV8): the rows row_start[b] .. row_start[b + 1] are the last of
+    sequence b's seq_lens[b] positions and see the keys up to their own. scale
+    defaults to hd^-0.5. max_rows and max_len, the most rows and the longest
+    length where the program knows them, choose how the work is split. Returns
+    (out like q, lse [rows, n_heads] f32); a row without keys has zeros and
+    -inf; rows behind the last sequence stay as `out` and `lse` have them."""
+    stride, batch = _queries(q, cache, seq_lens, row_start, max_rows, max_len)
+    rows, nh, hd = q.shape
+    if out is None:
+        out = torch.empty(rows, nh, hd, device=q.device, dtype=q.dtype)
+    if lse is None:
+        lse = torch.empty(rows, nh, device=q.device, dtype=torch.float32)
+    _dev(out, lse)
+    _need(out, q.dtype, rows * nh * hd, "out")
+    _need(lse, torch.float32, rows * nh, "lse")
+    _same_device(q.device, out=out, lse=lse)
+    lib, need = load(), C.c_uint64()
+    check(lib.bh_paged_attention_i8_workspace(C.byref(cache.desc), C.byref(batch), nh, C.byref(need)))
+    ws = torch.empty(need.value, device=q.device, dtype=torch.uint8) if need.value else None
+    check(lib.bh_paged_attention_i8(_stream(), q.data_ptr(), stride, _ACT[q.dtype], nh, C.byref(cache.desc),
+                                    C.byref(batch), hd ** -0.5 if scale is None else scale, out.data_ptr(),
+                                    lse.data_ptr(), _ptr(ws), need.value))
+    return out, lse
+
+
+def paged_weight_sums_i8(q, lse, cache, seq_lens, acc, row_start=None, scale=None, max_rows=None, max_len=None):
+    """acc [batch, n_kv, cap] f32 += the weight exp(s - lse) that the rows of
+    q gave each cached key in paged_attention_i8 (same arguments, its lse),
+    summed over rows and a kv head's query heads; the chunk's own keys start
+    from 0. Returns acc."""
+    stride, batch = _queries(q, cache, seq_lens, row_start, max_rows, max_len)
+    rows, nh, hd = q.shape
+    _dev(lse, acc)
+    _need(lse, torch.float32, rows * nh, "lse")
+    if acc.dim() != 3 or acc.shape[0] < seq_lens.numel() or acc.shape[1] != cache.n_kv:
+        raise ValueError(f"acc: shape {tuple(acc.shape)}, expected [{seq_lens.numel()}, {cache.n_kv}, cap]")
+    _need(acc, torch.float32, 0, "acc")
+    _same_device(q.device, lse=lse, acc=acc)
+    check(load().bh_paged_weight_sums_i8(_stream(), q.data_ptr(), stride, _ACT[q.dtype], nh, _ptr(lse),
+                                         C.byref(cache.desc), C.byref(batch), hd ** -0.5 if scale is None else scale,
+                                         _ptr(acc), acc.shape[2]))
+    return acc
+
+
+def paged_kv_evict_i8(cache, seq_lens, acc, budget, sink=0, recent=0, out_tables=None, acc_out=None, keep=None,
+                      new_lens=None):
+    """Cut sequences longer than `budget` down to it: each kv head keeps its
+    first `sink` positions, its last `recent` and the heaviest between by acc
+    [batch, n_kv, cap] (ties: the lower position). The entries kept move, in
+    order, to the front of the sequence: of out_tables' blocks [batch, blocks],
+    or, without, of its own. acc_out [batch, n_kv, >= budget] takes their acc
+    (it may be acc). Returns (keep [batch, n_kv, budget] int32, -1 behind the
+    last one, new_lens [batch])."""
+    batch = seq_lens.numel()
+    _dev(seq_lens, acc, out_tables, acc_out, keep, new_lens)
+    _need(seq_lens, torch.int32, batch, "seq_lens")
+    _need(acc, torch.float32, 0, "acc")
+    if batch > cache.block_tables.shape[0]:
+        raise ValueError(f"seq_lens: {batch} sequences, block_tables has {cache.block_tables.shape[0]}")
+    if acc.dim() != 3 or acc.shape[0] < batch or acc.shape[1] != cache.n_kv:
+        raise ValueError(f"acc: shape {tuple(acc.shape)}, expected [{batch}, {cache.n_kv}, cap]")
+    if budget <= 0 or sink < 0 or recent < 0 or sink + recent > budget:
+        raise ValueError(f"budget {budget} with sink {sink} and recent {recent}")
+    if out_tables is not None:
+        _need(out_tables, torch.int32, 0, "out_tables")
+        if out_tables.dim() != 2 or out_tables.shape[0] < batch:
+            raise ValueError(f"out_tables: shape {tuple(out_tables.shape)}, expected [{batch}, blocks]")
+    if acc_out is not None:
+        _need(acc_out, torch.float32, 0, "acc_out")
+        if acc_out.dim() != 3 or acc_out.shape[0] < batch or acc_out.shape[1] != cache.n_kv:
+            raise ValueError(f"acc_out: shape {tuple(acc_out.shape)}, expected [{batch}, {cache.n_kv}, >= {budget}]")
+    keep = torch.empty(batch, cache.n_kv, budget, device=acc.device, dtype=torch.int32) if keep is None else keep
+    new_lens = torch.empty(batch, device=acc.device, dtype=torch.int32) if new_lens is None else new_lens
+    _need(keep, torch.int32, batch * cache.n_kv * budget, "keep")
+    _need(new_lens, torch.int32, batch, "new_lens")
+    _same_device(cache.device, seq_lens=seq_lens, acc=acc, out_tables=out_tables, acc_out=acc_out, keep=keep,
+                 new_lens=new_lens)
+    check(load().bh_paged_kv_evict_i8(_stream(), C.byref(cache.desc), _ptr(seq_lens), batch, _ptr(acc), acc.shape[2],
+                                      budget, sink, recent, _ptr(out_tables),
+                                      out_tables.shape[1] if out_tables is not None else 0, _ptr(acc_out),
+                                      acc_out.shape[2] if acc_out is not None else 0, _ptr(keep), _ptr(new_lens)))
+    return keep, new_lens

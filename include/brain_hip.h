@@ -232,6 +232,102 @@ int bh_paged_decode_apply_i8(void* stream, const float* probs, const uint32_t* p
                              uint32_t head_dim, uint32_t block_size, uint32_t kv_stride, uint32_t cap,
                              uint32_t max_bt);
 
+/* ----------------------------------------------------------------------
+ * The life of a token in the int8 paged KV cache, for ragged batches. A cache
+ * is what bh_paged_kv_append_i8 fills, keys and values together; several
+ * sequences' chunks of new tokens go through one call. No counterpart in the
+ * reference beyond the one-token kernels above (its chunks are one sequence's).
+ * ---------------------------------------------------------------------- */
+typedef struct {
+    uint32_t *k_pool, *v_pool;     /* int8 codes, 4 per word, n_kv_heads * head_dim bytes a slot */
+    float *k_scales, *v_scales;    /* [slot][n_kv_heads] */
+    uint64_t pool_words, n_scales; /* the lengths of each */
+    const uint32_t* block_tables;  /* [batch][max_blocks]: position j of sequence b is slot
+                                      table[b][j / block_size] * block_size + j % block_size. An entry that
+                                      names a slot outside the pool or the scales is skipped: nothing is
+                                      stored there, and a query does not see the key */
+    uint32_t max_blocks, block_size, n_kv_heads, head_dim; /* head_dim % 4 == 0, <= 256 */
+} bh_kv8;
+
+/* Sequence b has the rows row_start[b] .. row_start[b+1] of the activations
+ * (ascending; none is fine; rows from row_start[batch] on are left as they
+ * are), and they are the last of its seq_lens[b] positions: row i of n sits at
+ * position seq_lens[b] - n + i. A row whose position that makes negative is
+ * stored nowhere and sees no key. max_rows and max_len are the most rows and the longest length that the program knows
+ * of: they choose how the work is split (0: not known), the results of a call
+ * hold without them. */
+typedef struct {
+    const uint32_t* row_start; /* [batch + 1], or NULL: one row for each sequence (rows == batch) */
+    const uint32_t* seq_lens;  /* [batch], the chunk's rows included */
+    uint32_t batch, rows, max_rows, max_len;
+} bh_kv8_batch;
+
+/* The queries, keys (and values) of `rows` rows, row strides in elements, the
+ * heads of a row side by side: views of a joined projection are fine. */
+typedef struct {
+    const void *q, *k, *v;     /* [rows][n_heads | n_kv_heads][head_dim], dtype BH_OUT_F32 or BH_OUT_BF16 */
+    uint64_t q_stride, k_stride, v_stride;
+    int dtype;
+    uint32_t rows, n_heads, n_kv_heads, head_dim;
+    const uint32_t* positions; /* [rows] of the rotation */
+    const double* inv_freq;    /* [rotary_dim / 2] radians a position, on the device */
+    uint32_t rotary_dim;       /* even, <= head_dim; the elements behind it are not turned */
+    const float *q_weight, *k_weight; /* [head_dim] norm gains, or NULL: no norm */
+    float eps;
+} bh_qk_rows;
+
+/* y = x * rsqrt(mean(x^2) + eps) * weight for each head of q and k, then the
+ * pairs (i, i + rotary_dim/2) of y turned by positions[row] * inv_freq[i] (the
+ * angle in f64). Outputs of the inputs' dtype; q_out may be q and k_out k, with
+ * the same strides. */
+int bh_qk_norm_rope(void* stream, const bh_qk_rows* in, void* q_out, uint64_t q_out_stride, void* k_out,
+                    uint64_t k_out_stride);
+/* The same, and the turned keys and the values into the cache at each row's
+ * position, quantised from f32 as bh_paged_kv_append_i8 does: scale =
+ * min(max|x|, clip[kv head]) / 127 (1 where that is 0). k_clip / v_clip
+ * [n_kv_heads] or NULL (FLT_MAX). The rows of a batch must have slots of their own. */
+int bh_qk_norm_rope_append_i8(void* stream, const bh_qk_rows* in, const bh_kv8* kv, const bh_kv8_batch* batch,
+                              const float* k_clip, const float* v_clip, void* q_out, uint64_t q_out_stride);
+
+/* Causal attention of the batch's rows over the cached keys: for each row and
+ * query head h, with kv head h / (n_heads / n_kv_heads), over the keys at
+ * positions <= the row's,
+ *   s_j = scale * k_scale_j * (q . k_code_j),  out = sum_j softmax(s)_j * v_scale_j * v_code_j.
+ * q and out [rows][n_heads][head_dim] of dtype BH_OUT_F32 or BH_OUT_BF16, q_stride elements from row to row, out
+ * contiguous; lse [rows][n_heads] f32 = log sum_j exp(s_j), or NULL. A row that sees no key gets zeros and -inf. Sums and statistics are f32; with bf16
+ * activations the weights are rounded to bf16 before the product with the
+ * values, with f32 they keep 24 bits. `ws`: ws_bytes of device memory, at least
+ * what bh_paged_attention_i8_workspace gives for the call (may be 0: NULL), which the call
+ * writes before it reads. */
+int bh_paged_attention_i8_workspace(const bh_kv8* kv, const bh_kv8_batch* batch, uint32_t n_heads, uint64_t* bytes);
+int bh_paged_attention_i8(void* stream, const void* q, uint64_t q_stride, int dtype, uint32_t n_heads, const bh_kv8* kv,
+                          const bh_kv8_batch* batch, float scale, void* out, float* lse, void* ws, uint64_t ws_bytes);
+
+/* The weight that the batch's rows give to each cached key, from the lse of
+ * bh_paged_attention_i8: acc[b][kv head][j] = (j < seq_lens[b] - n ? acc[b][kv head][j] : 0) + the sum of exp(s_j - lse)
+ * over the n rows of sequence b that see key j and the kv head's query heads, in
+ * a fixed order. acc [batch][n_kv_heads][acc_stride] f32; positions from
+ * min(seq_lens[b], acc_stride) on are left as they are. */
+int bh_paged_weight_sums_i8(void* stream, const void* q, uint64_t q_stride, int dtype, uint32_t n_heads, const float* lse,
+                            const bh_kv8* kv, const bh_kv8_batch* batch, float scale, float* acc, uint32_t acc_stride);
+
+/* Cuts sequences down to `budget` positions. Where seq_lens[b] > budget, each kv head keeps its first
+ * `sink` positions, its last `recent`, and of those between the ones of
+ * largest acc (ties: the lower position; NaN counts as -inf; sink + recent <= budget), else all.
+ * keep [batch][n_kv_heads][budget]: the positions kept, ascending, -1 behind
+ * them; new_lens[b] = min(seq_lens[b], budget). The codes and scales of
+ * position keep[i] move to position i of out_tables [batch][out_max_blocks]
+ * (blocks of the same pool; NULL: the cache's own tables, in place), and acc to
+ * acc_out [batch][n_kv_heads][acc_out_stride] (may be acc itself; NULL: not
+ * wanted). Different heads of a slot then hold different tokens: what was
+ * turned by its position stays so. Each block written to must belong to one
+ * sequence, and, unless in place, be none that is read. seq_lens[b] past
+ * acc_stride counts as acc_stride. new_lens may be seq_lens. */
+int bh_paged_kv_evict_i8(void* stream, const bh_kv8* kv, const uint32_t* seq_lens, uint32_t batch, const float* acc,
+                         uint32_t acc_stride, uint32_t budget, uint32_t sink, uint32_t recent,
+                         const uint32_t* out_tables, uint32_t out_max_blocks, float* acc_out, uint32_t acc_out_stride,
+                         int32_t* keep, uint32_t* new_lens);
+
 /* f32 -> bf16 bits, round to nearest even, NaN -> (bits >> 16) | 0x0040: the
  * conversion every bf16 output of this library goes through
  * (crates/model/src/half.rs:49-58, f32_to_bf16). x [n] f32 -> out [n] u16. */
