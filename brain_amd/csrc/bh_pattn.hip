@@ -7,6 +7,9 @@ namespace {
 
 constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.693147180559945309f;
 
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+
 struct AttnArgs {
     const void* q;
     uint64_t qs;  // row stride, elements
@@ -16,6 +19,12 @@ struct AttnArgs {
     Kv8Rows bt;
     uint32_t nh, group;
     float scale2;  // scale * log2(e): softmax in base 2
+    // The matrix kernels: blocks of query vectors, splits of the keys, what the
+    // splits leave for the join.
+    uint32_t blocks, nsplit, span;  // span: keys of a split
+    float* part;                    // [unit][kv head][vectors][hd], then
+    float2* ml;                     // [unit][kv head][vectors] maximum and sum
+    uint32_t qvec;                  // queries can be loaded 16 bytes at a time
 };
 struct SumsArgs {
     const void* q;
@@ -119,6 +128,479 @@ __global__ __launch_bounds__(64) void paged_weight_sums_any_kernel(SumsArgs p, u
     *dst = old ? *dst + sum : sum;
 }
 
+// ---------------------------------------------------------------- few rows
+//
+// Up to 32 query vectors (rows x heads of one kv head) of a sequence at a time:
+// the cache is read once and each code used for few products, so the stream of
+// the codes bounds it. A wave takes 32 keys at a time straight into the operand
+// layout of v_mfma_f32_16x16x32_bf16 (codes are exact in bf16), the next 32 in
+// flight: no LDS, no barrier in the loop. Scores are computed transposed (keys x
+// queries): lane (c, g) = (l % 16, l / 16) then holds the scores of query c and
+// keys 4g..4g+3 and 16+4g..16+4g+3, which is the operand layout of the second
+// product for an order of its 32 keys that V's loads follow.
+//
+// A query of f32 is the exact sum of three bf16 numbers, and so is a weight:
+// three products each, 24 bits. With bf16 activations the query is exact, and
+// the weight times its value scale is rounded to bf16, half a step 2^-9 of the
+// next power of two: the size of the output's own rounding.
+
+__device__ __forceinline__ uint32_t fbits(float f) { return __builtin_bit_cast(uint32_t, f); }
+__device__ __forceinline__ float bitsf(uint32_t u) { return __builtin_bit_cast(float, u); }
+// The upper halves of two floats, packed (exact where they are bf16 numbers).
+__device__ __forceinline__ uint32_t hi16x2(float lo, float hi) {
+    return __builtin_amdgcn_perm(fbits(hi), fbits(lo), 0x07060302u);
+}
+// Eight floats as PARTS bf16 fragments: one, rounded to nearest, or three that
+// add up to them: the first is cut, so that none rounds to infinity.
+template <int PARTS>
+__device__ __forceinline__ void split8(const float (&x)[8], v4i (&f)[PARTS]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float x0 = x[2 * i], x1 = x[2 * i + 1];
+        if constexpr (PARTS == 1) {
+            f[0][i] = (int)pack_bf16x2(x0, x1);
+        } else {
+            f[0][i] = (int)hi16x2(x0, x1);
+            const float r0 = x0 - bitsf(fbits(x0) & 0xffff0000u), r1 = x1 - bitsf(fbits(x1) & 0xffff0000u);
+            const uint32_t q = pack_bf16x2(r0, r1);
+            f[1][i] = (int)q;
+            f[2][i] = (int)hi16x2(r0 - bitsf(q << 16), r1 - bitsf(q & 0xffff0000u));  // at most 8 bits are left
+        }
+    }
+}
+// Eight codes (along one key's dimensions) as a fragment.
+__device__ __forceinline__ v4i codes8(uint32_t lo, uint32_t hi) {
+    return v4i{(int)hi16x2(code_f(lo, 0), code_f(lo, 1)), (int)hi16x2(code_f(lo, 2), code_f(lo, 3)),
+               (int)hi16x2(code_f(hi, 0), code_f(hi, 1)), (int)hi16x2(code_f(hi, 2), code_f(hi, 3))};
+}
+__device__ __forceinline__ v4f mfma16(v4i a, v4i b, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+}
+// Eight elements of a query from d on.
+template <class T>
+__device__ __forceinline__ void query8(const typename T::elem* p, bool vec, float (&x)[8]) {
+    if (vec) {
+        float a[4], b[4];
+        T::get4(p, a);
+        T::get4(p + 4, b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = T::get(p + i);
+    }
+}
+
+// Where a workgroup works: sequence b, VB of its query vectors from v0 on (of
+// nv = rows x group; vector v is head v % group of row v / group). Block numbers
+// are given out so that sequence b's start at row_start[b] * group / VB + b:
+// no list of them is needed, at the price of some that are empty.
+struct Block {
+    uint32_t b, r0, n, v0, nv, len;
+};
+template <int VB>
+__device__ __forceinline__ bool find_block(const Kv8Rows& bt, uint32_t group, uint32_t blk, uint32_t lane, Block& o) {
+    uint32_t b;
+    if (!bt.start && group <= VB) b = blk;  // one block each
+    else b = wave_last(bt.batch, lane, [&](uint32_t i) { return bt.first(i) * group / VB + i <= blk; });
+    b = __builtin_amdgcn_readfirstlane((int)b);
+    if (b >= bt.batch) return false;
+    const uint32_t r0 = bt.first(b), r1 = bt.end(b);
+    if (r1 <= r0) return false;
+    o.b = b, o.r0 = r0, o.n = r1 - r0, o.nv = o.n * group;
+    o.v0 = !bt.start && group <= VB ? 0 : (blk - (r0 * group / VB + b)) * VB;
+    o.len = bt.lens[b];
+    return o.v0 < o.nv;
+}
+// The number of keys that row i of a block's sequence sees.
+__device__ __forceinline__ uint32_t keys_seen(const Block& o, uint32_t i) {
+    return o.len + i + 1 > o.n && o.len + i + 1 > i ? o.len + i + 1 - o.n : 0u;
+}
+
+constexpr int SW = 4;  // waves
+
+// Waves per SIMD that the registers allow: queries, context and codes in flight.
+template <class T, int HD, int NQ>
+constexpr int stream_waves() {
+    return (sizeof(typename T::elem) == 4 ? 3 : 1) * NQ * HD <= (sizeof(typename T::elem) == 4 ? 3 : 2) * 128 ? 2 : 1;
+}
+
+template <class T, int HD, int NQ, bool B16>
+__global__ __launch_bounds__(SW * 64, (stream_waves<T, HD, NQ>())) void paged_attention_stream_kernel(AttnArgs p) {
+    typedef typename T::elem E;
+    constexpr int PARTS = sizeof(E) == 4 ? 3 : 1, VB = 16 * NQ, KT = HD / 64, VW = HD / 64;  // VW: words of V a lane takes of a key
+    constexpr int OST = HD + 4;
+    __shared__ __attribute__((aligned(16))) float so[SW][16][OST];
+    __shared__ float sm[SW][VB], sl[SW][VB];
+    __shared__ __attribute__((aligned(16))) float ssc[SW][64];
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // All kv heads of a unit run on one XCD (workgroups go round the eight):
+    // their scales share cache lines.
+    const uint32_t nkv = p.kv.nkv, unit = blockIdx.x / (8 * nkv) * 8 + blockIdx.x % 8, kvh = blockIdx.x / 8 % nkv;
+    if (unit >= p.blocks * p.nsplit) return;
+    const uint32_t split = unit % p.nsplit;
+    Block bl;
+    if (!find_block<VB>(p.bt, p.group, unit / p.nsplit, lane, bl)) return;
+    const uint32_t reach = (uint32_t)min((uint64_t)p.kv.max_bt * p.kv.bs, (uint64_t)0x7fffffffu);
+    const uint32_t vend = min(bl.v0 + VB, bl.nv);
+    const uint32_t kend = min(keys_seen(bl, (vend - 1) / p.group), reach);  // keys that any of the vectors sees
+    const uint32_t kall = min(keys_seen(bl, bl.v0 / p.group), reach);       // ... that all see
+    const uint32_t k0 = split * p.span, k1 = split + 1 == p.nsplit ? kend : min(kend, k0 + p.span);
+    if (k0 >= k1 && split) return;
+
+    // Queries: fragment (t, half) holds d = 16 (g + 4t) + 8 half ..+7 of vector c.
+    v4i qf[NQ][2 * KT][PARTS];
+    uint32_t seen[NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        const uint32_t v = min(bl.v0 + 16 * q + c, vend - 1), i = v / p.group, h = kvh * p.group + v % p.group;
+        seen[q] = bl.v0 + 16 * q + c < vend ? min(keys_seen(bl, i), reach) : 0u;
+        const E* src = (const E*)p.q + (bl.r0 + i) * p.qs + (uint64_t)h * HD;
+#pragma unroll
+        for (int t = 0; t < 2 * KT; ++t) {
+            float x[8];
+            query8<T>(src + 16 * (g + 4 * (t >> 1)) + 8 * (t & 1), p.qvec, x);
+            split8<PARTS>(x, qf[q][t]);
+        }
+    }
+    v4f o[NQ][HD / 16];
+    float m[NQ], l[NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        m[q] = -INFINITY, l[q] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < HD / 16; ++j) o[q][j] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+
+    const uint32_t kvs = nkv * HD;
+    const uint8_t* kp = (const uint8_t*)p.kv.pool[0] + (size_t)kvh * HD;
+    const uint8_t* vp = (const uint8_t*)p.kv.pool[1] + (size_t)kvh * HD;
+    const float* sp = (lane < 32 ? p.kv.scales[0] : p.kv.scales[1]) + kvh;  // half the lanes take the keys' scales
+    const uint32_t* tb = p.kv.bt + (uint64_t)bl.b * p.kv.max_bt;
+    // Slots of the 32 keys from j on. B16: the blocks hold whole groups of 16
+    // keys (and the pool as well), so two uniform slots say where all are;
+    // else lane l has that of key l % 32. ok: which of the keys have a slot.
+    struct Slots {
+        uint32_t s0, s1, ok;
+    };
+    auto slots_of = [&](uint32_t j) -> Slots {
+        Slots r{0, 0, 0};
+        if constexpr (B16) {
+            auto group = [&](uint32_t ju) -> uint32_t {
+                if (ju >= kend) return NO_SLOT;
+                const uint32_t blk = p.kv.block_of(ju);
+                const uint64_t s = (uint64_t)tb[blk] * p.kv.bs + (ju - blk * p.kv.bs);
+                return s < p.kv.nslots ? (uint32_t)s : NO_SLOT;
+            };
+            const uint32_t a = group(j), b = group(j + 16);
+            r.s0 = a != NO_SLOT ? a : 0u, r.s1 = b != NO_SLOT ? b : 0u;
+            r.ok = (a != NO_SLOT ? 0xffffu : 0u) | (b != NO_SLOT ? 0xffff0000u : 0u);
+        } else {
+            const uint32_t jl = j + (lane & 31), s = jl < kend ? p.kv.slot(bl.b, jl) : NO_SLOT;
+            r.s0 = s != NO_SLOT ? s : 0u;
+            r.ok = (uint32_t)__ballot(s != NO_SLOT);
+        }
+        return r;
+    };
+    v4i kc[2][KT];       // codes of the keys in flight: lane (c, g) has key 16 u + c, bytes 16 (g + 4 i) ..+15
+    uint32_t vc[8][VW];  // of the values: key 16 (e / 4) + 4 g + e % 4, bytes 4 VW c ..
+    float sc;
+    auto load_k = [&](const Slots& at) {
+        const uint32_t lo = (uint32_t)c * kvs + 16 * g;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const uint8_t* k = B16 ? kp + (size_t)(u ? at.s1 : at.s0) * kvs + lo
+                                   : kp + (size_t)(uint32_t)__shfl((int)at.s0, 16 * u + c, 64) * kvs + 16 * g;
+#pragma unroll
+            for (int i = 0; i < KT; ++i) kc[u][i] = *reinterpret_cast<const v4i*>(k + 64 * i);
+        }
+    };
+    auto load_v = [&](const Slots& at) {
+        const uint32_t lo = (uint32_t)(4 * g) * kvs + 4 * VW * c;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint8_t* v = B16 ? vp + (size_t)((e >> 2 ? at.s1 : at.s0) + (e & 3)) * kvs + lo
+                                   : vp + (size_t)(uint32_t)__shfl((int)at.s0, 16 * (e >> 2) + 4 * g + (e & 3), 64) * kvs + 4 * VW * c;
+            if constexpr (VW == 2) {
+                const uint2 w = *reinterpret_cast<const uint2*>(v);
+                vc[e][0] = w.x, vc[e][1] = w.y;
+            } else {
+                vc[e][0] = *reinterpret_cast<const uint32_t*>(v);
+            }
+        }
+        sc = sp[B16 ? (size_t)((lane & 16 ? at.s1 : at.s0) + c) * nkv : (size_t)at.s0 * nkv];
+    };
+    const uint32_t first = k0 + 32 * wave, step = 32 * SW;
+    Slots at{0, 0, 0}, next{0, 0, 0};
+    if (first < k1) {
+        at = slots_of(first);
+        load_k(at);
+        load_v(at);
+        next = slots_of(first + step);
+    }
+#pragma unroll 1
+    for (uint32_t j0 = first; j0 < k1; j0 += step) {
+        const bool more = j0 + step < k1;
+        uint32_t vt[8][VW];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int i = 0; i < VW; ++i) vt[e][i] = vc[e][i];
+        // Scales by key: this wave's 64 floats, keys' then values'.
+        ssc[wave][lane] = sc;
+        const uint32_t ok = at.ok;
+        if (more) load_v(next);
+        __builtin_amdgcn_sched_barrier(0);
+        v4f s[NQ][2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            v4i kf[2 * KT];
+#pragma unroll
+            for (int i = 0; i < KT; ++i) {
+                kf[2 * i] = codes8((uint32_t)kc[u][i][0], (uint32_t)kc[u][i][1]);
+                kf[2 * i + 1] = codes8((uint32_t)kc[u][i][2], (uint32_t)kc[u][i][3]);
+            }
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) {
+                s[q][u] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int part = PARTS - 1; part >= 0; --part)  // small products first
+#pragma unroll
+                    for (int i = 0; i < 2 * KT; ++i) s[q][u] = mfma16(kf[i], qf[q][i][part], s[q][u]);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (more) {
+            load_k(next);
+            at = next;
+            next = slots_of(j0 + 2 * step);
+        }
+        __builtin_amdgcn_wave_barrier();
+        float ks[8], vs[8];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const float4 a = *reinterpret_cast<const float4*>(&ssc[wave][16 * u + 4 * g]);
+            const float4 b = *reinterpret_cast<const float4*>(&ssc[wave][32 + 16 * u + 4 * g]);
+            ks[4 * u] = a.x, ks[4 * u + 1] = a.y, ks[4 * u + 2] = a.z, ks[4 * u + 3] = a.w;
+            vs[4 * u] = b.x, vs[4 * u + 1] = b.y, vs[4 * u + 2] = b.z, vs[4 * u + 3] = b.w;
+        }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ks[e] = ks[e] * p.scale2;
+        const bool masked = j0 + 32 > kall || ok != 0xffffffffu;
+        v4i pf[NQ][PARTS];
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+            float w[8], x[8], mx = -INFINITY;
+            uint32_t unseen = 0;  // bit e: not a key of this query, whatever its scales are
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = s[q][e >> 2][e & 3] * ks[e];
+            if (masked) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t key = 16 * (e >> 2) + 4 * g + (e & 3);
+                    if (j0 + key >= seen[q] || !((ok >> key) & 1u)) {
+                        w[e] = -INFINITY;
+                        unseen |= 1u << e;
+                    }
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mx = fmaxf(mx, w[e]);
+            mx = fmaxf(mx, xor_lane<16>(mx));
+            mx = fmaxf(mx, xor_lane<32>(mx));
+            if (__any(mx > m[q])) {
+                const float mn = fmaxf(m[q], mx);
+                const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[q] - mn);
+                l[q] = l[q] * alpha;
+#pragma unroll
+                for (int j = 0; j < HD / 16; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[q][j][e] = o[q][j][e] * alpha;
+                m[q] = mn;
+            }
+            const float ref = m[q] == -INFINITY ? 0.0f : m[q];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                w[e] = __builtin_amdgcn_exp2f(w[e] - ref);
+                l[q] = l[q] + w[e];
+                x[e] = w[e] * vs[e];
+            }
+            if (masked) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if ((unseen >> e) & 1u) x[e] = 0.0f;
+            }
+            split8<PARTS>(x, pf[q]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        // O^T: product j takes dimension 4 VW c + j of V for its row c.
+#pragma unroll
+        for (int j = 0; j < HD / 16; ++j) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = code_f(vt[e][j >> 2], j & 3);
+            const v4i vf = v4i{(int)hi16x2(x[0], x[1]), (int)hi16x2(x[2], x[3]), (int)hi16x2(x[4], x[5]), (int)hi16x2(x[6], x[7])};
+#pragma unroll
+            for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                for (int part = PARTS - 1; part >= 0; --part) o[q][j] = mfma16(vf, pf[q][part], o[q][j]);
+        }
+    }
+
+    // The waves' parts, 16 vectors at a time: register (j, r) of lane (c, g) is
+    // dimension 4 VW (4g + r) + j of vector c.
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        l[q] = l[q] + xor_lane<16>(l[q]);
+        l[q] = l[q] + xor_lane<32>(l[q]);
+        if (g == 0) sm[wave][16 * q + c] = m[q], sl[wave][16 * q + c] = l[q];
+    }
+    constexpr int DT = HD / 16;  // a thread's dimensions of vector tid / 16
+    const int mv = tid >> 4, d0 = (tid & 15) * DT;
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < HD / 16; j += 4)
+                *reinterpret_cast<float4*>(&so[wave][c][DT * (4 * g + r) + j]) =
+                    make_float4(o[q][j][r], o[q][j + 1][r], o[q][j + 2][r], o[q][j + 3][r]);
+        __syncthreads();
+        const uint32_t v = bl.v0 + 16 * q + mv;
+        if (v >= vend) continue;
+        float mm = -INFINITY, ll = 0.0f, acc[DT];
+#pragma unroll
+        for (int i = 0; i < DT; ++i) acc[i] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < SW; ++w) mm = fmaxf(mm, sm[w][16 * q + mv]);
+        const float ref = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll
+        for (int w = 0; w < SW; ++w) {
+            const float a = __builtin_amdgcn_exp2f(sm[w][16 * q + mv] - ref);
+            ll = ll + sl[w][16 * q + mv] * a;
+#pragma unroll
+            for (int i = 0; i < DT; i += 4) {
+                const float4 x = *reinterpret_cast<const float4*>(&so[w][mv][d0 + i]);
+                acc[i] = acc[i] + x.x * a, acc[i + 1] = acc[i + 1] + x.y * a;
+                acc[i + 2] = acc[i + 2] + x.z * a, acc[i + 3] = acc[i + 3] + x.w * a;
+            }
+        }
+        if (p.nsplit > 1) {
+            const uint64_t at = ((uint64_t)unit * nkv + kvh) * VB + 16 * q + mv;
+#pragma unroll
+            for (int i = 0; i < DT; i += 4)
+                *reinterpret_cast<float4*>(p.part + at * HD + d0 + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+            if (d0 == 0) p.ml[at] = make_float2(mm, ll);
+        } else {
+            const uint64_t row = (uint64_t)(bl.r0 + v / p.group) * p.nh + kvh * p.group + v % p.group;
+            E* dst = (E*)p.out + row * HD + d0;
+#pragma unroll
+            for (int i = 0; i < DT; ++i) T::put(dst + i, ll == 0.0f ? 0.0f : acc[i] / ll);
+            if (p.lse && d0 == 0) p.lse[row] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * LN2;
+        }
+    }
+}
+
+// Joins the splits of a vector: one wave for each vector of a block.
+template <class T, int HD, int VB>
+__global__ __launch_bounds__(256) void paged_attention_join_kernel(AttnArgs p) {
+    typedef typename T::elem E;
+    const uint32_t lane = threadIdx.x & 63, nkv = p.kv.nkv;
+    const uint32_t bk = blockIdx.x / (VB / 4), blk = bk / nkv, kvh = bk % nkv;
+    const uint32_t u = (blockIdx.x % (VB / 4)) * 4 + (threadIdx.x >> 6);
+    Block bl;
+    if (!find_block<VB>(p.bt, p.group, blk, lane, bl)) return;
+    const uint32_t v = bl.v0 + u;
+    if (v >= bl.nv) return;
+    const uint32_t reach = (uint32_t)min((uint64_t)p.kv.max_bt * p.kv.bs, (uint64_t)0x7fffffffu);
+    const uint32_t kend = min(keys_seen(bl, (min(bl.v0 + VB, bl.nv) - 1) / p.group), reach);
+    const uint32_t live = max(1u, min(p.nsplit, (kend + p.span - 1) / p.span));  // splits that had keys
+    const uint64_t at = ((uint64_t)blk * p.nsplit * nkv + kvh) * VB + u, far = (uint64_t)nkv * VB;
+    float mm = -INFINITY, ll = 0.0f, acc[HD / 64];
+    for (uint32_t s = 0; s < live; ++s) mm = fmaxf(mm, p.ml[at + s * far].x);
+    const float ref = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll
+    for (int i = 0; i < HD / 64; ++i) acc[i] = 0.0f;
+#pragma unroll 4
+    for (uint32_t s = 0; s < live; ++s) {
+        const float2 x = p.ml[at + s * far];
+        const float a = __builtin_amdgcn_exp2f(x.x - ref);
+        ll = ll + x.y * a;
+        const float* src = p.part + (at + s * far) * HD + lane * (HD / 64);
+#pragma unroll
+        for (int i = 0; i < HD / 64; ++i) acc[i] = acc[i] + src[i] * a;
+    }
+    const uint64_t row = (uint64_t)(bl.r0 + v / p.group) * p.nh + kvh * p.group + v % p.group;
+    E* dst = (E*)p.out + row * HD + lane * (HD / 64);
+#pragma unroll
+    for (int i = 0; i < HD / 64; ++i) T::put(dst + i, ll == 0.0f ? 0.0f : acc[i] / ll);
+    if (p.lse && lane == 0) p.lse[row] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * LN2;
+}
+
+// How a call is run.
+struct Plan {
+    int kind;                       // 0: the plain kernel, 1: the streaming kernel
+    uint32_t nq, blocks, nsplit, span;
+    uint64_t part_floats, ml_pairs;
+};
+constexpr uint32_t CUS = 256;
+
+Plan plan_attention(const Kv8& kv, const Kv8Rows& bt, const bh_kv8_batch* hint, uint32_t nh) {
+    Plan r{};
+    const uint32_t group = nh / kv.nkv;
+    if ((kv.hd != 64 && kv.hd != 128) || kv.nslots == 0 || !aligned_to(kv.pool[0], 16) || !aligned_to(kv.pool[1], 16)) return r;
+    r.kind = 1;
+    const uint32_t most = bt.start ? (hint->max_rows ? std::min(hint->max_rows, bt.rows) : bt.rows) : 1;
+    const uint64_t vectors = (uint64_t)most * group;
+    r.nq = vectors <= 16 ? 1 : 2;
+    const uint32_t vb = 16 * r.nq;
+    r.blocks = !bt.start && group <= vb ? bt.batch : (uint32_t)((uint64_t)bt.rows * group / vb) + bt.batch;
+    const uint64_t reach = (uint64_t)kv.max_bt * kv.bs;
+    const uint64_t len = std::max<uint64_t>(1, hint->max_len ? std::min<uint64_t>(hint->max_len, reach) : reach);
+    // Splits of whole rounds of the workgroup's waves (32 keys each).
+    const uint32_t round = 32 * SW;
+    const uint64_t rounds = (len + round - 1) / round, wgs = (uint64_t)r.blocks * kv.nkv;
+    const uint64_t want = std::max<uint64_t>(1, std::min<uint64_t>({rounds, (4 * CUS + wgs - 1) / wgs, 64}));
+    r.span = (uint32_t)std::min<uint64_t>((rounds + want - 1) / want * round, 0x40000000u);
+    r.nsplit = (uint32_t)((len + r.span - 1) / r.span);
+    if (r.nsplit > 1) {
+        r.ml_pairs = (uint64_t)r.blocks * r.nsplit * kv.nkv * vb;
+        r.part_floats = r.ml_pairs * kv.hd;
+    }
+    return r;
+}
+
+template <class T, int HD, int NQ>
+hipError_t go_stream(hipStream_t s, const AttnArgs& a, bool b16) {
+    const uint64_t units = ((uint64_t)a.blocks * a.nsplit + 7) / 8 * 8 * a.kv.nkv;
+    const uint64_t joins = (uint64_t)a.blocks * a.kv.nkv * (16 * NQ / 4);
+    if (units > 0x7fffffffull || joins > 0x7fffffffull) return hipErrorInvalidConfiguration;
+    if (b16) paged_attention_stream_kernel<T, HD, NQ, true><<<(unsigned)units, SW * 64, 0, s>>>(a);
+    else paged_attention_stream_kernel<T, HD, NQ, false><<<(unsigned)units, SW * 64, 0, s>>>(a);
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess && a.nsplit > 1) {
+        paged_attention_join_kernel<T, HD, 16 * NQ><<<(unsigned)joins, 256, 0, s>>>(a);
+        e = hipGetLastError();
+    }
+    return e;
+}
+template <class T, int HD>
+hipError_t go_hd(hipStream_t s, const AttnArgs& a, const Plan& pl) {
+    const bool b16 = a.kv.bs % 16 == 0 && a.kv.nslots % 16 == 0;
+    return pl.nq == 1 ? go_stream<T, HD, 1>(s, a, b16) : go_stream<T, HD, 2>(s, a, b16);
+}
+template <class T>
+hipError_t go_attention(hipStream_t s, const AttnArgs& a, const Plan& pl) {
+    if (pl.kind == 0) {
+        paged_attention_any_kernel<T><<<a.bt.rows * a.nh, 64, 0, s>>>(a);
+        return hipGetLastError();
+    }
+    return a.kv.hd == 128 ? go_hd<T, 128>(s, a, pl) : go_hd<T, 64>(s, a, pl);
+}
+
 int done(hipError_t e, const char* who) {
     return e == hipSuccess ? BH_OK : fail(BH_ERR_HIP, "%s: %s", who, hipGetErrorString(e));
 }
@@ -152,7 +634,8 @@ extern "C" int bh_paged_attention_i8_workspace(const bh_kv8* kv, const bh_kv8_ba
     if (!bytes) return fail(BH_ERR_INVALID, "%s: null result", who);
     const int rc = check_call(who, kv, batch, n_heads, BH_OUT_F32, (uint64_t)-1, &k, &r);
     if (rc) return rc;
-    *bytes = 0;
+    const Plan pl = plan_attention(k, r, batch, n_heads);
+    *bytes = pl.part_floats * 4 + pl.ml_pairs * 8;
     return BH_OK;
 }
 
@@ -167,10 +650,17 @@ extern "C" int bh_paged_attention_i8(void* stream, const void* q, uint64_t q_str
     if (!q || !out) return fail(BH_ERR_INVALID, "%s: null buffer", who);
     a.q = q, a.qs = q_stride, a.out = out, a.lse = lse;
     a.nh = n_heads, a.group = n_heads / kv->n_kv_heads, a.scale2 = scale * LOG2E;
+    const Plan pl = plan_attention(a.kv, a.bt, batch, n_heads);
+    const uint64_t need = pl.part_floats * 4 + pl.ml_pairs * 8;
+    if (ws_bytes < need || (need && (!ws || !aligned_to(ws, 16))))
+        return fail(BH_ERR_INVALID, "%s: a workspace of %llu bytes, 16-byte aligned, is needed, %llu given", who,
+                    (unsigned long long)need, (unsigned long long)ws_bytes);
+    a.blocks = pl.blocks, a.nsplit = pl.nsplit, a.span = pl.span;
+    a.part = (float*)ws, a.ml = (float2*)((float*)ws + pl.part_floats);
+    const size_t es = dtype == BH_OUT_F32 ? 4 : 2;
+    a.qvec = aligned_to(q, 4 * es) && q_stride % 4 == 0;
     const hipStream_t s = (hipStream_t)stream;
-    if (dtype == BH_OUT_F32) paged_attention_any_kernel<F32><<<batch->rows * n_heads, 64, 0, s>>>(a);
-    else paged_attention_any_kernel<Bf16><<<batch->rows * n_heads, 64, 0, s>>>(a);
-    return done(hipGetLastError(), who);
+    return done(dtype == BH_OUT_F32 ? go_attention<F32>(s, a, pl) : go_attention<Bf16>(s, a, pl), who);
 }
 
 extern "C" int bh_paged_weight_sums_i8(void* stream, const void* q, uint64_t q_stride, int dtype, uint32_t n_heads,
