@@ -24,7 +24,7 @@ struct AttnArgs {
     uint32_t blocks, nsplit, span;  // span: keys of a split
     float* part;                    // [unit][kv head][vectors][hd], then
     float2* ml;                     // [unit][kv head][vectors] maximum and sum
-    uint32_t qvec;                  // queries can be loaded 16 bytes at a time
+    uint32_t qvec, ovec;            // queries and outputs lie at multiples of 4 elements
 };
 struct SumsArgs {
     const void* q;
@@ -504,6 +504,342 @@ __global__ __launch_bounds__(SW * 64, (stream_waves<T, HD, NQ>())) void paged_at
     }
 }
 
+// ---------------------------------------------------------------- many rows
+//
+// Four waves of QW query vectors each walk the keys 64 at a time, through LDS:
+// codes go global -> registers -> bf16 -> LDS once for the four, one tile in LDS
+// and one in registers ahead of the products, with one barrier a tile.
+// v_mfma_f32_32x32x16_bf16 on scores transposed (keys x queries), so that a lane
+// has 16 keys of one query, which are the operand of the second product for the
+// order of keys that V^T is stored in.
+//
+// The vector unit's work for each score is kept small, since it takes as long as
+// the products: the key's scale goes into the exponent's fma, and the reference
+// of the softmax is not the running maximum but within 2^SLACK below it (floats
+// lose nothing by it). Whether it must move is seen from a bound, the largest
+// product times the tile's largest scale, without scaling each.
+constexpr int TK = 64;  // keys of a tile
+constexpr float SLACK = 6.0f;
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ v16f mfma32(v4i a, v4i b, v16f c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+}
+
+template <class T, int HD, int QW>
+__global__ __launch_bounds__(256, (QW == 64 ? 1 : 2)) void paged_attention_tile_kernel(AttnArgs p) {
+    typedef typename T::elem E;
+    constexpr int PARTS = sizeof(E) == 4 ? 3 : 1, NB = QW / 32, VB = 4 * QW, KB = TK * HD * 2;
+    __shared__ __attribute__((aligned(1024))) uint8_t kt[2][KB], vt[2][KB];
+    __shared__ __attribute__((aligned(16))) float kcs[2][TK], vss[2][TK];
+    __shared__ __attribute__((aligned(16))) uint32_t ring[4][TK];
+    __shared__ unsigned long long okm[4];
+    __shared__ float kmx[2];
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t nkv = p.kv.nkv, kvs = nkv * HD, units = p.blocks * p.nsplit;
+    uint32_t unit = blockIdx.x / (8 * nkv) * 8 + blockIdx.x % 8;
+    const uint32_t kvh = blockIdx.x / 8 % nkv;
+    if (unit >= units) return;
+    unit = units - 1 - unit;  // a chunk's last rows see the most keys: they start first
+    const uint32_t split = unit % p.nsplit;
+    Block bl;
+    if (!find_block<VB>(p.bt, p.group, unit / p.nsplit, lane, bl)) return;
+    const uint32_t reach = (uint32_t)min((uint64_t)p.kv.max_bt * p.kv.bs, (uint64_t)0x7fffffffu);
+    const uint32_t vend = min(bl.v0 + VB, bl.nv);
+    const uint32_t kend = min(keys_seen(bl, (vend - 1) / p.group), reach);
+    const uint32_t k0 = split * p.span, k1 = split + 1 == p.nsplit ? kend : min(kend, k0 + p.span);
+    if (k0 >= k1 && split) return;
+    const int nt = k1 > k0 ? (int)((k1 - k0 + TK - 1) / TK) : 0;
+
+    // This wave's vectors, and what its first and last see.
+    const uint32_t wv0 = bl.v0 + QW * wave, wv1 = min(wv0 + QW, vend);
+    const bool wlive = wv0 < vend;
+    const uint32_t wall = wlive ? min(keys_seen(bl, wv0 / p.group), reach) : 0u;
+    const uint32_t wend = wlive ? min(keys_seen(bl, (wv1 - 1) / p.group), reach) : 0u;
+    uint32_t seen[NB];
+    v4i qf[NB][HD / 16][PARTS];  // step t: d = 16 t + 8 half ..+7 of vector 32 n + col
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+        const uint32_t v = min(wv0 + 32 * n + col, vend - 1), i = v / p.group, h = kvh * p.group + v % p.group;
+        seen[n] = wv0 + 32 * n + col < vend ? min(keys_seen(bl, i), reach) : 0u;
+        const E* src = (const E*)p.q + (bl.r0 + i) * p.qs + (uint64_t)h * HD + 8 * half;
+#pragma unroll
+        for (int t = 0; t < HD / 16; ++t) {
+            float x[8];
+            query8<T>(src + 16 * t, p.qvec, x);
+            split8<PARTS>(x, qf[n][t]);
+        }
+    }
+    v16f o[NB][HD / 32];
+    float m[NB], l[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+        m[n] = -INFINITY, l[n] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < HD / 32; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[n][j][e] = 0.0f;
+    }
+
+    // ---- staging
+    const uint8_t* kp = (const uint8_t*)p.kv.pool[0] + (size_t)kvh * HD;
+    const uint8_t* vp = (const uint8_t*)p.kv.pool[1] + (size_t)kvh * HD;
+    const float* sp = (tid < TK ? p.kv.scales[0] : p.kv.scales[1]) + kvh;
+    auto barrier = [&]() {  // orders LDS only: loads in flight go on
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // Slots of tile t's keys, by wave 0: a key behind the end or without a slot
+    // gets slot 0 and no bit in okm.
+    auto slot_at = [&](int t) -> uint32_t {
+        const uint32_t j = k0 + (uint32_t)t * TK + lane;
+        return t < nt && j < k1 ? p.kv.slot(bl.b, j) : NO_SLOT;
+    };
+    auto put_slots = [&](int t, uint32_t s) {
+        ring[t & 3][lane] = s != NO_SLOT ? s : 0u;
+        const unsigned long long ok = __ballot(s != NO_SLOT);
+        if (lane == 0) okm[t & 3] = ok;
+    };
+    constexpr int CPK = HD / 16, KPP = 256 / CPK, NK = TK / KPP;  // 16-byte pieces of a key; keys a pass; passes
+    constexpr int DG = HD / 4;
+    const bool vlive = tid < TK / 8 * DG;
+    v4i kr[NK];
+    uint32_t vr[8];
+    float sr = 0.0f;
+    const int kkey = tid / CPK, kpc = tid % CPK, oct = tid / DG, dg = tid % DG;
+    const int vkey = 16 * (oct >> 1) + 4 * (oct & 1);  // octet's keys: vkey ..+3, vkey + 8 ..+11
+    auto load = [&](int t) {
+        const uint32_t* sl = ring[t & 3];
+#pragma unroll
+        for (int u = 0; u < NK; ++u)
+            kr[u] = *reinterpret_cast<const v4i*>(kp + (size_t)sl[kkey + KPP * u] * kvs + 16 * kpc);
+        if (vlive) {
+            const uint4 a = *reinterpret_cast<const uint4*>(sl + vkey), b = *reinterpret_cast<const uint4*>(sl + vkey + 8);
+            const uint32_t ss[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) vr[i] = *reinterpret_cast<const uint32_t*>(vp + (size_t)ss[i] * kvs + 4 * dg);
+        }
+        if (tid < 2 * TK) sr = sp[(size_t)sl[tid & (TK - 1)] * nkv];
+    };
+    // LDS images. K: chunk c (8 d) of key r. V^T: 32 keys at a time, lines of 256
+    // bytes hold 4 d x 32 keys. In both the 16 lanes that meet go to 16 slots.
+    auto kchunk = [&](int r, int c) -> int { return r * (HD * 2) + ((HD == 128 ? c ^ (r & 15) : c ^ ((r >> 1) & 7)) << 4); };
+    auto vchunk = [&](int d, int oc) -> int {
+        return (oc >> 2) * (64 * HD) + (d >> 2) * 256 + (((4 * (d & 3) + (oc & 3)) ^ ((d >> 2) & 15)) << 4);
+    };
+    auto store = [&](int t) {
+        const int bu = t & 1;
+#pragma unroll
+        for (int u = 0; u < NK; ++u) {
+            const int key = kkey + KPP * u;
+            *reinterpret_cast<v4i*>(kt[bu] + kchunk(key, 2 * kpc)) = codes8((uint32_t)kr[u][0], (uint32_t)kr[u][1]);
+            *reinterpret_cast<v4i*>(kt[bu] + kchunk(key, 2 * kpc + 1)) = codes8((uint32_t)kr[u][2], (uint32_t)kr[u][3]);
+        }
+        if (vlive) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = code_f(vr[i], e);
+                *reinterpret_cast<v4i*>(vt[bu] + vchunk(4 * dg + e, oct)) =
+                    v4i{(int)hi16x2(x[0], x[1]), (int)hi16x2(x[2], x[3]), (int)hi16x2(x[4], x[5]), (int)hi16x2(x[6], x[7])};
+            }
+        }
+        if (wave < 2) {  // a key without a slot has scales of 0
+            const bool ok = (okm[t & 3] >> lane) & 1ull;
+            if (wave == 0) {
+                const float kc = ok ? sr * p.scale2 : 0.0f;
+                kcs[bu][lane] = kc;
+                const float mx = xor_max<32>(fabsf(kc));
+                if (lane == 0) kmx[bu] = mx;
+            } else {
+                vss[bu][lane] = ok ? sr : 0.0f;
+            }
+        }
+    };
+
+    uint32_t sl_next = NO_SLOT;
+    if (wave == 0) {
+        put_slots(0, slot_at(0));
+        put_slots(1, slot_at(1));
+        put_slots(2, slot_at(2));
+        sl_next = slot_at(3);
+    }
+    barrier();
+    if (nt) {
+        load(0);
+        store(0);
+        load(1);
+    }
+    barrier();
+#pragma unroll 1
+    for (int t = 0; t < nt; ++t) {
+        const int bu = t & 1;
+        store(t + 1);
+        if (t + 2 < nt) load(t + 2);
+        if (wave == 0) {
+            put_slots(t + 3, sl_next);
+            sl_next = slot_at(t + 4);
+        }
+        const uint32_t j0 = k0 + (uint32_t)t * TK;
+        __builtin_amdgcn_sched_barrier(0);
+        if (j0 < wend) {
+            const float kb = kmx[bu];
+            const unsigned long long ok = okm[t & 3];
+            const bool masked = j0 + TK > wall || ok != ~0ull;
+#pragma unroll
+            for (int kh = 0; kh < 2; ++kh) {
+                v16f s[NB];
+#pragma unroll
+                for (int n = 0; n < NB; ++n)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[n][e] = 0.0f;
+#pragma unroll
+                for (int d = 0; d < HD / 16; ++d) {
+                    const v4i k = *reinterpret_cast<const v4i*>(kt[bu] + kchunk(32 * kh + col, 2 * d + half));
+#pragma unroll
+                    for (int n = 0; n < NB; ++n)
+#pragma unroll
+                        for (int part = PARTS - 1; part >= 0; --part) s[n] = mfma32(k, qf[n][d][part], s[n]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                // Register e: key 32 kh + 8 (e / 4) + 4 half + e % 4.
+                const float* kcp = &kcs[bu][32 * kh + 4 * half];
+                const float* vsp = &vss[bu][32 * kh + 4 * half];
+                uint32_t hid[NB];  // bit e: a key that this query does not see
+                if (masked) {
+                    const uint32_t okh = (uint32_t)(ok >> (32 * kh));
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) {
+                        hid[n] = 0;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const uint32_t key = 8 * (e >> 2) + 4 * half + (e & 3);
+                            if (j0 + 32 * kh + key >= seen[n] || !((okh >> key) & 1u)) hid[n] |= 1u << e;
+                        }
+                    }
+                }
+                bool any = false;
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    float mx = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) mx = fmaxf(fmaxf(mx, fabsf(s[n][e])), fabsf(s[n][e + 1]));
+                    any |= !(mx * kb <= m[n] + SLACK);
+                }
+                if (__any(any)) {  // the bound may be exceeded: look at the scores themselves
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) {
+                        float mx = -INFINITY;
+#pragma unroll
+                        for (int e4 = 0; e4 < 4; ++e4) {
+                            const float4 kc = *reinterpret_cast<const float4*>(kcp + 8 * e4);
+                            const float kk[4] = {kc.x, kc.y, kc.z, kc.w};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float a = s[n][4 * e4 + i] * kk[i];
+                                mx = fmaxf(mx, masked && ((hid[n] >> (4 * e4 + i)) & 1u) ? -INFINITY : a);
+                            }
+                        }
+                        mx = fmaxf(mx, xor_lane<32>(mx));
+                        const float mn = mx > m[n] + SLACK ? mx : m[n];  // each query for itself
+                        const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[n] - mn);
+                        l[n] = l[n] * alpha;
+#pragma unroll
+                        for (int j = 0; j < HD / 32; ++j)
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[n][j][e] = o[n][j][e] * alpha;
+                        m[n] = mn;
+                    }
+                }
+                v4i pf[NB][2][PARTS];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    float kk[8], vv[8];
+#pragma unroll
+                    for (int e4 = 0; e4 < 2; ++e4) {
+                        const float4 kc = *reinterpret_cast<const float4*>(kcp + 16 * u + 8 * e4);
+                        const float4 vs = *reinterpret_cast<const float4*>(vsp + 16 * u + 8 * e4);
+                        kk[4 * e4] = kc.x, kk[4 * e4 + 1] = kc.y, kk[4 * e4 + 2] = kc.z, kk[4 * e4 + 3] = kc.w;
+                        vv[4 * e4] = vs.x, vv[4 * e4 + 1] = vs.y, vv[4 * e4 + 2] = vs.z, vv[4 * e4 + 3] = vs.w;
+                    }
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) {
+                        const float ref = m[n] == -INFINITY ? 0.0f : m[n];
+                        float x[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) x[i] = __builtin_fmaf(s[n][8 * u + i], kk[i], -ref);
+                        if (masked) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                if ((hid[n] >> (8 * u + i)) & 1u) x[i] = -INFINITY;
+                        }
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float w = __builtin_amdgcn_exp2f(x[i]);
+                            l[n] = l[n] + w;
+                            x[i] = w * vv[i];
+                        }
+                        if (masked) {  // whatever its scale is
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                if ((hid[n] >> (8 * u + i)) & 1u) x[i] = 0.0f;
+                        }
+                        split8<PARTS>(x, pf[n][u]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int j = 0; j < HD / 32; ++j) {
+                        const v4i v = *reinterpret_cast<const v4i*>(vt[bu] + vchunk(32 * j + col, 4 * kh + 2 * u + half));
+#pragma unroll
+                        for (int n = 0; n < NB; ++n)
+#pragma unroll
+                            for (int part = PARTS - 1; part >= 0; --part) o[n][j] = mfma32(v, pf[n][u][part], o[n][j]);
+                    }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        barrier();
+    }
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+        const uint32_t v = wv0 + 32 * n + col;
+        const float ll = l[n] + xor_lane<32>(l[n]);
+        if (v >= vend) continue;
+        if (p.nsplit > 1) {
+            const uint64_t at = ((uint64_t)unit * nkv + kvh) * VB + (v - bl.v0);
+#pragma unroll
+            for (int j = 0; j < HD / 32; ++j)
+#pragma unroll
+                for (int e4 = 0; e4 < 4; ++e4)
+                    *reinterpret_cast<float4*>(p.part + at * HD + 32 * j + 8 * e4 + 4 * half) =
+                        make_float4(o[n][j][4 * e4], o[n][j][4 * e4 + 1], o[n][j][4 * e4 + 2], o[n][j][4 * e4 + 3]);
+            if (half == 0) p.ml[at] = make_float2(m[n], ll);
+        } else {
+            const uint64_t row = (uint64_t)(bl.r0 + v / p.group) * p.nh + kvh * p.group + v % p.group;
+            const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+            E* dst = (E*)p.out + row * HD;
+#pragma unroll
+            for (int j = 0; j < HD / 32; ++j)
+#pragma unroll
+                for (int e4 = 0; e4 < 4; ++e4) {
+                    const float y[4] = {o[n][j][4 * e4] * inv, o[n][j][4 * e4 + 1] * inv, o[n][j][4 * e4 + 2] * inv,
+                                        o[n][j][4 * e4 + 3] * inv};
+                    if (p.ovec) T::put4(dst + 32 * j + 8 * e4 + 4 * half, y);
+                    else
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) T::put(dst + 32 * j + 8 * e4 + 4 * half + i, y[i]);
+                }
+            if (p.lse && half == 0) p.lse[row] = ll == 0.0f ? -INFINITY : (m[n] + log2f(ll)) * LN2;
+        }
+    }
+}
+
 // Joins the splits of a vector: one wave for each vector of a block.
 template <class T, int HD, int VB>
 __global__ __launch_bounds__(256) void paged_attention_join_kernel(AttnArgs p) {
@@ -541,48 +877,58 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(AttnArgs p) {
 }
 
 // How a call is run.
+enum Kind { PLAIN, STREAM, TILE };
 struct Plan {
-    int kind;                       // 0: the plain kernel, 1: the streaming kernel
-    uint32_t nq, blocks, nsplit, span;
+    Kind kind;
+    uint32_t vb, blocks, nsplit, span;  // vb: query vectors of a block
     uint64_t part_floats, ml_pairs;
 };
 constexpr uint32_t CUS = 256;
 
-Plan plan_attention(const Kv8& kv, const Kv8Rows& bt, const bh_kv8_batch* hint, uint32_t nh) {
+Plan plan_attention(const Kv8& kv, const Kv8Rows& bt, const bh_kv8_batch* hint, uint32_t nh, int dtype) {
     Plan r{};
     const uint32_t group = nh / kv.nkv;
     if ((kv.hd != 64 && kv.hd != 128) || kv.nslots == 0 || !aligned_to(kv.pool[0], 16) || !aligned_to(kv.pool[1], 16)) return r;
-    r.kind = 1;
     const uint32_t most = bt.start ? (hint->max_rows ? std::min(hint->max_rows, bt.rows) : bt.rows) : 1;
-    const uint64_t vectors = (uint64_t)most * group;
-    r.nq = vectors <= 16 ? 1 : 2;
-    const uint32_t vb = 16 * r.nq;
-    r.blocks = !bt.start && group <= vb ? bt.batch : (uint32_t)((uint64_t)bt.rows * group / vb) + bt.batch;
+    const uint64_t vectors = (uint64_t)most * group, all = (uint64_t)bt.rows * group;
+    r.kind = vectors <= 32 ? STREAM : TILE;
+    r.vb = vectors <= 16 ? 16 : vectors <= 32 ? 32 : 128;
+    if (r.kind == TILE && dtype == BH_OUT_BF16 && all * kv.nkv >= 256ull * CUS) r.vb = 256;
+    r.blocks = !bt.start && group <= r.vb ? bt.batch : (uint32_t)(all / r.vb) + bt.batch;
     const uint64_t reach = (uint64_t)kv.max_bt * kv.bs;
     const uint64_t len = std::max<uint64_t>(1, hint->max_len ? std::min<uint64_t>(hint->max_len, reach) : reach);
-    // Splits of whole rounds of the workgroup's waves (32 keys each).
-    const uint32_t round = 32 * SW;
-    const uint64_t rounds = (len + round - 1) / round, wgs = (uint64_t)r.blocks * kv.nkv;
-    const uint64_t want = std::max<uint64_t>(1, std::min<uint64_t>({rounds, (4 * CUS + wgs - 1) / wgs, 64}));
+    // Splits of whole rounds: 32 keys for each wave, or two tiles.
+    const uint32_t round = 128;
+    const uint64_t rounds = (len + round - 1) / round;
+    uint64_t wgs = (uint64_t)r.blocks * kv.nkv, want;
+    if (r.kind == STREAM) {
+        want = std::min<uint64_t>({rounds, (4 * CUS + wgs - 1) / wgs, 64});
+    } else {
+        wgs = std::max<uint64_t>(1, all / r.vb) * kv.nkv;
+        want = std::min<uint64_t>({(rounds + 1) / 2, (2 * CUS + wgs - 1) / wgs, 32});
+        if (wgs * 4 >= 3 * CUS) want = 1;
+    }
+    want = std::max<uint64_t>(1, want);
     r.span = (uint32_t)std::min<uint64_t>((rounds + want - 1) / want * round, 0x40000000u);
     r.nsplit = (uint32_t)((len + r.span - 1) / r.span);
     if (r.nsplit > 1) {
-        r.ml_pairs = (uint64_t)r.blocks * r.nsplit * kv.nkv * vb;
+        r.ml_pairs = (uint64_t)r.blocks * r.nsplit * kv.nkv * r.vb;
         r.part_floats = r.ml_pairs * kv.hd;
     }
     return r;
 }
 
-template <class T, int HD, int NQ>
-hipError_t go_stream(hipStream_t s, const AttnArgs& a, bool b16) {
+template <class T, int HD, int VB>
+hipError_t go_matrix(hipStream_t s, const AttnArgs& a, bool b16) {
     const uint64_t units = ((uint64_t)a.blocks * a.nsplit + 7) / 8 * 8 * a.kv.nkv;
-    const uint64_t joins = (uint64_t)a.blocks * a.kv.nkv * (16 * NQ / 4);
+    const uint64_t joins = (uint64_t)a.blocks * a.kv.nkv * (VB / 4);
     if (units > 0x7fffffffull || joins > 0x7fffffffull) return hipErrorInvalidConfiguration;
-    if (b16) paged_attention_stream_kernel<T, HD, NQ, true><<<(unsigned)units, SW * 64, 0, s>>>(a);
-    else paged_attention_stream_kernel<T, HD, NQ, false><<<(unsigned)units, SW * 64, 0, s>>>(a);
+    if constexpr (VB > 32) paged_attention_tile_kernel<T, HD, VB / 4><<<(unsigned)units, 256, 0, s>>>(a);
+    else if (b16) paged_attention_stream_kernel<T, HD, VB / 16, true><<<(unsigned)units, SW * 64, 0, s>>>(a);
+    else paged_attention_stream_kernel<T, HD, VB / 16, false><<<(unsigned)units, SW * 64, 0, s>>>(a);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && a.nsplit > 1) {
-        paged_attention_join_kernel<T, HD, 16 * NQ><<<(unsigned)joins, 256, 0, s>>>(a);
+        paged_attention_join_kernel<T, HD, VB><<<(unsigned)joins, 256, 0, s>>>(a);
         e = hipGetLastError();
     }
     return e;
@@ -590,11 +936,17 @@ hipError_t go_stream(hipStream_t s, const AttnArgs& a, bool b16) {
 template <class T, int HD>
 hipError_t go_hd(hipStream_t s, const AttnArgs& a, const Plan& pl) {
     const bool b16 = a.kv.bs % 16 == 0 && a.kv.nslots % 16 == 0;
-    return pl.nq == 1 ? go_stream<T, HD, 1>(s, a, b16) : go_stream<T, HD, 2>(s, a, b16);
+    switch (pl.vb) {
+        case 16: return go_matrix<T, HD, 16>(s, a, b16);
+        case 32: return go_matrix<T, HD, 32>(s, a, b16);
+        case 128: return go_matrix<T, HD, 128>(s, a, b16);
+    }
+    if constexpr (sizeof(typename T::elem) == 2) return go_matrix<T, HD, 256>(s, a, b16);
+    return hipErrorInvalidValue;
 }
 template <class T>
 hipError_t go_attention(hipStream_t s, const AttnArgs& a, const Plan& pl) {
-    if (pl.kind == 0) {
+    if (pl.kind == PLAIN) {
         paged_attention_any_kernel<T><<<a.bt.rows * a.nh, 64, 0, s>>>(a);
         return hipGetLastError();
     }
@@ -634,8 +986,12 @@ extern "C" int bh_paged_attention_i8_workspace(const bh_kv8* kv, const bh_kv8_ba
     if (!bytes) return fail(BH_ERR_INVALID, "%s: null result", who);
     const int rc = check_call(who, kv, batch, n_heads, BH_OUT_F32, (uint64_t)-1, &k, &r);
     if (rc) return rc;
-    const Plan pl = plan_attention(k, r, batch, n_heads);
-    *bytes = pl.part_floats * 4 + pl.ml_pairs * 8;
+    uint64_t need = 0;
+    for (const int dtype : {BH_OUT_F32, BH_OUT_BF16}) {
+        const Plan pl = plan_attention(k, r, batch, n_heads, dtype);
+        need = std::max(need, pl.part_floats * 4 + pl.ml_pairs * 8);
+    }
+    *bytes = need;
     return BH_OK;
 }
 
@@ -650,7 +1006,7 @@ extern "C" int bh_paged_attention_i8(void* stream, const void* q, uint64_t q_str
     if (!q || !out) return fail(BH_ERR_INVALID, "%s: null buffer", who);
     a.q = q, a.qs = q_stride, a.out = out, a.lse = lse;
     a.nh = n_heads, a.group = n_heads / kv->n_kv_heads, a.scale2 = scale * LOG2E;
-    const Plan pl = plan_attention(a.kv, a.bt, batch, n_heads);
+    const Plan pl = plan_attention(a.kv, a.bt, batch, n_heads, dtype);
     const uint64_t need = pl.part_floats * 4 + pl.ml_pairs * 8;
     if (ws_bytes < need || (need && (!ws || !aligned_to(ws, 16))))
         return fail(BH_ERR_INVALID, "%s: a workspace of %llu bytes, 16-byte aligned, is needed, %llu given", who,
@@ -659,6 +1015,7 @@ extern "C" int bh_paged_attention_i8(void* stream, const void* q, uint64_t q_str
     a.part = (float*)ws, a.ml = (float2*)((float*)ws + pl.part_floats);
     const size_t es = dtype == BH_OUT_F32 ? 4 : 2;
     a.qvec = aligned_to(q, 4 * es) && q_stride % 4 == 0;
+    a.ovec = aligned_to(out, 4 * es);
     const hipStream_t s = (hipStream_t)stream;
     return done(dtype == BH_OUT_F32 ? go_attention<F32>(s, a, pl) : go_attention<Bf16>(s, a, pl), who);
 }
