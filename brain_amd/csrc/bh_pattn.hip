@@ -35,6 +35,7 @@ struct SumsArgs {
     Kv8Rows bt;
     uint32_t nh, group, cap;
     float scale2;
+    uint32_t qvec, nchunk;  // as AttnArgs; workgroups of a (sequence, kv head)
 };
 
 __device__ __forceinline__ float code_f(uint32_t w, int e) { return (float)(int8_t)(uint8_t)(w >> (8 * e)); }
@@ -876,6 +877,174 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(AttnArgs p) {
     if (p.lse && lane == 0) p.lse[row] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * LN2;
 }
 
+// ---------------------------------------------------------------- weight sums
+//
+// The keys stay, the queries pass by: a wave holds the codes of 16 KG keys as
+// operands of v_mfma_f32_16x16x32_bf16, loaded straight in its layout, and the
+// workgroup's queries go through LDS 32 at a time, two buffers. A lane then has
+// four queries' scores of one key, so a key's sum needs no exchange until the
+// end, and its order is that of the rows. A workgroup takes 64 KG keys of one
+// kv head, and more of them when the grid (made for max_len) does not reach.
+template <class T, int HD, int KG>
+__global__ __launch_bounds__(256, 2) void paged_weight_sums_kernel(SumsArgs p) {
+    typedef typename T::elem E;
+    constexpr int PARTS = sizeof(E) == 4 ? 3 : 1, TQ = 32, ST = HD / 32, PB = TQ * HD * 2;
+    __shared__ __attribute__((aligned(1024))) uint8_t qt[2][PARTS][PB];
+    __shared__ __attribute__((aligned(16))) float lses[2][TQ];
+    __shared__ __attribute__((aligned(16))) uint32_t sees[2][TQ];
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // All kv heads of a unit on one XCD: their scales share cache lines.
+    const uint32_t nkv = p.kv.nkv, unit = blockIdx.x / (8 * nkv) * 8 + blockIdx.x % 8, kvh = blockIdx.x / 8 % nkv;
+    if (unit >= p.bt.batch * p.nchunk) return;
+    Block bl;
+    bl.b = unit / p.nchunk;
+    const uint32_t r1 = p.bt.end(bl.b);
+    bl.r0 = p.bt.first(bl.b);
+    bl.n = r1 > bl.r0 ? r1 - bl.r0 : 0u;
+    bl.nv = bl.n * p.group, bl.v0 = 0, bl.len = p.bt.lens[bl.b];
+    const uint32_t end = min(bl.len, p.cap), kvs = nkv * HD;
+    float* acc = p.acc + ((uint64_t)bl.b * nkv + kvh) * p.cap;
+    auto kchunk = [&](int r, int ch) -> int { return r * (HD * 2) + ((HD == 128 ? ch ^ (r & 15) : ch ^ ((r >> 1) & 7)) << 4); };
+    // A thread brings HD / 8 elements of vector tid / 8 of a tile.
+    constexpr int QE = HD / 8;
+    const int qv = tid >> 3, qd = (tid & 7) * QE;
+    for (uint64_t j0 = (uint64_t)(unit % p.nchunk) * (64 * KG); j0 < end; j0 += (uint64_t)p.nchunk * (64 * KG)) {
+        // Keys: group k of the wave, key c of it.
+        v4i kf[KG][2 * HD / 64];
+        float kc[KG], sum[KG], old[KG];
+        bool live[KG];
+        const uint32_t jw = (uint32_t)j0 + 16 * KG * wave;
+#pragma unroll
+        for (int k = 0; k < KG; ++k) {
+            const uint32_t j = jw + 16 * k + c, slot = j < end ? p.kv.slot(bl.b, j) : NO_SLOT, s = slot != NO_SLOT ? slot : 0u;
+            live[k] = slot != NO_SLOT;
+            const uint8_t* src = (const uint8_t*)p.kv.pool[0] + (size_t)s * kvs + kvh * HD + 16 * g;
+#pragma unroll
+            for (int i = 0; i < HD / 64; ++i) {
+                const v4i w = *reinterpret_cast<const v4i*>(src + 64 * i);
+                kf[k][2 * i] = codes8((uint32_t)w[0], (uint32_t)w[1]);
+                kf[k][2 * i + 1] = codes8((uint32_t)w[2], (uint32_t)w[3]);
+            }
+            kc[k] = p.kv.scales[0][(size_t)s * nkv + kvh] * p.scale2;
+            sum[k] = 0.0f;
+            old[k] = j < end && (uint64_t)j + bl.n < bl.len ? acc[j] : 0.0f;
+        }
+        // The first row that sees the first key, from a whole tile on.
+        const uint64_t i0 = j0 + bl.n > bl.len ? j0 + bl.n - bl.len : 0;
+        const uint32_t v0 = (uint32_t)min(i0 * p.group, (uint64_t)bl.nv) / TQ * TQ;
+        float x[QE], xl = 0.0f;
+        uint32_t xs = 0;
+        auto load = [&](uint32_t v) {
+            const uint32_t vv = min(v + qv, bl.nv - 1), i = vv / p.group, h = kvh * p.group + vv % p.group;
+            const E* src = (const E*)p.q + (bl.r0 + i) * p.qs + (uint64_t)h * HD + qd;
+#pragma unroll
+            for (int u = 0; u < QE; u += 8) {
+                float y[8];
+                query8<T>(src + u, p.qvec, y);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[u + e] = y[e];
+            }
+            xl = p.lse[(uint64_t)(bl.r0 + i) * p.nh + h] * LOG2E;
+            xs = v + qv < bl.nv ? keys_seen(bl, i) : 0u;
+        };
+        auto store = [&](int bu) {
+#pragma unroll
+            for (int u = 0; u < QE; u += 8) {
+                float y[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = x[u + e];
+                v4i f[PARTS];
+                split8<PARTS>(y, f);
+#pragma unroll
+                for (int part = 0; part < PARTS; ++part)
+                    *reinterpret_cast<v4i*>(&qt[bu][part][kchunk(qv, (qd + u) / 8)]) = f[part];
+            }
+            if ((tid & 7) == 0) lses[bu][qv] = xl, sees[bu][qv] = xs;
+        };
+        __syncthreads();  // the buffers are free
+        if (v0 < bl.nv) {
+            load(v0);
+            store(0);
+        }
+        __syncthreads();
+        int bu = 0;
+#pragma unroll 1
+        for (uint32_t v = v0; v < bl.nv; v += TQ, bu ^= 1) {
+            const bool more = v + TQ < bl.nv;
+            if (more) load(v + TQ);
+            // Every vector of the tile sees every key of the wave.
+            const bool masked = v + TQ > bl.nv || keys_seen(bl, v / p.group) < (uint64_t)jw + 16 * KG;
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub) {
+                v4f s[KG];
+#pragma unroll
+                for (int k = 0; k < KG; ++k) s[k] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int part = PARTS - 1; part >= 0; --part)
+#pragma unroll
+                    for (int t = 0; t < ST; ++t) {
+                        const v4i a = *reinterpret_cast<const v4i*>(&qt[bu][part][kchunk(16 * sub + c, 2 * (g + 4 * (t >> 1)) + (t & 1))]);
+#pragma unroll
+                        for (int k = 0; k < KG; ++k) s[k] = mfma16(a, kf[k][t], s[k]);
+                    }
+                const float4 l4 = *reinterpret_cast<const float4*>(&lses[bu][16 * sub + 4 * g]);
+                const float ll[4] = {l4.x, l4.y, l4.z, l4.w};
+                if (!masked) {
+#pragma unroll
+                    for (int k = 0; k < KG; ++k)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            sum[k] = sum[k] + __builtin_amdgcn_exp2f(__builtin_fmaf(s[k][r], kc[k], -ll[r]));
+                } else {
+                    const uint4 n4 = *reinterpret_cast<const uint4*>(&sees[bu][16 * sub + 4 * g]);
+                    const uint32_t nn[4] = {n4.x, n4.y, n4.z, n4.w};
+#pragma unroll
+                    for (int k = 0; k < KG; ++k)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k][r], kc[k], -ll[r]));
+                            sum[k] = sum[k] + (jw + 16 * k + c < nn[r] ? w : 0.0f);
+                        }
+                }
+            }
+            if (more) store(bu ^ 1);
+            __syncthreads();
+        }
+#pragma unroll
+        for (int k = 0; k < KG; ++k) {
+            float w = sum[k] + xor_lane<16>(sum[k]);
+            w = w + xor_lane<32>(w);
+            const uint32_t j = jw + 16 * k + c;
+            if (g == k % 4 && j < end) acc[j] = (live[k] ? w : 0.0f) + old[k];
+        }
+    }
+}
+
+template <class T, int HD, int KG>
+hipError_t go_sums(hipStream_t s, SumsArgs a, uint64_t len) {
+    const uint64_t most = std::max<uint64_t>(1, 0x7fffffffull / 8 / a.kv.nkv / a.bt.batch);
+    a.nchunk = (uint32_t)std::min<uint64_t>((len + 64 * KG - 1) / (64 * KG), most);
+    const uint64_t grid = ((uint64_t)a.bt.batch * a.nchunk + 7) / 8 * 8 * a.kv.nkv;
+    if (grid > 0x7fffffffull) return hipErrorInvalidConfiguration;
+    paged_weight_sums_kernel<T, HD, KG><<<(unsigned)grid, 256, 0, s>>>(a);
+    return hipGetLastError();
+}
+template <class T>
+hipError_t go_weight_sums(hipStream_t s, const SumsArgs& a, const bh_kv8_batch* hint) {
+    if ((a.kv.hd != 64 && a.kv.hd != 128) || a.kv.nslots == 0 || !aligned_to(a.kv.pool[0], 16)) {
+        const uint32_t nchunk = (a.cap - 1) / 64 + 1;
+        const uint64_t grid = (uint64_t)a.bt.batch * a.kv.nkv * nchunk;
+        if (grid > 0x7fffffffull) return hipErrorInvalidConfiguration;
+        paged_weight_sums_any_kernel<T><<<(unsigned)grid, 64, 0, s>>>(a, nchunk);
+        return hipGetLastError();
+    }
+    const uint64_t len = std::max<uint64_t>(1, hint->max_len ? std::min(hint->max_len, a.cap) : a.cap);
+    const bool few = (uint64_t)a.bt.batch * a.kv.nkv * ((len + 255) / 256) < 256;
+    if (a.kv.hd == 128) return few ? go_sums<T, 128, 1>(s, a, len) : go_sums<T, 128, 4>(s, a, len);
+    return few ? go_sums<T, 64, 1>(s, a, len) : go_sums<T, 64, 4>(s, a, len);
+}
+
 // How a call is run.
 enum Kind { PLAIN, STREAM, TILE };
 struct Plan {
@@ -1031,11 +1200,7 @@ extern "C" int bh_paged_weight_sums_i8(void* stream, const void* q, uint64_t q_s
     if (!q || !lse || !acc) return fail(BH_ERR_INVALID, "%s: null buffer", who);
     a.q = q, a.qs = q_stride, a.lse = lse, a.acc = acc, a.cap = acc_stride;
     a.nh = n_heads, a.group = n_heads / kv->n_kv_heads, a.scale2 = scale * LOG2E;
-    const uint32_t nchunk = (acc_stride - 1) / 64 + 1;
-    const uint64_t grid = (uint64_t)batch->batch * kv->n_kv_heads * nchunk;
-    if (grid > 0x7fffffffull) return fail(BH_ERR_INVALID, "%s: grid too large", who);
+    a.qvec = aligned_to(q, dtype == BH_OUT_F32 ? 16 : 8) && q_stride % 4 == 0;
     const hipStream_t s = (hipStream_t)stream;
-    if (dtype == BH_OUT_F32) paged_weight_sums_any_kernel<F32><<<(unsigned)grid, 64, 0, s>>>(a, nchunk);
-    else paged_weight_sums_any_kernel<Bf16><<<(unsigned)grid, 64, 0, s>>>(a, nchunk);
-    return done(hipGetLastError(), who);
+    return done(dtype == BH_OUT_F32 ? go_weight_sums<F32>(s, a, batch) : go_weight_sums<Bf16>(s, a, batch), who);
 }
