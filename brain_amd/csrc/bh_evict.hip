@@ -24,24 +24,136 @@ __device__ __forceinline__ uint32_t place(float v) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// One workgroup for each (sequence, kv head). The weight of the last entry
-// kept is found digit by digit from the top (8 bits at a time, a histogram in
-// LDS for each): 4 passes over the weights. A last pass in order writes the
-// kept positions and their weights.
 constexpr uint32_t ET = 1024;
+
+// A sequence within its budget keeps all.
+__device__ __forceinline__ void keep_all(const EvictArgs& p, uint32_t len, const float* acc, float* acc_out, int32_t* keep) {
+    for (uint32_t j = threadIdx.x; j < p.budget; j += ET) keep[j] = j < len ? (int32_t)j : -1;
+    if (acc_out && acc_out != acc)
+        for (uint32_t j = threadIdx.x; j < len; j += ET) acc_out[j] = acc[j];
+}
+
+// One workgroup for each (sequence, kv head), its weights in registers (VPT a
+// thread, wave w those of positions 64 VPT w .. on): latency bounds it, so each
+// weight is loaded once and the steps that the workgroup takes together are few.
+// The weight of the last entry kept is found digit by digit from the top, 11, 11
+// and 10 bits, a histogram in LDS for each (the first of 8 bits would hold little
+// but exponents, a few bins for all weights to queue at); then a count of each
+// wave's kept entries says where it writes them.
+template <int VPT>
 __global__ __launch_bounds__(ET) void kv_evict_select_kernel(EvictArgs p) {
+    constexpr int NW = ET / 64, BINS = 2048;
+    __shared__ uint32_t hist[BINS], wtot[NW], pick[2];
+    const uint32_t b = blockIdx.x / p.kv.nkv, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint32_t len = min(p.lens[b], p.cap);
+    const float* acc = p.acc + (uint64_t)blockIdx.x * p.cap;
+    float* acc_out = p.acc_out ? p.acc_out + (uint64_t)blockIdx.x * p.cap_out : nullptr;
+    int32_t* keep = p.keep + (uint64_t)blockIdx.x * p.budget;
+    if (len <= p.budget) return keep_all(p, len, acc, acc_out, keep);
+    // The candidates are positions [lo, hi); `need` of them stay.
+    const uint32_t lo = p.sink, hi = len - p.recent, need = p.budget - p.sink - p.recent;
+    const uint32_t j0 = wave * 64 * VPT + lane;
+    float v[VPT];
+    uint32_t u[VPT];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) v[i] = j0 + 64 * i < len ? acc[j0 + 64 * i] : 0.0f;
+    uint32_t prefix = 0, left = need;  // of the digits found; how many of the weights that share them stay
+    if (need) {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) u[i] = place(v[i]);
+#pragma unroll
+        for (int d = 0; d < 3; ++d) {
+            const int shift = d == 0 ? 21 : d == 1 ? 10 : 0;
+            const uint32_t digit = d == 2 ? 1023u : 2047u, mask = d == 0 ? 0u : ~0u << (d == 1 ? 21 : 10);
+            for (uint32_t i = tid; i < BINS; i += ET) hist[i] = 0;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) {
+                const uint32_t j = j0 + 64 * i;
+                if (j >= lo && j < hi && (u[i] & mask) == prefix) atomicAdd(&hist[(u[i] >> shift) & digit], 1u);
+            }
+            __syncthreads();
+            // The highest digit with at least `left` weights at or above it:
+            // thread t looks at two, from the top.
+            const uint32_t c1 = hist[BINS - 1 - 2 * tid], c0 = hist[BINS - 2 - 2 * tid];
+            uint32_t upto = c1 + c0;
+#pragma unroll
+            for (int off = 1; off < 64; off *= 2) {
+                const uint32_t o = __shfl_up(upto, off, 64);
+                if ((int)lane >= off) upto += o;
+            }
+            if (lane == 63) wtot[wave] = upto;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < NW; ++w)
+                if (w < (int)wave) upto += wtot[w];
+            const uint32_t above = upto - c1 - c0;
+            if (above < left && left <= upto) {
+                const bool first = above + c1 >= left;
+                pick[0] = BINS - 2 - 2 * tid + (first ? 1 : 0);
+                pick[1] = left - above - (first ? 0 : c1);
+            }
+            __syncthreads();
+            prefix |= pick[0] << shift;
+            left = pick[1];
+        }
+    }
+    // All weights above `prefix` stay, and the first `left` equal to it.
+    const unsigned long long below = (1ull << lane) - 1;
+    uint32_t n = 0;
+    if (need) {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const uint32_t j = j0 + 64 * i;
+            n += (uint32_t)__popcll(__ballot(j >= lo && j < hi && u[i] == prefix));
+        }
+    }
+    if (lane == 0) wtot[wave] = n;
+    __syncthreads();
+    uint32_t before = 0, kept = 0, stay = 0;  // stay: bit i, entry i of this thread
+#pragma unroll
+    for (int w = 0; w < NW; ++w)
+        if (w < (int)wave) before += wtot[w];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        const uint32_t j = j0 + 64 * i;
+        const bool mid = j >= lo && j < hi, eq = need && mid && u[i] == prefix;
+        const unsigned long long em = __ballot(eq);
+        const bool s = j < len && (!mid || (need && (u[i] > prefix || (eq && before + (uint32_t)__popcll(em & below) < left))));
+        before += (uint32_t)__popcll(em);
+        kept += (uint32_t)__popcll(__ballot(s));
+        stay |= (s ? 1u : 0u) << i;
+    }
+    __syncthreads();
+    if (lane == 0) wtot[wave] = kept;
+    __syncthreads();
+    uint32_t to = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w)
+        if (w < (int)wave) to += wtot[w];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        const bool s = (stay >> i) & 1u;
+        const unsigned long long km = __ballot(s);
+        const uint32_t at = to + (uint32_t)__popcll(km & below);
+        if (s && at < p.budget) {  // (acc_out may be acc: all of it has been read)
+            keep[at] = (int32_t)(j0 + 64 * i);
+            if (acc_out) acc_out[at] = v[i];
+        }
+        to += (uint32_t)__popcll(km);
+    }
+}
+
+// The same for any length, its weights read again for each digit (8 bits at a
+// time) and for the last pass, which goes through them in order.
+__global__ __launch_bounds__(ET) void kv_evict_select_long_kernel(EvictArgs p) {
     __shared__ uint32_t hist[256], wtot[ET / 64], pick[2];
     const uint32_t b = blockIdx.x / p.kv.nkv, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const uint32_t len = min(p.lens[b], p.cap);
     const float* acc = p.acc + (uint64_t)blockIdx.x * p.cap;
     float* acc_out = p.acc_out ? p.acc_out + (uint64_t)blockIdx.x * p.cap_out : nullptr;
     int32_t* keep = p.keep + (uint64_t)blockIdx.x * p.budget;
-    if (len <= p.budget) {
-        for (uint32_t j = tid; j < p.budget; j += ET) keep[j] = j < len ? (int32_t)j : -1;
-        if (acc_out && acc_out != acc)
-            for (uint32_t j = tid; j < len; j += ET) acc_out[j] = acc[j];
-        return;
-    }
+    if (len <= p.budget) return keep_all(p, len, acc, acc_out, keep);
     // The candidates are positions [lo, hi); `need` of them stay.
     const uint32_t lo = p.sink, hi = len - p.recent, need = p.budget - p.sink - p.recent;
     uint32_t prefix = 0, left = need;  // of the digits found; how many of the weights that share them stay
@@ -117,39 +229,66 @@ __global__ __launch_bounds__(ET) void kv_evict_select_kernel(EvictArgs p) {
     }
 }
 
-// One workgroup for each (sequence, kv head, keys or values), MK entries at a
-// time in order. Position i's entry comes from keep[i] >= i: what a step
-// writes, in place, no later step reads, so a barrier between a step's reads
-// and its writes is enough.
+// Moves the entries of a (sequence, kv head), keys or values. A thread takes a
+// piece of W, MU entries of a step at a time in flight. Position i's entry comes
+// from keep[i] >= i, so in place a workgroup goes through all of them in order:
+// what a step writes no later step reads, and a barrier between its reads and
+// its writes is enough. To other blocks the steps are spread over workgroups.
 constexpr uint32_t MT = 256;
-__global__ __launch_bounds__(MT) void kv_evict_move_kernel(EvictArgs p) {
-    const uint32_t which = blockIdx.x & 1, bk = blockIdx.x >> 1, b = bk / p.kv.nkv, kvh = bk % p.kv.nkv;
-    const uint32_t words = p.kv.hd / 4;
+constexpr int MU = 4;
+template <class W, bool IN_PLACE>
+__global__ __launch_bounds__(MT) void kv_evict_move_kernel(EvictArgs p, uint32_t steps, uint32_t per) {
+    const uint32_t group = blockIdx.x / steps, which = group & 1, bk = group >> 1, b = bk / p.kv.nkv, kvh = bk % p.kv.nkv;
+    const uint32_t pieces = p.kv.hd / sizeof(W), e = threadIdx.x / pieces, w = threadIdx.x % pieces;
     const int32_t* keep = p.keep + (uint64_t)bk * p.budget;
-    if (kvh == 0 && which == 0 && threadIdx.x == 0) p.new_lens[b] = min(min(p.lens[b], p.cap), p.budget);
-    // A thread moves one word of an entry (lane groups of `words`).
-    const uint32_t per = MT / words, e = threadIdx.x / words, w = threadIdx.x % words;
-    for (uint32_t i0 = 0; i0 < p.budget; i0 += per) {
-        const uint32_t i = i0 + e;
-        const int32_t src = e < per && i < p.budget ? keep[i] : -1;
-        uint32_t from = NO_SLOT, to = NO_SLOT;
-        uint32_t c = 0;
-        float s = 0.0f;
-        if (src >= 0 && !(p.in_place && (uint32_t)src == i)) {
-            from = p.kv.slot(b, (uint32_t)src);
-            to = p.kv.slot_in(p.to, p.to_cols, b, i);
-            if (from != NO_SLOT && to != NO_SLOT) {
-                c = p.kv.pool[which][(p.kv.row(from) + (uint64_t)kvh * p.kv.hd) / 4 + w];
-                if (w == 0) s = p.kv.scales[which][(uint64_t)from * p.kv.nkv + kvh];
+    if (kvh == 0 && blockIdx.x % (2 * steps * p.kv.nkv) == 0 && threadIdx.x == 0)
+        p.new_lens[b] = min(min(p.lens[b], p.cap), p.budget);
+    uint8_t* pool = (uint8_t*)(which ? p.kv.pool[1] : p.kv.pool[0]) + (size_t)kvh * p.kv.hd + w * sizeof(W);
+    float* scales = (which ? p.kv.scales[1] : p.kv.scales[0]) + kvh;
+    for (uint64_t i0 = (uint64_t)(blockIdx.x % steps) * MU * per; i0 < p.budget; i0 += (uint64_t)steps * MU * per) {
+        uint32_t from[MU], to[MU];
+        W c[MU];
+        float s[MU];
+#pragma unroll
+        for (int u = 0; u < MU; ++u) {
+            const uint64_t i = i0 + u * per + e;
+            const int32_t src = e < per && i < p.budget ? keep[i] : -1;
+            const bool move = src >= 0 && !(IN_PLACE && (uint32_t)src == (uint32_t)i);
+            from[u] = move ? p.kv.slot(b, (uint32_t)src) : NO_SLOT;
+            to[u] = move ? p.kv.slot_in(p.to, p.to_cols, b, (uint32_t)i) : NO_SLOT;
+        }
+#pragma unroll
+        for (int u = 0; u < MU; ++u) {
+            if (to[u] == NO_SLOT) from[u] = NO_SLOT;
+            c[u] = W{};
+            s[u] = 0.0f;
+            if (from[u] != NO_SLOT) {
+                c[u] = *reinterpret_cast<const W*>(pool + p.kv.row(from[u]));
+                if (w == 0) s[u] = scales[(uint64_t)from[u] * p.kv.nkv];
             }
         }
-        __syncthreads();
-        if (from != NO_SLOT && to != NO_SLOT) {
-            p.kv.pool[which][(p.kv.row(to) + (uint64_t)kvh * p.kv.hd) / 4 + w] = c;
-            if (w == 0) p.kv.scales[which][(uint64_t)to * p.kv.nkv + kvh] = s;
+        if constexpr (IN_PLACE) __syncthreads();
+#pragma unroll
+        for (int u = 0; u < MU; ++u) {
+            if (from[u] == NO_SLOT) continue;
+            *reinterpret_cast<W*>(pool + p.kv.row(to[u])) = c[u];
+            if (w == 0) scales[(uint64_t)to[u] * p.kv.nkv] = s[u];
         }
-        __syncthreads();
+        if constexpr (IN_PLACE) __syncthreads();
     }
+}
+
+template <class W>
+hipError_t go_move(hipStream_t s, const EvictArgs& a, uint64_t heads) {
+    const uint32_t per = MT / (a.kv.hd / sizeof(W));  // entries of a pass
+    const uint64_t all = (a.budget + (uint64_t)per * MU - 1) / (per * MU);
+    if (a.in_place) {
+        kv_evict_move_kernel<W, true><<<(unsigned)(2 * heads), MT, 0, s>>>(a, 1, per);
+    } else {
+        const uint32_t steps = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(all, 0x7fffffffull / (2 * heads)));
+        kv_evict_move_kernel<W, false><<<(unsigned)(2 * heads * steps), MT, 0, s>>>(a, steps, per);
+    }
+    return hipGetLastError();
 }
 
 }  // namespace
@@ -181,11 +320,11 @@ extern "C" int bh_paged_kv_evict_i8(void* stream, const bh_kv8* kv, const uint32
     a.to_cols = a.in_place ? kv->max_blocks : out_max_blocks;
     a.cap = acc_stride, a.cap_out = acc_out_stride, a.budget = budget, a.sink = sink, a.recent = recent;
     const hipStream_t s = (hipStream_t)stream;
-    kv_evict_select_kernel<<<(unsigned)heads, ET, 0, s>>>(a);
+    if (acc_stride <= 4 * ET) kv_evict_select_kernel<4><<<(unsigned)heads, ET, 0, s>>>(a);
+    else if (acc_stride <= 16 * ET) kv_evict_select_kernel<16><<<(unsigned)heads, ET, 0, s>>>(a);
+    else kv_evict_select_long_kernel<<<(unsigned)heads, ET, 0, s>>>(a);
     hipError_t e = hipGetLastError();
-    if (e == hipSuccess) {
-        kv_evict_move_kernel<<<(unsigned)(2 * heads), MT, 0, s>>>(a);
-        e = hipGetLastError();
-    }
+    const bool wide = kv->head_dim % 16 == 0 && aligned_to(kv->k_pool, 16) && aligned_to(kv->v_pool, 16);
+    if (e == hipSuccess) e = wide ? go_move<uint4>(s, a, heads) : go_move<uint32_t>(s, a, heads);
     return e == hipSuccess ? BH_OK : fail(BH_ERR_HIP, "%s: %s", who, hipGetErrorString(e));
 }

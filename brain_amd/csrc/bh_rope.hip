@@ -114,9 +114,126 @@ __global__ __launch_bounds__(64) void qk_norm_rope_any_kernel(RopeRowsArgs p) {
     }
 }
 
+// Heads of 64, 128 or 256 turned whole: HD / 8 lanes hold a head, lane i its
+// elements 4i ..+3 of both halves, so a pair meets in a lane and a wave works on
+// 512 / HD heads at once. Memory traffic bounds it: a wave takes one row (or a
+// `part` of its heads, where there are few rows) and computes its angles once
+// for all of them; the next heads' loads are in flight while it works.
+template <class T, int HD, bool APPEND>
+__global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeRowsArgs p, uint32_t parts) {
+    typedef typename T::elem E;
+    constexpr int LPH = HD / 8, HPW = 64 / LPH, HALF = HD / 2;
+    const uint32_t lane = threadIdx.x & 63, li = lane % LPH;
+    const uint32_t w = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
+    const uint32_t r = w / parts, heads = p.nh + p.nkv * (APPEND ? 2 : 1);
+    if (r >= p.rows) return;
+    uint32_t h = (w % parts) * HPW + lane / LPH;
+    struct In {
+        float a[4], b[4];
+    };
+    auto source = [&](uint32_t hh) -> const E* {
+        const E* base = hh < p.nh ? (const E*)p.q + r * p.qs + (uint64_t)hh * HD
+                        : hh < p.nh + p.nkv ? (const E*)p.k + r * p.ks + (uint64_t)(hh - p.nh) * HD
+                                            : (const E*)p.v + r * p.vs + (uint64_t)(hh - p.nh - p.nkv) * HD;
+        return base + 4 * li;
+    };
+    auto load = [&](uint32_t hh, In& x) {  // a head behind the last one reads the last
+        const E* src = source(min(hh, heads - 1));
+        T::get4(src, x.a);
+        T::get4(src + HALF, x.b);
+    };
+    In x;
+    load(h, x);
+    const uint32_t pos = p.pos[r];
+    float cs[4], sn[4], qw[8], kw[8];
+    double f[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = p.freq[4 * li + e];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const uint32_t d = (e < 4 ? 0 : HALF) + 4 * li + (e & 3);
+        qw[e] = p.qw ? p.qw[d] : 1.0f;
+        kw[e] = p.kw ? p.kw[d] : 1.0f;
+    }
+    uint32_t slot = 0;
+    if constexpr (APPEND)
+        if (!row_slot(p.kv, p.bt, r, lane, slot)) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) turn(pos, f[e], cs[e], sn[e]);
+    // The whole wave stays for the exchanges.
+    for (; __any(h < heads); h += parts * HPW) {
+        In cur = x;
+        load(h + parts * HPW, x);
+        const bool real = h < heads, is_q = h < p.nh, rot = h < p.nh + p.nkv;
+        if (__any(rot)) {
+            float ss = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) ss = ss + (cur.a[e] * cur.a[e] + cur.b[e] * cur.b[e]);
+            ss = xor_sum<LPH / 2>(ss);
+            const float rs = rsqrtf(ss * (1.0f / HD) + p.eps);
+            const bool norm = is_q ? p.qw != nullptr : p.kw != nullptr;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float a = cur.a[e], b = cur.b[e];
+                if (norm) {
+                    a = a * rs * (is_q ? qw[e] : kw[e]);
+                    b = b * rs * (is_q ? qw[4 + e] : kw[4 + e]);
+                }
+                if (rot) {
+                    cur.a[e] = a * cs[e] - b * sn[e];
+                    cur.b[e] = b * cs[e] + a * sn[e];
+                }
+            }
+        }
+        if (is_q || (!APPEND && real)) {
+            E* dst = (is_q ? (E*)p.qo + r * p.qos + (uint64_t)h * HD : (E*)p.ko + r * p.kos + (uint64_t)(h - p.nh) * HD) + 4 * li;
+            T::put4(dst, cur.a);
+            T::put4(dst + HALF, cur.b);
+        }
+        if constexpr (APPEND) {
+            if (!__any(!is_q)) continue;
+            float mx = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fmaxf(fabsf(cur.a[e]), fabsf(cur.b[e])));
+            mx = xor_max<LPH / 2>(mx);
+            if (real && !is_q && slot != NO_SLOT) {
+                const uint32_t kvh = h - p.nh - (rot ? 0 : p.nkv);
+                const float scale = code_scale(mx, rot ? p.kclip : p.vclip, kvh);
+                uint32_t wa = 0, wb = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    wa |= (uint32_t)kv8_code(cur.a[e], scale) << (8 * e);
+                    wb |= (uint32_t)kv8_code(cur.b[e], scale) << (8 * e);
+                }
+                uint32_t* pool = (rot ? p.kv.pool[0] : p.kv.pool[1]) + (p.kv.row(slot) + (uint64_t)kvh * HD) / 4 + li;
+                pool[0] = wa;
+                pool[HALF / 4] = wb;
+                if (li == 0) (rot ? p.kv.scales[0] : p.kv.scales[1])[(uint64_t)slot * p.nkv + kvh] = scale;
+            }
+        }
+    }
+}
+
+template <class T, int HD, bool APPEND>
+hipError_t go_whole(hipStream_t s, const RopeRowsArgs& a) {
+    const uint32_t heads = a.nh + a.nkv * (APPEND ? 2 : 1), groups = (heads + 512 / HD - 1) / (512 / HD);
+    // Waves for the whole chip first, then rows whose angles are computed once.
+    const uint32_t parts = std::min<uint32_t>(groups, std::max<uint32_t>(1, 4096 / a.rows));
+    const uint64_t waves = (uint64_t)a.rows * parts;
+    qk_norm_rope_kernel<T, HD, APPEND><<<(unsigned)((waves + 3) / 4), 256, 0, s>>>(a, parts);
+    return hipGetLastError();
+}
+
 template <class T, bool APPEND>
 hipError_t go(hipStream_t s, const RopeRowsArgs& a) {
     const uint32_t heads = a.nh + a.nkv * (APPEND ? 2 : 1);
+    const size_t es = 4 * sizeof(typename T::elem);
+    const bool whole = a.rot == a.hd && aligned_to(a.q, es) && aligned_to(a.k, es) && aligned_to(a.qo, es) &&
+                       (a.qs | a.ks | a.qos) % 4 == 0 &&
+                       (APPEND ? aligned_to(a.v, es) && a.vs % 4 == 0 : aligned_to(a.ko, es) && a.kos % 4 == 0);
+    if (whole && a.hd == 64) return go_whole<T, 64, APPEND>(s, a);
+    if (whole && a.hd == 128) return go_whole<T, 128, APPEND>(s, a);
+    if (whole && a.hd == 256) return go_whole<T, 256, APPEND>(s, a);
     qk_norm_rope_any_kernel<T, APPEND><<<a.rows * heads, 64, 0, s>>>(a);
     return hipGetLastError();
 }

@@ -255,6 +255,30 @@ def moe_linear_gated_i8(xq, wq, sx, sw, gate, e_idx, out=None):
     return out
 
 
+# ---------------------------------------------------------------- the int8 paged cache
+# These calls take a few microseconds on the device in a decode step, so their
+# checks are kept short: _here looks at a tensor once.
+
+_current = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _here(dev, *ts):
+    """Every tensor (or None) contiguous and on device `dev`."""
+    for t in ts:
+        if t is not None and (t.get_device() != dev or not t.is_contiguous()):
+            raise ValueError(f"brain_amd.ops: tensors must be contiguous and on one GPU (device {dev}, got "
+                             f"{tuple(t.shape)} on {t.get_device()}, strides {t.stride()})")
+
+
+def _stream_of(dev):
+    # The launches go to the current device.
+    if dev < 0:
+        raise ValueError("brain_amd.ops: tensors must live on the GPU")
+    if dev != _current():
+        raise ValueError(f"brain_amd.ops: the tensors are on GPU {dev}, the current device is {_current()}")
+    return _stream()
+
+
 class PagedKV8:
     """An int8 paged KV cache (bh_kv8): pools of int32 words (4 codes each,
     n_kv * head_dim bytes a slot) and f32 scales [slots, n_kv] for keys and
@@ -263,7 +287,6 @@ class PagedKV8:
     the tensors; make it once for a cache."""
 
     def __init__(self, k_pool, v_pool, k_scales, v_scales, block_tables, block_size, head_dim):
-        _dev(k_pool, v_pool, k_scales, v_scales, block_tables)
         if head_dim <= 0 or head_dim % 4 or head_dim > 256:
             raise ValueError(f"PagedKV8: head_dim {head_dim}, a multiple of 4 up to 256")
         if block_size <= 0:
@@ -271,90 +294,83 @@ class PagedKV8:
         if k_scales.dim() != 2 or block_tables.dim() != 2:
             raise ValueError("PagedKV8: scales [slots, n_kv] and block_tables [batch, max_blocks] expected")
         slots, n_kv = k_scales.shape
-        for name, t, dtype, numel in (("k_pool", k_pool, torch.int32, slots * n_kv * head_dim // 4),
-                                      ("v_pool", v_pool, torch.int32, slots * n_kv * head_dim // 4),
+        words = slots * n_kv * head_dim // 4
+        for name, t, dtype, numel in (("k_pool", k_pool, torch.int32, words), ("v_pool", v_pool, torch.int32, words),
                                       ("k_scales", k_scales, torch.float32, slots * n_kv),
                                       ("v_scales", v_scales, torch.float32, slots * n_kv),
                                       ("block_tables", block_tables, torch.int32, 0)):
             _need(t, dtype, numel, name)
-            if t.device != k_pool.device:
-                raise ValueError(f"PagedKV8: {name} is on {t.device}, k_pool on {k_pool.device}")
+        self.dev = k_pool.get_device()
+        _here(self.dev, k_pool, v_pool, k_scales, v_scales, block_tables)
         self.k_pool, self.v_pool, self.k_scales, self.v_scales = k_pool, v_pool, k_scales, v_scales
         self.block_tables, self.block_size, self.head_dim, self.n_kv = block_tables, block_size, head_dim, n_kv
-        self.device = k_pool.device
-        self.desc = Kv8T(_ptr(k_pool), _ptr(v_pool), _ptr(k_scales), _ptr(v_scales), slots * n_kv * head_dim // 4,
-                         slots * n_kv, _ptr(block_tables), block_tables.shape[1], block_size, n_kv, head_dim)
+        self.desc = Kv8T(_ptr(k_pool), _ptr(v_pool), _ptr(k_scales), _ptr(v_scales), words, slots * n_kv,
+                         _ptr(block_tables), block_tables.shape[1], block_size, n_kv, head_dim)
+        self.ref = C.byref(self.desc)
+        self.sequences = block_tables.shape[0]
+        self.needs = {}  # workspace bytes of paged_attention_i8, by the sizes of the call
 
 
 def _heads(t, dtype, hd, name):
-    """Row stride (elements) of [rows, heads, hd] `t`, whose heads lie side by side."""
+    """(rows, heads, row stride in elements) of [rows, heads, hd] `t`, whose heads lie side by side."""
     if t.dtype != dtype:
         raise ValueError(f"{name}: dtype {t.dtype}, expected {dtype}")
-    if not t.is_cuda:
-        raise ValueError("brain_amd.ops: tensors must live on the GPU")
-    if t.dim() != 3 or t.shape[2] != hd:
-        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected [rows, heads, {hd}]")
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != hd:
+        raise ValueError(f"{name}: shape {tuple(shape)}, expected [rows, heads, {hd}]")
+    rows, heads, _ = shape
     rs, hs, es = t.stride()
-    rows, heads = t.shape[0], t.shape[1]
-    if (hd > 1 and es != 1) or (heads > 1 and hs != hd) or (rows > 1 and rs < heads * hd):
+    if es != 1 or (heads > 1 and hs != hd) or (rows > 1 and rs < heads * hd):
         raise ValueError(f"{name}: strides {t.stride()}; the heads of a row must lie side by side")
-    return rs if rows > 1 else heads * hd
-
-
-def _same_device(device, **ts):
-    # The launches go to the current device's current stream.
-    if device.index is not None and device.index != torch.cuda.current_device():
-        raise ValueError(f"brain_amd.ops: the tensors are on {device}, the current device is "
-                         f"{torch.cuda.current_device()}")
-    for name, t in ts.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, expected {device}")
+    return rows, heads, rs if rows > 1 else heads * hd
 
 
 def _kv_batch(cache, rows, seq_lens, row_start, max_rows, max_len):
     batch = seq_lens.numel()
-    _dev(seq_lens, row_start)
     _need(seq_lens, torch.int32, batch, "seq_lens")
-    if batch > cache.block_tables.shape[0]:
-        raise ValueError(f"seq_lens: {batch} sequences, block_tables has {cache.block_tables.shape[0]}")
+    if batch > cache.sequences:
+        raise ValueError(f"seq_lens: {batch} sequences, block_tables has {cache.sequences}")
     if row_start is None:
         if rows != batch:
             raise ValueError(f"row_start: {rows} rows of {batch} sequences need one")
-    else:
-        _need(row_start, torch.int32, batch + 1, "row_start")
-        if row_start.numel() != batch + 1:
-            raise ValueError(f"row_start: {row_start.numel()} entries for {batch} sequences")
-    return Kv8BatchT(_ptr(row_start), _ptr(seq_lens), batch, rows, max_rows or 0, max_len or 0)
+    elif row_start.dtype != torch.int32 or row_start.numel() != batch + 1:
+        raise ValueError(f"row_start: {row_start.numel()} entries of {row_start.dtype} for {batch} sequences")
+    return Kv8BatchT(_ptr(row_start), seq_lens.data_ptr(), batch, rows, max_rows or 0, max_len or 0)
 
 
 _ACT = {torch.float32: BH_OUT_F32, torch.bfloat16: BH_OUT_BF16}
 
 
-def _qk_rows(q, k, v, positions, inv_freq, q_weight, k_weight, eps):
-    if q.dtype not in _ACT:
-        raise ValueError(f"q: dtype {q.dtype}, expected float32 or bfloat16")
-    if q.dim() != 3 or k.dim() != 3:
-        raise ValueError("q, k: [rows, heads, head_dim] expected")
-    rows, nh, hd = q.shape
-    nkv = k.shape[1]
-    strides = [_heads(q, q.dtype, hd, "q"), _heads(k, q.dtype, hd, "k"), 0]
-    if k.shape[0] != rows:
-        raise ValueError(f"k: {k.shape[0]} rows, q has {rows}")
+def _qk_rows(dev, q, k, v, positions, inv_freq, q_weight, k_weight, eps):
+    dtype = q.dtype
+    if dtype not in _ACT:
+        raise ValueError(f"q: dtype {dtype}, expected float32 or bfloat16")
+    hd = q.shape[-1]
+    rows, nh, qs = _heads(q, dtype, hd, "q")
+    k_rows, nkv, ks = _heads(k, dtype, hd, "k")
+    if k_rows != rows:
+        raise ValueError(f"k: {k_rows} rows, q has {rows}")
+    vs = 0
     if v is not None:
-        strides[2] = _heads(v, q.dtype, hd, "v")
+        vs = _heads(v, dtype, hd, "v")[2]
         if v.shape != k.shape:
             raise ValueError(f"v: shape {tuple(v.shape)}, k has {tuple(k.shape)}")
-    _dev(positions, inv_freq, q_weight, k_weight)
+        if v.get_device() != dev:
+            raise ValueError(f"v is on {v.get_device()}, q on {dev}")
+    if k.get_device() != dev:
+        raise ValueError(f"k is on {k.get_device()}, q on {dev}")
     _need(positions, torch.int32, rows, "positions")
+    pairs = inv_freq.numel()
     _need(inv_freq, torch.float64, 0, "inv_freq")
-    if 2 * inv_freq.numel() > hd:
-        raise ValueError(f"inv_freq: {inv_freq.numel()} pairs, head_dim {hd}")
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None:
-            _need(w, torch.float32, hd, name)
-    _same_device(q.device, k=k, v=v, positions=positions, inv_freq=inv_freq, q_weight=q_weight, k_weight=k_weight)
-    return QkRowsT(q.data_ptr(), k.data_ptr(), _ptr(v), *strides, _ACT[q.dtype], rows, nh, nkv, hd, _ptr(positions),
-                   _ptr(inv_freq), 2 * inv_freq.numel(), _ptr(q_weight), _ptr(k_weight), eps)
+    if 2 * pairs > hd:
+        raise ValueError(f"inv_freq: {pairs} pairs, head_dim {hd}")
+    if q_weight is not None:
+        _need(q_weight, torch.float32, hd, "q_weight")
+    if k_weight is not None:
+        _need(k_weight, torch.float32, hd, "k_weight")
+    _here(dev, positions, inv_freq, q_weight, k_weight)
+    return QkRowsT(q.data_ptr(), k.data_ptr(), _ptr(v), qs, ks, vs, _ACT[dtype], rows, nh, nkv, hd, positions.data_ptr(),
+                   inv_freq.data_ptr(), 2 * pairs, _ptr(q_weight), _ptr(k_weight), eps)
 
 
 def rope_frequencies(rotary_dim, theta, device="cuda"):
@@ -362,13 +378,13 @@ def rope_frequencies(rotary_dim, theta, device="cuda"):
     return theta ** (-torch.arange(0, rotary_dim, 2, device=device, dtype=torch.float64) / rotary_dim)
 
 
-def _out_like(out, t, name):
+def _out_like(dev, out, t, name):
     if out is None:
-        return torch.empty(t.shape, device=t.device, dtype=t.dtype), t.shape[1] * t.shape[2]
-    stride = _heads(out, t.dtype, t.shape[2], name)
-    if out.shape != t.shape:
-        raise ValueError(f"{name}: shape {tuple(out.shape)}, expected {tuple(t.shape)}")
-    _same_device(t.device, **{name: out})
+        out = torch.empty_like(t, memory_format=torch.contiguous_format)
+        return out, out.stride(0)
+    stride = _heads(out, t.dtype, t.shape[2], name)[2]
+    if out.shape != t.shape or out.get_device() != dev:
+        raise ValueError(f"{name}: shape {tuple(out.shape)} on {out.get_device()}, expected {tuple(t.shape)} on {dev}")
     return out, stride
 
 
@@ -378,10 +394,11 @@ def qk_norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e
     projection included: pair (i, i + rotary_dim/2) is turned by
     positions[row] * inv_freq[i], rotary_dim = 2 * inv_freq.numel(). Returns
     (q_out, k_out), which may be q and k themselves."""
-    rows = _qk_rows(q, k, None, positions, inv_freq, q_weight, k_weight, eps)
-    q_out, qs = _out_like(q_out, q, "q_out")
-    k_out, ks = _out_like(k_out, k, "k_out")
-    check(load().bh_qk_norm_rope(_stream(), C.byref(rows), q_out.data_ptr(), qs, k_out.data_ptr(), ks))
+    dev = q.get_device()
+    rows = _qk_rows(dev, q, k, None, positions, inv_freq, q_weight, k_weight, eps)
+    q_out, qs = _out_like(dev, q_out, q, "q_out")
+    k_out, ks = _out_like(dev, k_out, k, "k_out")
+    check(load().bh_qk_norm_rope(_stream_of(dev), C.byref(rows), q_out.data_ptr(), qs, k_out.data_ptr(), ks))
     return q_out, k_out
 
 
@@ -391,17 +408,20 @@ def qk_norm_rope_append_i8(q, k, v, positions, inv_freq, cache, seq_lens, row_st
     cache (PagedKV8): the rows row_start[b] .. row_start[b + 1] become the last
     positions of sequence b's seq_lens[b] (row_start None: one row each).
     Returns q_out."""
-    rows = _qk_rows(q, k, v, positions, inv_freq, q_weight, k_weight, eps)
-    if (k.shape[1], k.shape[2]) != (cache.n_kv, cache.head_dim):
+    dev = cache.dev
+    rows = _qk_rows(dev, q, k, v, positions, inv_freq, q_weight, k_weight, eps)
+    if rows.n_kv_heads != cache.n_kv or rows.head_dim != cache.head_dim:
         raise ValueError(f"k: heads {tuple(k.shape[1:])}, the cache has {(cache.n_kv, cache.head_dim)}")
-    batch = _kv_batch(cache, q.shape[0], seq_lens, row_start, 0, 0)
-    _dev(k_clip, v_clip)
-    for name, t in (("k_clip", k_clip), ("v_clip", v_clip)):
-        if t is not None:
-            _need(t, torch.float32, cache.n_kv, name)
-    _same_device(q.device, cache=cache, seq_lens=seq_lens, row_start=row_start, k_clip=k_clip, v_clip=v_clip)
-    q_out, qs = _out_like(q_out, q, "q_out")
-    check(load().bh_qk_norm_rope_append_i8(_stream(), C.byref(rows), C.byref(cache.desc), C.byref(batch), _ptr(k_clip),
+    if q.get_device() != dev:
+        raise ValueError(f"q is on {q.get_device()}, the cache on {dev}")
+    batch = _kv_batch(cache, rows.rows, seq_lens, row_start, 0, 0)
+    if k_clip is not None:
+        _need(k_clip, torch.float32, cache.n_kv, "k_clip")
+    if v_clip is not None:
+        _need(v_clip, torch.float32, cache.n_kv, "v_clip")
+    _here(dev, seq_lens, row_start, k_clip, v_clip)
+    q_out, qs = _out_like(dev, q_out, q, "q_out")
+    check(load().bh_qk_norm_rope_append_i8(_stream_of(dev), C.byref(rows), cache.ref, C.byref(batch), _ptr(k_clip),
                                            _ptr(v_clip), q_out.data_ptr(), qs))
     return q_out
 
@@ -409,12 +429,13 @@ def qk_norm_rope_append_i8(q, k, v, positions, inv_freq, cache, seq_lens, row_st
 def _queries(q, cache, seq_lens, row_start, max_rows, max_len):
     if q.dtype not in _ACT:
         raise ValueError(f"q: dtype {q.dtype}, expected float32 or bfloat16")
-    stride = _heads(q, q.dtype, cache.head_dim, "q")
-    if q.shape[1] == 0 or q.shape[1] % cache.n_kv:
-        raise ValueError(f"q: {q.shape[1]} heads over {cache.n_kv} kv heads")
-    batch = _kv_batch(cache, q.shape[0], seq_lens, row_start, max_rows, max_len)
-    _same_device(q.device, cache=cache, seq_lens=seq_lens, row_start=row_start)
-    return stride, batch
+    rows, nh, stride = _heads(q, q.dtype, cache.head_dim, "q")
+    if nh == 0 or nh % cache.n_kv:
+        raise ValueError(f"q: {nh} heads over {cache.n_kv} kv heads")
+    if q.get_device() != cache.dev:
+        raise ValueError(f"q is on {q.get_device()}, the cache on {cache.dev}")
+    batch = _kv_batch(cache, rows, seq_lens, row_start, max_rows, max_len)
+    return rows, nh, stride, batch
 
 
 def paged_attention_i8(q, cache, seq_lens, row_start=None, scale=None, max_rows=None, max_len=None, out=None, lse=None):
@@ -425,22 +446,30 @@ def paged_attention_i8(q, cache, seq_lens, row_start=None, scale=None, max_rows=
     length where the program knows them, choose how the work is split. Returns
     (out like q, lse [rows, n_heads] f32); a row without keys has zeros and
     -inf; rows behind the last sequence stay as `out` and `lse` have them."""
-    stride, batch = _queries(q, cache, seq_lens, row_start, max_rows, max_len)
-    rows, nh, hd = q.shape
+    rows, nh, stride, batch = _queries(q, cache, seq_lens, row_start, max_rows, max_len)
+    hd, device, dtype = cache.head_dim, q.device, q.dtype
     if out is None:
-        out = torch.empty(rows, nh, hd, device=q.device, dtype=q.dtype)
+        out = q.new_empty((rows, nh, hd))
+    else:
+        _need(out, dtype, rows * nh * hd, "out")
     if lse is None:
-        lse = torch.empty(rows, nh, device=q.device, dtype=torch.float32)
-    _dev(out, lse)
-    _need(out, q.dtype, rows * nh * hd, "out")
-    _need(lse, torch.float32, rows * nh, "lse")
-    _same_device(q.device, out=out, lse=lse)
-    lib, need = load(), C.c_uint64()
-    check(lib.bh_paged_attention_i8_workspace(C.byref(cache.desc), C.byref(batch), nh, C.byref(need)))
-    ws = torch.empty(need.value, device=q.device, dtype=torch.uint8) if need.value else None
-    check(lib.bh_paged_attention_i8(_stream(), q.data_ptr(), stride, _ACT[q.dtype], nh, C.byref(cache.desc),
-                                    C.byref(batch), hd ** -0.5 if scale is None else scale, out.data_ptr(),
-                                    lse.data_ptr(), _ptr(ws), need.value))
+        lse = torch.empty((rows, nh), device=device, dtype=torch.float32)
+    else:
+        _need(lse, torch.float32, rows * nh, "lse")
+    _here(cache.dev, seq_lens, row_start, out, lse)
+    lib, ref = load(), C.byref(batch)
+    sizes = (nh, rows, batch.batch, batch.max_rows, batch.max_len, row_start is None)
+    need = cache.needs.get(sizes)
+    if need is None:
+        n = C.c_uint64()
+        check(lib.bh_paged_attention_i8_workspace(cache.ref, ref, nh, C.byref(n)))
+        if len(cache.needs) > 4096:
+            cache.needs.clear()
+        need = cache.needs[sizes] = n.value
+    ws = torch.empty(need, device=device, dtype=torch.uint8) if need else None
+    check(lib.bh_paged_attention_i8(_stream_of(cache.dev), q.data_ptr(), stride, _ACT[dtype], nh, cache.ref, ref,
+                                    hd ** -0.5 if scale is None else scale, out.data_ptr(), lse.data_ptr(), _ptr(ws),
+                                    need))
     return out, lse
 
 
@@ -449,17 +478,15 @@ def paged_weight_sums_i8(q, lse, cache, seq_lens, acc, row_start=None, scale=Non
     q gave each cached key in paged_attention_i8 (same arguments, its lse),
     summed over rows and a kv head's query heads; the chunk's own keys start
     from 0. Returns acc."""
-    stride, batch = _queries(q, cache, seq_lens, row_start, max_rows, max_len)
-    rows, nh, hd = q.shape
-    _dev(lse, acc)
+    rows, nh, stride, batch = _queries(q, cache, seq_lens, row_start, max_rows, max_len)
     _need(lse, torch.float32, rows * nh, "lse")
-    if acc.dim() != 3 or acc.shape[0] < seq_lens.numel() or acc.shape[1] != cache.n_kv:
-        raise ValueError(f"acc: shape {tuple(acc.shape)}, expected [{seq_lens.numel()}, {cache.n_kv}, cap]")
+    if acc.dim() != 3 or acc.shape[0] < batch.batch or acc.shape[1] != cache.n_kv:
+        raise ValueError(f"acc: shape {tuple(acc.shape)}, expected [{batch.batch}, {cache.n_kv}, cap]")
     _need(acc, torch.float32, 0, "acc")
-    _same_device(q.device, lse=lse, acc=acc)
-    check(load().bh_paged_weight_sums_i8(_stream(), q.data_ptr(), stride, _ACT[q.dtype], nh, _ptr(lse),
-                                         C.byref(cache.desc), C.byref(batch), hd ** -0.5 if scale is None else scale,
-                                         _ptr(acc), acc.shape[2]))
+    _here(cache.dev, seq_lens, row_start, lse, acc)
+    check(load().bh_paged_weight_sums_i8(_stream_of(cache.dev), q.data_ptr(), stride, _ACT[q.dtype], nh, lse.data_ptr(),
+                                         cache.ref, C.byref(batch), cache.head_dim ** -0.5 if scale is None else scale,
+                                         acc.data_ptr(), acc.shape[2]))
     return acc
 
 
@@ -473,31 +500,35 @@ def paged_kv_evict_i8(cache, seq_lens, acc, budget, sink=0, recent=0, out_tables
     (it may be acc). Returns (keep [batch, n_kv, budget] int32, -1 behind the
     last one, new_lens [batch])."""
     batch = seq_lens.numel()
-    _dev(seq_lens, acc, out_tables, acc_out, keep, new_lens)
     _need(seq_lens, torch.int32, batch, "seq_lens")
     _need(acc, torch.float32, 0, "acc")
-    if batch > cache.block_tables.shape[0]:
-        raise ValueError(f"seq_lens: {batch} sequences, block_tables has {cache.block_tables.shape[0]}")
+    if batch > cache.sequences:
+        raise ValueError(f"seq_lens: {batch} sequences, block_tables has {cache.sequences}")
     if acc.dim() != 3 or acc.shape[0] < batch or acc.shape[1] != cache.n_kv:
         raise ValueError(f"acc: shape {tuple(acc.shape)}, expected [{batch}, {cache.n_kv}, cap]")
     if budget <= 0 or sink < 0 or recent < 0 or sink + recent > budget:
         raise ValueError(f"budget {budget} with sink {sink} and recent {recent}")
+    to_ptr = to_cols = out_ptr = out_cap = 0
     if out_tables is not None:
         _need(out_tables, torch.int32, 0, "out_tables")
         if out_tables.dim() != 2 or out_tables.shape[0] < batch:
             raise ValueError(f"out_tables: shape {tuple(out_tables.shape)}, expected [{batch}, blocks]")
+        to_ptr, to_cols = out_tables.data_ptr(), out_tables.shape[1]
     if acc_out is not None:
         _need(acc_out, torch.float32, 0, "acc_out")
         if acc_out.dim() != 3 or acc_out.shape[0] < batch or acc_out.shape[1] != cache.n_kv:
             raise ValueError(f"acc_out: shape {tuple(acc_out.shape)}, expected [{batch}, {cache.n_kv}, >= {budget}]")
-    keep = torch.empty(batch, cache.n_kv, budget, device=acc.device, dtype=torch.int32) if keep is None else keep
-    new_lens = torch.empty(batch, device=acc.device, dtype=torch.int32) if new_lens is None else new_lens
-    _need(keep, torch.int32, batch * cache.n_kv * budget, "keep")
-    _need(new_lens, torch.int32, batch, "new_lens")
-    _same_device(cache.device, seq_lens=seq_lens, acc=acc, out_tables=out_tables, acc_out=acc_out, keep=keep,
-                 new_lens=new_lens)
-    check(load().bh_paged_kv_evict_i8(_stream(), C.byref(cache.desc), _ptr(seq_lens), batch, _ptr(acc), acc.shape[2],
-                                      budget, sink, recent, _ptr(out_tables),
-                                      out_tables.shape[1] if out_tables is not None else 0, _ptr(acc_out),
-                                      acc_out.shape[2] if acc_out is not None else 0, _ptr(keep), _ptr(new_lens)))
+        out_ptr, out_cap = acc_out.data_ptr(), acc_out.shape[2]
+    if keep is None:
+        keep = torch.empty((batch, cache.n_kv, budget), device=acc.device, dtype=torch.int32)
+    else:
+        _need(keep, torch.int32, batch * cache.n_kv * budget, "keep")
+    if new_lens is None:
+        new_lens = torch.empty(batch, device=acc.device, dtype=torch.int32)
+    else:
+        _need(new_lens, torch.int32, batch, "new_lens")
+    _here(cache.dev, seq_lens, acc, out_tables, acc_out, keep, new_lens)
+    check(load().bh_paged_kv_evict_i8(_stream_of(cache.dev), cache.ref, seq_lens.data_ptr(), batch, acc.data_ptr(),
+                                      acc.shape[2], budget, sink, recent, to_ptr, to_cols, out_ptr, out_cap,
+                                      keep.data_ptr(), new_lens.data_ptr()))
     return keep, new_lens

@@ -409,7 +409,7 @@ def test_weight_sums_unseen_blocks(gpu):
 
 EVICT = [([50, 7, 0, 31], 20, 2, 5, 8, 64, 16), ([300], 299, 0, 0, 1, 128, 32), ([300, 100], 1, 0, 0, 3, 36, 7), ([64, 65], 64, 64, 0, 2, 64, 8),
          ([2000, 3000], 700, 4, 100, 2, 128, 16), ([5000], 4999, 4000, 999, 1, 4, 64), ([40, 41], 40, 0, 40, 2, 256, 1),
-         ([9000], 3000, 0, 1, 1, 64, 24)]
+         ([9000], 3000, 0, 1, 1, 64, 24), ([17000, 20], 5000, 3, 50, 1, 64, 16)]
 
 
 @pytest.mark.parametrize("in_place", [True, False], ids=["in_place", "copied"])

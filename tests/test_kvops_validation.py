@@ -139,10 +139,13 @@ def test_evict():
 
 
 class Fake:
-    """A CPU tensor that says it is on the GPU; whoever asks for its memory launches."""
+    """A CPU tensor that says it is on GPU 0; whoever asks for its memory launches."""
 
     def __init__(self, t, ptr=None):
-        self.t, self.ptr, self.is_cuda = t, ptr, True
+        self.t, self.ptr = t, ptr
+
+    def get_device(self):
+        return 0
 
     def __getattr__(self, name):
         return getattr(self.t, name)
@@ -178,7 +181,7 @@ def test_ops_cache(change, word):
 
 def test_ops_attention():
     c = cache()
-    ok = dict(q=f(3, 4, 64), cache=c, seq_lens=i(2, ptr=P), row_start=i(3, ptr=P))
+    ok = dict(q=f(3, 4, 64), cache=c, seq_lens=i(2, ptr=P), row_start=i(3, ptr=P), out=f(3, 4, 64), lse=f(3, 4))
 
     def no(word, **change):
         with pytest.raises(ValueError, match=word):
@@ -196,6 +199,9 @@ def test_ops_attention():
     no("out: dtype", out=f(3, 4, 64, dtype=torch.bfloat16), lse=f(3, 4))
     no("out: 700", out=f(700), lse=f(3, 4))
     no("lse: 11", out=f(3, 4, 64), lse=f(11))
+    no("one GPU", lse=torch.zeros(3, 4))
+    no("one GPU", row_start=Fake(torch.zeros(6, dtype=torch.int32)[::2], ptr=P))
+    no("q is on -1", q=torch.zeros(3, 4, 64))
     with pytest.raises(ValueError, match="acc"):
         ops.paged_weight_sums_i8(ok["q"], f(3, 4), c, ok["seq_lens"], f(2, 3, 9), ok["row_start"])
     with pytest.raises(ValueError, match="acc"):
