@@ -1,5 +1,7 @@
 // Attention of a ragged batch's new rows over the int8 paged KV cache, and the
 // weight that each cached key receives from it.
+#include <type_traits>
+
 #include "bh_kvops.h"
 
 namespace bh {
@@ -243,7 +245,7 @@ __global__ __launch_bounds__(SW * 64, (stream_waves<T, HD, NQ>())) void paged_at
     const uint32_t split = unit % p.nsplit;
     Block bl;
     if (!find_block<VB>(p.bt, p.group, unit / p.nsplit, lane, bl)) return;
-    const uint32_t reach = (uint32_t)min((uint64_t)p.kv.max_bt * p.kv.bs, (uint64_t)0x7fffffffu);
+    const uint32_t reach = (uint32_t)min((uint64_t)p.kv.max_bt * p.kv.bs, (uint64_t)0x7fff0000u);
     const uint32_t vend = min(bl.v0 + VB, bl.nv);
     const uint32_t kend = min(keys_seen(bl, (vend - 1) / p.group), reach);  // keys that any of the vectors sees
     const uint32_t kall = min(keys_seen(bl, bl.v0 / p.group), reach);       // ... that all see
@@ -507,8 +509,8 @@ __global__ __launch_bounds__(SW * 64, (stream_waves<T, HD, NQ>())) void paged_at
 
 // ---------------------------------------------------------------- many rows
 //
-// Four waves of QW query vectors each walk the keys 64 at a time, through LDS:
-// codes go global -> registers -> bf16 -> LDS once for the four, one tile in LDS
+// NW waves of 32 query vectors each walk the keys 64 at a time, through LDS:
+// codes go global -> registers -> bf16 -> LDS once for all, one tile in LDS
 // and one in registers ahead of the products, with one barrier a tile.
 // v_mfma_f32_32x32x16_bf16 on scores transposed (keys x queries), so that a lane
 // has 16 keys of one query, which are the operand of the second product for the
@@ -527,15 +529,14 @@ __device__ __forceinline__ v16f mfma32(v4i a, v4i b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
 }
 
-template <class T, int HD, int QW>
-__global__ __launch_bounds__(256, (QW == 64 ? 1 : 2)) void paged_attention_tile_kernel(AttnArgs p) {
+template <class T, int HD, int NW>
+__global__ __launch_bounds__(NW * 64, 2) void paged_attention_tile_kernel(AttnArgs p) {
     typedef typename T::elem E;
-    constexpr int PARTS = sizeof(E) == 4 ? 3 : 1, NB = QW / 32, VB = 4 * QW, KB = TK * HD * 2;
+    constexpr int PARTS = sizeof(E) == 4 ? 3 : 1, NT = NW * 64, VB = 32 * NW, KB = TK * HD * 2;
     __shared__ __attribute__((aligned(1024))) uint8_t kt[2][KB], vt[2][KB];
-    __shared__ __attribute__((aligned(16))) float kcs[2][TK], vss[2][TK];
+    __shared__ __attribute__((aligned(16))) float scs[2][2][TK];  // [buffer][keys', values'] scales
     __shared__ __attribute__((aligned(16))) uint32_t ring[4][TK];
-    __shared__ unsigned long long okm[4];
-    __shared__ float kmx[2];
+    __shared__ float kmx[2][2];
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t nkv = p.kv.nkv, kvs = nkv * HD, units = p.blocks * p.nsplit;
@@ -546,66 +547,61 @@ __global__ __launch_bounds__(256, (QW == 64 ? 1 : 2)) void paged_attention_tile_
     const uint32_t split = unit % p.nsplit;
     Block bl;
     if (!find_block<VB>(p.bt, p.group, unit / p.nsplit, lane, bl)) return;
-    const uint32_t reach = (uint32_t)min((uint64_t)p.kv.max_bt * p.kv.bs, (uint64_t)0x7fffffffu);
+    const uint32_t reach = (uint32_t)min((uint64_t)p.kv.max_bt * p.kv.bs, (uint64_t)0x7fff0000u);
     const uint32_t vend = min(bl.v0 + VB, bl.nv);
     const uint32_t kend = min(keys_seen(bl, (vend - 1) / p.group), reach);
     const uint32_t k0 = split * p.span, k1 = split + 1 == p.nsplit ? kend : min(kend, k0 + p.span);
     if (k0 >= k1 && split) return;
     const int nt = k1 > k0 ? (int)((k1 - k0 + TK - 1) / TK) : 0;
 
-    // This wave's vectors, and what its first and last see.
-    const uint32_t wv0 = bl.v0 + QW * wave, wv1 = min(wv0 + QW, vend);
+    // This wave's 32 vectors, and what its first and last see.
+    const uint32_t wv0 = bl.v0 + 32 * wave, wv1 = min(wv0 + 32, vend);
     const bool wlive = wv0 < vend;
     const uint32_t wall = wlive ? min(keys_seen(bl, wv0 / p.group), reach) : 0u;
     const uint32_t wend = wlive ? min(keys_seen(bl, (wv1 - 1) / p.group), reach) : 0u;
-    uint32_t seen[NB];
-    v4i qf[NB][HD / 16][PARTS];  // step t: d = 16 t + 8 half ..+7 of vector 32 n + col
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-        const uint32_t v = min(wv0 + 32 * n + col, vend - 1), i = v / p.group, h = kvh * p.group + v % p.group;
-        seen[n] = wv0 + 32 * n + col < vend ? min(keys_seen(bl, i), reach) : 0u;
+    uint32_t seen;
+    v4i qf[HD / 16][PARTS];  // step t: d = 16 t + 8 half ..+7 of vector col
+    {
+        const uint32_t v = min(wv0 + col, vend - 1), i = v / p.group, h = kvh * p.group + v % p.group;
+        seen = wv0 + col < vend ? min(keys_seen(bl, i), reach) : 0u;
         const E* src = (const E*)p.q + (bl.r0 + i) * p.qs + (uint64_t)h * HD + 8 * half;
 #pragma unroll
         for (int t = 0; t < HD / 16; ++t) {
             float x[8];
             query8<T>(src + 16 * t, p.qvec, x);
-            split8<PARTS>(x, qf[n][t]);
+            split8<PARTS>(x, qf[t]);
         }
     }
-    v16f o[NB][HD / 32];
-    float m[NB], l[NB];
+    v16f o[HD / 32];
+    float m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-        m[n] = -INFINITY, l[n] = 0.0f;
+    for (int j = 0; j < HD / 32; ++j)
 #pragma unroll
-        for (int j = 0; j < HD / 32; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[n][j][e] = 0.0f;
-    }
+        for (int e = 0; e < 16; ++e) o[j][e] = 0.0f;
 
     // ---- staging
     const uint8_t* kp = (const uint8_t*)p.kv.pool[0] + (size_t)kvh * HD;
     const uint8_t* vp = (const uint8_t*)p.kv.pool[1] + (size_t)kvh * HD;
-    const float* sp = (tid < TK ? p.kv.scales[0] : p.kv.scales[1]) + kvh;
+    const float* sp = (wave & 1 ? p.kv.scales[1] : p.kv.scales[0]) + kvh;  // even waves take the keys' scales
     auto barrier = [&]() {  // orders LDS only: loads in flight go on
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
     };
-    // Slots of tile t's keys, by wave 0: a key behind the end or without a slot
-    // gets slot 0 and no bit in okm.
+    // Slots of tile t's keys: every wave looks all of them up, so that each has
+    // the mask of those that exist in scalar registers. A key behind the end or
+    // without a slot gets slot 0.
     auto slot_at = [&](int t) -> uint32_t {
         const uint32_t j = k0 + (uint32_t)t * TK + lane;
-        return t < nt && j < k1 ? p.kv.slot(bl.b, j) : NO_SLOT;
+        return j < k1 ? p.kv.slot(bl.b, j) : NO_SLOT;
     };
-    auto put_slots = [&](int t, uint32_t s) {
+    auto put_slots = [&](int t, uint32_t s) -> unsigned long long {
         ring[t & 3][lane] = s != NO_SLOT ? s : 0u;
-        const unsigned long long ok = __ballot(s != NO_SLOT);
-        if (lane == 0) okm[t & 3] = ok;
+        return __ballot(s != NO_SLOT);
     };
-    constexpr int CPK = HD / 16, KPP = 256 / CPK, NK = TK / KPP;  // 16-byte pieces of a key; keys a pass; passes
+    constexpr int CPK = HD / 16, KPP = NT / CPK, NK = KPP < TK ? TK / KPP : 1;  // 16-byte pieces of a key; keys a pass; passes
     constexpr int DG = HD / 4;
-    const bool vlive = tid < TK / 8 * DG;
+    const bool klive = NT <= TK * CPK || tid < TK * CPK, vlive = NT <= TK / 8 * DG || tid < TK / 8 * DG;
     v4i kr[NK];
     uint32_t vr[8];
     float sr = 0.0f;
@@ -613,16 +609,17 @@ __global__ __launch_bounds__(256, (QW == 64 ? 1 : 2)) void paged_attention_tile_
     const int vkey = 16 * (oct >> 1) + 4 * (oct & 1);  // octet's keys: vkey ..+3, vkey + 8 ..+11
     auto load = [&](int t) {
         const uint32_t* sl = ring[t & 3];
+        if (klive)
 #pragma unroll
-        for (int u = 0; u < NK; ++u)
-            kr[u] = *reinterpret_cast<const v4i*>(kp + (size_t)sl[kkey + KPP * u] * kvs + 16 * kpc);
+            for (int u = 0; u < NK; ++u)
+                kr[u] = *reinterpret_cast<const v4i*>(kp + (size_t)sl[kkey + KPP * u] * kvs + 16 * kpc);
         if (vlive) {
             const uint4 a = *reinterpret_cast<const uint4*>(sl + vkey), b = *reinterpret_cast<const uint4*>(sl + vkey + 8);
             const uint32_t ss[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
             for (int i = 0; i < 8; ++i) vr[i] = *reinterpret_cast<const uint32_t*>(vp + (size_t)ss[i] * kvs + 4 * dg);
         }
-        if (tid < 2 * TK) sr = sp[(size_t)sl[tid & (TK - 1)] * nkv];
+        sr = sp[(size_t)sl[lane] * nkv];
     };
     // LDS images. K: chunk c (8 d) of key r. V^T: 32 keys at a time, lines of 256
     // bytes hold 4 d x 32 keys. In both the 16 lanes that meet go to 16 slots.
@@ -630,14 +627,15 @@ __global__ __launch_bounds__(256, (QW == 64 ? 1 : 2)) void paged_attention_tile_
     auto vchunk = [&](int d, int oc) -> int {
         return (oc >> 2) * (64 * HD) + (d >> 2) * 256 + (((4 * (d & 3) + (oc & 3)) ^ ((d >> 2) & 15)) << 4);
     };
-    auto store = [&](int t) {
+    auto store = [&](int t, unsigned long long ok) __attribute__((always_inline)) {
         const int bu = t & 1;
+        if (klive)
 #pragma unroll
-        for (int u = 0; u < NK; ++u) {
-            const int key = kkey + KPP * u;
-            *reinterpret_cast<v4i*>(kt[bu] + kchunk(key, 2 * kpc)) = codes8((uint32_t)kr[u][0], (uint32_t)kr[u][1]);
-            *reinterpret_cast<v4i*>(kt[bu] + kchunk(key, 2 * kpc + 1)) = codes8((uint32_t)kr[u][2], (uint32_t)kr[u][3]);
-        }
+            for (int u = 0; u < NK; ++u) {
+                const int key = kkey + KPP * u;
+                *reinterpret_cast<v4i*>(kt[bu] + kchunk(key, 2 * kpc)) = codes8((uint32_t)kr[u][0], (uint32_t)kr[u][1]);
+                *reinterpret_cast<v4i*>(kt[bu] + kchunk(key, 2 * kpc + 1)) = codes8((uint32_t)kr[u][2], (uint32_t)kr[u][3]);
+            }
         if (vlive) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -648,197 +646,160 @@ __global__ __launch_bounds__(256, (QW == 64 ? 1 : 2)) void paged_attention_tile_
                     v4i{(int)hi16x2(x[0], x[1]), (int)hi16x2(x[2], x[3]), (int)hi16x2(x[4], x[5]), (int)hi16x2(x[6], x[7])};
             }
         }
-        if (wave < 2) {  // a key without a slot has scales of 0
-            const bool ok = (okm[t & 3] >> lane) & 1ull;
-            if (wave == 0) {
-                const float kc = ok ? sr * p.scale2 : 0.0f;
-                kcs[bu][lane] = kc;
-                const float mx = xor_max<32>(fabsf(kc));
-                if (lane == 0) kmx[bu] = mx;
-            } else {
-                vss[bu][lane] = ok ? sr : 0.0f;
-            }
-        }
+        // A key without a slot has scales of 0. (Waves of a kind write the same.)
+        const float sc = (ok >> lane) & 1ull ? (wave & 1 ? sr : sr * p.scale2) : 0.0f;
+        scs[bu][wave & 1][lane] = sc;
+        kmx[bu][wave & 1] = xor_max<32>(fabsf(sc));
     };
 
-    uint32_t sl_next = NO_SLOT;
-    if (wave == 0) {
-        put_slots(0, slot_at(0));
-        put_slots(1, slot_at(1));
-        put_slots(2, slot_at(2));
-        sl_next = slot_at(3);
-    }
-    barrier();
-    if (nt) {
-        load(0);
-        store(0);
-        load(1);
-    }
-    barrier();
-#pragma unroll 1
-    for (int t = 0; t < nt; ++t) {
-        const int bu = t & 1;
-        store(t + 1);
-        if (t + 2 < nt) load(t + 2);
-        if (wave == 0) {
-            put_slots(t + 3, sl_next);
-            sl_next = slot_at(t + 4);
+    // The products of one tile. HIDE: some of its keys are hidden from some query
+    // (ok: the keys that have a slot).
+    auto attend = [&](auto hide_, int bu, uint32_t j0, unsigned long long ok) __attribute__((always_inline)) {
+        constexpr bool HIDE = decltype(hide_)::value;
+        // Register e of half kh: key 32 kh + 8 (e / 4) + 4 half + e % 4.
+        v16f s[2];
+        // kchunk(32 kh + col, 2 d + half) and vchunk(32 j + col, 4 kh + 2 u + half)
+        // from one address each. (The empty asm keeps the rest of them from being
+        // carried in registers from tile to tile.)
+        int ka = bu * KB + kchunk(col, half), va = bu * KB + vchunk(col, half);
+        asm volatile("" : "+v"(ka), "+v"(va));
+#pragma unroll
+        for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[kh][e] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d) {
+            v4i k[2];
+#pragma unroll
+            for (int kh = 0; kh < 2; ++kh) k[kh] = *reinterpret_cast<const v4i*>(kt[0] + (ka ^ (d << 5)) + kh * (64 * HD));
+#pragma unroll
+            for (int part = PARTS - 1; part >= 0; --part)
+#pragma unroll
+                for (int kh = 0; kh < 2; ++kh) s[kh] = mfma32(k[kh], qf[d][part], s[kh]);
         }
-        const uint32_t j0 = k0 + (uint32_t)t * TK;
-        __builtin_amdgcn_sched_barrier(0);
-        if (j0 < wend) {
-            const float kb = kmx[bu];
-            const unsigned long long ok = okm[t & 3];
-            const bool masked = j0 + TK > wall || ok != ~0ull;
+        const float *kcp = &scs[bu][0][4 * half], *vsp = &scs[bu][1][4 * half];
+        const unsigned long long okl = ok >> (4 * half);
+        const int lim = (int)(seen - j0) - 4 * half;  // (2^31 keys at most)
+        auto hidden = [&](int key) -> bool { return key >= lim || !((okl >> key) & 1ull); };
+        float mx = 0.0f;
 #pragma unroll
-            for (int kh = 0; kh < 2; ++kh) {
-                v16f s[NB];
+        for (int kh = 0; kh < 2; ++kh)
 #pragma unroll
-                for (int n = 0; n < NB; ++n)
+            for (int e = 0; e < 16; e += 2) mx = fmaxf(fmaxf(mx, fabsf(s[kh][e])), fabsf(s[kh][e + 1]));
+        if (__builtin_expect(__any(!(mx * kmx[bu][0] <= m + SLACK)), 0)) {  // the bound may be exceeded: look at the scores themselves
+            mx = -INFINITY;
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) s[n][e] = 0.0f;
+            for (int kh = 0; kh < 2; ++kh)
 #pragma unroll
-                for (int d = 0; d < HD / 16; ++d) {
-                    const v4i k = *reinterpret_cast<const v4i*>(kt[bu] + kchunk(32 * kh + col, 2 * d + half));
-#pragma unroll
-                    for (int n = 0; n < NB; ++n)
-#pragma unroll
-                        for (int part = PARTS - 1; part >= 0; --part) s[n] = mfma32(k, qf[n][d][part], s[n]);
+                for (int e = 0; e < 16; ++e) {
+                    const int key = 32 * kh + 8 * (e >> 2) + (e & 3);
+                    const float a = s[kh][e] * kcp[key];
+                    mx = fmaxf(mx, HIDE && hidden(key) ? -INFINITY : a);
                 }
-                __builtin_amdgcn_sched_barrier(0);
-                // Register e: key 32 kh + 8 (e / 4) + 4 half + e % 4.
-                const float* kcp = &kcs[bu][32 * kh + 4 * half];
-                const float* vsp = &vss[bu][32 * kh + 4 * half];
-                uint32_t hid[NB];  // bit e: a key that this query does not see
-                if (masked) {
-                    const uint32_t okh = (uint32_t)(ok >> (32 * kh));
+            mx = fmaxf(mx, xor_lane<32>(mx));
+            const float mn = mx > m + SLACK ? mx : m;  // each query for itself
+            const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            l = l * alpha;
 #pragma unroll
-                    for (int n = 0; n < NB; ++n) {
-                        hid[n] = 0;
+            for (int j = 0; j < HD / 32; ++j)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const uint32_t key = 8 * (e >> 2) + 4 * half + (e & 3);
-                            if (j0 + 32 * kh + key >= seen[n] || !((okh >> key) & 1u)) hid[n] |= 1u << e;
-                        }
+                for (int e = 0; e < 16; ++e) o[j][e] = o[j][e] * alpha;
+            m = mn;
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                float x[8];
+#pragma unroll
+                for (int i4 = 0; i4 < 2; ++i4) {
+                    const int k0_ = 32 * kh + 16 * u + 8 * i4;
+                    const float4 kc = *reinterpret_cast<const float4*>(kcp + k0_), vs = *reinterpret_cast<const float4*>(vsp + k0_);
+                    const float kk[4] = {kc.x, kc.y, kc.z, kc.w}, vv[4] = {vs.x, vs.y, vs.z, vs.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float a = __builtin_fmaf(s[kh][8 * u + 4 * i4 + i], kk[i], -ref);
+                        if (HIDE && hidden(k0_ + i)) a = -INFINITY;
+                        const float w = __builtin_amdgcn_exp2f(a);
+                        l = l + w;
+                        x[4 * i4 + i] = HIDE && hidden(k0_ + i) ? 0.0f : w * vv[i];  // whatever its scale is
                     }
                 }
-                bool any = false;
+                v4i pf[PARTS];
+                split8<PARTS>(x, pf);
 #pragma unroll
-                for (int n = 0; n < NB; ++n) {
-                    float mx = 0.0f;
+                for (int j = 0; j < HD / 32; ++j) {
+                    const v4i v = *reinterpret_cast<const v4i*>(vt[0] + (va ^ (u << 5) ^ ((j & 1) << 7)) + j * 2048 + kh * (64 * HD));
 #pragma unroll
-                    for (int e = 0; e < 16; e += 2) mx = fmaxf(fmaxf(mx, fabsf(s[n][e])), fabsf(s[n][e + 1]));
-                    any |= !(mx * kb <= m[n] + SLACK);
+                    for (int part = PARTS - 1; part >= 0; --part) o[j] = mfma32(v, pf[part], o[j]);
                 }
-                if (__any(any)) {  // the bound may be exceeded: look at the scores themselves
-#pragma unroll
-                    for (int n = 0; n < NB; ++n) {
-                        float mx = -INFINITY;
-#pragma unroll
-                        for (int e4 = 0; e4 < 4; ++e4) {
-                            const float4 kc = *reinterpret_cast<const float4*>(kcp + 8 * e4);
-                            const float kk[4] = {kc.x, kc.y, kc.z, kc.w};
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const float a = s[n][4 * e4 + i] * kk[i];
-                                mx = fmaxf(mx, masked && ((hid[n] >> (4 * e4 + i)) & 1u) ? -INFINITY : a);
-                            }
-                        }
-                        mx = fmaxf(mx, xor_lane<32>(mx));
-                        const float mn = mx > m[n] + SLACK ? mx : m[n];  // each query for itself
-                        const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[n] - mn);
-                        l[n] = l[n] * alpha;
-#pragma unroll
-                        for (int j = 0; j < HD / 32; ++j)
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) o[n][j][e] = o[n][j][e] * alpha;
-                        m[n] = mn;
-                    }
-                }
-                v4i pf[NB][2][PARTS];
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    float kk[8], vv[8];
-#pragma unroll
-                    for (int e4 = 0; e4 < 2; ++e4) {
-                        const float4 kc = *reinterpret_cast<const float4*>(kcp + 16 * u + 8 * e4);
-                        const float4 vs = *reinterpret_cast<const float4*>(vsp + 16 * u + 8 * e4);
-                        kk[4 * e4] = kc.x, kk[4 * e4 + 1] = kc.y, kk[4 * e4 + 2] = kc.z, kk[4 * e4 + 3] = kc.w;
-                        vv[4 * e4] = vs.x, vv[4 * e4 + 1] = vs.y, vv[4 * e4 + 2] = vs.z, vv[4 * e4 + 3] = vs.w;
-                    }
-#pragma unroll
-                    for (int n = 0; n < NB; ++n) {
-                        const float ref = m[n] == -INFINITY ? 0.0f : m[n];
-                        float x[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) x[i] = __builtin_fmaf(s[n][8 * u + i], kk[i], -ref);
-                        if (masked) {
-#pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                if ((hid[n] >> (8 * u + i)) & 1u) x[i] = -INFINITY;
-                        }
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const float w = __builtin_amdgcn_exp2f(x[i]);
-                            l[n] = l[n] + w;
-                            x[i] = w * vv[i];
-                        }
-                        if (masked) {  // whatever its scale is
-#pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                if ((hid[n] >> (8 * u + i)) & 1u) x[i] = 0.0f;
-                        }
-                        split8<PARTS>(x, pf[n][u]);
-                    }
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int j = 0; j < HD / 32; ++j) {
-                        const v4i v = *reinterpret_cast<const v4i*>(vt[bu] + vchunk(32 * j + col, 4 * kh + 2 * u + half));
-#pragma unroll
-                        for (int n = 0; n < NB; ++n)
-#pragma unroll
-                            for (int part = PARTS - 1; part >= 0; --part) o[n][j] = mfma32(v, pf[n][u][part], o[n][j]);
-                    }
-                __builtin_amdgcn_sched_barrier(0);
             }
+    };
+
+    // Masks of tiles t .. t + 2, and the slot that this lane puts next.
+    unsigned long long ok0 = put_slots(0, slot_at(0)), ok1 = put_slots(1, slot_at(1)), ok2 = put_slots(2, slot_at(2));
+    uint32_t sl_next = slot_at(3);
+    barrier();
+    load(0);
+    store(0, ok0);
+    load(1);
+    barrier();
+    auto stage = [&](int t) __attribute__((always_inline)) {
+        store(t + 1, ok1);
+        load(t + 2);
+        ok0 = ok1, ok1 = ok2, ok2 = put_slots(t + 3, sl_next);
+        sl_next = slot_at(t + 4);
+    };
+    // Tiles that all of this wave's queries see whole go through a loop of their
+    // own, without the comparisons. (Each wave passes one barrier a tile in
+    // whichever loop it is.)
+    for (int t = 0; t < nt;) {
+#pragma unroll 1
+        for (; t < nt; ++t) {
+            const uint32_t j0 = k0 + (uint32_t)t * TK;
+            if (j0 + TK > wall || ok0 != ~0ull) break;
+            stage(t);
+            attend(std::false_type{}, t & 1, j0, ~0ull);
+            barrier();
         }
-        barrier();
-    }
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-        const uint32_t v = wv0 + 32 * n + col;
-        const float ll = l[n] + xor_lane<32>(l[n]);
-        if (v >= vend) continue;
-        if (p.nsplit > 1) {
-            const uint64_t at = ((uint64_t)unit * nkv + kvh) * VB + (v - bl.v0);
-#pragma unroll
-            for (int j = 0; j < HD / 32; ++j)
-#pragma unroll
-                for (int e4 = 0; e4 < 4; ++e4)
-                    *reinterpret_cast<float4*>(p.part + at * HD + 32 * j + 8 * e4 + 4 * half) =
-                        make_float4(o[n][j][4 * e4], o[n][j][4 * e4 + 1], o[n][j][4 * e4 + 2], o[n][j][4 * e4 + 3]);
-            if (half == 0) p.ml[at] = make_float2(m[n], ll);
-        } else {
-            const uint64_t row = (uint64_t)(bl.r0 + v / p.group) * p.nh + kvh * p.group + v % p.group;
-            const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-            E* dst = (E*)p.out + row * HD;
-#pragma unroll
-            for (int j = 0; j < HD / 32; ++j)
-#pragma unroll
-                for (int e4 = 0; e4 < 4; ++e4) {
-                    const float y[4] = {o[n][j][4 * e4] * inv, o[n][j][4 * e4 + 1] * inv, o[n][j][4 * e4 + 2] * inv,
-                                        o[n][j][4 * e4 + 3] * inv};
-                    if (p.ovec) T::put4(dst + 32 * j + 8 * e4 + 4 * half, y);
-                    else
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) T::put(dst + 32 * j + 8 * e4 + 4 * half + i, y[i]);
-                }
-            if (p.lse && half == 0) p.lse[row] = ll == 0.0f ? -INFINITY : (m[n] + log2f(ll)) * LN2;
+        if (t < nt) {
+            const uint32_t j0 = k0 + (uint32_t)t * TK;
+            const unsigned long long ok = ok0;
+            stage(t);
+            if (j0 < wend) attend(std::true_type{}, t & 1, j0, ok);
+            barrier();
+            ++t;
         }
     }
+    const uint32_t v = wv0 + col;
+    l = l + xor_lane<32>(l);
+    if (v >= vend) return;
+    if (p.nsplit > 1) {
+        const uint64_t at = ((uint64_t)unit * nkv + kvh) * VB + (v - bl.v0);
+#pragma unroll
+        for (int j = 0; j < HD / 32; ++j)
+#pragma unroll
+            for (int e4 = 0; e4 < 4; ++e4)
+                *reinterpret_cast<float4*>(p.part + at * HD + 32 * j + 8 * e4 + 4 * half) =
+                    make_float4(o[j][4 * e4], o[j][4 * e4 + 1], o[j][4 * e4 + 2], o[j][4 * e4 + 3]);
+        if (half == 0) p.ml[at] = make_float2(m, l);
+        return;
+    }
+    const uint64_t row = (uint64_t)(bl.r0 + v / p.group) * p.nh + kvh * p.group + v % p.group;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    E* dst = (E*)p.out + row * HD;
+#pragma unroll
+    for (int j = 0; j < HD / 32; ++j)
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4) {
+            const float y[4] = {o[j][4 * e4] * inv, o[j][4 * e4 + 1] * inv, o[j][4 * e4 + 2] * inv, o[j][4 * e4 + 3] * inv};
+            if (p.ovec) T::put4(dst + 32 * j + 8 * e4 + 4 * half, y);
+            else
+#pragma unroll
+                for (int i = 0; i < 4; ++i) T::put(dst + 32 * j + 8 * e4 + 4 * half + i, y[i]);
+        }
+    if (p.lse && half == 0) p.lse[row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
 }
 
 // Joins the splits of a vector: one wave for each vector of a block.
@@ -852,7 +813,7 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(AttnArgs p) {
     if (!find_block<VB>(p.bt, p.group, blk, lane, bl)) return;
     const uint32_t v = bl.v0 + u;
     if (v >= bl.nv) return;
-    const uint32_t reach = (uint32_t)min((uint64_t)p.kv.max_bt * p.kv.bs, (uint64_t)0x7fffffffu);
+    const uint32_t reach = (uint32_t)min((uint64_t)p.kv.max_bt * p.kv.bs, (uint64_t)0x7fff0000u);
     const uint32_t kend = min(keys_seen(bl, (min(bl.v0 + VB, bl.nv) - 1) / p.group), reach);
     const uint32_t live = max(1u, min(p.nsplit, (kend + p.span - 1) / p.span));  // splits that had keys
     const uint64_t at = ((uint64_t)blk * p.nsplit * nkv + kvh) * VB + u, far = (uint64_t)nkv * VB;
@@ -1062,7 +1023,6 @@ Plan plan_attention(const Kv8& kv, const Kv8Rows& bt, const bh_kv8_batch* hint, 
     const uint64_t vectors = (uint64_t)most * group, all = (uint64_t)bt.rows * group;
     r.kind = vectors <= 32 ? STREAM : TILE;
     r.vb = vectors <= 16 ? 16 : vectors <= 32 ? 32 : 128;
-    if (r.kind == TILE && dtype == BH_OUT_BF16 && all * kv.nkv >= 256ull * CUS) r.vb = 256;
     r.blocks = !bt.start && group <= r.vb ? bt.batch : (uint32_t)(all / r.vb) + bt.batch;
     const uint64_t reach = (uint64_t)kv.max_bt * kv.bs;
     const uint64_t len = std::max<uint64_t>(1, hint->max_len ? std::min<uint64_t>(hint->max_len, reach) : reach);
@@ -1092,7 +1052,7 @@ hipError_t go_matrix(hipStream_t s, const AttnArgs& a, bool b16) {
     const uint64_t units = ((uint64_t)a.blocks * a.nsplit + 7) / 8 * 8 * a.kv.nkv;
     const uint64_t joins = (uint64_t)a.blocks * a.kv.nkv * (VB / 4);
     if (units > 0x7fffffffull || joins > 0x7fffffffull) return hipErrorInvalidConfiguration;
-    if constexpr (VB > 32) paged_attention_tile_kernel<T, HD, VB / 4><<<(unsigned)units, 256, 0, s>>>(a);
+    if constexpr (VB > 32) paged_attention_tile_kernel<T, HD, VB / 32><<<(unsigned)units, 2 * VB, 0, s>>>(a);
     else if (b16) paged_attention_stream_kernel<T, HD, VB / 16, true><<<(unsigned)units, SW * 64, 0, s>>>(a);
     else paged_attention_stream_kernel<T, HD, VB / 16, false><<<(unsigned)units, SW * 64, 0, s>>>(a);
     hipError_t e = hipGetLastError();
@@ -1110,7 +1070,7 @@ hipError_t go_hd(hipStream_t s, const AttnArgs& a, const Plan& pl) {
         case 32: return go_matrix<T, HD, 32>(s, a, b16);
         case 128: return go_matrix<T, HD, 128>(s, a, b16);
     }
-    if constexpr (sizeof(typename T::elem) == 2) return go_matrix<T, HD, 256>(s, a, b16);
+    if (pl.vb == 256) return go_matrix<T, HD, 256>(s, a, b16);
     return hipErrorInvalidValue;
 }
 template <class T>
