@@ -518,25 +518,48 @@ __global__ __launch_bounds__(SW * 64, (stream_waves<T, HD, NQ>())) void paged_at
 //
 // The vector unit's work for each score is kept small, since it takes as long as
 // the products: the key's scale goes into the exponent's fma, and the reference
-// of the softmax is not the running maximum but within 2^SLACK below it (floats
-// lose nothing by it). Whether it must move is seen from a bound, the largest
-// product times the tile's largest scale, without scaling each.
+// of the softmax is not the running maximum but below it by up to 2^ROOM, which
+// floats hold as well (the exponent's rounding is that of the score itself). That
+// a tile stays within ROOM is seen before it is computed, from |q| |k|, so that
+// the loop of most tiles has no comparisons and no rescaling of the context (the
+// registers of the two are what lets the products of one half tile run beside
+// the exponentials of another). A tile for which the bound says nothing, such as
+// a sequence's first, takes a step that looks at the scores and moves the
+// reference where one lies more than 2^SLACK above it.
 constexpr int TK = 64;  // keys of a tile
-constexpr float SLACK = 6.0f;
+// 2^(ROOM + 7) (codes) times value scales below VMOST times 2^28 keys is finite.
+constexpr float SLACK = 6.0f, ROOM = 72.0f, VMOST = 1048576.0f;
 typedef float v16f __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ v16f mfma32(v4i a, v4i b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
 }
 
-template <class T, int HD, int NW>
-__global__ __launch_bounds__(NW * 64, 2) void paged_attention_tile_kernel(AttnArgs p) {
+constexpr int TW = 8, TVB = 32 * TW;  // waves, query vectors of a workgroup
+
+// N matrix products of a region, each followed by an LDS read and VALU vector
+// instructions of it.
+template <int N, int VALU>
+__device__ __forceinline__ void interleave() {
+    __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, VALU, 0);
+    }
+}
+
+template <class T, int HD>
+__global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnArgs p) {
     typedef typename T::elem E;
-    constexpr int PARTS = sizeof(E) == 4 ? 3 : 1, NT = NW * 64, VB = 32 * NW, KB = TK * HD * 2;
-    __shared__ __attribute__((aligned(1024))) uint8_t kt[2][KB], vt[2][KB];
-    __shared__ __attribute__((aligned(16))) float scs[2][2][TK];  // [buffer][keys', values'] scales
+    constexpr int PARTS = sizeof(E) == 4 ? 3 : 1, NT = TW * 64, KB = TK * HD * 2, NBUF = 3;
+    constexpr bool PIPE = PARTS == 1;
+    __shared__ __attribute__((aligned(1024))) uint8_t kt[NBUF][KB], vt[NBUF][KB];
+    __shared__ __attribute__((aligned(16))) float scs[NBUF][2][TK];  // keys', values' scales
     __shared__ __attribute__((aligned(16))) uint32_t ring[4][TK];
-    __shared__ float kmx[2][2];
+    __shared__ float kmx[NBUF][2];                               // their largest
+    __shared__ __attribute__((aligned(16))) int kn2[NBUF][TW];  // largest |codes|^2 of a wave's keys
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t nkv = p.kv.nkv, kvs = nkv * HD, units = p.blocks * p.nsplit;
@@ -546,9 +569,9 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_tile_kernel(AttnAr
     unit = units - 1 - unit;  // a chunk's last rows see the most keys: they start first
     const uint32_t split = unit % p.nsplit;
     Block bl;
-    if (!find_block<VB>(p.bt, p.group, unit / p.nsplit, lane, bl)) return;
+    if (!find_block<TVB>(p.bt, p.group, unit / p.nsplit, lane, bl)) return;
     const uint32_t reach = (uint32_t)min((uint64_t)p.kv.max_bt * p.kv.bs, (uint64_t)0x7fff0000u);
-    const uint32_t vend = min(bl.v0 + VB, bl.nv);
+    const uint32_t vend = min(bl.v0 + TVB, bl.nv);
     const uint32_t kend = min(keys_seen(bl, (vend - 1) / p.group), reach);
     const uint32_t k0 = split * p.span, k1 = split + 1 == p.nsplit ? kend : min(kend, k0 + p.span);
     if (k0 >= k1 && split) return;
@@ -560,17 +583,22 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_tile_kernel(AttnAr
     const uint32_t wall = wlive ? min(keys_seen(bl, wv0 / p.group), reach) : 0u;
     const uint32_t wend = wlive ? min(keys_seen(bl, (wv1 - 1) / p.group), reach) : 0u;
     uint32_t seen;
+    float qn;
     v4i qf[HD / 16][PARTS];  // step t: d = 16 t + 8 half ..+7 of vector col
     {
         const uint32_t v = min(wv0 + col, vend - 1), i = v / p.group, h = kvh * p.group + v % p.group;
         seen = wv0 + col < vend ? min(keys_seen(bl, i), reach) : 0u;
         const E* src = (const E*)p.q + (bl.r0 + i) * p.qs + (uint64_t)h * HD + 8 * half;
+        qn = 0.0f;
 #pragma unroll
         for (int t = 0; t < HD / 16; ++t) {
             float x[8];
             query8<T>(src + 16 * t, p.qvec, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) qn = qn + x[e] * x[e];
             split8<PARTS>(x, qf[t]);
         }
+        qn = sqrtf(qn + xor_lane<32>(qn)) * 1.001f;  // above |q|, whatever the roundings (infinite or NaN: no bound)
     }
     v16f o[HD / 32];
     float m = -INFINITY, l = 0.0f;
@@ -599,184 +627,224 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_tile_kernel(AttnAr
         ring[t & 3][lane] = s != NO_SLOT ? s : 0u;
         return __ballot(s != NO_SLOT);
     };
-    constexpr int CPK = HD / 16, KPP = NT / CPK, NK = KPP < TK ? TK / KPP : 1;  // 16-byte pieces of a key; keys a pass; passes
-    constexpr int DG = HD / 4;
-    const bool klive = NT <= TK * CPK || tid < TK * CPK, vlive = NT <= TK / 8 * DG || tid < TK / 8 * DG;
-    v4i kr[NK];
-    uint32_t vr[8];
+    // A thread takes 16 bytes of a key and four values' four bytes (HD 64: one
+    // of the two).
+    constexpr int CPK = HD / 16, DG = HD / 4, VT = NT - TK / 4 * DG;  // VT: the first thread with values
+    static_assert(VT >= 0 && TK * CPK <= NT, "a piece for each thread");
+    const bool klive = TK * CPK == NT || tid < TK * CPK, vlive = VT == 0 || tid >= VT;
+    const int kkey = tid / CPK, kpc = tid % CPK, quad = (tid - VT) / DG, dg = (tid - VT) % DG;
+    v4i kr;
+    uint32_t vr[4];
     float sr = 0.0f;
-    const int kkey = tid / CPK, kpc = tid % CPK, oct = tid / DG, dg = tid % DG;
-    const int vkey = 16 * (oct >> 1) + 4 * (oct & 1);  // octet's keys: vkey ..+3, vkey + 8 ..+11
-    auto load = [&](int t) {
+    auto load = [&](int t) __attribute__((always_inline)) {
         const uint32_t* sl = ring[t & 3];
-        if (klive)
-#pragma unroll
-            for (int u = 0; u < NK; ++u)
-                kr[u] = *reinterpret_cast<const v4i*>(kp + (size_t)sl[kkey + KPP * u] * kvs + 16 * kpc);
+        if (klive) kr = *reinterpret_cast<const v4i*>(kp + (size_t)sl[kkey] * kvs + 16 * kpc);
         if (vlive) {
-            const uint4 a = *reinterpret_cast<const uint4*>(sl + vkey), b = *reinterpret_cast<const uint4*>(sl + vkey + 8);
-            const uint32_t ss[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+            const uint4 a = *reinterpret_cast<const uint4*>(sl + 4 * quad);
+            const uint32_t ss[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-            for (int i = 0; i < 8; ++i) vr[i] = *reinterpret_cast<const uint32_t*>(vp + (size_t)ss[i] * kvs + 4 * dg);
+            for (int i = 0; i < 4; ++i) vr[i] = *reinterpret_cast<const uint32_t*>(vp + (size_t)ss[i] * kvs + 4 * dg);
         }
         sr = sp[(size_t)sl[lane] * nkv];
     };
     // LDS images. K: chunk c (8 d) of key r. V^T: 32 keys at a time, lines of 256
-    // bytes hold 4 d x 32 keys. In both the 16 lanes that meet go to 16 slots.
+    // bytes hold 4 d x 32 keys, 8 keys a chunk in the order of a lane's scores:
+    // chunk 2u + h has keys 16u + 4h ..+3 and 16u + 8 + 4h ..+3. In both the 16
+    // lanes that meet go to 16 slots.
     auto kchunk = [&](int r, int c) -> int { return r * (HD * 2) + ((HD == 128 ? c ^ (r & 15) : c ^ ((r >> 1) & 7)) << 4); };
     auto vchunk = [&](int d, int oc) -> int {
         return (oc >> 2) * (64 * HD) + (d >> 2) * 256 + (((4 * (d & 3) + (oc & 3)) ^ ((d >> 2) & 15)) << 4);
     };
-    auto store = [&](int t, unsigned long long ok) __attribute__((always_inline)) {
-        const int bu = t & 1;
-        if (klive)
+    const int kst = klive ? kchunk(kkey, 2 * kpc) : 0;  // chunk 2 kpc + 1 is at kst ^ 16
+    // quad: keys 4 quad ..+3 = 16 u' + 4 x: chunk (quad / 4) * 2 + (quad & 1), its half (quad >> 1) & 1
+    const int vst = vlive ? vchunk(4 * dg, 2 * (quad >> 2) + (quad & 1)) + 8 * ((quad >> 1) & 1) : 0;
+    auto store_k = [&](int bu) __attribute__((always_inline)) {
+        if (klive) {
+            *reinterpret_cast<v4i*>(kt[0] + bu * KB + kst) = codes8((uint32_t)kr[0], (uint32_t)kr[1]);
+            *reinterpret_cast<v4i*>(kt[0] + bu * KB + (kst ^ 16)) = codes8((uint32_t)kr[2], (uint32_t)kr[3]);
+            int n2 = 0;
 #pragma unroll
-            for (int u = 0; u < NK; ++u) {
-                const int key = kkey + KPP * u;
-                *reinterpret_cast<v4i*>(kt[bu] + kchunk(key, 2 * kpc)) = codes8((uint32_t)kr[u][0], (uint32_t)kr[u][1]);
-                *reinterpret_cast<v4i*>(kt[bu] + kchunk(key, 2 * kpc + 1)) = codes8((uint32_t)kr[u][2], (uint32_t)kr[u][3]);
-            }
+            for (int i = 0; i < 4; ++i) n2 = __builtin_amdgcn_sdot4(kr[i], kr[i], n2, false);
+            n2 += (int)xor_lane_u<1>((uint32_t)n2);  // the CPK lanes of a key
+            n2 += (int)xor_lane_u<2>((uint32_t)n2);
+            if constexpr (CPK == 8) n2 += (int)xor_lane_u<4>((uint32_t)n2);
+            float f = (float)n2;  // exact
+            f = fmaxf(f, xor_lane<8>(f));
+            f = fmaxf(f, xor_lane<16>(f));
+            f = fmaxf(f, xor_lane<32>(f));
+            if constexpr (CPK == 4) f = fmaxf(f, xor_lane<4>(f));
+            kn2[bu][wave] = (int)f;
+        }
+    };
+    auto store_v = [&](int bu, unsigned long long ok) __attribute__((always_inline)) {
         if (vlive) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float x[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = code_f(vr[i], e);
-                *reinterpret_cast<v4i*>(vt[bu] + vchunk(4 * dg + e, oct)) =
-                    v4i{(int)hi16x2(x[0], x[1]), (int)hi16x2(x[2], x[3]), (int)hi16x2(x[4], x[5]), (int)hi16x2(x[6], x[7])};
-            }
+            for (int e = 0; e < 4; ++e)  // dimension 4 dg + e: chunk index + 4 e
+                *reinterpret_cast<uint2*>(vt[0] + bu * KB + (vst ^ (e << 6))) =
+                    make_uint2(hi16x2(code_f(vr[0], e), code_f(vr[1], e)), hi16x2(code_f(vr[2], e), code_f(vr[3], e)));
         }
         // A key without a slot has scales of 0. (Waves of a kind write the same.)
         const float sc = (ok >> lane) & 1ull ? (wave & 1 ? sr : sr * p.scale2) : 0.0f;
         scs[bu][wave & 1][lane] = sc;
         kmx[bu][wave & 1] = xor_max<32>(fabsf(sc));
     };
-
-    // The products of one tile. HIDE: some of its keys are hidden from some query
-    // (ok: the keys that have a slot).
-    auto attend = [&](auto hide_, int bu, uint32_t j0, unsigned long long ok) __attribute__((always_inline)) {
-        constexpr bool HIDE = decltype(hide_)::value;
-        // Register e of half kh: key 32 kh + 8 (e / 4) + 4 half + e % 4.
-        v16f s[2];
-        // kchunk(32 kh + col, 2 d + half) and vchunk(32 j + col, 4 kh + 2 u + half)
-        // from one address each. (The empty asm keeps the rest of them from being
-        // carried in registers from tile to tile.)
-        int ka = bu * KB + kchunk(col, half), va = bu * KB + vchunk(col, half);
-        asm volatile("" : "+v"(ka), "+v"(va));
+    // Scores of half kh of the tile in buffer bu. Register e: key 32 kh +
+    // 8 (e / 4) + 4 half + e % 4.
+    auto scores = [&](int bu, int kh, v16f& s) __attribute__((always_inline)) {
+        int ka = bu * KB + kh * (64 * HD) + kchunk(col, half);  // chunk 2 d + half is at ka ^ (d << 5)
+        asm volatile("" : "+v"(ka));  // the others are not carried from tile to tile in registers
 #pragma unroll
-        for (int kh = 0; kh < 2; ++kh)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) s[kh][e] = 0.0f;
+        for (int e = 0; e < 16; ++e) s[e] = 0.0f;
 #pragma unroll
         for (int d = 0; d < HD / 16; ++d) {
-            v4i k[2];
+            const v4i k = *reinterpret_cast<const v4i*>(kt[0] + (ka ^ (d << 5)));
 #pragma unroll
-            for (int kh = 0; kh < 2; ++kh) k[kh] = *reinterpret_cast<const v4i*>(kt[0] + (ka ^ (d << 5)) + kh * (64 * HD));
-#pragma unroll
-            for (int part = PARTS - 1; part >= 0; --part)
-#pragma unroll
-                for (int kh = 0; kh < 2; ++kh) s[kh] = mfma32(k[kh], qf[d][part], s[kh]);
+            for (int part = PARTS - 1; part >= 0; --part) s = mfma32(k, qf[d][part], s);
         }
-        const float *kcp = &scs[bu][0][4 * half], *vsp = &scs[bu][1][4 * half];
-        const unsigned long long okl = ok >> (4 * half);
-        const int lim = (int)(seen - j0) - 4 * half;  // (2^31 keys at most)
-        auto hidden = [&](int key) -> bool { return key >= lim || !((okl >> key) & 1ull); };
-        float mx = 0.0f;
+    };
+    // Whether the tile in buffer bu stays within ROOM of every query's reference.
+    auto within = [&](int bu) -> bool {
+        int n2 = 0;
 #pragma unroll
-        for (int kh = 0; kh < 2; ++kh)
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) mx = fmaxf(fmaxf(mx, fabsf(s[kh][e])), fabsf(s[kh][e + 1]));
-        if (__builtin_expect(__any(!(mx * kmx[bu][0] <= m + SLACK)), 0)) {  // the bound may be exceeded: look at the scores themselves
-            mx = -INFINITY;
-#pragma unroll
-            for (int kh = 0; kh < 2; ++kh)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int key = 32 * kh + 8 * (e >> 2) + (e & 3);
-                    const float a = s[kh][e] * kcp[key];
-                    mx = fmaxf(mx, HIDE && hidden(key) ? -INFINITY : a);
-                }
-            mx = fmaxf(mx, xor_lane<32>(mx));
-            const float mn = mx > m + SLACK ? mx : m;  // each query for itself
-            const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-            l = l * alpha;
-#pragma unroll
-            for (int j = 0; j < HD / 32; ++j)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) o[j][e] = o[j][e] * alpha;
-            m = mn;
+        for (int w = 0; w < TW; w += 4) {
+            const v4i n = *reinterpret_cast<const v4i*>(&kn2[bu][w]);
+            n2 = max(max(max(n2, n[0]), max(n[1], n[2])), n[3]);
         }
-        const float ref = m == -INFINITY ? 0.0f : m;
+        const bool ok = qn * (__builtin_amdgcn_sqrtf((float)n2) * kmx[bu][0]) <= m + ROOM && kmx[bu][1] < VMOST;
+        return __all(ok);
+    };
+    // Moves the reference to the largest score where that is more than SLACK
+    // above it, each query for itself (ok: the keys that have a slot).
+    auto refer = [&](int bu, int kh, uint32_t j0, unsigned long long ok, const v16f& s) __attribute__((always_inline)) {
+        const float* kcp = &scs[bu][0][32 * kh + 4 * half];
+        const uint32_t okl = (uint32_t)(ok >> (32 * kh)) >> (4 * half);
+        const int lim = (int)(seen - j0) - 32 * kh - 4 * half;
+        float mx = -INFINITY;
 #pragma unroll
-        for (int kh = 0; kh < 2; ++kh)
+        for (int e = 0; e < 16; ++e) {
+            const int key = 8 * (e >> 2) + (e & 3);
+            const float a = s[e] * kcp[key];
+            mx = fmaxf(mx, key >= lim || !((okl >> key) & 1u) ? -INFINITY : a);
+        }
+        mx = fmaxf(mx, xor_lane<32>(mx));
+        const bool up = mx > m + SLACK;
+        if (!__any(up)) return;
+        const float alpha = up ? __builtin_amdgcn_exp2f(m - mx) : 1.0f;
+        l = l * alpha;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                float x[8];
+        for (int j = 0; j < HD / 32; ++j)
 #pragma unroll
-                for (int i4 = 0; i4 < 2; ++i4) {
-                    const int k0_ = 32 * kh + 16 * u + 8 * i4;
-                    const float4 kc = *reinterpret_cast<const float4*>(kcp + k0_), vs = *reinterpret_cast<const float4*>(vsp + k0_);
-                    const float kk[4] = {kc.x, kc.y, kc.z, kc.w}, vv[4] = {vs.x, vs.y, vs.z, vs.w};
+            for (int e = 0; e < 16; ++e) o[j][e] = o[j][e] * alpha;
+        m = up ? mx : m;
+    };
+    // Weights of registers 8 u ..+7 of a half's scores, times their values' scales.
+    auto weights = [&](auto hide_, int bu, int kh, int u, uint32_t j0, unsigned long long ok, const v16f& s,
+                       v4i (&pf)[PARTS]) __attribute__((always_inline)) {
+        constexpr bool HIDE = decltype(hide_)::value;
+        const float *kcp = &scs[bu][0][32 * kh + 4 * half], *vsp = &scs[bu][1][32 * kh + 4 * half];
+        const uint32_t okl = (uint32_t)(ok >> (32 * kh)) >> (4 * half);
+        const int lim = (int)(seen - j0) - 32 * kh - 4 * half;
+        const float ref = HIDE && m == -INFINITY ? 0.0f : m;
+        float x[8];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float a = __builtin_fmaf(s[kh][8 * u + 4 * i4 + i], kk[i], -ref);
-                        if (HIDE && hidden(k0_ + i)) a = -INFINITY;
-                        const float w = __builtin_amdgcn_exp2f(a);
-                        l = l + w;
-                        x[4 * i4 + i] = HIDE && hidden(k0_ + i) ? 0.0f : w * vv[i];  // whatever its scale is
-                    }
-                }
-                v4i pf[PARTS];
-                split8<PARTS>(x, pf);
+        for (int i4 = 0; i4 < 2; ++i4) {
+            const int k_ = 16 * u + 8 * i4;
+            const float4 kc = *reinterpret_cast<const float4*>(kcp + k_), vs = *reinterpret_cast<const float4*>(vsp + k_);
+            const float kk[4] = {kc.x, kc.y, kc.z, kc.w}, vv[4] = {vs.x, vs.y, vs.z, vs.w};
 #pragma unroll
-                for (int j = 0; j < HD / 32; ++j) {
-                    const v4i v = *reinterpret_cast<const v4i*>(vt[0] + (va ^ (u << 5) ^ ((j & 1) << 7)) + j * 2048 + kh * (64 * HD));
-#pragma unroll
-                    for (int part = PARTS - 1; part >= 0; --part) o[j] = mfma32(v, pf[part], o[j]);
-                }
+            for (int i = 0; i < 4; ++i) {
+                const bool hid = HIDE && (k_ + i >= lim || !((okl >> (k_ + i)) & 1u));
+                float a = __builtin_fmaf(s[8 * u + 4 * i4 + i], kk[i], -ref);
+                if (hid) a = -INFINITY;
+                const float w = __builtin_amdgcn_exp2f(a);
+                l = l + w;
+                x[4 * i4 + i] = hid ? 0.0f : w * vv[i];  // whatever its scale is
             }
+        }
+        split8<PARTS>(x, pf);
+    };
+    // Their product with the values.
+    auto values = [&](int bu, int kh, int u, const v4i (&pf)[PARTS]) __attribute__((always_inline)) {
+        int va = bu * KB + kh * (64 * HD) + (vchunk(col, half) ^ (u << 5));  // vchunk(32 j + col, 2 u + half): see there
+        asm volatile("" : "+v"(va));
+#pragma unroll
+        for (int j = 0; j < HD / 32; ++j) {
+            const v4i v = *reinterpret_cast<const v4i*>(vt[0] + (va ^ ((j & 1) << 7)) + j * 2048);
+#pragma unroll
+            for (int part = PARTS - 1; part >= 0; --part) o[j] = mfma32(v, pf[part], o[j]);
+        }
     };
 
-    // Masks of tiles t .. t + 2, and the slot that this lane puts next.
-    unsigned long long ok0 = put_slots(0, slot_at(0)), ok1 = put_slots(1, slot_at(1)), ok2 = put_slots(2, slot_at(2));
-    uint32_t sl_next = slot_at(3);
+    // Masks of tiles t .. t + 3, and the slot that this lane puts next.
+    unsigned long long ok0 = put_slots(0, slot_at(0)), ok1 = put_slots(1, slot_at(1)), ok2 = put_slots(2, slot_at(2)),
+                       ok3 = put_slots(3, slot_at(3));
+    uint32_t sl_next = slot_at(4);
     barrier();
     load(0);
-    store(0, ok0);
+    store_k(0), store_v(0, ok0);
     load(1);
+    store_k(1), store_v(1, ok1);
+    load(2);
     barrier();
-    auto stage = [&](int t) __attribute__((always_inline)) {
-        store(t + 1, ok1);
-        load(t + 2);
-        ok0 = ok1, ok1 = ok2, ok2 = put_slots(t + 3, sl_next);
-        sl_next = slot_at(t + 4);
+    // In step t tile t + 2 goes to LDS, whose buffer was last read in step t - 1.
+    // bf16: the scores of a half are computed beside the weights of the half
+    // before (with three parts the products alone fill the time, and the
+    // registers). Regions between the scheduling barriers are what is to run
+    // together; interleave in which order their kinds are issued.
+    int b0 = 0, b1 = 1, b2 = 2;
+    v16f s0, s1;
+    if constexpr (PIPE) scores(0, 0, s0);
+    bool calm = false;  // the next tile is within its bound and seen whole by all of the wave's queries
+    auto step = [&](auto look, int t) __attribute__((always_inline)) {
+        constexpr bool LOOK = decltype(look)::value;
+        const uint32_t j0 = k0 + (uint32_t)t * TK;
+        if (!LOOK || j0 < wend) {
+            v4i pf[PARTS], pg[PARTS];
+#pragma unroll
+            for (int kh = 0; kh < 2; ++kh) {
+                v16f& s = PIPE && kh ? s1 : s0;
+                if constexpr (!PIPE) scores(b0, kh, s);
+                if constexpr (LOOK) refer(b0, kh, j0, ok0, s);
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (PIPE) {
+                    if (kh == 0) scores(b0, 1, s1);
+                    else scores(b1, 0, s0);
+                }
+                weights(look, b0, kh, 0, j0, ok0, s, pf);
+                if constexpr (PIPE && !LOOK) interleave<HD / 16, 6>();
+                __builtin_amdgcn_sched_barrier(0);
+                values(b0, kh, 0, pf);
+                weights(look, b0, kh, 1, j0, ok0, s, pg);
+                if constexpr (!LOOK) interleave<PARTS * HD / 32, 9>();
+                __builtin_amdgcn_sched_barrier(0);
+                values(b0, kh, 1, pg);
+                if (kh == 0) store_k(b2);
+                else store_v(b2, ok2);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+            store_k(b2);
+            store_v(b2, ok2);
+        }
+        load(t + 3);
+        calm = j0 + 2 * TK <= wall && ok1 == ~0ull && within(b1);
+        ok0 = ok1, ok1 = ok2, ok2 = ok3, ok3 = put_slots(t + 4, sl_next);
+        sl_next = slot_at(t + 5);
+        const int b = b0;
+        b0 = b1, b1 = b2, b2 = b;
+        barrier();
     };
-    // Tiles that all of this wave's queries see whole go through a loop of their
-    // own, without the comparisons. (Each wave passes one barrier a tile in
-    // whichever loop it is.)
+    // (Each wave passes one barrier a tile in whichever loop it is.)
     for (int t = 0; t < nt;) {
+        step(std::true_type{}, t++);
 #pragma unroll 1
-        for (; t < nt; ++t) {
-            const uint32_t j0 = k0 + (uint32_t)t * TK;
-            if (j0 + TK > wall || ok0 != ~0ull) break;
-            stage(t);
-            attend(std::false_type{}, t & 1, j0, ~0ull);
-            barrier();
-        }
-        if (t < nt) {
-            const uint32_t j0 = k0 + (uint32_t)t * TK;
-            const unsigned long long ok = ok0;
-            stage(t);
-            if (j0 < wend) attend(std::true_type{}, t & 1, j0, ok);
-            barrier();
-            ++t;
-        }
+        while (t < nt && calm) step(std::false_type{}, t++);
     }
     const uint32_t v = wv0 + col;
     l = l + xor_lane<32>(l);
     if (v >= vend) return;
     if (p.nsplit > 1) {
-        const uint64_t at = ((uint64_t)unit * nkv + kvh) * VB + (v - bl.v0);
+        const uint64_t at = ((uint64_t)unit * nkv + kvh) * TVB + (v - bl.v0);
 #pragma unroll
         for (int j = 0; j < HD / 32; ++j)
 #pragma unroll
@@ -1022,7 +1090,7 @@ Plan plan_attention(const Kv8& kv, const Kv8Rows& bt, const bh_kv8_batch* hint, 
     const uint32_t most = bt.start ? (hint->max_rows ? std::min(hint->max_rows, bt.rows) : bt.rows) : 1;
     const uint64_t vectors = (uint64_t)most * group, all = (uint64_t)bt.rows * group;
     r.kind = vectors <= 32 ? STREAM : TILE;
-    r.vb = vectors <= 16 ? 16 : vectors <= 32 ? 32 : 128;
+    r.vb = vectors <= 16 ? 16 : vectors <= 32 ? 32 : TVB;
     r.blocks = !bt.start && group <= r.vb ? bt.batch : (uint32_t)(all / r.vb) + bt.batch;
     const uint64_t reach = (uint64_t)kv.max_bt * kv.bs;
     const uint64_t len = std::max<uint64_t>(1, hint->max_len ? std::min<uint64_t>(hint->max_len, reach) : reach);
@@ -1052,7 +1120,7 @@ hipError_t go_matrix(hipStream_t s, const AttnArgs& a, bool b16) {
     const uint64_t units = ((uint64_t)a.blocks * a.nsplit + 7) / 8 * 8 * a.kv.nkv;
     const uint64_t joins = (uint64_t)a.blocks * a.kv.nkv * (VB / 4);
     if (units > 0x7fffffffull || joins > 0x7fffffffull) return hipErrorInvalidConfiguration;
-    if constexpr (VB > 32) paged_attention_tile_kernel<T, HD, VB / 32><<<(unsigned)units, 2 * VB, 0, s>>>(a);
+    if constexpr (VB > 32) paged_attention_tile_kernel<T, HD><<<(unsigned)units, TW * 64, 0, s>>>(a);
     else if (b16) paged_attention_stream_kernel<T, HD, VB / 16, true><<<(unsigned)units, SW * 64, 0, s>>>(a);
     else paged_attention_stream_kernel<T, HD, VB / 16, false><<<(unsigned)units, SW * 64, 0, s>>>(a);
     hipError_t e = hipGetLastError();
@@ -1068,10 +1136,8 @@ hipError_t go_hd(hipStream_t s, const AttnArgs& a, const Plan& pl) {
     switch (pl.vb) {
         case 16: return go_matrix<T, HD, 16>(s, a, b16);
         case 32: return go_matrix<T, HD, 32>(s, a, b16);
-        case 128: return go_matrix<T, HD, 128>(s, a, b16);
     }
-    if (pl.vb == 256) return go_matrix<T, HD, 256>(s, a, b16);
-    return hipErrorInvalidValue;
+    return go_matrix<T, HD, TVB>(s, a, b16);
 }
 template <class T>
 hipError_t go_attention(hipStream_t s, const AttnArgs& a, const Plan& pl) {
