@@ -537,19 +537,6 @@ __device__ __forceinline__ v16f mfma32(v4i a, v4i b, v16f c) {
 
 constexpr int TW = 8, TVB = 32 * TW;  // waves, query vectors of a workgroup
 
-// N matrix products of a region, each followed by an LDS read and VALU vector
-// instructions of it.
-template <int N, int VALU>
-__device__ __forceinline__ void interleave() {
-    __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x2, VALU, 0);
-    }
-}
-
 template <class T, int HD>
 __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnArgs p) {
     typedef typename T::elem E;
@@ -738,9 +725,10 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
         m = up ? mx : m;
     };
     // Weights of registers 8 u ..+7 of a half's scores, times their values' scales.
-    auto weights = [&](auto hide_, int bu, int kh, int u, uint32_t j0, unsigned long long ok, const v16f& s,
-                       v4i (&pf)[PARTS]) __attribute__((always_inline)) {
-        constexpr bool HIDE = decltype(hide_)::value;
+    // HIDE: some of the keys are hidden from some query.
+    auto weights = [&](int bu, int kh, int u, uint32_t j0, unsigned long long ok, const v16f& s, v4i (&pf)[PARTS],
+                       auto hide) __attribute__((always_inline)) {
+        constexpr bool HIDE = decltype(hide)::value;
         const float *kcp = &scs[bu][0][32 * kh + 4 * half], *vsp = &scs[bu][1][32 * kh + 4 * half];
         const uint32_t okl = (uint32_t)(ok >> (32 * kh)) >> (4 * half);
         const int lim = (int)(seen - j0) - 32 * kh - 4 * half;
@@ -787,45 +775,11 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
     load(2);
     barrier();
     // In step t tile t + 2 goes to LDS, whose buffer was last read in step t - 1.
-    // bf16: the scores of a half are computed beside the weights of the half
-    // before (with three parts the products alone fill the time, and the
-    // registers). Regions between the scheduling barriers are what is to run
-    // together; interleave in which order their kinds are issued.
     int b0 = 0, b1 = 1, b2 = 2;
     v16f s0, s1;
-    if constexpr (PIPE) scores(0, 0, s0);
     bool calm = false;  // the next tile is within its bound and seen whole by all of the wave's queries
-    auto step = [&](auto look, int t) __attribute__((always_inline)) {
-        constexpr bool LOOK = decltype(look)::value;
+    auto rest = [&](int t) __attribute__((always_inline)) {
         const uint32_t j0 = k0 + (uint32_t)t * TK;
-        if (!LOOK || j0 < wend) {
-            v4i pf[PARTS], pg[PARTS];
-#pragma unroll
-            for (int kh = 0; kh < 2; ++kh) {
-                v16f& s = PIPE && kh ? s1 : s0;
-                if constexpr (!PIPE) scores(b0, kh, s);
-                if constexpr (LOOK) refer(b0, kh, j0, ok0, s);
-                __builtin_amdgcn_sched_barrier(0);
-                if constexpr (PIPE) {
-                    if (kh == 0) scores(b0, 1, s1);
-                    else scores(b1, 0, s0);
-                }
-                weights(look, b0, kh, 0, j0, ok0, s, pf);
-                if constexpr (PIPE && !LOOK) interleave<HD / 16, 6>();
-                __builtin_amdgcn_sched_barrier(0);
-                values(b0, kh, 0, pf);
-                weights(look, b0, kh, 1, j0, ok0, s, pg);
-                if constexpr (!LOOK) interleave<PARTS * HD / 32, 9>();
-                __builtin_amdgcn_sched_barrier(0);
-                values(b0, kh, 1, pg);
-                if (kh == 0) store_k(b2);
-                else store_v(b2, ok2);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        } else {
-            store_k(b2);
-            store_v(b2, ok2);
-        }
         load(t + 3);
         calm = j0 + 2 * TK <= wall && ok1 == ~0ull && within(b1);
         ok0 = ok1, ok1 = ok2, ok2 = ok3, ok3 = put_slots(t + 4, sl_next);
@@ -834,11 +788,155 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
         b0 = b1, b1 = b2, b2 = b;
         barrier();
     };
+    // Any tile, one thing after another.
+    auto step = [&](int t) __attribute__((always_inline)) {
+        const uint32_t j0 = k0 + (uint32_t)t * TK;
+        store_k(b2);
+        store_v(b2, ok2);
+        if (j0 < wend) {
+#pragma unroll
+            for (int kh = 0; kh < 2; ++kh) {
+                v4i pf[PARTS];
+                scores(b0, kh, s0);
+                refer(b0, kh, j0, ok0, s0);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    weights(b0, kh, u, j0, ok0, s0, pf, std::true_type{});
+                    values(b0, kh, u, pf);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        rest(t);
+    };
+    // A calm tile. The products are laid out with the vector work that is to run
+    // beside them, one product (32 cycles) and its share between two scheduling
+    // barriers, and the operands of a product are read two products ahead. bf16:
+    // beside the next half's scores go the weights of 8 of this half's keys;
+    // beside their product with V the weights of the other 8; beside those'
+    // product the conversion of a tile to come. f32: three products for each,
+    // and no registers for the next half's scores.
+    constexpr int NS = HD / 16, NJ = HD / 32;
+    v4i ka_[2];     // the first two operands of the next scores
+    float4 kc_, vs_;  // scales of the next 4 keys
+    auto fence = [&]() { __builtin_amdgcn_sched_barrier(0); };
+    auto kaddr = [&](int bu, int kh) -> int { return bu * KB + kh * (64 * HD) + kchunk(col, half); };
+    auto prime = [&](int kbase, int bu, int kh) __attribute__((always_inline)) {
+        kc_ = *reinterpret_cast<const float4*>(&scs[bu][0][32 * kh + 4 * half]);
+        vs_ = *reinterpret_cast<const float4*>(&scs[bu][1][32 * kh + 4 * half]);
+        ka_[0] = *reinterpret_cast<const v4i*>(kt[0] + kbase);
+        ka_[1] = *reinterpret_cast<const v4i*>(kt[0] + (kbase ^ 32));
+    };
+    auto calm_half = [&](int kh, int kbase, const v16f& s, v16f& nx, int nbase, int nbu, int nkh) __attribute__((always_inline)) {
+        const float* kcp = &scs[b0][0][32 * kh + 4 * half];  // values' scales: TK floats on
+        int va0 = b0 * KB + kh * (64 * HD) + vchunk(col, half), va1 = va0 ^ 32;
+        asm volatile("" : "+v"(va0), "+v"(va1), "+v"(kbase));
+        auto vread = [&](int va, int j) -> v4i { return *reinterpret_cast<const v4i*>(vt[0] + (va ^ ((j & 1) << 7)) + j * 2048); };
+        float x[16];
+        float4 kc[4], vs[4];
+        v4i kf[NS], vf[2][NJ], pf[PARTS], pg[PARTS];
+        kc[0] = kc_, vs[0] = vs_, kf[0] = ka_[0], kf[1] = ka_[1];
+        // Key register e: its weight's exponential, then (one product later) the rest.
+        float w[16];
+        auto at = [](const float4& v, int i) -> float { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; };
+        auto raise = [&](int e) { w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], at(kc[e >> 2], e & 3), -m)); };
+        auto finish = [&](int e) {
+            l = l + w[e];
+            x[e] = w[e] * at(vs[e >> 2], e & 3);
+        };
+        auto scales = [&](int g4) {  // of keys 8 g4 ..
+            kc[g4] = *reinterpret_cast<const float4*>(kcp + 8 * g4);
+            vs[g4] = *reinterpret_cast<const float4*>(kcp + TK + 8 * g4);
+        };
+        auto pack = [&](int u, v4i (&f)[PARTS]) {
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = x[8 * u + i];
+            split8<PARTS>(y, f);
+        };
+        constexpr int EP = 8 / NS;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) nx[e] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < NS; ++d) {
+            nx = mfma32(kf[d], qf[d][0], nx);
+            if (d + 2 < NS) kf[d + 2] = *reinterpret_cast<const v4i*>(kt[0] + (kbase ^ ((d + 2) << 5)));
+            if (d == 0) scales(1);
+            if (d == NS - 2) vf[0][0] = vread(va0, 0), scales(2);
+            if (d == NS - 1) vf[0][1] = vread(va0, 1);
+#pragma unroll
+            for (int i = 0; i < EP; ++i) raise(EP * d + i);
+            if (d)
+#pragma unroll
+                for (int i = 0; i < EP; ++i) finish(EP * (d - 1) + i);
+            fence();
+        }
+#pragma unroll
+        for (int i = 0; i < EP; ++i) finish(8 - EP + i);
+        pack(0, pf);
+        fence();
+        constexpr int EV = 8 / NJ;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            o[j] = mfma32(vf[0][j], pf[0], o[j]);
+            if (j + 2 < NJ) vf[0][j + 2] = vread(va0, j + 2);
+            else vf[1][j + 2 - NJ] = vread(va1, j + 2 - NJ);
+            if (j == 0) scales(3);
+#pragma unroll
+            for (int i = 0; i < EV; ++i) raise(8 + EV * j + i);
+            if (j)
+#pragma unroll
+                for (int i = 0; i < EV; ++i) finish(8 + EV * (j - 1) + i);
+            fence();
+        }
+#pragma unroll
+        for (int i = 0; i < EV; ++i) finish(16 - EV + i);
+        pack(1, pg);
+        fence();
+        prime(nbase, nbu, nkh);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            o[j] = mfma32(vf[1][j], pg[0], o[j]);
+            if (j + 2 < NJ) vf[1][j + 2] = vread(va1, j + 2);
+        }
+        if (kh == 0) store_k(b2);
+        else store_v(b2, ok2);
+        fence();
+    };
+    auto calm_step = [&](int t) __attribute__((always_inline)) {
+        if constexpr (PIPE) {
+            const int kb0 = kaddr(b0, 1), kb1 = kaddr(b1, 0), kb2 = kaddr(b1, 1);
+            calm_half(0, kb0, s0, s1, kb1, b0, 1);
+            calm_half(1, kb1, s1, s0, kb2, b1, 0);
+        } else {
+#pragma unroll
+            for (int kh = 0; kh < 2; ++kh) {
+                v4i pf[PARTS], pg[PARTS];
+                scores(b0, kh, s0);
+                fence();
+                weights(b0, kh, 0, 0u, ~0ull, s0, pf, std::false_type{});
+                fence();
+                values(b0, kh, 0, pf);
+                weights(b0, kh, 1, 0u, ~0ull, s0, pg, std::false_type{});
+                fence();
+                values(b0, kh, 1, pg);
+                if (kh == 0) store_k(b2);
+                else store_v(b2, ok2);
+                fence();
+            }
+        }
+        rest(t);
+    };
     // (Each wave passes one barrier a tile in whichever loop it is.)
     for (int t = 0; t < nt;) {
-        step(std::true_type{}, t++);
+        step(t++);
+        if (t < nt && calm && PIPE) {
+            scores(b0, 0, s0);
+            prime(kaddr(b0, 1), b0, 0);
+        }
 #pragma unroll 1
-        while (t < nt && calm) step(std::false_type{}, t++);
+        while (t < nt && calm) calm_step(t++);
     }
     const uint32_t v = wv0 + col;
     l = l + xor_lane<32>(l);
