@@ -544,9 +544,9 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
     constexpr bool PIPE = PARTS == 1;
     __shared__ __attribute__((aligned(1024))) uint8_t kt[NBUF][KB], vt[NBUF][KB];
     __shared__ __attribute__((aligned(16))) float scs[NBUF][2][TK];  // keys', values' scales
-    __shared__ __attribute__((aligned(16))) uint32_t ring[4][TK];
-    __shared__ float kmx[NBUF][2];                               // their largest
-    __shared__ __attribute__((aligned(16))) int kn2[NBUF][TW];  // largest |codes|^2 of a wave's keys
+    __shared__ int kn2[NBUF][TK];                                      // |codes|^2 of each key
+    __shared__ __attribute__((aligned(16))) uint64_t ring[4][TK];      // bytes to each key's slot
+    __shared__ unsigned long long okm[4];                              // which keys have one
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t nkv = p.kv.nkv, kvs = nkv * HD, units = p.blocks * p.nsplit;
@@ -571,6 +571,7 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
     const uint32_t wend = wlive ? min(keys_seen(bl, (wv1 - 1) / p.group), reach) : 0u;
     uint32_t seen;
     float qn;
+    const bool dead = wv0 + col >= vend;  // no vector: computes the last one's again, its sums are not used
     v4i qf[HD / 16][PARTS];  // step t: d = 16 t + 8 half ..+7 of vector col
     {
         const uint32_t v = min(wv0 + col, vend - 1), i = v / p.group, h = kvh * p.group + v % p.group;
@@ -585,7 +586,10 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
             for (int e = 0; e < 8; ++e) qn = qn + x[e] * x[e];
             split8<PARTS>(x, qf[t]);
         }
-        qn = sqrtf(qn + xor_lane<32>(qn)) * 1.001f;  // above |q|, whatever the roundings (infinite or NaN: no bound)
+        // Above |q|, whatever the roundings; infinite or NaN (no bound: a NaN here
+        // would be lost in the maximum) becomes infinite.
+        qn = sqrtf(qn + xor_lane<32>(qn)) * 1.001f;
+        qn = dead ? 0.0f : qn < INFINITY ? qn : INFINITY;
     }
     v16f o[HD / 32];
     float m = -INFINITY, l = 0.0f;
@@ -597,22 +601,21 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
     // ---- staging
     const uint8_t* kp = (const uint8_t*)p.kv.pool[0] + (size_t)kvh * HD;
     const uint8_t* vp = (const uint8_t*)p.kv.pool[1] + (size_t)kvh * HD;
-    const float* sp = (wave & 1 ? p.kv.scales[1] : p.kv.scales[0]) + kvh;  // even waves take the keys' scales
+    const uint8_t* sp = (const uint8_t*)((wave & 1 ? p.kv.scales[1] : p.kv.scales[0]) + kvh);  // even waves take the keys' scales
     auto barrier = [&]() {  // orders LDS only: loads in flight go on
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
     };
-    // Slots of tile t's keys: every wave looks all of them up, so that each has
-    // the mask of those that exist in scalar registers. A key behind the end or
-    // without a slot gets slot 0.
+    // Where tile t's keys lie: wave t % 8 looks the tables up, two steps before
+    // the loads need it. A key behind the end or without a slot gets slot 0.
     auto slot_at = [&](int t) -> uint32_t {
         const uint32_t j = k0 + (uint32_t)t * TK + lane;
         return j < k1 ? p.kv.slot(bl.b, j) : NO_SLOT;
     };
-    auto put_slots = [&](int t, uint32_t s) -> unsigned long long {
-        ring[t & 3][lane] = s != NO_SLOT ? s : 0u;
-        return __ballot(s != NO_SLOT);
+    auto put_slots = [&](int t, uint32_t s) {
+        ring[t & 3][lane] = s != NO_SLOT ? (uint64_t)s * kvs : 0u;
+        okm[t & 3] = __ballot(s != NO_SLOT);
     };
     // A thread takes 16 bytes of a key and four values' four bytes (HD 64: one
     // of the two).
@@ -624,15 +627,13 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
     uint32_t vr[4];
     float sr = 0.0f;
     auto load = [&](int t) __attribute__((always_inline)) {
-        const uint32_t* sl = ring[t & 3];
-        if (klive) kr = *reinterpret_cast<const v4i*>(kp + (size_t)sl[kkey] * kvs + 16 * kpc);
+        const uint64_t* sl = ring[t & 3];
+        if (klive) kr = *reinterpret_cast<const v4i*>(kp + sl[kkey] + 16 * kpc);
         if (vlive) {
-            const uint4 a = *reinterpret_cast<const uint4*>(sl + 4 * quad);
-            const uint32_t ss[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) vr[i] = *reinterpret_cast<const uint32_t*>(vp + (size_t)ss[i] * kvs + 4 * dg);
+            for (int i = 0; i < 4; ++i) vr[i] = *reinterpret_cast<const uint32_t*>(vp + sl[4 * quad + i] + 4 * dg);
         }
-        sr = sp[(size_t)sl[lane] * nkv];
+        sr = *reinterpret_cast<const float*>(sp + sl[lane] / (HD / 4));
     };
     // LDS images. K: chunk c (8 d) of key r. V^T: 32 keys at a time, lines of 256
     // bytes hold 4 d x 32 keys, 8 keys a chunk in the order of a lane's scores:
@@ -655,12 +656,7 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
             n2 += (int)xor_lane_u<1>((uint32_t)n2);  // the CPK lanes of a key
             n2 += (int)xor_lane_u<2>((uint32_t)n2);
             if constexpr (CPK == 8) n2 += (int)xor_lane_u<4>((uint32_t)n2);
-            float f = (float)n2;  // exact
-            f = fmaxf(f, xor_lane<8>(f));
-            f = fmaxf(f, xor_lane<16>(f));
-            f = fmaxf(f, xor_lane<32>(f));
-            if constexpr (CPK == 4) f = fmaxf(f, xor_lane<4>(f));
-            kn2[bu][wave] = (int)f;
+            kn2[bu][kkey] = n2;
         }
     };
     auto store_v = [&](int bu, unsigned long long ok) __attribute__((always_inline)) {
@@ -673,7 +669,6 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
         // A key without a slot has scales of 0. (Waves of a kind write the same.)
         const float sc = (ok >> lane) & 1ull ? (wave & 1 ? sr : sr * p.scale2) : 0.0f;
         scs[bu][wave & 1][lane] = sc;
-        kmx[bu][wave & 1] = xor_max<32>(fabsf(sc));
     };
     // Scores of half kh of the tile in buffer bu. Register e: key 32 kh +
     // 8 (e / 4) + 4 half + e % 4.
@@ -689,16 +684,14 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
             for (int part = PARTS - 1; part >= 0; --part) s = mfma32(k, qf[d][part], s);
         }
     };
-    // Whether the tile in buffer bu stays within ROOM of every query's reference.
+    // Whether the tile in buffer bu stays within ROOM of every query's reference
+    // (lane l looks at key l, for the longest query and the lowest reference; a
+    // scale that is not a number says no).
+    const float qmost = xor_max<32>(qn);
+    float mleast = -INFINITY;
     auto within = [&](int bu) -> bool {
-        int n2 = 0;
-#pragma unroll
-        for (int w = 0; w < TW; w += 4) {
-            const v4i n = *reinterpret_cast<const v4i*>(&kn2[bu][w]);
-            n2 = max(max(max(n2, n[0]), max(n[1], n[2])), n[3]);
-        }
-        const bool ok = qn * (__builtin_amdgcn_sqrtf((float)n2) * kmx[bu][0]) <= m + ROOM && kmx[bu][1] < VMOST;
-        return __all(ok);
+        const float size = __builtin_amdgcn_sqrtf((float)kn2[bu][lane]) * fabsf(scs[bu][0][lane]);
+        return __all(qmost * size <= mleast + ROOM && scs[bu][1][lane] < VMOST);
     };
     // Moves the reference to the largest score where that is more than SLACK
     // above it, each query for itself (ok: the keys that have a slot).
@@ -723,6 +716,8 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[j][e] = o[j][e] * alpha;
         m = up ? mx : m;
+        const float none = dead ? 0.0f : m;
+        mleast = -xor_max<32>(-none);
     };
     // Weights of registers 8 u ..+7 of a half's scores, times their values' scales.
     // HIDE: some of the keys are hidden from some query.
@@ -732,7 +727,7 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
         const float *kcp = &scs[bu][0][32 * kh + 4 * half], *vsp = &scs[bu][1][32 * kh + 4 * half];
         const uint32_t okl = (uint32_t)(ok >> (32 * kh)) >> (4 * half);
         const int lim = (int)(seen - j0) - 32 * kh - 4 * half;
-        const float ref = HIDE && m == -INFINITY ? 0.0f : m;
+        const float ref = m == -INFINITY ? 0.0f : m;
         float x[8];
 #pragma unroll
         for (int i4 = 0; i4 < 2; ++i4) {
@@ -763,11 +758,15 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
         }
     };
 
-    // Masks of tiles t .. t + 3, and the slot that this lane puts next.
-    unsigned long long ok0 = put_slots(0, slot_at(0)), ok1 = put_slots(1, slot_at(1)), ok2 = put_slots(2, slot_at(2)),
-                       ok3 = put_slots(3, slot_at(3));
-    uint32_t sl_next = slot_at(4);
+    if (wave < 4) put_slots(wave, slot_at(wave));
+    uint32_t sl_next = wave == 4 ? slot_at(4) : NO_SLOT;
     barrier();
+    auto ok_of = [&](int t) -> unsigned long long {
+        const unsigned long long ok = okm[t & 3];
+        return (unsigned long long)(uint32_t)__builtin_amdgcn_readfirstlane((int)(ok >> 32)) << 32 |
+               (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)ok);
+    };
+    unsigned long long ok0 = ok_of(0), ok1 = ok_of(1), ok2 = ok_of(2);  // of tiles t .. t + 2
     load(0);
     store_k(0), store_v(0, ok0);
     load(1);
@@ -782,8 +781,9 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
         const uint32_t j0 = k0 + (uint32_t)t * TK;
         load(t + 3);
         calm = j0 + 2 * TK <= wall && ok1 == ~0ull && within(b1);
-        ok0 = ok1, ok1 = ok2, ok2 = ok3, ok3 = put_slots(t + 4, sl_next);
-        sl_next = slot_at(t + 5);
+        ok0 = ok1, ok1 = ok2, ok2 = ok_of(t + 3);
+        if (((t + 4) & (TW - 1)) == wave) put_slots(t + 4, sl_next);
+        if (((t + 5) & (TW - 1)) == wave) sl_next = slot_at(t + 5);
         const int b = b0;
         b0 = b1, b1 = b2, b2 = b;
         barrier();
@@ -838,9 +838,10 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
         v4i kf[NS], vf[2][NJ], pf[PARTS], pg[PARTS];
         kc[0] = kc_, vs[0] = vs_, kf[0] = ka_[0], kf[1] = ka_[1];
         // Key register e: its weight's exponential, then (one product later) the rest.
+        const float ref = dead ? 0.0f : m;  // (finite where not dead: mleast is)
         float w[16];
         auto at = [](const float4& v, int i) -> float { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; };
-        auto raise = [&](int e) { w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], at(kc[e >> 2], e & 3), -m)); };
+        auto raise = [&](int e) { w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], at(kc[e >> 2], e & 3), -ref)); };
         auto finish = [&](int e) {
             l = l + w[e];
             x[e] = w[e] * at(vs[e >> 2], e & 3);
