@@ -309,6 +309,7 @@ extern "C" int bh_paged_kv_evict_i8(void* stream, const bh_kv8* kv, const uint32
                     sink, recent, acc_stride);
     if (batch == 0) return BH_OK;
     if (!seq_lens || !acc || !keep || !new_lens) return fail(BH_ERR_INVALID, "%s: null buffer", who);
+    if (out_tables && out_max_blocks == 0) return fail(BH_ERR_INVALID, "%s: out_max_blocks 0", who);
     if (acc_out && (acc_out_stride < std::min(budget, acc_stride) || (acc_out == acc && acc_out_stride != acc_stride)))
         return fail(BH_ERR_INVALID, "%s: rows of %u in acc_out for a budget of %u (acc_stride %u)", who, acc_out_stride,
                     budget, acc_stride);

@@ -14,6 +14,23 @@ namespace bh {
 
 constexpr uint32_t NO_SLOT = 0xffffffffu;
 
+// n / d for n < 2^31 without the division's dozen dependent steps: for d no
+// power of two the upper half of n * m, m = ceil(2^(31 + l) / d) with
+// l = ceil(log2 d), shifted by l - 1; n m / 2^(31 + l) is above n / d by less
+// than 1 / d then (n < 2^31, m 2^-(31 + l) above 1 / d by less than 2^-(31 + l)).
+struct Div {
+    uint32_t m, s;  // m = 0: a shift
+    static Div by(uint32_t d) {
+        uint32_t l = 0;
+        while (l < 32 && (1ull << l) < d) ++l;
+        if ((1ull << l) == d) return Div{0, l};
+        return Div{(uint32_t)(((1ull << (31 + l)) + d - 1) / d), l - 1};
+    }
+    __host__ __device__ __forceinline__ uint32_t of(uint32_t n) const {
+        return (m ? (uint32_t)(((uint64_t)n * m) >> 32) : n) >> s;
+    }
+};
+
 // A bh_kv8 whose geometry has been checked. Slots from `nslots` on lie outside
 // the pool or the scales: a table entry that names one is skipped.
 struct Kv8 {
@@ -21,15 +38,14 @@ struct Kv8 {
     float* scales[2];
     const uint32_t* bt;
     uint32_t max_bt, bs, nkv, hd, nslots;
-    int bs_shift;  // log2(bs), or -1
+    Div by_bs;
 
-    __device__ __forceinline__ uint32_t block_of(uint32_t j) const { return bs_shift >= 0 ? j >> bs_shift : j / bs; }
-    // Slot of position j of sequence b in a table of `cols` entries a row.
+    // Slot of position j of sequence b in a table of `cols` > 0 entries a row.
+    // (Unconditional: the load is at an entry of the row in any case.)
     __device__ __forceinline__ uint32_t slot_in(const uint32_t* tables, uint32_t cols, uint32_t b, uint32_t j) const {
-        const uint32_t blk = block_of(j);
-        if (blk >= cols) return NO_SLOT;
-        const uint64_t s = (uint64_t)tables[(uint64_t)b * cols + blk] * bs + (j - blk * bs);
-        return s < nslots ? (uint32_t)s : NO_SLOT;
+        const uint32_t blk = by_bs.of(j & 0x7fffffffu);
+        const uint64_t s = (uint64_t)tables[(uint64_t)b * cols + min(blk, cols - 1)] * bs + (j - blk * bs);
+        return blk < cols && j < 0x80000000u && s < nslots ? (uint32_t)s : NO_SLOT;
     }
     __device__ __forceinline__ uint32_t slot(uint32_t b, uint32_t j) const { return slot_in(bt, max_bt, b, j); }
     __device__ __forceinline__ size_t row(uint32_t slot) const { return (size_t)slot * (nkv * hd); }  // bytes

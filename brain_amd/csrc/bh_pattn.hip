@@ -20,13 +20,14 @@ struct AttnArgs {
     Kv8 kv;
     Kv8Rows bt;
     uint32_t nh, group;
+    Div by_group, by_nsplit, by_nkv;
     float scale2;  // scale * log2(e): softmax in base 2
     // The matrix kernels: blocks of query vectors, splits of the keys, what the
     // splits leave for the join.
     uint32_t blocks, nsplit, span;  // span: keys of a split
     float* part;                    // [unit][kv head][vectors][hd], then
     float2* ml;                     // [unit][kv head][vectors] maximum and sum
-    uint32_t qvec, ovec;            // queries and outputs lie at multiples of 4 elements
+    uint32_t ovec;                  // outputs lie at multiples of 4 elements
 };
 struct SumsArgs {
     const void* q;
@@ -36,8 +37,9 @@ struct SumsArgs {
     Kv8 kv;
     Kv8Rows bt;
     uint32_t nh, group, cap;
+    Div by_group, by_nchunk, by_nkv;
     float scale2;
-    uint32_t qvec, nchunk;  // as AttnArgs; workgroups of a (sequence, kv head)
+    uint32_t nchunk;  // workgroups of a (sequence, kv head)
 };
 
 __device__ __forceinline__ float code_f(uint32_t w, int e) { return (float)(int8_t)(uint8_t)(w >> (8 * e)); }
@@ -179,19 +181,14 @@ __device__ __forceinline__ v4i codes8(uint32_t lo, uint32_t hi) {
 __device__ __forceinline__ v4f mfma16(v4i a, v4i b, v4f c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
 }
-// Eight elements of a query from d on.
-template <class T>
-__device__ __forceinline__ void query8(const typename T::elem* p, bool vec, float (&x)[8]) {
-    if (vec) {
-        float a[4], b[4];
-        T::get4(p, a);
-        T::get4(p + 4, b);
+// N times eight elements of a query, the n-th from p + at(n) on. (Wide loads all
+// the same: the hardware takes them at any element's address.)
+template <class T, int N, class At>
+__device__ __forceinline__ void query8(const typename T::elem* p, float (&x)[N][8], At at) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
-    } else {
+    for (int n = 0; n < N; ++n)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = T::get(p + i);
-    }
+        for (int i = 0; i < 8; ++i) x[n][i] = T::get(p + at(n) + i);
 }
 
 // Where a workgroup works: sequence b, VB of its query vectors from v0 on (of
@@ -202,17 +199,31 @@ struct Block {
     uint32_t b, r0, n, v0, nv, len;
 };
 template <int VB>
+__device__ __forceinline__ uint32_t block_at(const Kv8Rows& bt, uint32_t group, uint32_t b, uint32_t r0) {
+    return !bt.start && group <= VB ? b : r0 * group / VB + b;  // (without row_start and within VB: one block each)
+}
+template <int VB>
 __device__ __forceinline__ bool find_block(const Kv8Rows& bt, uint32_t group, uint32_t blk, uint32_t lane, Block& o) {
-    uint32_t b;
-    if (!bt.start && group <= VB) b = blk;  // one block each
-    else b = wave_last(bt.batch, lane, [&](uint32_t i) { return bt.first(i) * group / VB + i <= blk; });
-    b = __builtin_amdgcn_readfirstlane((int)b);
-    if (b >= bt.batch) return false;
-    const uint32_t r0 = bt.first(b), r1 = bt.end(b);
+    uint32_t b, r0, r1;
+    if (bt.start && bt.batch < 64) {  // one round trip: lane i has row_start[i] and sequence i's length
+        const uint32_t st = min(bt.start[min(lane, bt.batch)], bt.rows), ln = bt.lens[min(lane, bt.batch - 1)];
+        asm volatile("" ::"v"(ln));  // both on their way before the branch
+        const unsigned long long m = __ballot(lane < bt.batch && st * group / VB + lane <= blk);
+        if (!m) return false;
+        b = 63u - (uint32_t)__builtin_clzll(m);
+        r0 = (uint32_t)__builtin_amdgcn_readlane((int)st, (int)b);
+        r1 = (uint32_t)__builtin_amdgcn_readlane((int)st, (int)b + 1);
+        o.len = (uint32_t)__builtin_amdgcn_readlane((int)ln, (int)b);
+    } else {
+        if (!bt.start && group <= VB) b = blk;
+        else b = wave_last(bt.batch, lane, [&](uint32_t i) { return bt.first(i) * group / VB + i <= blk; });
+        b = __builtin_amdgcn_readfirstlane((int)b);
+        if (b >= bt.batch) return false;
+        r0 = bt.first(b), r1 = bt.end(b), o.len = bt.lens[b];
+    }
     if (r1 <= r0) return false;
     o.b = b, o.r0 = r0, o.n = r1 - r0, o.nv = o.n * group;
-    o.v0 = !bt.start && group <= VB ? 0 : (blk - (r0 * group / VB + b)) * VB;
-    o.len = bt.lens[b];
+    o.v0 = (blk - block_at<VB>(bt, group, b, r0)) * VB;
     return o.v0 < o.nv;
 }
 // The number of keys that row i of a block's sequence sees.
@@ -240,33 +251,18 @@ __global__ __launch_bounds__(SW * 64, (stream_waves<T, HD, NQ>())) void paged_at
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // All kv heads of a unit run on one XCD (workgroups go round the eight):
     // their scales share cache lines.
-    const uint32_t nkv = p.kv.nkv, unit = blockIdx.x / (8 * nkv) * 8 + blockIdx.x % 8, kvh = blockIdx.x / 8 % nkv;
+    const uint32_t nkv = p.kv.nkv, turn = p.by_nkv.of(blockIdx.x / 8), unit = turn * 8 + blockIdx.x % 8, kvh = blockIdx.x / 8 - turn * nkv;
     if (unit >= p.blocks * p.nsplit) return;
-    const uint32_t split = unit % p.nsplit;
+    const uint32_t blk = p.by_nsplit.of(unit), split = unit - blk * p.nsplit;
     Block bl;
-    if (!find_block<VB>(p.bt, p.group, unit / p.nsplit, lane, bl)) return;
+    if (!find_block<VB>(p.bt, p.group, blk, lane, bl)) return;
     const uint32_t reach = (uint32_t)min((uint64_t)p.kv.max_bt * p.kv.bs, (uint64_t)0x7fff0000u);
     const uint32_t vend = min(bl.v0 + VB, bl.nv);
-    const uint32_t kend = min(keys_seen(bl, (vend - 1) / p.group), reach);  // keys that any of the vectors sees
-    const uint32_t kall = min(keys_seen(bl, bl.v0 / p.group), reach);       // ... that all see
+    const uint32_t kend = min(keys_seen(bl, p.by_group.of(vend - 1)), reach);  // keys that any of the vectors sees
+    const uint32_t kall = min(keys_seen(bl, p.by_group.of(bl.v0)), reach);       // ... that all see
     const uint32_t k0 = split * p.span, k1 = split + 1 == p.nsplit ? kend : min(kend, k0 + p.span);
     if (k0 >= k1 && split) return;
 
-    // Queries: fragment (t, half) holds d = 16 (g + 4t) + 8 half ..+7 of vector c.
-    v4i qf[NQ][2 * KT][PARTS];
-    uint32_t seen[NQ];
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-        const uint32_t v = min(bl.v0 + 16 * q + c, vend - 1), i = v / p.group, h = kvh * p.group + v % p.group;
-        seen[q] = bl.v0 + 16 * q + c < vend ? min(keys_seen(bl, i), reach) : 0u;
-        const E* src = (const E*)p.q + (bl.r0 + i) * p.qs + (uint64_t)h * HD;
-#pragma unroll
-        for (int t = 0; t < 2 * KT; ++t) {
-            float x[8];
-            query8<T>(src + 16 * (g + 4 * (t >> 1)) + 8 * (t & 1), p.qvec, x);
-            split8<PARTS>(x, qf[q][t]);
-        }
-    }
     v4f o[NQ][HD / 16];
     float m[NQ], l[NQ];
 #pragma unroll
@@ -280,27 +276,32 @@ __global__ __launch_bounds__(SW * 64, (stream_waves<T, HD, NQ>())) void paged_at
     const uint8_t* kp = (const uint8_t*)p.kv.pool[0] + (size_t)kvh * HD;
     const uint8_t* vp = (const uint8_t*)p.kv.pool[1] + (size_t)kvh * HD;
     const float* sp = (lane < 32 ? p.kv.scales[0] : p.kv.scales[1]) + kvh;  // half the lanes take the keys' scales
-    const uint32_t* tb = p.kv.bt + (uint64_t)bl.b * p.kv.max_bt;
-    // Slots of the 32 keys from j on. B16: the blocks hold whole groups of 16
-    // keys (and the pool as well), so two uniform slots say where all are;
-    // else lane l has that of key l % 32. ok: which of the keys have a slot.
+    const uint32_t first = k0 + 32 * wave, step = 32 * SW;
+    // Slots of the 32 keys of the wave's i-th tile. B16: the blocks hold whole
+    // groups of 16 keys (and the pool as well), so two slots say where all are;
+    // lane l looks those of tile l up, 64 tiles at a time (a look-up for each
+    // tile would be waited for, tile by tile). Else lane l has that of key l % 32.
+    // ok: which of the keys have a slot.
     struct Slots {
         uint32_t s0, s1, ok;
     };
-    auto slots_of = [&](uint32_t j) -> Slots {
+    uint32_t mine0 = NO_SLOT, mine1 = NO_SLOT;
+    auto slots_of = [&](uint32_t i) -> Slots {
         Slots r{0, 0, 0};
         if constexpr (B16) {
-            auto group = [&](uint32_t ju) -> uint32_t {
-                if (ju >= kend) return NO_SLOT;
-                const uint32_t blk = p.kv.block_of(ju);
-                const uint64_t s = (uint64_t)tb[blk] * p.kv.bs + (ju - blk * p.kv.bs);
-                return s < p.kv.nslots ? (uint32_t)s : NO_SLOT;
-            };
-            const uint32_t a = group(j), b = group(j + 16);
+            if ((i & 63) == 0) {
+                const uint32_t j = first + (i + lane) * step;
+                uint32_t a = p.kv.slot(bl.b, j), b = p.kv.slot(bl.b, j + 16);
+                asm volatile("" : "+v"(a), "+v"(b));  // both look-ups, then the comparisons
+                mine0 = j < k1 ? a : NO_SLOT;
+                mine1 = j + 16 < k1 ? b : NO_SLOT;
+            }
+            const uint32_t a = (uint32_t)__builtin_amdgcn_readlane((int)mine0, (int)(i & 63));
+            const uint32_t b = (uint32_t)__builtin_amdgcn_readlane((int)mine1, (int)(i & 63));
             r.s0 = a != NO_SLOT ? a : 0u, r.s1 = b != NO_SLOT ? b : 0u;
             r.ok = (a != NO_SLOT ? 0xffffu : 0u) | (b != NO_SLOT ? 0xffff0000u : 0u);
         } else {
-            const uint32_t jl = j + (lane & 31), s = jl < kend ? p.kv.slot(bl.b, jl) : NO_SLOT;
+            const uint32_t j = first + i * step + (lane & 31), s = j < k1 ? p.kv.slot(bl.b, j) : NO_SLOT;
             r.s0 = s != NO_SLOT ? s : 0u;
             r.ok = (uint32_t)__ballot(s != NO_SLOT);
         }
@@ -332,16 +333,32 @@ __global__ __launch_bounds__(SW * 64, (stream_waves<T, HD, NQ>())) void paged_at
                 vc[e][0] = *reinterpret_cast<const uint32_t*>(v);
             }
         }
-        sc = sp[B16 ? (size_t)((lane & 16 ? at.s1 : at.s0) + c) * nkv : (size_t)at.s0 * nkv];
+        const uint32_t a0 = at.s0, a1 = B16 ? at.s1 : 0u;
+        sc = sp[(size_t)(B16 ? (lane & 16 ? a1 : a0) + c : a0) * nkv];
     };
-    const uint32_t first = k0 + 32 * wave, step = 32 * SW;
-    Slots at{0, 0, 0}, next{0, 0, 0};
-    if (first < k1) {
-        at = slots_of(first);
-        load_k(at);
-        load_v(at);
-        next = slots_of(first + step);
+    // The look-ups, the queries and the first tile go out before anything waits
+    // for the queries.
+    Slots at = slots_of(0);
+    // Queries: fragment (t, half) holds d = 16 (g + 4t) + 8 half ..+7 of vector c.
+    v4i qf[NQ][2 * KT][PARTS];
+    float qx[NQ][2 * KT][8];
+    uint32_t seen[NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        const uint32_t v = min(bl.v0 + 16 * q + c, vend - 1), i = p.by_group.of(v), h = kvh * p.group + (v - i * p.group);
+        seen[q] = bl.v0 + 16 * q + c < vend ? min(keys_seen(bl, i), reach) : 0u;
+        const E* src = (const E*)p.q + (bl.r0 + i) * p.qs + (uint64_t)h * HD;
+        query8<T>(src, qx[q], [&](int t) { return 16 * (g + 4 * (t >> 1)) + 8 * (t & 1); });
     }
+    load_k(at);
+    load_v(at);
+    Slots next = slots_of(1);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int q = 0; q < NQ; ++q)
+#pragma unroll
+        for (int t = 0; t < 2 * KT; ++t) split8<PARTS>(qx[q][t], qf[q][t]);
+    uint32_t tile = 2;  // the one whose slots come next
 #pragma unroll 1
     for (uint32_t j0 = first; j0 < k1; j0 += step) {
         const bool more = j0 + step < k1;
@@ -377,7 +394,7 @@ __global__ __launch_bounds__(SW * 64, (stream_waves<T, HD, NQ>())) void paged_at
         if (more) {
             load_k(next);
             at = next;
-            next = slots_of(j0 + 2 * step);
+            next = slots_of(tile++);
         }
         __builtin_amdgcn_wave_barrier();
         float ks[8], vs[8];
@@ -498,7 +515,8 @@ __global__ __launch_bounds__(SW * 64, (stream_waves<T, HD, NQ>())) void paged_at
                 *reinterpret_cast<float4*>(p.part + at * HD + d0 + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
             if (d0 == 0) p.ml[at] = make_float2(mm, ll);
         } else {
-            const uint64_t row = (uint64_t)(bl.r0 + v / p.group) * p.nh + kvh * p.group + v % p.group;
+            const uint32_t i = p.by_group.of(v);
+            const uint64_t row = (uint64_t)(bl.r0 + i) * p.nh + kvh * p.group + (v - i * p.group);
             E* dst = (E*)p.out + row * HD + d0;
 #pragma unroll
             for (int i = 0; i < DT; ++i) T::put(dst + i, ll == 0.0f ? 0.0f : acc[i] / ll);
@@ -550,16 +568,16 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t nkv = p.kv.nkv, kvs = nkv * HD, units = p.blocks * p.nsplit;
-    uint32_t unit = blockIdx.x / (8 * nkv) * 8 + blockIdx.x % 8;
-    const uint32_t kvh = blockIdx.x / 8 % nkv;
+    const uint32_t turn = p.by_nkv.of(blockIdx.x / 8), kvh = blockIdx.x / 8 - turn * nkv;
+    uint32_t unit = turn * 8 + blockIdx.x % 8;
     if (unit >= units) return;
     unit = units - 1 - unit;  // a chunk's last rows see the most keys: they start first
-    const uint32_t split = unit % p.nsplit;
+    const uint32_t blk = p.by_nsplit.of(unit), split = unit - blk * p.nsplit;
     Block bl;
-    if (!find_block<TVB>(p.bt, p.group, unit / p.nsplit, lane, bl)) return;
+    if (!find_block<TVB>(p.bt, p.group, blk, lane, bl)) return;
     const uint32_t reach = (uint32_t)min((uint64_t)p.kv.max_bt * p.kv.bs, (uint64_t)0x7fff0000u);
     const uint32_t vend = min(bl.v0 + TVB, bl.nv);
-    const uint32_t kend = min(keys_seen(bl, (vend - 1) / p.group), reach);
+    const uint32_t kend = min(keys_seen(bl, p.by_group.of(vend - 1)), reach);
     const uint32_t k0 = split * p.span, k1 = split + 1 == p.nsplit ? kend : min(kend, k0 + p.span);
     if (k0 >= k1 && split) return;
     const int nt = k1 > k0 ? (int)((k1 - k0 + TK - 1) / TK) : 0;
@@ -567,24 +585,24 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
     // This wave's 32 vectors, and what its first and last see.
     const uint32_t wv0 = bl.v0 + 32 * wave, wv1 = min(wv0 + 32, vend);
     const bool wlive = wv0 < vend;
-    const uint32_t wall = wlive ? min(keys_seen(bl, wv0 / p.group), reach) : 0u;
-    const uint32_t wend = wlive ? min(keys_seen(bl, (wv1 - 1) / p.group), reach) : 0u;
+    const uint32_t wall = wlive ? min(keys_seen(bl, p.by_group.of(wv0)), reach) : 0u;
+    const uint32_t wend = wlive ? min(keys_seen(bl, p.by_group.of(wv1 - 1)), reach) : 0u;
     uint32_t seen;
     float qn;
     const bool dead = wv0 + col >= vend;  // no vector: computes the last one's again, its sums are not used
     v4i qf[HD / 16][PARTS];  // step t: d = 16 t + 8 half ..+7 of vector col
     {
-        const uint32_t v = min(wv0 + col, vend - 1), i = v / p.group, h = kvh * p.group + v % p.group;
+        const uint32_t v = min(wv0 + col, vend - 1), i = p.by_group.of(v), h = kvh * p.group + (v - i * p.group);
         seen = wv0 + col < vend ? min(keys_seen(bl, i), reach) : 0u;
         const E* src = (const E*)p.q + (bl.r0 + i) * p.qs + (uint64_t)h * HD + 8 * half;
         qn = 0.0f;
+        float x[HD / 16][8];
+        query8<T>(src, x, [](int t) { return 16 * t; });
 #pragma unroll
         for (int t = 0; t < HD / 16; ++t) {
-            float x[8];
-            query8<T>(src + 16 * t, p.qvec, x);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) qn = qn + x[e] * x[e];
-            split8<PARTS>(x, qf[t]);
+            for (int e = 0; e < 8; ++e) qn = qn + x[t][e] * x[t][e];
+            split8<PARTS>(x[t], qf[t]);
         }
         // Above |q|, whatever the roundings; infinite or NaN (no bound: a NaN here
         // would be lost in the maximum) becomes infinite.
@@ -953,7 +971,8 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
         if (half == 0) p.ml[at] = make_float2(m, l);
         return;
     }
-    const uint64_t row = (uint64_t)(bl.r0 + v / p.group) * p.nh + kvh * p.group + v % p.group;
+    const uint32_t iv = p.by_group.of(v);
+    const uint64_t row = (uint64_t)(bl.r0 + iv) * p.nh + kvh * p.group + (v - iv * p.group);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     E* dst = (E*)p.out + row * HD;
 #pragma unroll
@@ -969,40 +988,56 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
     if (p.lse && half == 0) p.lse[row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
 }
 
-// Joins the splits of a vector: one wave for each vector of a block.
+// Joins the splits of a row and head, one wave for each: lane s takes split s's
+// maximum and sum (at most 64 splits), then all take their dimensions.
 template <class T, int HD, int VB>
 __global__ __launch_bounds__(256) void paged_attention_join_kernel(AttnArgs p) {
     typedef typename T::elem E;
     const uint32_t lane = threadIdx.x & 63, nkv = p.kv.nkv;
-    const uint32_t bk = blockIdx.x / (VB / 4), blk = bk / nkv, kvh = bk % nkv;
-    const uint32_t u = (blockIdx.x % (VB / 4)) * 4 + (threadIdx.x >> 6);
+    const uint32_t rh = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
+    const uint32_t r = rh / p.nh, h = rh % p.nh, kvh = h / p.group;
+    if (r >= p.bt.rows) return;
+    uint32_t b = r;
+    if (p.bt.start) b = wave_last(p.bt.batch, lane, [&](uint32_t i) { return p.bt.start[i] <= r; });
+    b = __builtin_amdgcn_readfirstlane((int)b);
+    if (b >= p.bt.batch) return;
     Block bl;
-    if (!find_block<VB>(p.bt, p.group, blk, lane, bl)) return;
-    const uint32_t v = bl.v0 + u;
-    if (v >= bl.nv) return;
+    bl.b = b, bl.r0 = p.bt.first(b);
+    const uint32_t r1 = p.bt.end(b);
+    if (r >= r1) return;
+    bl.n = r1 - bl.r0, bl.nv = bl.n * p.group, bl.len = p.bt.lens[b];
+    const uint32_t v = (r - bl.r0) * p.group + h % p.group, blk = block_at<VB>(p.bt, p.group, b, bl.r0) + v / VB;
     const uint32_t reach = (uint32_t)min((uint64_t)p.kv.max_bt * p.kv.bs, (uint64_t)0x7fff0000u);
-    const uint32_t kend = min(keys_seen(bl, (min(bl.v0 + VB, bl.nv) - 1) / p.group), reach);
-    const uint32_t live = max(1u, min(p.nsplit, (kend + p.span - 1) / p.span));  // splits that had keys
-    const uint64_t at = ((uint64_t)blk * p.nsplit * nkv + kvh) * VB + u, far = (uint64_t)nkv * VB;
-    float mm = -INFINITY, ll = 0.0f, acc[HD / 64];
-    for (uint32_t s = 0; s < live; ++s) mm = fmaxf(mm, p.ml[at + s * far].x);
-    const float ref = mm == -INFINITY ? 0.0f : mm;
+    const uint32_t kend = min(keys_seen(bl, (min((v / VB + 1) * VB, bl.nv) - 1) / p.group), reach);  // of the vector's block
+    const uint32_t live = max(1u, min(p.nsplit, (kend + p.span - 1) / p.span));                  // splits that had keys
+    const uint64_t at = ((uint64_t)blk * p.nsplit * nkv + kvh) * VB + v % VB, far = (uint64_t)nkv * VB;
+    const float2 ml = lane < live ? p.ml[at + lane * far] : make_float2(-INFINITY, 0.0f);
+    const float mm = xor_max<32>(ml.x), ref = mm == -INFINITY ? 0.0f : mm;
+    const float a = __builtin_amdgcn_exp2f(ml.x - ref);
+    const float ll = xor_sum<32>(lane < live ? ml.y * a : 0.0f);
+    constexpr int DL = HD / 64;
+    float acc[DL];
 #pragma unroll
-    for (int i = 0; i < HD / 64; ++i) acc[i] = 0.0f;
-#pragma unroll 4
-    for (uint32_t s = 0; s < live; ++s) {
-        const float2 x = p.ml[at + s * far];
-        const float a = __builtin_amdgcn_exp2f(x.x - ref);
-        ll = ll + x.y * a;
-        const float* src = p.part + (at + s * far) * HD + lane * (HD / 64);
+    for (int i = 0; i < DL; ++i) acc[i] = 0.0f;
+    const float* src = p.part + at * HD + lane * DL;
+    for (uint32_t s0 = 0; s0 < live; s0 += 8) {
+        float x[8][DL];
 #pragma unroll
-        for (int i = 0; i < HD / 64; ++i) acc[i] = acc[i] + src[i] * a;
+        for (int u = 0; u < 8; ++u)
+#pragma unroll
+            for (int i = 0; i < DL; ++i) x[u][i] = src[min(s0 + u, live - 1) * far * HD + i];
+        __builtin_amdgcn_sched_barrier(0);  // all on their way
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, a), (int)min(s0 + u, 63u)));
+#pragma unroll
+            for (int i = 0; i < DL; ++i) acc[i] = s0 + u < live ? acc[i] + x[u][i] * w : acc[i];
+        }
     }
-    const uint64_t row = (uint64_t)(bl.r0 + v / p.group) * p.nh + kvh * p.group + v % p.group;
-    E* dst = (E*)p.out + row * HD + lane * (HD / 64);
+    E* dst = (E*)p.out + (uint64_t)rh * HD + lane * DL;
 #pragma unroll
-    for (int i = 0; i < HD / 64; ++i) T::put(dst + i, ll == 0.0f ? 0.0f : acc[i] / ll);
-    if (p.lse && lane == 0) p.lse[row] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * LN2;
+    for (int i = 0; i < DL; ++i) T::put(dst + i, ll == 0.0f ? 0.0f : acc[i] / ll);
+    if (p.lse && lane == 0) p.lse[rh] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * LN2;
 }
 
 // ---------------------------------------------------------------- weight sums
@@ -1023,10 +1058,10 @@ __global__ __launch_bounds__(256, 2) void paged_weight_sums_kernel(SumsArgs p) {
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // All kv heads of a unit on one XCD: their scales share cache lines.
-    const uint32_t nkv = p.kv.nkv, unit = blockIdx.x / (8 * nkv) * 8 + blockIdx.x % 8, kvh = blockIdx.x / 8 % nkv;
+    const uint32_t nkv = p.kv.nkv, turn = p.by_nkv.of(blockIdx.x / 8), unit = turn * 8 + blockIdx.x % 8, kvh = blockIdx.x / 8 - turn * nkv;
     if (unit >= p.bt.batch * p.nchunk) return;
     Block bl;
-    bl.b = unit / p.nchunk;
+    bl.b = p.by_nchunk.of(unit);
     const uint32_t r1 = p.bt.end(bl.b);
     bl.r0 = p.bt.first(bl.b);
     bl.n = r1 > bl.r0 ? r1 - bl.r0 : 0u;
@@ -1037,7 +1072,7 @@ __global__ __launch_bounds__(256, 2) void paged_weight_sums_kernel(SumsArgs p) {
     // A thread brings HD / 8 elements of vector tid / 8 of a tile.
     constexpr int QE = HD / 8;
     const int qv = tid >> 3, qd = (tid & 7) * QE;
-    for (uint64_t j0 = (uint64_t)(unit % p.nchunk) * (64 * KG); j0 < end; j0 += (uint64_t)p.nchunk * (64 * KG)) {
+    for (uint64_t j0 = (uint64_t)(unit - bl.b * p.nchunk) * (64 * KG); j0 < end; j0 += (uint64_t)p.nchunk * (64 * KG)) {
         // Keys: group k of the wave, key c of it.
         v4i kf[KG][2 * HD / 64];
         float kc[KG], sum[KG], old[KG];
@@ -1061,29 +1096,20 @@ __global__ __launch_bounds__(256, 2) void paged_weight_sums_kernel(SumsArgs p) {
         // The first row that sees the first key, from a whole tile on.
         const uint64_t i0 = j0 + bl.n > bl.len ? j0 + bl.n - bl.len : 0;
         const uint32_t v0 = (uint32_t)min(i0 * p.group, (uint64_t)bl.nv) / TQ * TQ;
-        float x[QE], xl = 0.0f;
+        float x[QE / 8][8], xl = 0.0f;
         uint32_t xs = 0;
         auto load = [&](uint32_t v) {
-            const uint32_t vv = min(v + qv, bl.nv - 1), i = vv / p.group, h = kvh * p.group + vv % p.group;
+            const uint32_t vv = min(v + qv, bl.nv - 1), i = p.by_group.of(vv), h = kvh * p.group + (vv - i * p.group);
             const E* src = (const E*)p.q + (bl.r0 + i) * p.qs + (uint64_t)h * HD + qd;
-#pragma unroll
-            for (int u = 0; u < QE; u += 8) {
-                float y[8];
-                query8<T>(src + u, p.qvec, y);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[u + e] = y[e];
-            }
+            query8<T>(src, x, [](int n) { return 8 * n; });
             xl = p.lse[(uint64_t)(bl.r0 + i) * p.nh + h] * LOG2E;
             xs = v + qv < bl.nv ? keys_seen(bl, i) : 0u;
         };
         auto store = [&](int bu) {
 #pragma unroll
             for (int u = 0; u < QE; u += 8) {
-                float y[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = x[u + e];
                 v4i f[PARTS];
-                split8<PARTS>(y, f);
+                split8<PARTS>(x[u / 8], f);
 #pragma unroll
                 for (int part = 0; part < PARTS; ++part)
                     *reinterpret_cast<v4i*>(&qt[bu][part][kchunk(qv, (qd + u) / 8)]) = f[part];
@@ -1102,7 +1128,7 @@ __global__ __launch_bounds__(256, 2) void paged_weight_sums_kernel(SumsArgs p) {
             const bool more = v + TQ < bl.nv;
             if (more) load(v + TQ);
             // Every vector of the tile sees every key of the wave.
-            const bool masked = v + TQ > bl.nv || keys_seen(bl, v / p.group) < (uint64_t)jw + 16 * KG;
+            const bool masked = v + TQ > bl.nv || keys_seen(bl, p.by_group.of(v)) < (uint64_t)jw + 16 * KG;
 #pragma unroll
             for (int sub = 0; sub < 2; ++sub) {
                 v4f s[KG];
@@ -1153,6 +1179,7 @@ template <class T, int HD, int KG>
 hipError_t go_sums(hipStream_t s, SumsArgs a, uint64_t len) {
     const uint64_t most = std::max<uint64_t>(1, 0x7fffffffull / 8 / a.kv.nkv / a.bt.batch);
     a.nchunk = (uint32_t)std::min<uint64_t>((len + 64 * KG - 1) / (64 * KG), most);
+    a.by_nchunk = Div::by(a.nchunk);
     const uint64_t grid = ((uint64_t)a.bt.batch * a.nchunk + 7) / 8 * 8 * a.kv.nkv;
     if (grid > 0x7fffffffull) return hipErrorInvalidConfiguration;
     paged_weight_sums_kernel<T, HD, KG><<<(unsigned)grid, 256, 0, s>>>(a);
@@ -1198,10 +1225,10 @@ Plan plan_attention(const Kv8& kv, const Kv8Rows& bt, const bh_kv8_batch* hint, 
     const uint64_t rounds = (len + round - 1) / round;
     uint64_t wgs = (uint64_t)r.blocks * kv.nkv, want;
     if (r.kind == STREAM) {
-        want = std::min<uint64_t>({rounds, (4 * CUS + wgs - 1) / wgs, 64});
+        want = std::min<uint64_t>({rounds, (16 * CUS + wgs - 1) / wgs, 64});
     } else {
         wgs = std::max<uint64_t>(1, all / r.vb) * kv.nkv;
-        want = std::min<uint64_t>({(rounds + 1) / 2, (2 * CUS + wgs - 1) / wgs, 32});
+        want = std::min<uint64_t>({(rounds + 1) / 2, (3 * CUS + wgs - 1) / wgs, 32});
         if (wgs * 4 >= 3 * CUS) want = 1;
     }
     want = std::max<uint64_t>(1, want);
@@ -1217,7 +1244,7 @@ Plan plan_attention(const Kv8& kv, const Kv8Rows& bt, const bh_kv8_batch* hint, 
 template <class T, int HD, int VB>
 hipError_t go_matrix(hipStream_t s, const AttnArgs& a, bool b16) {
     const uint64_t units = ((uint64_t)a.blocks * a.nsplit + 7) / 8 * 8 * a.kv.nkv;
-    const uint64_t joins = (uint64_t)a.blocks * a.kv.nkv * (VB / 4);
+    const uint64_t joins = ((uint64_t)a.bt.rows * a.nh + 3) / 4;
     if (units > 0x7fffffffull || joins > 0x7fffffffull) return hipErrorInvalidConfiguration;
     if constexpr (VB > 32) paged_attention_tile_kernel<T, HD><<<(unsigned)units, TW * 64, 0, s>>>(a);
     else if (b16) paged_attention_stream_kernel<T, HD, VB / 16, true><<<(unsigned)units, SW * 64, 0, s>>>(a);
@@ -1300,15 +1327,16 @@ extern "C" int bh_paged_attention_i8(void* stream, const void* q, uint64_t q_str
     if (!q || !out) return fail(BH_ERR_INVALID, "%s: null buffer", who);
     a.q = q, a.qs = q_stride, a.out = out, a.lse = lse;
     a.nh = n_heads, a.group = n_heads / kv->n_kv_heads, a.scale2 = scale * LOG2E;
+    a.by_group = Div::by(a.group), a.by_nkv = Div::by(kv->n_kv_heads);
     const Plan pl = plan_attention(a.kv, a.bt, batch, n_heads, dtype);
     const uint64_t need = pl.part_floats * 4 + pl.ml_pairs * 8;
     if (ws_bytes < need || (need && (!ws || !aligned_to(ws, 16))))
         return fail(BH_ERR_INVALID, "%s: a workspace of %llu bytes, 16-byte aligned, is needed, %llu given", who,
                     (unsigned long long)need, (unsigned long long)ws_bytes);
     a.blocks = pl.blocks, a.nsplit = pl.nsplit, a.span = pl.span;
+    if (pl.nsplit) a.by_nsplit = Div::by(pl.nsplit);
     a.part = (float*)ws, a.ml = (float2*)((float*)ws + pl.part_floats);
     const size_t es = dtype == BH_OUT_F32 ? 4 : 2;
-    a.qvec = aligned_to(q, 4 * es) && q_stride % 4 == 0;
     a.ovec = aligned_to(out, 4 * es);
     const hipStream_t s = (hipStream_t)stream;
     return done(dtype == BH_OUT_F32 ? go_attention<F32>(s, a, pl) : go_attention<Bf16>(s, a, pl), who);
@@ -1325,7 +1353,7 @@ extern "C" int bh_paged_weight_sums_i8(void* stream, const void* q, uint64_t q_s
     if (!q || !lse || !acc) return fail(BH_ERR_INVALID, "%s: null buffer", who);
     a.q = q, a.qs = q_stride, a.lse = lse, a.acc = acc, a.cap = acc_stride;
     a.nh = n_heads, a.group = n_heads / kv->n_kv_heads, a.scale2 = scale * LOG2E;
-    a.qvec = aligned_to(q, dtype == BH_OUT_F32 ? 16 : 8) && q_stride % 4 == 0;
+    a.by_group = Div::by(a.group), a.by_nkv = Div::by(kv->n_kv_heads);
     const hipStream_t s = (hipStream_t)stream;
     return done(dtype == BH_OUT_F32 ? go_weight_sums<F32>(s, a, batch) : go_weight_sums<Bf16>(s, a, batch), who);
 }

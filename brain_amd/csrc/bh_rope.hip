@@ -276,16 +276,17 @@ int done(hipError_t e, const char* who) {
 int check_kv8(const char* who, const bh_kv8* kv, Kv8* out) {
     if (!kv) return fail(BH_ERR_INVALID, "%s: no cache", who);
     if (kv->head_dim == 0 || kv->head_dim % 4 || kv->head_dim > 256 || kv->n_kv_heads == 0 || kv->block_size == 0 ||
-        (uint64_t)kv->n_kv_heads * kv->head_dim > 0x7fffffffull)
-        return fail(BH_ERR_INVALID, "%s: head_dim %u (a multiple of 4, <= 256), %u kv heads and block_size %u do not fit",
-                    who, kv->head_dim, kv->n_kv_heads, kv->block_size);
+        kv->max_blocks == 0 || (uint64_t)kv->n_kv_heads * kv->head_dim > 0x7fffffffull)
+        return fail(BH_ERR_INVALID,
+                    "%s: head_dim %u (a multiple of 4, <= 256), %u kv heads, block_size %u and max_blocks %u do not fit", who,
+                    kv->head_dim, kv->n_kv_heads, kv->block_size, kv->max_blocks);
     if (!kv->k_pool || !kv->v_pool || !kv->k_scales || !kv->v_scales || !kv->block_tables)
         return fail(BH_ERR_INVALID, "%s: the cache has a null buffer", who);
     const uint64_t stride = (uint64_t)kv->n_kv_heads * kv->head_dim;
     const uint64_t n = std::min(kv->pool_words / (stride / 4), kv->n_scales / kv->n_kv_heads);
     *out = Kv8{{kv->k_pool, kv->v_pool}, {kv->k_scales, kv->v_scales}, kv->block_tables, kv->max_blocks,
                kv->block_size, kv->n_kv_heads, kv->head_dim, (uint32_t)std::min<uint64_t>(n, NO_SLOT),
-               (kv->block_size & (kv->block_size - 1)) == 0 ? __builtin_ctz(kv->block_size) : -1};
+               Div::by(kv->block_size)};
     return BH_OK;
 }
 

@@ -246,7 +246,7 @@ typedef struct {
                                       table[b][j / block_size] * block_size + j % block_size. An entry that
                                       names a slot outside the pool or the scales is skipped: nothing is
                                       stored there, and a query does not see the key */
-    uint32_t max_blocks, block_size, n_kv_heads, head_dim; /* head_dim % 4 == 0, <= 256 */
+    uint32_t max_blocks, block_size, n_kv_heads, head_dim; /* none 0; head_dim % 4 == 0, <= 256 */
 } bh_kv8;
 
 /* Sequence b has the rows row_start[b] .. row_start[b+1] of the activations

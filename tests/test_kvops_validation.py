@@ -39,7 +39,7 @@ def refused(rc, *words):
 
 BAD_KV = [(dict(head_dim=0), "head_dim 0"), (dict(head_dim=66), "head_dim 66"), (dict(head_dim=260), "head_dim 260"),
           (dict(n_kv_heads=0), "0 kv heads"), (dict(block_size=0), "block_size 0"), (dict(k_pool=None), "null"),
-          (dict(v_scales=None), "null"), (dict(block_tables=None), "null"), (dict(n_kv_heads=1 << 26), "fit")]
+          (dict(v_scales=None), "null"), (dict(block_tables=None), "null"), (dict(max_blocks=0), "max_blocks 0"), (dict(n_kv_heads=1 << 26), "fit")]
 
 
 @pytest.mark.parametrize("change,word", BAD_KV)
@@ -135,6 +135,7 @@ def test_evict():
     refused(call(acc_out=P + 4096, cap_out=7), "acc_out")
     refused(call(acc_out=P, cap_out=32), "acc_out")
     refused(call(n=1 << 30), "grid")
+    refused(call(to=P, cols=0), "out_max_blocks")
     assert call(n=0, lens=None, acc=None, keep=None, new=None) == BH_OK
 
 
