@@ -133,6 +133,8 @@ __global__ __launch_bounds__(64) void paged_weight_sums_any_kernel(SumsArgs p, u
     *dst = old ? *dst + sum : sum;
 }
 
+constexpr uint32_t CUS = 256;  // compute units
+
 // ---------------------------------------------------------------- few rows
 //
 // Up to 32 query vectors (rows x heads of one kv head) of a sequence at a time:
@@ -1175,14 +1177,146 @@ __global__ __launch_bounds__(256, 2) void paged_weight_sums_kernel(SumsArgs p) {
     }
 }
 
+// Few query vectors (rows x heads of a kv head up to 32, or 32 at a time): they
+// stay in LDS and the keys stream by, each wave with the next 64 in flight and no
+// barrier between.
+template <class T, int HD>
+__global__ __launch_bounds__(256, 2) void paged_weight_sums_stream_kernel(SumsArgs p) {
+    typedef typename T::elem E;
+    constexpr int PARTS = sizeof(E) == 4 ? 3 : 1, TQ = 32, ST = HD / 32, PB = TQ * HD * 2, KG = 4;
+    __shared__ __attribute__((aligned(1024))) uint8_t qt[PARTS][PB];
+    __shared__ __attribute__((aligned(16))) float lses[TQ];
+    __shared__ __attribute__((aligned(16))) uint32_t sees[TQ];
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t nkv = p.kv.nkv, turn = p.by_nkv.of(blockIdx.x / 8), unit = turn * 8 + blockIdx.x % 8;
+    const uint32_t kvh = blockIdx.x / 8 - turn * nkv;
+    if (unit >= p.bt.batch * p.nchunk) return;
+    Block bl;
+    bl.b = p.by_nchunk.of(unit);
+    const uint32_t r1 = p.bt.end(bl.b);
+    bl.r0 = p.bt.first(bl.b), bl.len = p.bt.lens[bl.b];
+    if (r1 <= bl.r0) return;
+    bl.n = r1 - bl.r0, bl.nv = bl.n * p.group, bl.v0 = 0;
+    const uint32_t end = min(min(bl.len, p.cap), 0x7fff0000u), kvs = nkv * HD;
+    float* acc = p.acc + ((uint64_t)bl.b * nkv + kvh) * p.cap;
+    auto kchunk = [&](int r, int ch) -> int { return r * (HD * 2) + ((HD == 128 ? ch ^ (r & 15) : ch ^ ((r >> 1) & 7)) << 4); };
+    constexpr int QE = HD / 8;
+    const int qv = tid >> 3, qd = (tid & 7) * QE;
+    const uint32_t first = ((unit - bl.b * p.nchunk) * 4 + wave) * 64, step = p.nchunk * 256;
+    v4i kr[KG][HD / 64];  // codes of the keys in flight: group k of the wave, key c of it, bytes 16 (g + 4 i)
+    float sr[KG], ar[KG];
+    uint32_t slot[KG];
+    auto look = [&](uint32_t j) {
+#pragma unroll
+        for (int k = 0; k < KG; ++k) slot[k] = p.kv.slot(bl.b, j + 16 * k + c);
+    };
+    auto load = [&](uint32_t j) {
+#pragma unroll
+        for (int k = 0; k < KG; ++k) {
+            const uint32_t s = slot[k] != NO_SLOT ? slot[k] : 0u;
+            const uint8_t* src = (const uint8_t*)p.kv.pool[0] + (size_t)s * kvs + kvh * HD + 16 * g;
+#pragma unroll
+            for (int i = 0; i < HD / 64; ++i) kr[k][i] = *reinterpret_cast<const v4i*>(src + 64 * i);
+            sr[k] = p.kv.scales[0][(size_t)s * nkv + kvh];
+            ar[k] = acc[min(j + 16 * k + c, end - 1)];
+        }
+    };
+    for (uint32_t v = 0; v < bl.nv; v += TQ) {
+        if (first < end) {
+            look(first);
+            load(first);
+        }
+        {  // thread: HD / 8 elements of vector tid / 8
+            const uint32_t vv = min(v + qv, bl.nv - 1), i = p.by_group.of(vv), h = kvh * p.group + (vv - i * p.group);
+            const E* src = (const E*)p.q + (bl.r0 + i) * p.qs + (uint64_t)h * HD + qd;
+            float x[QE / 8][8];
+            query8<T>(src, x, [](int n) { return 8 * n; });
+            const float xl = p.lse[(uint64_t)(bl.r0 + i) * p.nh + h] * LOG2E;
+            if (v) __syncthreads();  // the last vectors are done with
+#pragma unroll
+            for (int u = 0; u < QE / 8; ++u) {
+                v4i f[PARTS];
+                split8<PARTS>(x[u], f);
+#pragma unroll
+                for (int part = 0; part < PARTS; ++part) *reinterpret_cast<v4i*>(&qt[part][kchunk(qv, qd / 8 + u)]) = f[part];
+            }
+            if ((tid & 7) == 0) lses[qv] = xl, sees[qv] = v + qv < bl.nv ? keys_seen(bl, i) : 0u;
+        }
+        __syncthreads();
+        const uint32_t all = v + TQ <= bl.nv ? keys_seen(bl, p.by_group.of(v)) : 0u;  // keys that all of the vectors see
+        const int subs = bl.nv - v > 16 ? 2 : 1;
+#pragma unroll 1
+        for (uint32_t j0 = first; j0 < end; j0 += step) {
+            v4i kf[KG][ST];
+            float kc[KG], sum[KG], old[KG];
+            bool live[KG];
+#pragma unroll
+            for (int k = 0; k < KG; ++k) {
+#pragma unroll
+                for (int i = 0; i < HD / 64; ++i) {
+                    asm volatile("" : "+v"(kr[k][i]));  // (else they are carried from step to step byte by byte)
+                    kf[k][2 * i] = codes8((uint32_t)kr[k][i][0], (uint32_t)kr[k][i][1]);
+                    kf[k][2 * i + 1] = codes8((uint32_t)kr[k][i][2], (uint32_t)kr[k][i][3]);
+                }
+                kc[k] = sr[k] * p.scale2, sum[k] = 0.0f, live[k] = slot[k] != NO_SLOT;
+                // The chunk's own keys start from 0, at the first vectors.
+                old[k] = v || (uint64_t)(j0 + 16 * k + c) + bl.n < bl.len ? ar[k] : 0.0f;
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (j0 + step < end) {
+                look(j0 + step);
+                load(j0 + step);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            const bool masked = all < j0 + 64;
+            for (int sub = 0; sub < subs; ++sub) {
+                v4f s[KG];
+#pragma unroll
+                for (int k = 0; k < KG; ++k) s[k] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int part = PARTS - 1; part >= 0; --part)
+#pragma unroll
+                    for (int t = 0; t < ST; ++t) {
+                        const v4i a = *reinterpret_cast<const v4i*>(&qt[part][kchunk(16 * sub + c, 2 * (g + 4 * (t >> 1)) + (t & 1))]);
+#pragma unroll
+                        for (int k = 0; k < KG; ++k) s[k] = mfma16(a, kf[k][t], s[k]);
+                    }
+                const float4 l4 = *reinterpret_cast<const float4*>(&lses[16 * sub + 4 * g]);
+                const uint4 n4 = *reinterpret_cast<const uint4*>(&sees[16 * sub + 4 * g]);
+                const float ll[4] = {l4.x, l4.y, l4.z, l4.w};
+                const uint32_t nn[4] = {n4.x, n4.y, n4.z, n4.w};
+#pragma unroll
+                for (int k = 0; k < KG; ++k)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k][r], kc[k], -ll[r]));
+                        sum[k] = sum[k] + (!masked || j0 + 16 * k + c < nn[r] ? w : 0.0f);
+                    }
+            }
+#pragma unroll
+            for (int k = 0; k < KG; ++k) {
+                float w = sum[k] + xor_lane<16>(sum[k]);
+                w = w + xor_lane<32>(w);
+                const uint32_t j = j0 + 16 * k + c;
+                if (g == k && j < end) acc[j] = (live[k] ? w : 0.0f) + old[k];
+            }
+        }
+    }
+}
+
+// KG 0: the streaming kernel.
 template <class T, int HD, int KG>
 hipError_t go_sums(hipStream_t s, SumsArgs a, uint64_t len) {
-    const uint64_t most = std::max<uint64_t>(1, 0x7fffffffull / 8 / a.kv.nkv / a.bt.batch);
-    a.nchunk = (uint32_t)std::min<uint64_t>((len + 64 * KG - 1) / (64 * KG), most);
-    a.by_nchunk = Div::by(a.nchunk);
+    constexpr uint32_t keys = KG ? 64 * KG : 256;
+    const uint64_t pairs = (uint64_t)a.bt.batch * a.kv.nkv, most = std::max<uint64_t>(1, 0x7fffffffull / 8 / pairs);
+    uint64_t chunks = std::min<uint64_t>((len + keys - 1) / keys, most);
+    if (KG == 0) chunks = std::min<uint64_t>(chunks, (2 * CUS + pairs - 1) / pairs);
+    a.nchunk = (uint32_t)chunks, a.by_nchunk = Div::by(a.nchunk);
     const uint64_t grid = ((uint64_t)a.bt.batch * a.nchunk + 7) / 8 * 8 * a.kv.nkv;
     if (grid > 0x7fffffffull) return hipErrorInvalidConfiguration;
-    paged_weight_sums_kernel<T, HD, KG><<<(unsigned)grid, 256, 0, s>>>(a);
+    if constexpr (KG) paged_weight_sums_kernel<T, HD, KG><<<(unsigned)grid, 256, 0, s>>>(a);
+    else paged_weight_sums_stream_kernel<T, HD><<<(unsigned)grid, 256, 0, s>>>(a);
     return hipGetLastError();
 }
 template <class T>
@@ -1195,6 +1329,8 @@ hipError_t go_weight_sums(hipStream_t s, const SumsArgs& a, const bh_kv8_batch* 
         return hipGetLastError();
     }
     const uint64_t len = std::max<uint64_t>(1, hint->max_len ? std::min(hint->max_len, a.cap) : a.cap);
+    const uint32_t most = a.bt.start ? (hint->max_rows ? std::min(hint->max_rows, a.bt.rows) : a.bt.rows) : 1;
+    if ((uint64_t)most * a.group <= 32) return a.kv.hd == 128 ? go_sums<T, 128, 0>(s, a, len) : go_sums<T, 64, 0>(s, a, len);
     const bool few = (uint64_t)a.bt.batch * a.kv.nkv * ((len + 255) / 256) < 256;
     if (a.kv.hd == 128) return few ? go_sums<T, 128, 1>(s, a, len) : go_sums<T, 128, 4>(s, a, len);
     return few ? go_sums<T, 64, 1>(s, a, len) : go_sums<T, 64, 4>(s, a, len);
@@ -1207,8 +1343,6 @@ struct Plan {
     uint32_t vb, blocks, nsplit, span;  // vb: query vectors of a block
     uint64_t part_floats, ml_pairs;
 };
-constexpr uint32_t CUS = 256;
-
 Plan plan_attention(const Kv8& kv, const Kv8Rows& bt, const bh_kv8_batch* hint, uint32_t nh, int dtype) {
     Plan r{};
     const uint32_t group = nh / kv.nkv;
