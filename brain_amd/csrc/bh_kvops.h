@@ -92,9 +92,10 @@ inline bool aligned_to(const void* p, size_t n) { return (reinterpret_cast<uintp
 struct F32 {
     typedef float elem;
     static __device__ __forceinline__ float get(const float* p) { return *p; }
-    static __device__ __forceinline__ void get4(const float* p, float (&x)[4]) {
-        const float4 v = *reinterpret_cast<const float4*>(p);
-        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+    typedef float raw4 __attribute__((ext_vector_type(4)));  // four elements as loaded
+    static __device__ __forceinline__ void open4(raw4 v, float (&x)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = v[i];
     }
     static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
     static __device__ __forceinline__ void put4(float* p, const float (&x)[4]) {
@@ -106,10 +107,13 @@ struct Bf16 {
     static __device__ __forceinline__ float get(const uint16_t* p) {
         return __builtin_bit_cast(float, (uint32_t)*p << 16);
     }
-    static __device__ __forceinline__ void get4(const uint16_t* p, float (&x)[4]) {
-        const uint2 v = *reinterpret_cast<const uint2*>(p);
-        x[0] = __builtin_bit_cast(float, v.x << 16), x[1] = __builtin_bit_cast(float, v.x & 0xffff0000u);
-        x[2] = __builtin_bit_cast(float, v.y << 16), x[3] = __builtin_bit_cast(float, v.y & 0xffff0000u);
+    typedef int raw4 __attribute__((ext_vector_type(2)));
+    static __device__ __forceinline__ void open4(raw4 v, float (&x)[4]) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            x[2 * i] = __builtin_bit_cast(float, (uint32_t)v[i] << 16);
+            x[2 * i + 1] = __builtin_bit_cast(float, (uint32_t)v[i] & 0xffff0000u);
+        }
     }
     static __device__ __forceinline__ void put(uint16_t* p, float v) { *p = f32_to_bf16_rne(v); }
     static __device__ __forceinline__ void put4(uint16_t* p, const float (&x)[4]) {

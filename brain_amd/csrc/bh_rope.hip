@@ -39,18 +39,29 @@ __device__ __forceinline__ void turn(uint32_t pos, double freq, float& c, float&
 // its cache slot: NO_SLOT where its position is before the sequence's first or
 // has no block.
 __device__ __forceinline__ bool row_slot(const Kv8& kv, const Kv8Rows& bt, uint32_t r, uint32_t lane, uint32_t& slot) {
-    uint32_t b = r;
-    if (bt.start) b = wave_last(bt.batch, lane, [&](uint32_t i) { return bt.start[i] <= r; });
-    if (b >= bt.batch) return false;
-    const uint32_t e = bt.end(b), len = bt.lens[b];
+    uint32_t b = r, e, len;
+    if (bt.start && bt.batch < 64) {  // one round trip: lane i has row_start[i] and sequence i's length
+        const uint32_t st = min(bt.start[min(lane, bt.batch)], bt.rows), ln = bt.lens[min(lane, bt.batch - 1)];
+        asm volatile("" ::"v"(ln));  // both on their way before the branch
+        const unsigned long long m = __ballot(lane < bt.batch && st <= r);
+        if (!m) return false;
+        b = 63u - (uint32_t)__builtin_clzll(m);
+        e = (uint32_t)__builtin_amdgcn_readlane((int)st, (int)b + 1);
+        len = (uint32_t)__builtin_amdgcn_readlane((int)ln, (int)b);
+    } else {
+        if (bt.start) b = wave_last(bt.batch, lane, [&](uint32_t i) { return bt.start[i] <= r; });
+        if (b >= bt.batch) return false;
+        e = bt.end(b), len = bt.lens[b];
+    }
     if (r >= e) return false;
     slot = len < e - r ? NO_SLOT : kv.slot(b, len - (e - r));
     return true;
 }
 
 // Without ceilings the largest finite one, as the appends of the decoder have it.
-__device__ __forceinline__ float code_scale(float mx, const float* clip, uint32_t head) {
-    const float s = fminf(mx, clip ? clip[head] : 3.402823466e+38f) / 127.0f;
+constexpr float NO_CLIP = 3.402823466e+38f;
+__device__ __forceinline__ float code_scale(float mx, float clip) {
+    const float s = fminf(mx, clip) / 127.0f;
     return s == 0.0f ? 1.0f : s;
 }
 
@@ -105,7 +116,8 @@ __global__ __launch_bounds__(64) void qk_norm_rope_any_kernel(RopeRowsArgs p) {
     float mx = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
     mx = xor_max<32>(mx);
     const uint32_t which = kind - 1;
-    const float scale = code_scale(mx, which ? p.vclip : p.kclip, hh);
+    const float* clip = which ? p.vclip : p.kclip;
+    const float scale = code_scale(mx, clip ? clip[hh] : NO_CLIP);
     if (lane == 0) p.kv.scales[which][(uint64_t)slot * p.nkv + hh] = scale;
     if (live) {
         uint32_t w = 0;
@@ -129,40 +141,68 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeRowsArgs p, uint3
     if (r >= p.rows) return;
     uint32_t h = (w % parts) * HPW + lane / LPH;
     struct In {
-        float a[4], b[4];
-    };
-    auto source = [&](uint32_t hh) -> const E* {
-        const E* base = hh < p.nh ? (const E*)p.q + r * p.qs + (uint64_t)hh * HD
-                        : hh < p.nh + p.nkv ? (const E*)p.k + r * p.ks + (uint64_t)(hh - p.nh) * HD
-                                            : (const E*)p.v + r * p.vs + (uint64_t)(hh - p.nh - p.nkv) * HD;
-        return base + 4 * li;
+        typename T::raw4 a, b;
+        float clip;
     };
     auto load = [&](uint32_t hh, In& x) {  // a head behind the last one reads the last
-        const E* src = source(min(hh, heads - 1));
-        T::get4(src, x.a);
-        T::get4(src + HALF, x.b);
+        hh = min(hh, heads - 1);
+        const bool is_q = hh < p.nh, is_k = !is_q && hh < p.nh + p.nkv;
+        const uint32_t kvh = is_q ? 0 : hh - p.nh - (is_k ? 0 : p.nkv);
+        const E* src = is_q ? (const E*)p.q + r * p.qs + (uint64_t)hh * HD
+                            : (is_k ? (const E*)p.k + r * p.ks : (const E*)p.v + r * p.vs) + (uint64_t)kvh * HD;
+        x.a = *reinterpret_cast<const typename T::raw4*>(src + 4 * li);
+        x.b = *reinterpret_cast<const typename T::raw4*>(src + 4 * li + HALF);
+        // The ceiling goes out with the row: a load at its use would wait for the
+        // stores and the next row as well.
+        x.clip = 0.0f;
+        if constexpr (APPEND) {
+            const float* c = is_q ? nullptr : is_k ? p.kclip : p.vclip;
+            x.clip = *(c ? c + kvh : (const float*)p.pos);  // (without one: any word)
+        }
     };
     In x;
     load(h, x);
     const uint32_t pos = p.pos[r];
+    double f[(HALF + 63) / 64];  // lane l: pairs l, l + 64
+#pragma unroll
+    for (int i = 0; i < (HALF + 63) / 64; ++i) f[i] = p.freq[min(64 * i + lane, (uint32_t)HALF - 1)];
     float cs[4], sn[4], qw[8], kw[8];
-    double f[4];
+    auto gains = [&](const float* w, float (&g)[8]) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = p.freq[4 * li + e];
+        for (int e = 0; e < 8; ++e) g[e] = 1.0f;
+        if (w) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const uint32_t d = (e < 4 ? 0 : HALF) + 4 * li + (e & 3);
-        qw[e] = p.qw ? p.qw[d] : 1.0f;
-        kw[e] = p.kw ? p.kw[d] : 1.0f;
-    }
+            for (int e = 0; e < 4; ++e) g[e] = w[4 * li + e], g[4 + e] = w[HALF + 4 * li + e];
+        }
+    };
+    gains(p.qw, qw);
+    gains(p.kw, kw);
     uint32_t slot = 0;
     if constexpr (APPEND)
         if (!row_slot(p.kv, p.bt, r, lane, slot)) return;
+    // Each angle once for the wave (its lanes for different heads need the same).
+    __shared__ __attribute__((aligned(16))) float turns[4][2][HALF];
+    float(&tw)[2][HALF] = turns[threadIdx.x >> 6];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) turn(pos, f[e], cs[e], sn[e]);
+    for (int i = 0; i < (HALF + 63) / 64; ++i) {
+        float c, s;
+        turn(pos, f[i], c, s);
+        if (HALF >= 64 || lane < HALF) tw[0][64 * i + lane] = c, tw[1][64 * i + lane] = s;
+    }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int e = 0; e < 4; ++e) cs[e] = tw[0][4 * li + e], sn[e] = tw[1][4 * li + e];
     // The whole wave stays for the exchanges.
     for (; __any(h < heads); h += parts * HPW) {
-        In cur = x;
+        struct {
+            float a[4], b[4], clip;
+        } cur;
+        // (Opened here and not before: that would wait for the row's arrival, and
+        // for all stores before it, a round early.)
+        asm volatile("" : "+v"(x.a), "+v"(x.b), "+v"(x.clip));
+        T::open4(x.a, cur.a);
+        T::open4(x.b, cur.b);
+        cur.clip = x.clip;
         load(h + parts * HPW, x);
         const bool real = h < heads, is_q = h < p.nh, rot = h < p.nh + p.nkv;
         if (__any(rot)) {
@@ -198,7 +238,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeRowsArgs p, uint3
             mx = xor_max<LPH / 2>(mx);
             if (real && !is_q && slot != NO_SLOT) {
                 const uint32_t kvh = h - p.nh - (rot ? 0 : p.nkv);
-                const float scale = code_scale(mx, rot ? p.kclip : p.vclip, kvh);
+                const float scale = code_scale(mx, (rot ? p.kclip : p.vclip) ? cur.clip : NO_CLIP);
                 uint32_t wa = 0, wb = 0;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
