@@ -309,7 +309,10 @@ extern "C" int bh_paged_kv_evict_i8(void* stream, const bh_kv8* kv, const uint32
                     sink, recent, acc_stride);
     if (batch == 0) return BH_OK;
     if (!seq_lens || !acc || !keep || !new_lens) return fail(BH_ERR_INVALID, "%s: null buffer", who);
-    if (out_tables && out_max_blocks == 0) return fail(BH_ERR_INVALID, "%s: out_max_blocks 0", who);
+    const uint64_t most = std::min<uint64_t>({budget, acc_stride, (uint64_t)kv->max_blocks * kv->block_size});
+    if (out_tables && (out_max_blocks == 0 || (uint64_t)out_max_blocks * kv->block_size < most))
+        return fail(BH_ERR_INVALID, "%s: out_max_blocks %u, blocks of %u, for %llu positions", who, out_max_blocks,
+                    kv->block_size, (unsigned long long)most);
     if (acc_out && (acc_out_stride < std::min(budget, acc_stride) || (acc_out == acc && acc_out_stride != acc_stride)))
         return fail(BH_ERR_INVALID, "%s: rows of %u in acc_out for a budget of %u (acc_stride %u)", who, acc_out_stride,
                     budget, acc_stride);

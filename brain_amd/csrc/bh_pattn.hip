@@ -711,7 +711,7 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
     float mleast = -INFINITY;
     auto within = [&](int bu) -> bool {
         const float size = __builtin_amdgcn_sqrtf((float)kn2[bu][lane]) * fabsf(scs[bu][0][lane]);
-        return __all(qmost * size <= mleast + ROOM && scs[bu][1][lane] < VMOST);
+        return __all(qmost * size <= mleast + ROOM && fabsf(scs[bu][1][lane]) < VMOST);
     };
     // Moves the reference to the largest score where that is more than SLACK
     // above it, each query for itself (ok: the keys that have a slot).
@@ -1346,13 +1346,14 @@ struct Plan {
 Plan plan_attention(const Kv8& kv, const Kv8Rows& bt, const bh_kv8_batch* hint, uint32_t nh, int dtype) {
     Plan r{};
     const uint32_t group = nh / kv.nkv;
+    if (bt.rows == 0 || bt.batch == 0) return r;
     if ((kv.hd != 64 && kv.hd != 128) || kv.nslots == 0 || !aligned_to(kv.pool[0], 16) || !aligned_to(kv.pool[1], 16)) return r;
     const uint32_t most = bt.start ? (hint->max_rows ? std::min(hint->max_rows, bt.rows) : bt.rows) : 1;
     const uint64_t vectors = (uint64_t)most * group, all = (uint64_t)bt.rows * group;
     r.kind = vectors <= 32 ? STREAM : TILE;
     r.vb = vectors <= 16 ? 16 : vectors <= 32 ? 32 : TVB;
     r.blocks = !bt.start && group <= r.vb ? bt.batch : (uint32_t)(all / r.vb) + bt.batch;
-    const uint64_t reach = (uint64_t)kv.max_bt * kv.bs;
+    const uint64_t reach = std::min<uint64_t>((uint64_t)kv.max_bt * kv.bs, 0x7fff0000u);
     const uint64_t len = std::max<uint64_t>(1, hint->max_len ? std::min<uint64_t>(hint->max_len, reach) : reach);
     // Splits of whole rounds: 32 keys for each wave, or two tiles.
     const uint32_t round = 128;
@@ -1483,6 +1484,7 @@ extern "C" int bh_paged_weight_sums_i8(void* stream, const void* q, uint64_t q_s
     SumsArgs a{};
     const int rc = check_call(who, kv, batch, n_heads, dtype, q_stride, &a.kv, &a.bt);
     if (rc) return rc;
+    if (acc_stride > 0x7fff0000u) return fail(BH_ERR_INVALID, "%s: acc_stride %u", who, acc_stride);
     if (batch->rows == 0 || batch->batch == 0 || acc_stride == 0) return BH_OK;
     if (!q || !lse || !acc) return fail(BH_ERR_INVALID, "%s: null buffer", who);
     a.q = q, a.qs = q_stride, a.lse = lse, a.acc = acc, a.cap = acc_stride;

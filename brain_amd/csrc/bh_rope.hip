@@ -332,6 +332,7 @@ int check_kv8(const char* who, const bh_kv8* kv, Kv8* out) {
 
 int check_kv8_batch(const char* who, const bh_kv8_batch* bt, Kv8Rows* out) {
     if (!bt) return fail(BH_ERR_INVALID, "%s: no batch", who);
+    if (bt->batch > 0x3fffffffu) return fail(BH_ERR_INVALID, "%s: %u sequences", who, bt->batch);
     if (bt->batch && bt->rows && !bt->seq_lens) return fail(BH_ERR_INVALID, "%s: no sequence lengths", who);
     if (!bt->row_start && bt->rows != bt->batch)
         return fail(BH_ERR_INVALID, "%s: %u rows of %u sequences need row_start", who, bt->rows, bt->batch);

@@ -321,8 +321,10 @@ int bh_paged_weight_sums_i8(void* stream, const void* q, uint64_t q_stride, int 
  * acc_out [batch][n_kv_heads][acc_out_stride] (may be acc itself; NULL: not
  * wanted). Different heads of a slot then hold different tokens: what was
  * turned by its position stays so. Each block written to must belong to one
- * sequence, and, unless in place, be none that is read. seq_lens[b] past
- * acc_stride counts as acc_stride. new_lens may be seq_lens. */
+ * sequence, and, unless in place, be none that is read; out_tables has room for min(budget, acc_stride, the cache's
+ * max_blocks * block_size) positions. seq_lens[b] past
+ * acc_stride counts as acc_stride. new_lens may be seq_lens. An entry kept whose position has no slot (a table entry
+ * outside the pool) does not move: its new place holds what it held. */
 int bh_paged_kv_evict_i8(void* stream, const bh_kv8* kv, const uint32_t* seq_lens, uint32_t batch, const float* acc,
                          uint32_t acc_stride, uint32_t budget, uint32_t sink, uint32_t recent,
                          const uint32_t* out_tables, uint32_t out_max_blocks, float* acc_out, uint32_t acc_out_stride,

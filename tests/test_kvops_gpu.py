@@ -603,3 +603,69 @@ def test_two_streams(gpu):
     for i in range(2):
         for out, lse in got[i]:
             assert torch.equal(out, alone[i][0]) and torch.equal(lse, alone[i][1])
+
+
+# ------------------------------------------------------------------ hints, and batches without rows
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows,lens,nh,nkv,hd,bs", [ATTN[3], ATTN[5], ATTN[6], ATTN[11], ([1, 1], [5000, 129], 8, 2, 128, 16)])
+def test_wrong_hints(gpu, rows, lens, nh, nkv, hd, bs, dtype):
+    """max_rows and max_len only choose how the work is split: too small or too large ones give the same values."""
+    g = gen(sum(lens), nh, hd, bs, 2)
+    c = ref.Cache(g, len(rows), max(1, (max(lens) + bs - 1) // bs), bs, nkv, hd)
+    start = ref.starts(rows)
+    q = torch.randn(int(start[-1]), nh, hd, generator=g).to(dtype)
+    want, lse, ob, lb = ref.attention(c, q, start, lens, 0.1)
+    acc = torch.randn(len(rows), nkv, max(lens), generator=g)
+    given = lse.float()
+    want_acc, bound = ref.weight_sums(c, q, given, start, lens, 0.1, acc)
+    dl = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    for max_rows in (1, 9, 1 << 30):
+        for max_len in (1, 200, 1 << 30):
+            hints = dict(max_rows=max_rows, max_len=max_len)
+            out, got = run_attention(gpu, c, q.to(gpu), start, lens, 0.1, **hints)
+            near(out, want, ob, f"out {hints}")
+            near(got, lse, lb, f"lse {hints}")
+            sums = ops.paged_weight_sums_i8(q.to(gpu), given.to(gpu), c.kv(ops, gpu), dl, acc.to(gpu), start.to(gpu), 0.1, **hints)
+            near(sums, want_acc, bound, f"acc {hints}")
+
+
+def test_no_rows(gpu):
+    """Batches without sequences or without rows: nothing is done, acc keeps what it has."""
+    g = gen(21)
+    c = ref.Cache(g, 2, 3, 16, 2, 64)
+    kv, none = c.kv(ops, gpu), torch.zeros(0, dtype=torch.int32, device=gpu)
+    lens, start = torch.tensor([40, 3], dtype=torch.int32, device=gpu), torch.zeros(3, dtype=torch.int32, device=gpu)
+    q, k, pos = torch.zeros(0, 4, 64, device=gpu), torch.zeros(0, 2, 64, device=gpu), none
+    freq = ops.rope_frequencies(64, 1e4)
+    acc = torch.rand(2, 2, 48, generator=g).to(gpu)
+    old = acc.clone()
+    for at, st in ((none, None), (lens, start)):
+        assert ops.qk_norm_rope(q, k, pos, freq)[0].shape == q.shape
+        ops.qk_norm_rope_append_i8(q, k, k, pos, freq, kv, at, st)
+        out, lse = ops.paged_attention_i8(q, kv, at, st)
+        assert out.shape == q.shape and lse.shape == (0, 4)
+        ops.paged_weight_sums_i8(q, lse, kv, at, acc, st)
+    assert ops.paged_kv_evict_i8(kv, none, acc, 5)[0].shape == (0, 2, 5)
+    assert torch.equal(acc, old) and torch.equal(kv.k_scales.cpu(), c.scales[0]) and torch.equal(kv.k_pool.cpu(), c.words(0))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_attention_large_value_scales(gpu, sign, dtype):
+    """Value scales of 2^60 at a key whose score is far above those before it: the weighted values stay finite."""
+    g = gen(22)
+    rows, t, nh, nkv, hd, bs = 40, 470, 4, 2, 128, 16
+    c = ref.Cache(g, 1, (t + bs - 1) // bs, bs, nkv, hd)
+    c.codes[0].zero_()
+    for j in (200, 210):
+        c.codes[0][c.slot(0, j)] = 127
+        c.scales[0][c.slot(0, j)] = 45.0 / 127 / 128
+        c.scales[1][c.slot(0, j)] = sign * 2.0 ** 60
+    start, lens = ref.starts([rows]), [t]
+    q = torch.ones(rows, nh, hd).to(dtype)
+    want, lse, ob, lb = ref.attention(c, q, start, lens, 1.0)  # scores 45 = 65 binades, and 0
+    out, got = run_attention(gpu, c, q.to(gpu), start, lens, 1.0)
+    near(out, want, ob, "out")
+    near(got, lse, lb, "lse")

@@ -264,3 +264,21 @@ def test_ops_evict():
     no("acc_out", c, lens, acc, 4, acc_out=f(2, 1, 4))
     no("keep", c, lens, acc, 4, keep=i(2, 2, 3), new_lens=i(2))
     no("new_lens", c, lens, acc, 4, keep=i(2, 2, 4), new_lens=i(1))
+
+
+def test_sizes_at_the_ends():
+    lib = load()
+    for some in (dict(batch=0, rows=0, row_start=None, seq_lens=None), dict(batch=0, rows=0), dict(rows=0)):
+        n = C.c_uint64(1)
+        assert lib.bh_paged_attention_i8_workspace(kv(), batch(**some), 4, C.byref(n)) == BH_OK and n.value == 0
+    refused(lib.bh_paged_attention_i8_workspace(kv(), batch(batch=1 << 30), 4, C.byref(C.c_uint64())), "sequences")
+    refused(lib.bh_paged_weight_sums_i8(None, P, 256, 0, 4, P, kv(), batch(), 0.1, P, 0x7FFFFFFF), "acc_stride")
+    # max_blocks * block_size past 32 bits: no more than the positions there can be.
+    n = C.c_uint64()
+    assert lib.bh_paged_attention_i8_workspace(kv(max_blocks=0xFFFFFFFF, block_size=1 << 20), batch(max_len=0), 4, C.byref(n)) == BH_OK
+    assert 0 < n.value < 1 << 22  # 2 blocks of 16 vectors, 2 heads, 64 splits at most
+    # Tables without room for what is kept.
+    evict = lambda budget, cap, cols: lib.bh_paged_kv_evict_i8(None, kv(), P, 2, P, cap, budget, 0, 0, P + 64, cols, None, 0,  # noqa: E731
+                                                               P, P)
+    refused(evict(9, 64, 8 // kv()._obj.block_size), "for 9 positions")
+    refused(evict(64, 9, 8 // kv()._obj.block_size), "for 9 positions")
