@@ -160,20 +160,21 @@ __device__ __forceinline__ uint32_t hi16x2(float lo, float hi) {
 // Eight floats as PARTS bf16 fragments: one, rounded to nearest, or three that
 // add up to them: the first is cut, so that none rounds to infinity.
 template <int PARTS>
+__device__ __forceinline__ void split2(float x0, float x1, int i, v4i (&f)[PARTS]) {  // elements 2 i, 2 i + 1 of a fragment
+    if constexpr (PARTS == 1) {
+        f[0][i] = (int)pack_bf16x2(x0, x1);
+    } else {
+        f[0][i] = (int)hi16x2(x0, x1);
+        const float r0 = x0 - bitsf(fbits(x0) & 0xffff0000u), r1 = x1 - bitsf(fbits(x1) & 0xffff0000u);
+        const uint32_t q = pack_bf16x2(r0, r1);
+        f[1][i] = (int)q;
+        f[2][i] = (int)hi16x2(r0 - bitsf(q << 16), r1 - bitsf(q & 0xffff0000u));  // at most 8 bits are left
+    }
+}
+template <int PARTS>
 __device__ __forceinline__ void split8(const float (&x)[8], v4i (&f)[PARTS]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float x0 = x[2 * i], x1 = x[2 * i + 1];
-        if constexpr (PARTS == 1) {
-            f[0][i] = (int)pack_bf16x2(x0, x1);
-        } else {
-            f[0][i] = (int)hi16x2(x0, x1);
-            const float r0 = x0 - bitsf(fbits(x0) & 0xffff0000u), r1 = x1 - bitsf(fbits(x1) & 0xffff0000u);
-            const uint32_t q = pack_bf16x2(r0, r1);
-            f[1][i] = (int)q;
-            f[2][i] = (int)hi16x2(r0 - bitsf(q << 16), r1 - bitsf(q & 0xffff0000u));  // at most 8 bits are left
-        }
-    }
+    for (int i = 0; i < 4; ++i) split2<PARTS>(x[2 * i], x[2 * i + 1], i, f);
 }
 // Eight codes (along one key's dimensions) as a fragment.
 __device__ __forceinline__ v4i codes8(uint32_t lo, uint32_t hi) {
@@ -555,13 +556,17 @@ __device__ __forceinline__ v16f mfma32(v4i a, v4i b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
 }
 
-constexpr int TW = 8, TVB = 32 * TW;  // waves, query vectors of a workgroup
+// Waves of a workgroup (one workgroup a compute unit: LDS), 32 query vectors each.
+template <class T, int HD>
+constexpr int tile_waves() {
+    return sizeof(typename T::elem) == 4 && HD == 128 ? 4 : 8;
+}
 
 template <class T, int HD>
-__global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnArgs p) {
+__global__ __launch_bounds__((tile_waves<T, HD>() * 64), (tile_waves<T, HD>() / 4)) void paged_attention_tile_kernel(AttnArgs p) {
     typedef typename T::elem E;
+    constexpr int TW = tile_waves<T, HD>(), TVB = 32 * TW;
     constexpr int PARTS = sizeof(E) == 4 ? 3 : 1, NT = TW * 64, KB = TK * HD * 2, NBUF = 3;
-    constexpr bool PIPE = PARTS == 1;
     __shared__ __attribute__((aligned(1024))) uint8_t kt[NBUF][KB], vt[NBUF][KB];
     __shared__ __attribute__((aligned(16))) float scs[NBUF][2][TK];  // keys', values' scales
     __shared__ int kn2[NBUF][TK];                                      // |codes|^2 of each key
@@ -571,9 +576,8 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t nkv = p.kv.nkv, kvs = nkv * HD, units = p.blocks * p.nsplit;
     const uint32_t turn = p.by_nkv.of(blockIdx.x / 8), kvh = blockIdx.x / 8 - turn * nkv;
-    uint32_t unit = turn * 8 + blockIdx.x % 8;
+    const uint32_t unit = turn * 8 + blockIdx.x % 8;
     if (unit >= units) return;
-    unit = units - 1 - unit;  // a chunk's last rows see the most keys: they start first
     const uint32_t blk = p.by_nsplit.of(unit), split = unit - blk * p.nsplit;
     Block bl;
     if (!find_block<TVB>(p.bt, p.group, blk, lane, bl)) return;
@@ -589,28 +593,6 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
     const bool wlive = wv0 < vend;
     const uint32_t wall = wlive ? min(keys_seen(bl, p.by_group.of(wv0)), reach) : 0u;
     const uint32_t wend = wlive ? min(keys_seen(bl, p.by_group.of(wv1 - 1)), reach) : 0u;
-    uint32_t seen;
-    float qn;
-    const bool dead = wv0 + col >= vend;  // no vector: computes the last one's again, its sums are not used
-    v4i qf[HD / 16][PARTS];  // step t: d = 16 t + 8 half ..+7 of vector col
-    {
-        const uint32_t v = min(wv0 + col, vend - 1), i = p.by_group.of(v), h = kvh * p.group + (v - i * p.group);
-        seen = wv0 + col < vend ? min(keys_seen(bl, i), reach) : 0u;
-        const E* src = (const E*)p.q + (bl.r0 + i) * p.qs + (uint64_t)h * HD + 8 * half;
-        qn = 0.0f;
-        float x[HD / 16][8];
-        query8<T>(src, x, [](int t) { return 16 * t; });
-#pragma unroll
-        for (int t = 0; t < HD / 16; ++t) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) qn = qn + x[t][e] * x[t][e];
-            split8<PARTS>(x[t], qf[t]);
-        }
-        // Above |q|, whatever the roundings; infinite or NaN (no bound: a NaN here
-        // would be lost in the maximum) becomes infinite.
-        qn = sqrtf(qn + xor_lane<32>(qn)) * 1.001f;
-        qn = dead ? 0.0f : qn < INFINITY ? qn : INFINITY;
-    }
     v16f o[HD / 32];
     float m = -INFINITY, l = 0.0f;
 #pragma unroll
@@ -627,7 +609,7 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
     };
-    // Where tile t's keys lie: wave t % 8 looks the tables up, two steps before
+    // Where tile t's keys lie: wave t % TW looks the tables up, two steps before
     // the loads need it. A key behind the end or without a slot gets slot 0.
     auto slot_at = [&](int t) -> uint32_t {
         const uint32_t j = k0 + (uint32_t)t * TK + lane;
@@ -637,24 +619,62 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
         ring[t & 3][lane] = s != NO_SLOT ? (uint64_t)s * kvs : 0u;
         okm[t & 3] = __ballot(s != NO_SLOT);
     };
-    // A thread takes 16 bytes of a key and four values' four bytes (HD 64: one
-    // of the two).
-    constexpr int CPK = HD / 16, DG = HD / 4, VT = NT - TK / 4 * DG;  // VT: the first thread with values
-    static_assert(VT >= 0 && TK * CPK <= NT, "a piece for each thread");
-    const bool klive = TK * CPK == NT || tid < TK * CPK, vlive = VT == 0 || tid >= VT;
+    // The first look-ups, the queries and the first two tiles go out before
+    // anything waits for the queries.
+    const uint32_t sl_first = wave < 4 ? slot_at(wave) : NO_SLOT;
+    uint32_t sl_next = wave == 4 % TW ? slot_at(4) : NO_SLOT;
+    uint32_t seen;
+    const bool dead = wv0 + col >= vend;  // no vector: computes the last one's again, its sums are not used
+    float qx[HD / 16][8];  // step t: d = 16 t + 8 half ..+7 of vector col
+    {
+        const uint32_t v = min(wv0 + col, vend - 1), i = p.by_group.of(v), h = kvh * p.group + (v - i * p.group);
+        seen = wv0 + col < vend ? min(keys_seen(bl, i), reach) : 0u;
+        const E* src = (const E*)p.q + (bl.r0 + i) * p.qs + (uint64_t)h * HD + 8 * half;
+        query8<T>(src, qx, [](int t) { return 16 * t; });
+    }
+    if (wave < 4) put_slots(wave, sl_first);
+    barrier();
+    // A thread takes 16 bytes of a key and four values' four bytes, PR times (8
+    // waves and HD 64: one of the two).
+    constexpr int CPK = HD / 16, DG = HD / 4, KP = TK * CPK, VP = TK / 4 * DG;  // pieces
+    static_assert(KP == VP && (KP % NT == 0 || NT == 2 * KP), "whole pieces for each thread");
+    constexpr int PR = KP > NT ? KP / NT : 1, VT = NT > VP ? NT - VP : 0;  // VT: the first thread with values
+    const bool klive = KP >= NT || tid < KP, vlive = VT == 0 || tid >= VT;
     const int kkey = tid / CPK, kpc = tid % CPK, quad = (tid - VT) / DG, dg = (tid - VT) % DG;
-    v4i kr;
-    uint32_t vr[4];
-    float sr = 0.0f;
-    auto load = [&](int t) __attribute__((always_inline)) {
-        const uint64_t* sl = ring[t & 3];
-        if (klive) kr = *reinterpret_cast<const v4i*>(kp + sl[kkey] + 16 * kpc);
-        if (vlive) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) vr[i] = *reinterpret_cast<const uint32_t*>(vp + sl[4 * quad + i] + 4 * dg);
-        }
-        sr = *reinterpret_cast<const float*>(sp + sl[lane] / (HD / 4));
+    struct Raw {
+        v4i k[PR];
+        uint32_t v[PR][4];
+        float s;
     };
+    auto load = [&](int t, Raw& x) __attribute__((always_inline)) {
+        const uint64_t* sl = ring[t & 3];
+#pragma unroll
+        for (int r = 0; r < PR; ++r) {
+            if (klive) x.k[r] = *reinterpret_cast<const v4i*>(kp + sl[kkey + r * (NT / CPK)] + 16 * kpc);
+            if (vlive) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    x.v[r][i] = *reinterpret_cast<const uint32_t*>(vp + sl[4 * (quad + r * (NT / DG)) + i] + 4 * dg);
+            }
+        }
+        x.s = *reinterpret_cast<const float*>(sp + sl[lane] / (HD / 4));
+    };
+    Raw raw, second;
+    load(0, raw);
+    load(1, second);
+    __builtin_amdgcn_sched_barrier(0);
+    float qn = 0.0f;
+    v4i qf[HD / 16][PARTS];
+#pragma unroll
+    for (int t = 0; t < HD / 16; ++t) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) qn = qn + qx[t][e] * qx[t][e];
+        split8<PARTS>(qx[t], qf[t]);
+    }
+    // Above |q|, whatever the roundings; infinite or NaN (no bound: a NaN here
+    // would be lost in the maximum) becomes infinite.
+    qn = sqrtf(qn + xor_lane<32>(qn)) * 1.001f;
+    qn = dead ? 0.0f : qn < INFINITY ? qn : INFINITY;
     // LDS images. K: chunk c (8 d) of key r. V^T: 32 keys at a time, lines of 256
     // bytes hold 4 d x 32 keys, 8 keys a chunk in the order of a lane's scores:
     // chunk 2u + h has keys 16u + 4h ..+3 and 16u + 8 + 4h ..+3. In both the 16
@@ -666,30 +686,38 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
     const int kst = klive ? kchunk(kkey, 2 * kpc) : 0;  // chunk 2 kpc + 1 is at kst ^ 16
     // quad: keys 4 quad ..+3 = 16 u' + 4 x: chunk (quad / 4) * 2 + (quad & 1), its half (quad >> 1) & 1
     const int vst = vlive ? vchunk(4 * dg, 2 * (quad >> 2) + (quad & 1)) + 8 * ((quad >> 1) & 1) : 0;
-    auto store_k = [&](int bu) __attribute__((always_inline)) {
-        if (klive) {
-            *reinterpret_cast<v4i*>(kt[0] + bu * KB + kst) = codes8((uint32_t)kr[0], (uint32_t)kr[1]);
-            *reinterpret_cast<v4i*>(kt[0] + bu * KB + (kst ^ 16)) = codes8((uint32_t)kr[2], (uint32_t)kr[3]);
-            int n2 = 0;
+    // Piece r: 16 n keys on, and 16 n values: the same place of a later line.
+    auto store_k = [&](int bu, int r) __attribute__((always_inline)) {
+        if (!klive) return;
+        uint8_t* at = kt[0] + bu * KB + r * (NT / CPK) * (HD * 2);
+        *reinterpret_cast<v4i*>(at + kst) = codes8((uint32_t)raw.k[r][0], (uint32_t)raw.k[r][1]);
+        *reinterpret_cast<v4i*>(at + (kst ^ 16)) = codes8((uint32_t)raw.k[r][2], (uint32_t)raw.k[r][3]);
+        int n2 = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) n2 = __builtin_amdgcn_sdot4(kr[i], kr[i], n2, false);
-            n2 += (int)xor_lane_u<1>((uint32_t)n2);  // the CPK lanes of a key
-            n2 += (int)xor_lane_u<2>((uint32_t)n2);
-            if constexpr (CPK == 8) n2 += (int)xor_lane_u<4>((uint32_t)n2);
-            kn2[bu][kkey] = n2;
-        }
+        for (int i = 0; i < 4; ++i) n2 = __builtin_amdgcn_sdot4(raw.k[r][i], raw.k[r][i], n2, false);
+        n2 += (int)xor_lane_u<1>((uint32_t)n2);  // the CPK lanes of a key
+        n2 += (int)xor_lane_u<2>((uint32_t)n2);
+        if constexpr (CPK == 8) n2 += (int)xor_lane_u<4>((uint32_t)n2);
+        kn2[bu][kkey + r * (NT / CPK)] = n2;
     };
-    auto store_v = [&](int bu, unsigned long long ok) __attribute__((always_inline)) {
+    auto store_v = [&](int bu, unsigned long long ok, int r) __attribute__((always_inline)) {
         if (vlive) {
+            uint8_t* at = vt[0] + bu * KB + r * (NT / DG / 8) * (64 * HD);
 #pragma unroll
             for (int e = 0; e < 4; ++e)  // dimension 4 dg + e: chunk index + 4 e
-                *reinterpret_cast<uint2*>(vt[0] + bu * KB + (vst ^ (e << 6))) =
-                    make_uint2(hi16x2(code_f(vr[0], e), code_f(vr[1], e)), hi16x2(code_f(vr[2], e), code_f(vr[3], e)));
+                *reinterpret_cast<uint2*>(at + (vst ^ (e << 6))) = make_uint2(
+                    hi16x2(code_f(raw.v[r][0], e), code_f(raw.v[r][1], e)), hi16x2(code_f(raw.v[r][2], e), code_f(raw.v[r][3], e)));
         }
+        if (r) return;
         // A key without a slot has scales of 0. (Waves of a kind write the same.)
-        const float sc = (ok >> lane) & 1ull ? (wave & 1 ? sr : sr * p.scale2) : 0.0f;
+        const float sc = (ok >> lane) & 1ull ? (wave & 1 ? raw.s : raw.s * p.scale2) : 0.0f;
         scs[bu][wave & 1][lane] = sc;
     };
+    auto store = [&](int bu, unsigned long long ok) __attribute__((always_inline)) {
+#pragma unroll
+        for (int r = 0; r < PR; ++r) store_k(bu, r), store_v(bu, ok, r);
+    };
+    static_assert(PR == 1 || ((NT / CPK) % 16 == 0 && (NT / DG) % 8 == 0), "the pieces' places");
     // Scores of half kh of the tile in buffer bu. Register e: key 32 kh +
     // 8 (e / 4) + 4 half + e % 4.
     auto scores = [&](int bu, int kh, v16f& s) __attribute__((always_inline)) {
@@ -713,18 +741,27 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
         const float size = __builtin_amdgcn_sqrtf((float)kn2[bu][lane]) * fabsf(scs[bu][0][lane]);
         return __all(qmost * size <= mleast + ROOM && fabsf(scs[bu][1][lane]) < VMOST);
     };
+    // The keys (bit 8 (e / 4) + e % 4 of register e) that this lane's query sees in
+    // half kh of the tile from j0 on.
+    auto visible = [&](int kh, uint32_t j0, unsigned long long ok) -> uint32_t {
+        const int lim = (int)(seen - j0) - 32 * kh - 4 * half;
+        return (uint32_t)(ok >> (32 * kh)) >> (4 * half) & (lim >= 32 ? ~0u : (1u << max(lim, 0)) - 1u);
+    };
     // Moves the reference to the largest score where that is more than SLACK
     // above it, each query for itself (ok: the keys that have a slot).
     auto refer = [&](int bu, int kh, uint32_t j0, unsigned long long ok, const v16f& s) __attribute__((always_inline)) {
         const float* kcp = &scs[bu][0][32 * kh + 4 * half];
-        const uint32_t okl = (uint32_t)(ok >> (32 * kh)) >> (4 * half);
-        const int lim = (int)(seen - j0) - 32 * kh - 4 * half;
+        const uint32_t vis = visible(kh, j0, ok);
         float mx = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const int key = 8 * (e >> 2) + (e & 3);
-            const float a = s[e] * kcp[key];
-            mx = fmaxf(mx, key >= lim || !((okl >> key) & 1u) ? -INFINITY : a);
+        for (int g = 0; g < 4; ++g) {
+            const float4 kc = *reinterpret_cast<const float4*>(kcp + 8 * g);
+            float a[4] = {s[4 * g] * kc.x, s[4 * g + 1] * kc.y, s[4 * g + 2] * kc.z, s[4 * g + 3] * kc.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                asm volatile("" : "+v"(a[i]));  // no branch around each
+                mx = fmaxf(mx, (vis >> (8 * g + i)) & 1u ? a[i] : -INFINITY);
+            }
         }
         mx = fmaxf(mx, xor_lane<32>(mx));
         const bool up = mx > m + SLACK;
@@ -740,13 +777,10 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
         mleast = -xor_max<32>(-none);
     };
     // Weights of registers 8 u ..+7 of a half's scores, times their values' scales.
-    // HIDE: some of the keys are hidden from some query.
-    auto weights = [&](int bu, int kh, int u, uint32_t j0, unsigned long long ok, const v16f& s, v4i (&pf)[PARTS],
-                       auto hide) __attribute__((always_inline)) {
-        constexpr bool HIDE = decltype(hide)::value;
+    auto weights = [&](int bu, int kh, int u, uint32_t j0, unsigned long long ok, const v16f& s,
+                       v4i (&pf)[PARTS]) __attribute__((always_inline)) {
         const float *kcp = &scs[bu][0][32 * kh + 4 * half], *vsp = &scs[bu][1][32 * kh + 4 * half];
-        const uint32_t okl = (uint32_t)(ok >> (32 * kh)) >> (4 * half);
-        const int lim = (int)(seen - j0) - 32 * kh - 4 * half;
+        const uint32_t vis = visible(kh, j0, ok);
         const float ref = m == -INFINITY ? 0.0f : m;
         float x[8];
 #pragma unroll
@@ -756,7 +790,7 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
             const float kk[4] = {kc.x, kc.y, kc.z, kc.w}, vv[4] = {vs.x, vs.y, vs.z, vs.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const bool hid = HIDE && (k_ + i >= lim || !((okl >> (k_ + i)) & 1u));
+                const bool hid = !((vis >> (k_ + i)) & 1u);
                 float a = __builtin_fmaf(s[8 * u + 4 * i4 + i], kk[i], -ref);
                 if (hid) a = -INFINITY;
                 const float w = __builtin_amdgcn_exp2f(a);
@@ -778,20 +812,16 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
         }
     };
 
-    if (wave < 4) put_slots(wave, slot_at(wave));
-    uint32_t sl_next = wave == 4 ? slot_at(4) : NO_SLOT;
-    barrier();
     auto ok_of = [&](int t) -> unsigned long long {
         const unsigned long long ok = okm[t & 3];
         return (unsigned long long)(uint32_t)__builtin_amdgcn_readfirstlane((int)(ok >> 32)) << 32 |
                (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)ok);
     };
     unsigned long long ok0 = ok_of(0), ok1 = ok_of(1), ok2 = ok_of(2);  // of tiles t .. t + 2
-    load(0);
-    store_k(0), store_v(0, ok0);
-    load(1);
-    store_k(1), store_v(1, ok1);
-    load(2);
+    store(0, ok0);
+    raw = second;
+    store(1, ok1);
+    load(2, raw);
     barrier();
     // In step t tile t + 2 goes to LDS, whose buffer was last read in step t - 1.
     int b0 = 0, b1 = 1, b2 = 2;
@@ -799,7 +829,7 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
     bool calm = false;  // the next tile is within its bound and seen whole by all of the wave's queries
     auto rest = [&](int t) __attribute__((always_inline)) {
         const uint32_t j0 = k0 + (uint32_t)t * TK;
-        load(t + 3);
+        load(t + 3, raw);
         calm = j0 + 2 * TK <= wall && ok1 == ~0ull && within(b1);
         ok0 = ok1, ok1 = ok2, ok2 = ok_of(t + 3);
         if (((t + 4) & (TW - 1)) == wave) put_slots(t + 4, sl_next);
@@ -811,8 +841,7 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
     // Any tile, one thing after another.
     auto step = [&](int t) __attribute__((always_inline)) {
         const uint32_t j0 = k0 + (uint32_t)t * TK;
-        store_k(b2);
-        store_v(b2, ok2);
+        store(b2, ok2);
         if (j0 < wend) {
 #pragma unroll
             for (int kh = 0; kh < 2; ++kh) {
@@ -822,7 +851,7 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     __builtin_amdgcn_sched_barrier(0);
-                    weights(b0, kh, u, j0, ok0, s0, pf, std::true_type{});
+                    weights(b0, kh, u, j0, ok0, s0, pf);
                     values(b0, kh, u, pf);
                 }
                 __builtin_amdgcn_sched_barrier(0);
@@ -836,8 +865,10 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
     // beside the next half's scores go the weights of 8 of this half's keys;
     // beside their product with V the weights of the other 8; beside those'
     // product the conversion of a tile to come. f32: three products for each,
-    // and no registers for the next half's scores.
+    // so that all weights fit beside the next scores; and since a wave has its
+    // SIMD for itself, the vector work is dealt out product by product.
     constexpr int NS = HD / 16, NJ = HD / 32;
+    constexpr bool WIDE = PARTS == 3;
     v4i ka_[2];     // the first two operands of the next scores
     float4 kc_, vs_;  // scales of the next 4 keys
     auto fence = [&]() { __builtin_amdgcn_sched_barrier(0); };
@@ -870,89 +901,116 @@ __global__ __launch_bounds__(TW * 64, 2) void paged_attention_tile_kernel(AttnAr
             kc[g4] = *reinterpret_cast<const float4*>(kcp + 8 * g4);
             vs[g4] = *reinterpret_cast<const float4*>(kcp + TK + 8 * g4);
         };
-        auto pack = [&](int u, v4i (&f)[PARTS]) {
-            float y[8];
+        auto pair = [&](int k) { split2<PARTS>(x[2 * k], x[2 * k + 1], k & 3, k < 4 ? pf : pg); };
+        auto products = [&](const v4i& a, const v4i (&b)[PARTS], v16f& c) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = x[8 * u + i];
-            split8<PARTS>(y, f);
+            for (int part = PARTS - 1; part >= 0; --part) c = mfma32(a, b[part], c);
         };
-        constexpr int EP = 8 / NS;
+        // f32: the vector work of a stretch of n products dealt out to each of them.
+        auto deal = [&](auto n, auto each) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < n(); ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x2, each(), 0);
+            }
+        };
+        typedef std::integral_constant<int, 3> N3;
+        typedef std::integral_constant<int, 7> N7;
+        typedef std::integral_constant<int, 8> N8;
+        typedef std::integral_constant<int, 3 * NJ> NV;
+        constexpr int EP = WIDE ? 16 / NS : 8 / NS;
 #pragma unroll
         for (int e = 0; e < 16; ++e) nx[e] = 0.0f;
 #pragma unroll
         for (int d = 0; d < NS; ++d) {
-            nx = mfma32(kf[d], qf[d][0], nx);
+            products(kf[d], qf[d], nx);
             if (d + 2 < NS) kf[d + 2] = *reinterpret_cast<const v4i*>(kt[0] + (kbase ^ ((d + 2) << 5)));
-            if (d == 0) scales(1);
-            if (d == NS - 2) vf[0][0] = vread(va0, 0), scales(2);
+            if constexpr (WIDE) {  // (of the slot after next, or the next)
+                if (EP * (d + 1) % 4 != 0 && EP * d / 4 < 3) scales(EP * d / 4 + 1);
+                if (EP == 4 && d < 3) scales(d + 1);
+            } else {
+                if (d == 0) scales(1);
+                if (d == NS - 2) scales(2);
+            }
+            if (d == NS - 2) vf[0][0] = vread(va0, 0);
             if (d == NS - 1) vf[0][1] = vread(va0, 1);
 #pragma unroll
             for (int i = 0; i < EP; ++i) raise(EP * d + i);
             if (d)
 #pragma unroll
-                for (int i = 0; i < EP; ++i) finish(EP * (d - 1) + i);
+                for (int i = 0; i < EP; ++i) {
+                    const int e = EP * (d - 1) + i;
+                    finish(e);
+                    if (WIDE && e % 2) pair(e / 2);
+                }
+            if constexpr (WIDE) deal(N3{}, N7{});
             fence();
         }
+        if constexpr (WIDE) {
 #pragma unroll
-        for (int i = 0; i < EP; ++i) finish(8 - EP + i);
-        pack(0, pf);
-        fence();
-        constexpr int EV = 8 / NJ;
+            for (int j = 0; j < NJ; ++j) {
+                products(vf[0][j], pf, o[j]);
+                if (j + 2 < NJ) vf[0][j + 2] = vread(va0, j + 2);
+                else vf[1][j + 2 - NJ] = vread(va1, j + 2 - NJ);
+            }
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            o[j] = mfma32(vf[0][j], pf[0], o[j]);
-            if (j + 2 < NJ) vf[0][j + 2] = vread(va0, j + 2);
-            else vf[1][j + 2 - NJ] = vread(va1, j + 2 - NJ);
-            if (j == 0) scales(3);
+            for (int e = 16 - EP; e < 16; ++e) {
+                finish(e);
+                if (e % 2) pair(e / 2);
+            }
+            if (PR == 2) {
+                if (kh == 0) store_k(b2, 1);
+                else store_v(b2, ok2, 1);
+            }
+            deal(NV{}, N8{});
+            fence();
+        } else {
 #pragma unroll
-            for (int i = 0; i < EV; ++i) raise(8 + EV * j + i);
-            if (j)
+            for (int i = 0; i < EP; ++i) finish(8 - EP + i);
 #pragma unroll
-                for (int i = 0; i < EV; ++i) finish(8 + EV * (j - 1) + i);
+            for (int k = 0; k < 4; ++k) pair(k);
+            fence();
+            constexpr int EV = 8 / NJ;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                products(vf[0][j], pf, o[j]);
+                if (j + 2 < NJ) vf[0][j + 2] = vread(va0, j + 2);
+                else vf[1][j + 2 - NJ] = vread(va1, j + 2 - NJ);
+                if (j == 0) scales(3);
+#pragma unroll
+                for (int i = 0; i < EV; ++i) raise(8 + EV * j + i);
+                if (j)
+#pragma unroll
+                    for (int i = 0; i < EV; ++i) finish(8 + EV * (j - 1) + i);
+                fence();
+            }
+#pragma unroll
+            for (int i = 0; i < EV; ++i) finish(16 - EV + i);
+#pragma unroll
+            for (int k = 4; k < 8; ++k) pair(k);
             fence();
         }
-#pragma unroll
-        for (int i = 0; i < EV; ++i) finish(16 - EV + i);
-        pack(1, pg);
-        fence();
         prime(nbase, nbu, nkh);
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            o[j] = mfma32(vf[1][j], pg[0], o[j]);
+            products(vf[1][j], pg, o[j]);
             if (j + 2 < NJ) vf[1][j + 2] = vread(va1, j + 2);
         }
-        if (kh == 0) store_k(b2);
-        else store_v(b2, ok2);
+        if (kh == 0) store_k(b2, 0);
+        else store_v(b2, ok2, 0);
+        if constexpr (WIDE) deal(NV{}, N8{});
         fence();
     };
     auto calm_step = [&](int t) __attribute__((always_inline)) {
-        if constexpr (PIPE) {
-            const int kb0 = kaddr(b0, 1), kb1 = kaddr(b1, 0), kb2 = kaddr(b1, 1);
-            calm_half(0, kb0, s0, s1, kb1, b0, 1);
-            calm_half(1, kb1, s1, s0, kb2, b1, 0);
-        } else {
-#pragma unroll
-            for (int kh = 0; kh < 2; ++kh) {
-                v4i pf[PARTS], pg[PARTS];
-                scores(b0, kh, s0);
-                fence();
-                weights(b0, kh, 0, 0u, ~0ull, s0, pf, std::false_type{});
-                fence();
-                values(b0, kh, 0, pf);
-                weights(b0, kh, 1, 0u, ~0ull, s0, pg, std::false_type{});
-                fence();
-                values(b0, kh, 1, pg);
-                if (kh == 0) store_k(b2);
-                else store_v(b2, ok2);
-                fence();
-            }
-        }
+        const int kb0 = kaddr(b0, 1), kb1 = kaddr(b1, 0), kb2 = kaddr(b1, 1);
+        calm_half(0, kb0, s0, s1, kb1, b0, 1);
+        calm_half(1, kb1, s1, s0, kb2, b1, 0);
         rest(t);
     };
     // (Each wave passes one barrier a tile in whichever loop it is.)
     for (int t = 0; t < nt;) {
         step(t++);
-        if (t < nt && calm && PIPE) {
+        if (t < nt && calm) {
             scores(b0, 0, s0);
             prime(kaddr(b0, 1), b0, 0);
         }
@@ -1351,7 +1409,7 @@ Plan plan_attention(const Kv8& kv, const Kv8Rows& bt, const bh_kv8_batch* hint, 
     const uint32_t most = bt.start ? (hint->max_rows ? std::min(hint->max_rows, bt.rows) : bt.rows) : 1;
     const uint64_t vectors = (uint64_t)most * group, all = (uint64_t)bt.rows * group;
     r.kind = vectors <= 32 ? STREAM : TILE;
-    r.vb = vectors <= 16 ? 16 : vectors <= 32 ? 32 : TVB;
+    r.vb = vectors <= 16 ? 16 : vectors <= 32 ? 32 : dtype == BH_OUT_F32 && kv.hd == 128 ? 32 * tile_waves<F32, 128>() : 256;
     r.blocks = !bt.start && group <= r.vb ? bt.batch : (uint32_t)(all / r.vb) + bt.batch;
     const uint64_t reach = std::min<uint64_t>((uint64_t)kv.max_bt * kv.bs, 0x7fff0000u);
     const uint64_t len = std::max<uint64_t>(1, hint->max_len ? std::min<uint64_t>(hint->max_len, reach) : reach);
@@ -1364,7 +1422,7 @@ Plan plan_attention(const Kv8& kv, const Kv8Rows& bt, const bh_kv8_batch* hint, 
     } else {
         wgs = std::max<uint64_t>(1, all / r.vb) * kv.nkv;
         want = std::min<uint64_t>({(rounds + 1) / 2, (3 * CUS + wgs - 1) / wgs, 32});
-        if (wgs * 4 >= 3 * CUS) want = 1;
+        if ((wgs + CUS - 1) / CUS * CUS * 3 <= wgs * 4) want = 1;
     }
     want = std::max<uint64_t>(1, want);
     r.span = (uint32_t)std::min<uint64_t>((rounds + want - 1) / want * round, 0x40000000u);
@@ -1381,7 +1439,7 @@ hipError_t go_matrix(hipStream_t s, const AttnArgs& a, bool b16) {
     const uint64_t units = ((uint64_t)a.blocks * a.nsplit + 7) / 8 * 8 * a.kv.nkv;
     const uint64_t joins = ((uint64_t)a.bt.rows * a.nh + 3) / 4;
     if (units > 0x7fffffffull || joins > 0x7fffffffull) return hipErrorInvalidConfiguration;
-    if constexpr (VB > 32) paged_attention_tile_kernel<T, HD><<<(unsigned)units, TW * 64, 0, s>>>(a);
+    if constexpr (VB > 32) paged_attention_tile_kernel<T, HD><<<(unsigned)units, tile_waves<T, HD>() * 64, 0, s>>>(a);
     else if (b16) paged_attention_stream_kernel<T, HD, VB / 16, true><<<(unsigned)units, SW * 64, 0, s>>>(a);
     else paged_attention_stream_kernel<T, HD, VB / 16, false><<<(unsigned)units, SW * 64, 0, s>>>(a);
     hipError_t e = hipGetLastError();
@@ -1398,7 +1456,7 @@ hipError_t go_hd(hipStream_t s, const AttnArgs& a, const Plan& pl) {
         case 16: return go_matrix<T, HD, 16>(s, a, b16);
         case 32: return go_matrix<T, HD, 32>(s, a, b16);
     }
-    return go_matrix<T, HD, TVB>(s, a, b16);
+    return go_matrix<T, HD, 32 * tile_waves<T, HD>()>(s, a, b16);
 }
 template <class T>
 hipError_t go_attention(hipStream_t s, const AttnArgs& a, const Plan& pl) {
