@@ -1389,7 +1389,7 @@ hipError_t go_weight_sums(hipStream_t s, const SumsArgs& a, const bh_kv8_batch* 
     const uint64_t len = std::max<uint64_t>(1, hint->max_len ? std::min(hint->max_len, a.cap) : a.cap);
     const uint32_t most = a.bt.start ? (hint->max_rows ? std::min(hint->max_rows, a.bt.rows) : a.bt.rows) : 1;
     if ((uint64_t)most * a.group <= 32) return a.kv.hd == 128 ? go_sums<T, 128, 0>(s, a, len) : go_sums<T, 64, 0>(s, a, len);
-    const bool few = (uint64_t)a.bt.batch * a.kv.nkv * ((len + 255) / 256) < 256;
+    const bool few = (uint64_t)a.bt.batch * a.kv.nkv * ((len + 255) / 256) <= CUS;
     if (a.kv.hd == 128) return few ? go_sums<T, 128, 1>(s, a, len) : go_sums<T, 128, 4>(s, a, len);
     return few ? go_sums<T, 64, 1>(s, a, len) : go_sums<T, 64, 4>(s, a, len);
 }
@@ -1408,8 +1408,9 @@ Plan plan_attention(const Kv8& kv, const Kv8Rows& bt, const bh_kv8_batch* hint, 
     if ((kv.hd != 64 && kv.hd != 128) || kv.nslots == 0 || !aligned_to(kv.pool[0], 16) || !aligned_to(kv.pool[1], 16)) return r;
     const uint32_t most = bt.start ? (hint->max_rows ? std::min(hint->max_rows, bt.rows) : bt.rows) : 1;
     const uint64_t vectors = (uint64_t)most * group, all = (uint64_t)bt.rows * group;
-    r.kind = vectors <= 32 ? STREAM : TILE;
-    r.vb = vectors <= 16 ? 16 : vectors <= 32 ? 32 : dtype == BH_OUT_F32 && kv.hd == 128 ? 32 * tile_waves<F32, 128>() : 256;
+    const bool f32 = dtype == BH_OUT_F32;
+    r.kind = vectors * kv.hd * (f32 ? 4 : 2) <= 40960 ? STREAM : TILE;
+    r.vb = r.kind == TILE ? (f32 && kv.hd == 128 ? 32 * tile_waves<F32, 128>() : 256) : vectors <= 16 ? 16 : 32;
     r.blocks = !bt.start && group <= r.vb ? bt.batch : (uint32_t)(all / r.vb) + bt.batch;
     const uint64_t reach = std::min<uint64_t>((uint64_t)kv.max_bt * kv.bs, 0x7fff0000u);
     const uint64_t len = std::max<uint64_t>(1, hint->max_len ? std::min<uint64_t>(hint->max_len, reach) : reach);
@@ -1418,7 +1419,7 @@ Plan plan_attention(const Kv8& kv, const Kv8Rows& bt, const bh_kv8_batch* hint, 
     const uint64_t rounds = (len + round - 1) / round;
     uint64_t wgs = (uint64_t)r.blocks * kv.nkv, want;
     if (r.kind == STREAM) {
-        want = std::min<uint64_t>({rounds, (16 * CUS + wgs - 1) / wgs, 64});
+        want = std::min<uint64_t>({rounds, ((r.vb == 16 ? 16 : 4) * CUS + wgs - 1) / wgs, 64});
     } else {
         wgs = std::max<uint64_t>(1, all / r.vb) * kv.nkv;
         want = std::min<uint64_t>({(rounds + 1) / 2, (3 * CUS + wgs - 1) / wgs, 32});
