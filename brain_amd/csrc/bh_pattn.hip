@@ -139,7 +139,9 @@ constexpr uint32_t CUS = 256;  // compute units
 //
 // Up to 32 query vectors (rows x heads of one kv head) of a sequence at a time:
 // the cache is read once and each code used for few products, so the stream of
-// the codes bounds it. A wave takes 32 keys at a time straight into the operand
+// the codes bounds it (64 sequences of up to 8192 keys, one row of 32 heads over
+// 8 of 128, bf16: 905 MB in 178 us, 5.1 TB/s, where a large copy moves 4.9 and a
+// read alone 6.2). A wave takes 32 keys at a time straight into the operand
 // layout of v_mfma_f32_16x16x32_bf16 (codes are exact in bf16), the next 32 in
 // flight: no LDS, no barrier in the loop. Scores are computed transposed (keys x
 // queries): lane (c, g) = (l % 16, l / 16) then holds the scores of query c and
@@ -150,6 +152,9 @@ constexpr uint32_t CUS = 256;  // compute units
 // three products each, 24 bits. With bf16 activations the query is exact, and
 // the weight times its value scale is rounded to bf16, half a step 2^-9 of the
 // next power of two: the size of the output's own rounding.
+//
+// A single sequence of 2000 keys (16 heads over 8, f32) takes 5.9 us, the chain
+// of look-up, codes, products and the workgroup's sum; the join behind it 4 us.
 
 __device__ __forceinline__ uint32_t fbits(float f) { return __builtin_bit_cast(uint32_t, f); }
 __device__ __forceinline__ float bitsf(uint32_t u) { return __builtin_bit_cast(float, u); }
@@ -547,6 +552,12 @@ __global__ __launch_bounds__(SW * 64, (stream_waves<T, HD, NQ>())) void paged_at
 // the exponentials of another). A tile for which the bound says nothing, such as
 // a sequence's first, takes a step that looks at the scores and moves the
 // reference where one lies more than 2^SLACK above it.
+//
+// A prompt's last 2048 rows over 32768 keys, 32 heads over 8 of 128, bf16: 1.12
+// ms, 950 TFLOP/s, where a large library product reaches 1190 (the matrix unit is
+// busy for 41 % of the cycles and the vector unit, with 32 exponentials a lane
+// and tile, for 65 %; 1.94 GHz under that load). f32, three products for one: 1000
+// rows over 8000 keys in 407 us, 900 TFLOP/s of products.
 constexpr int TK = 64;  // keys of a tile
 // 2^(ROOM + 7) (codes) times value scales below VMOST times 2^28 keys is finite.
 constexpr float SLACK = 6.0f, ROOM = 72.0f, VMOST = 1048576.0f;
@@ -556,7 +567,11 @@ __device__ __forceinline__ v16f mfma32(v4i a, v4i b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
 }
 
-// Waves of a workgroup (one workgroup a compute unit: LDS), 32 query vectors each.
+// Waves of a workgroup (one workgroup a compute unit: LDS), 32 query vectors
+// each: four, so that each has a SIMD's registers, where f32 queries of 128 in
+// three parts need them (1000 rows over 8000 keys 407 us; eight waves spilled,
+// 470), else eight, which stage each tile for twice the queries (f32 of 64, 500
+// rows of 4 sequences over 3000 keys: 36 us, with four 46).
 template <class T, int HD>
 constexpr int tile_waves() {
     return sizeof(typename T::elem) == 4 && HD == 128 ? 4 : 8;
@@ -1049,7 +1064,9 @@ __global__ __launch_bounds__((tile_waves<T, HD>() * 64), (tile_waves<T, HD>() / 
 }
 
 // Joins the splits of a row and head, one wave for each: lane s takes split s's
-// maximum and sum (at most 64 splits), then all take their dimensions.
+// maximum and sum (at most 64 splits), then all take their dimensions, eight
+// splits' loads at once. Bound by the trip to memory, 4 us for few rows, and by
+// the splits' bytes for many (1443 rows of 28 heads of 128, three splits: 24 us).
 template <class T, int HD, int VB>
 __global__ __launch_bounds__(256) void paged_attention_join_kernel(AttnArgs p) {
     typedef typename T::elem E;
@@ -1108,6 +1125,8 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(AttnArgs p) {
 // four queries' scores of one key, so a key's sum needs no exchange until the
 // end, and its order is that of the rows. A workgroup takes 64 KG keys of one
 // kv head, and more of them when the grid (made for max_len) does not reach.
+// 1024 rows over 16384 keys, 32 heads over 8 of 128, bf16: 168 us, 790 TFLOP/s,
+// with an exponential, an fma and a sum for every 128 multiply-adds.
 template <class T, int HD, int KG>
 __global__ __launch_bounds__(256, 2) void paged_weight_sums_kernel(SumsArgs p) {
     typedef typename T::elem E;
@@ -1237,7 +1256,9 @@ __global__ __launch_bounds__(256, 2) void paged_weight_sums_kernel(SumsArgs p) {
 
 // Few query vectors (rows x heads of a kv head up to 32, or 32 at a time): they
 // stay in LDS and the keys stream by, each wave with the next 64 in flight and no
-// barrier between.
+// barrier between. 32 sequences of up to 4096 keys, one row of 16 heads over 8 of
+// 128, f32: 113 MB in 39 us, 2.9 TB/s; a wave has few steps, so that the latency
+// of the first look-ups and codes shows. (Look-ups a step further ahead: 43 us.)
 template <class T, int HD>
 __global__ __launch_bounds__(256, 2) void paged_weight_sums_stream_kernel(SumsArgs p) {
     typedef typename T::elem E;
@@ -1388,13 +1409,20 @@ hipError_t go_weight_sums(hipStream_t s, const SumsArgs& a, const bh_kv8_batch* 
     }
     const uint64_t len = std::max<uint64_t>(1, hint->max_len ? std::min(hint->max_len, a.cap) : a.cap);
     const uint32_t most = a.bt.start ? (hint->max_rows ? std::min(hint->max_rows, a.bt.rows) : a.bt.rows) : 1;
+    // One row of 32 sequences over 4096 keys: streaming 39 us, the tiles below 48;
+    // 7 rows of 16 (28 vectors): 20 and 24; 16 rows (64 vectors, twice the keys'
+    // stream): 32 and 25.
     if ((uint64_t)most * a.group <= 32) return a.kv.hd == 128 ? go_sums<T, 128, 0>(s, a, len) : go_sums<T, 64, 0>(s, a, len);
+    // Keys for each wave: 16 where chunks of 256 would give no compute unit a
+    // second workgroup (64 rows of 4 sequences over 2000 keys: 10.3 us, 13.4 with
+    // 64 keys), else 64, which read a query's fragment a quarter as often (1024 rows
+    // over 12000 keys: 178 us, 277 with 16; over 8192, at the limit, 165 and 164).
     const bool few = (uint64_t)a.bt.batch * a.kv.nkv * ((len + 255) / 256) <= CUS;
     if (a.kv.hd == 128) return few ? go_sums<T, 128, 1>(s, a, len) : go_sums<T, 128, 4>(s, a, len);
     return few ? go_sums<T, 64, 1>(s, a, len) : go_sums<T, 64, 4>(s, a, len);
 }
 
-// How a call is run.
+// How a call is run. PLAIN: any head_dim, any alignment.
 enum Kind { PLAIN, STREAM, TILE };
 struct Plan {
     Kind kind;
@@ -1409,6 +1437,13 @@ Plan plan_attention(const Kv8& kv, const Kv8Rows& bt, const bh_kv8_batch* hint, 
     const uint32_t most = bt.start ? (hint->max_rows ? std::min(hint->max_rows, bt.rows) : bt.rows) : 1;
     const uint64_t vectors = (uint64_t)most * group, all = (uint64_t)bt.rows * group;
     const bool f32 = dtype == BH_OUT_F32;
+    // By the bytes of a sequence's queries: up to 160 vectors of 128 in bf16 and 80
+    // in f32, 32 to a block, whose blocks find the codes in the caches. Streaming
+    // and tiles (kernel time): 63 vectors of 16 sequences over 8000 keys 42 and 92
+    // us (bf16), 79 and 137 (f32); 80 of 8 sequences 37 and 84, 68 and 124; 128 of
+    // one 23 and 22 (bf16), 41 and 28 (f32); 240 of 8 over 2000 keys 30 and 33
+    // (bf16), 105 of 16 over 16000 225 and 204 (f32). Heads of 64: 300 vectors of 8
+    // over 4000 keys 26 and 48 (bf16).
     r.kind = vectors * kv.hd * (f32 ? 4 : 2) <= 40960 ? STREAM : TILE;
     r.vb = r.kind == TILE ? (f32 && kv.hd == 128 ? 32 * tile_waves<F32, 128>() : 256) : vectors <= 16 ? 16 : 32;
     r.blocks = !bt.start && group <= r.vb ? bt.batch : (uint32_t)(all / r.vb) + bt.batch;
@@ -1419,8 +1454,15 @@ Plan plan_attention(const Kv8& kv, const Kv8Rows& bt, const bh_kv8_batch* hint, 
     const uint64_t rounds = (len + round - 1) / round;
     uint64_t wgs = (uint64_t)r.blocks * kv.nkv, want;
     if (r.kind == STREAM) {
+        // Workgroups a compute unit: of 16 vectors 16 (64 sequences of up to 8192
+        // keys: 178 us; 8: 202, 32: 185), of 32, with twice the state to join, 4 (80
+        // vectors of 8 sequences, f32: 68 us; 2: 73, 8: 91).
         want = std::min<uint64_t>({rounds, ((r.vb == 16 ? 16 : 4) * CUS + wgs - 1) / wgs, 64});
     } else {
+        // Three workgroups a compute unit, or no splits where whole rounds of one
+        // leave less than a quarter of the chip idle (1000 f32 rows over 8000 keys,
+        // 250 workgroups: 407 us, 480 in three splits; a mixed batch's 312: 324 us
+        // whole and 300 split).
         wgs = std::max<uint64_t>(1, all / r.vb) * kv.nkv;
         want = std::min<uint64_t>({(rounds + 1) / 2, (3 * CUS + wgs - 1) / wgs, 32});
         if ((wgs + CUS - 1) / CUS * CUS * 3 <= wgs * 4) want = 1;

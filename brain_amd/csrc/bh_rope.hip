@@ -130,7 +130,11 @@ __global__ __launch_bounds__(64) void qk_norm_rope_any_kernel(RopeRowsArgs p) {
 // elements 4i ..+3 of both halves, so a pair meets in a lane and a wave works on
 // 512 / HD heads at once. Memory traffic bounds it: a wave takes one row (or a
 // `part` of its heads, where there are few rows) and computes its angles once
-// for all of them; the next heads' loads are in flight while it works.
+// for all of them; the next heads' loads are in flight while it works. 8192 rows
+// of 32 + 8 heads of 128, bf16: 168 MB in 28 us, 6.0 TB/s (a part of it from the
+// last-level cache; a large copy moves 4.9). With the append, 2113 rows of 16 + 8 + 8
+// heads: 15.6 us, two waves a SIMD that each walk eight steps; one row of 16 + 8
+// heads 2.7 us, the latency of its loads and the angles.
 template <class T, int HD, bool APPEND>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeRowsArgs p, uint32_t parts) {
     typedef typename T::elem E;
@@ -257,7 +261,9 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeRowsArgs p, uint3
 template <class T, int HD, bool APPEND>
 hipError_t go_whole(hipStream_t s, const RopeRowsArgs& a) {
     const uint32_t heads = a.nh + a.nkv * (APPEND ? 2 : 1), groups = (heads + 512 / HD - 1) / (512 / HD);
-    // Waves for the whole chip first, then rows whose angles are computed once.
+    // Waves for the whole chip first, then rows whose angles are computed once:
+    // 4096 waves (512 rows of 40 heads: 5.6 us, 6.2 with 1024 waves; 4 times more
+    // are no faster).
     const uint32_t parts = std::min<uint32_t>(groups, std::max<uint32_t>(1, 4096 / a.rows));
     const uint64_t waves = (uint64_t)a.rows * parts;
     qk_norm_rope_kernel<T, HD, APPEND><<<(unsigned)((waves + 3) / 4), 256, 0, s>>>(a, parts);
