@@ -581,8 +581,10 @@ template <class T, int HD>
 __global__ __launch_bounds__((tile_waves<T, HD>() * 64), (tile_waves<T, HD>() / 4)) void paged_attention_tile_kernel(AttnArgs p) {
     typedef typename T::elem E;
     constexpr int TW = tile_waves<T, HD>(), TVB = 32 * TW;
-    constexpr int PARTS = sizeof(E) == 4 ? 3 : 1, NT = TW * 64, KB = TK * HD * 2, NBUF = 3;
-    __shared__ __attribute__((aligned(1024))) uint8_t kt[NBUF][KB], vt[NBUF][KB];
+    constexpr int PARTS = sizeof(E) == 4 ? 3 : 1, NT = TW * 64, NBUF = 3;
+    // Bytes in LDS: a key, a line of values, those of 32 keys, a tile of each.
+    constexpr int KROW = HD * 2 + 16, VROW = 256 + 16, VHALF = HD / 4 * VROW, KB = TK * KROW, VB = 2 * VHALF;
+    __shared__ __attribute__((aligned(1024))) uint8_t kt[NBUF][KB], vt[NBUF][VB];
     __shared__ __attribute__((aligned(16))) float scs[NBUF][2][TK];  // keys', values' scales
     __shared__ int kn2[NBUF][TK];                                      // |codes|^2 of each key
     __shared__ __attribute__((aligned(16))) uint64_t ring[4][TK];      // bytes to each key's slot
@@ -692,21 +694,22 @@ __global__ __launch_bounds__((tile_waves<T, HD>() * 64), (tile_waves<T, HD>() / 
     qn = dead ? 0.0f : qn < INFINITY ? qn : INFINITY;
     // LDS images. K: chunk c (8 d) of key r. V^T: 32 keys at a time, lines of 256
     // bytes hold 4 d x 32 keys, 8 keys a chunk in the order of a lane's scores:
-    // chunk 2u + h has keys 16u + 4h ..+3 and 16u + 8 + 4h ..+3. In both the 16
-    // lanes that meet go to 16 slots.
-    auto kchunk = [&](int r, int c) -> int { return r * (HD * 2) + ((HD == 128 ? c ^ (r & 15) : c ^ ((r >> 1) & 7)) << 4); };
+    // chunk 2u + h has keys 16u + 4h ..+3 and 16u + 8 + 4h ..+3. In both 16
+    // bytes of padding send the 16 lanes that meet to different banks (and leave the
+    // places of a lane's reads constants apart).
+    auto kchunk = [&](int r, int c) -> int { return r * KROW + (c << 4); };
     auto vchunk = [&](int d, int oc) -> int {
-        return (oc >> 2) * (64 * HD) + (d >> 2) * 256 + (((4 * (d & 3) + (oc & 3)) ^ ((d >> 2) & 15)) << 4);
+        return (oc >> 2) * VHALF + (d >> 2) * VROW + ((4 * (d & 3) + (oc & 3)) << 4);
     };
-    const int kst = klive ? kchunk(kkey, 2 * kpc) : 0;  // chunk 2 kpc + 1 is at kst ^ 16
+    const int kst = klive ? kchunk(kkey, 2 * kpc) : 0;
     // quad: keys 4 quad ..+3 = 16 u' + 4 x: chunk (quad / 4) * 2 + (quad & 1), its half (quad >> 1) & 1
     const int vst = vlive ? vchunk(4 * dg, 2 * (quad >> 2) + (quad & 1)) + 8 * ((quad >> 1) & 1) : 0;
     // Piece r: 16 n keys on, and 16 n values: the same place of a later line.
     auto store_k = [&](int bu, int r) __attribute__((always_inline)) {
         if (!klive) return;
-        uint8_t* at = kt[0] + bu * KB + r * (NT / CPK) * (HD * 2);
+        uint8_t* at = kt[0] + bu * KB + r * (NT / CPK) * KROW;
         *reinterpret_cast<v4i*>(at + kst) = codes8((uint32_t)raw.k[r][0], (uint32_t)raw.k[r][1]);
-        *reinterpret_cast<v4i*>(at + (kst ^ 16)) = codes8((uint32_t)raw.k[r][2], (uint32_t)raw.k[r][3]);
+        *reinterpret_cast<v4i*>(at + (kst + 16)) = codes8((uint32_t)raw.k[r][2], (uint32_t)raw.k[r][3]);
         int n2 = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) n2 = __builtin_amdgcn_sdot4(raw.k[r][i], raw.k[r][i], n2, false);
@@ -717,10 +720,10 @@ __global__ __launch_bounds__((tile_waves<T, HD>() * 64), (tile_waves<T, HD>() / 
     };
     auto store_v = [&](int bu, unsigned long long ok, int r) __attribute__((always_inline)) {
         if (vlive) {
-            uint8_t* at = vt[0] + bu * KB + r * (NT / DG / 8) * (64 * HD);
+            uint8_t* at = vt[0] + bu * VB + r * (NT / DG / 8) * VHALF;
 #pragma unroll
             for (int e = 0; e < 4; ++e)  // dimension 4 dg + e: chunk index + 4 e
-                *reinterpret_cast<uint2*>(at + (vst ^ (e << 6))) = make_uint2(
+                *reinterpret_cast<uint2*>(at + vst + (e << 6)) = make_uint2(
                     hi16x2(code_f(raw.v[r][0], e), code_f(raw.v[r][1], e)), hi16x2(code_f(raw.v[r][2], e), code_f(raw.v[r][3], e)));
         }
         if (r) return;
@@ -732,17 +735,16 @@ __global__ __launch_bounds__((tile_waves<T, HD>() * 64), (tile_waves<T, HD>() / 
 #pragma unroll
         for (int r = 0; r < PR; ++r) store_k(bu, r), store_v(bu, ok, r);
     };
-    static_assert(PR == 1 || ((NT / CPK) % 16 == 0 && (NT / DG) % 8 == 0), "the pieces' places");
+    static_assert(PR == 1 || (NT / DG) % 8 == 0, "the pieces' places");
     // Scores of half kh of the tile in buffer bu. Register e: key 32 kh +
     // 8 (e / 4) + 4 half + e % 4.
     auto scores = [&](int bu, int kh, v16f& s) __attribute__((always_inline)) {
-        int ka = bu * KB + kh * (64 * HD) + kchunk(col, half);  // chunk 2 d + half is at ka ^ (d << 5)
-        asm volatile("" : "+v"(ka));  // the others are not carried from tile to tile in registers
+        const int ka = bu * KB + kh * (32 * KROW) + kchunk(col, half);
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] = 0.0f;
 #pragma unroll
         for (int d = 0; d < HD / 16; ++d) {
-            const v4i k = *reinterpret_cast<const v4i*>(kt[0] + (ka ^ (d << 5)));
+            const v4i k = *reinterpret_cast<const v4i*>(kt[0] + ka + (d << 5));
 #pragma unroll
             for (int part = PARTS - 1; part >= 0; --part) s = mfma32(k, qf[d][part], s);
         }
@@ -817,11 +819,10 @@ __global__ __launch_bounds__((tile_waves<T, HD>() * 64), (tile_waves<T, HD>() / 
     };
     // Their product with the values.
     auto values = [&](int bu, int kh, int u, const v4i (&pf)[PARTS]) __attribute__((always_inline)) {
-        int va = bu * KB + kh * (64 * HD) + (vchunk(col, half) ^ (u << 5));  // vchunk(32 j + col, 2 u + half): see there
-        asm volatile("" : "+v"(va));
+        const int va = bu * VB + kh * VHALF + vchunk(col, half) + (u << 5);  // vchunk(32 j + col, 2 u + half)
 #pragma unroll
         for (int j = 0; j < HD / 32; ++j) {
-            const v4i v = *reinterpret_cast<const v4i*>(vt[0] + (va ^ ((j & 1) << 7)) + j * 2048);
+            const v4i v = *reinterpret_cast<const v4i*>(vt[0] + va + j * (8 * VROW));
 #pragma unroll
             for (int part = PARTS - 1; part >= 0; --part) o[j] = mfma32(v, pf[part], o[j]);
         }
@@ -887,18 +888,17 @@ __global__ __launch_bounds__((tile_waves<T, HD>() * 64), (tile_waves<T, HD>() / 
     v4i ka_[2];     // the first two operands of the next scores
     float4 kc_, vs_;  // scales of the next 4 keys
     auto fence = [&]() { __builtin_amdgcn_sched_barrier(0); };
-    auto kaddr = [&](int bu, int kh) -> int { return bu * KB + kh * (64 * HD) + kchunk(col, half); };
+    auto kaddr = [&](int bu, int kh) -> int { return bu * KB + kh * (32 * KROW) + kchunk(col, half); };
     auto prime = [&](int kbase, int bu, int kh) __attribute__((always_inline)) {
         kc_ = *reinterpret_cast<const float4*>(&scs[bu][0][32 * kh + 4 * half]);
         vs_ = *reinterpret_cast<const float4*>(&scs[bu][1][32 * kh + 4 * half]);
         ka_[0] = *reinterpret_cast<const v4i*>(kt[0] + kbase);
-        ka_[1] = *reinterpret_cast<const v4i*>(kt[0] + (kbase ^ 32));
+        ka_[1] = *reinterpret_cast<const v4i*>(kt[0] + kbase + 32);
     };
     auto calm_half = [&](int kh, int kbase, const v16f& s, v16f& nx, int nbase, int nbu, int nkh) __attribute__((always_inline)) {
         const float* kcp = &scs[b0][0][32 * kh + 4 * half];  // values' scales: TK floats on
-        int va0 = b0 * KB + kh * (64 * HD) + vchunk(col, half), va1 = va0 ^ 32;
-        asm volatile("" : "+v"(va0), "+v"(va1), "+v"(kbase));
-        auto vread = [&](int va, int j) -> v4i { return *reinterpret_cast<const v4i*>(vt[0] + (va ^ ((j & 1) << 7)) + j * 2048); };
+        const int va0 = b0 * VB + kh * VHALF + vchunk(col, half), va1 = va0 + 32;
+        auto vread = [&](int va, int j) -> v4i { return *reinterpret_cast<const v4i*>(vt[0] + va + j * (8 * VROW)); };
         float x[16];
         float4 kc[4], vs[4];
         v4i kf[NS], vf[2][NJ], pf[PARTS], pg[PARTS];
@@ -939,7 +939,7 @@ __global__ __launch_bounds__((tile_waves<T, HD>() * 64), (tile_waves<T, HD>() / 
 #pragma unroll
         for (int d = 0; d < NS; ++d) {
             products(kf[d], qf[d], nx);
-            if (d + 2 < NS) kf[d + 2] = *reinterpret_cast<const v4i*>(kt[0] + (kbase ^ ((d + 2) << 5)));
+            if (d + 2 < NS) kf[d + 2] = *reinterpret_cast<const v4i*>(kt[0] + kbase + ((d + 2) << 5));
             if constexpr (WIDE) {  // (of the slot after next, or the next)
                 if (EP * (d + 1) % 4 != 0 && EP * d / 4 < 3) scales(EP * d / 4 + 1);
                 if (EP == 4 && d < 3) scales(d + 1);
