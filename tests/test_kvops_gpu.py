@@ -669,3 +669,49 @@ def test_attention_large_value_scales(gpu, sign, dtype):
     out, got = run_attention(gpu, c, q.to(gpu), start, lens, 1.0)
     near(out, want, ob, "out")
     near(got, lse, lb, "lse")
+
+
+# ------------------------------------------------------------------ many rows and long sequences together
+
+# Drafts of a few blocks of query vectors over split keys; prompts' pieces with heads of 64 and 128.
+LONG = [([20, 1, 11], [3000, 2500, 700], 16, 4, 128, 16), ([9, 20], [1111, 2049], 16, 4, 128, 24), ([70, 5], [1500, 64], 8, 2, 64, 16),
+        ([400, 7], [900, 1300], 8, 2, 64, 16), ([150, 90], [1000, 90], 8, 2, 128, 5)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows,lens,nh,nkv,hd,bs", LONG)
+def test_attention_long(gpu, rows, lens, nh, nkv, hd, bs, dtype):
+    """With a block outside the pool, and an output that is not aligned."""
+    g = gen(sum(lens), nh, hd, bs, 3)
+    c = ref.Cache(g, len(rows), (max(lens) + bs - 1) // bs, bs, nkv, hd)
+    c.table[0, 300 // bs] = -1
+    start = ref.starts(rows)
+    total = int(start[-1])
+    q = torch.randn(total, nh, hd, generator=g).to(dtype)
+    want, lse, ob, lb = ref.attention(c, q, start, lens, 0.1)
+    for hints in ({}, dict(max_rows=max(rows), max_len=max(lens))):
+        room = torch.full((total * nh * hd + 1,), math.nan, dtype=dtype, device=gpu)
+        out, got = run_attention(gpu, c, q.to(gpu), start, lens, 0.1, out=room[1:].view(total, nh, hd), **hints)
+        near(out, want, ob, f"out {hints}")
+        near(got, lse, lb, f"lse {hints}")
+        assert bool(torch.isnan(room[0]))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows", [[20, 3, 0], [1, 1, 1]])
+def test_weight_sums_long(gpu, rows, hd, dtype):
+    """More keys than there are workgroups at once, with a block outside the pool."""
+    g = gen(sum(rows), hd, 4)
+    nh, nkv, bs, lens = 32, 8, 16, [3500, 3111, 3300]
+    c = ref.Cache(g, 3, (max(lens) + bs - 1) // bs, bs, nkv, hd)
+    c.table[1, 100] = -1
+    start = ref.starts(rows)
+    q = torch.randn(int(start[-1]), nh, hd, generator=g).to(dtype)
+    lse = ref.attention(c, q, start, lens, 0.1)[1].float()
+    acc = torch.rand(3, nkv, 3600, generator=g)
+    want, bound = ref.weight_sums(c, q, lse, start, lens, 0.1, acc)
+    dl = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    for hints in ({}, dict(max_rows=max(rows), max_len=max(lens))):
+        got = ops.paged_weight_sums_i8(q.to(gpu), lse.to(gpu), c.kv(ops, gpu), dl, acc.to(gpu), start.to(gpu), 0.1, **hints)
+        near(got, want, bound, f"acc {hints}")
