@@ -43,7 +43,7 @@ __device__ __forceinline__ void keep_all(const EvictArgs& p, uint32_t len, const
 // 4096 positions (8 heads of 1111: 7.7 us), of 16 up to 16384 (16 sequences of up
 // to 8192, 128 workgroups: 12.6 us, histograms and barriers in turn).
 template <int VPT>
-__global__ __launch_bounds__(ET) void kv_evict_select_kernel(EvictArgs p) {
+__device__ __forceinline__ void select_entries(EvictArgs p) {
     constexpr int NW = ET / 64, BINS = 2048;
     __shared__ uint32_t hist[BINS], wtot[NW], pick[2];
     const uint32_t b = blockIdx.x / p.kv.nkv, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -146,6 +146,11 @@ __global__ __launch_bounds__(ET) void kv_evict_select_kernel(EvictArgs p) {
     }
 }
 
+template <int VPT>
+__global__ __launch_bounds__(ET) void kv_evict_select_kernel(EvictArgs p) {
+    select_entries<VPT>(p);
+}
+
 // The same for any length, its weights read again for each digit (8 bits at a
 // time) and for the last pass, which goes through them in order.
 __global__ __launch_bounds__(ET) void kv_evict_select_long_kernel(EvictArgs p) {
@@ -231,29 +236,27 @@ __global__ __launch_bounds__(ET) void kv_evict_select_long_kernel(EvictArgs p) {
     }
 }
 
-// Moves the entries of a (sequence, kv head), keys or values. A thread takes a
-// piece of W, MU entries of a step at a time in flight. Position i's entry comes
-// from keep[i] >= i, so in place a workgroup goes through all of them in order:
-// what a step writes no later step reads, and a barrier between its reads and
-// its writes is enough. To other blocks the steps are spread over workgroups.
-// 16 sequences cut to 2048 entries of 8 heads of 128: 138 MB in 26 us, 5.3 TB/s.
+// Moves the entries of a (sequence, kv head), keys or values, from entry i0 on, in
+// strides of `step`, by threads tid of NT. A thread takes a piece of W, M entries of a
+// pass at a time in flight. Position i's entry comes from keep[i] >= i, so in place a workgroup
+// goes through all of them in order: what a pass writes no later pass reads, and a
+// barrier between its reads and its writes is enough.
 constexpr uint32_t MT = 256;
-constexpr int MU = 4;
-template <class W, bool IN_PLACE>
-__global__ __launch_bounds__(MT) void kv_evict_move_kernel(EvictArgs p, uint32_t steps, uint32_t per) {
-    const uint32_t group = blockIdx.x / steps, which = group & 1, bk = group >> 1, b = bk / p.kv.nkv, kvh = bk % p.kv.nkv;
-    const uint32_t pieces = p.kv.hd / sizeof(W), e = threadIdx.x / pieces, w = threadIdx.x % pieces;
+constexpr int MU = 4, SU = 8;  // M of the kernel for the move alone, and for both
+template <class W, bool IN_PLACE, uint32_t NT, int M>
+__device__ __forceinline__ void move_entries(const EvictArgs& p, uint32_t bk, uint32_t which, uint32_t tid, uint64_t i0,
+                                             uint64_t step) {
+    const uint32_t b = bk / p.kv.nkv, kvh = bk % p.kv.nkv;
+    const uint32_t pieces = p.kv.hd / sizeof(W), per = NT / pieces, e = tid / pieces, w = tid % pieces;
     const int32_t* keep = p.keep + (uint64_t)bk * p.budget;
-    if (kvh == 0 && blockIdx.x % (2 * steps * p.kv.nkv) == 0 && threadIdx.x == 0)
-        p.new_lens[b] = min(min(p.lens[b], p.cap), p.budget);
     uint8_t* pool = (uint8_t*)(which ? p.kv.pool[1] : p.kv.pool[0]) + (size_t)kvh * p.kv.hd + w * sizeof(W);
     float* scales = (which ? p.kv.scales[1] : p.kv.scales[0]) + kvh;
-    for (uint64_t i0 = (uint64_t)(blockIdx.x % steps) * MU * per; i0 < p.budget; i0 += (uint64_t)steps * MU * per) {
-        uint32_t from[MU], to[MU];
-        W c[MU];
-        float s[MU];
+    for (; i0 < p.budget; i0 += step) {
+        uint32_t from[M], to[M];
+        W c[M];
+        float s[M];
 #pragma unroll
-        for (int u = 0; u < MU; ++u) {
+        for (int u = 0; u < M; ++u) {
             const uint64_t i = i0 + u * per + e;
             const int32_t src = e < per && i < p.budget ? keep[i] : -1;
             const bool move = src >= 0 && !(IN_PLACE && (uint32_t)src == (uint32_t)i);
@@ -261,7 +264,7 @@ __global__ __launch_bounds__(MT) void kv_evict_move_kernel(EvictArgs p, uint32_t
             to[u] = move ? p.kv.slot_in(p.to, p.to_cols, b, (uint32_t)i) : NO_SLOT;
         }
 #pragma unroll
-        for (int u = 0; u < MU; ++u) {
+        for (int u = 0; u < M; ++u) {
             if (to[u] == NO_SLOT) from[u] = NO_SLOT;
             c[u] = W{};
             s[u] = 0.0f;
@@ -272,13 +275,40 @@ __global__ __launch_bounds__(MT) void kv_evict_move_kernel(EvictArgs p, uint32_t
         }
         if constexpr (IN_PLACE) __syncthreads();
 #pragma unroll
-        for (int u = 0; u < MU; ++u) {
+        for (int u = 0; u < M; ++u) {
             if (from[u] == NO_SLOT) continue;
             *reinterpret_cast<W*>(pool + p.kv.row(to[u])) = c[u];
             if (w == 0) scales[(uint64_t)to[u] * p.kv.nkv] = s[u];
         }
         if constexpr (IN_PLACE) __syncthreads();
     }
+}
+
+// To other blocks the passes are spread over `steps` workgroups. 16 sequences cut
+// to 2048 entries of 8 heads of 128: 138 MB in 26 us, 5.3 TB/s.
+template <class W, bool IN_PLACE>
+__global__ __launch_bounds__(MT) void kv_evict_move_kernel(EvictArgs p, uint32_t steps, uint32_t per) {
+    const uint32_t group = blockIdx.x / steps, bk = group >> 1;
+    if (bk % p.kv.nkv == 0 && blockIdx.x % (2 * steps * p.kv.nkv) == 0 && threadIdx.x == 0) {
+        const uint32_t b = bk / p.kv.nkv;
+        p.new_lens[b] = min(min(p.lens[b], p.cap), p.budget);
+    }
+    move_entries<W, IN_PLACE, MT, MU>(p, bk, group & 1, threadIdx.x, (uint64_t)(blockIdx.x % steps) * MU * per,
+                                      (uint64_t)steps * MU * per);
+}
+
+// Selection and move of a (sequence, kv head) in one workgroup, half of it moving
+// the keys and half the values.
+template <class W, bool IN_PLACE>
+__global__ __launch_bounds__(ET) void kv_evict_small_kernel(EvictArgs p) {
+    select_entries<4>(p);
+    __syncthreads();  // keep[] is written
+    if (blockIdx.x % p.kv.nkv == 0 && threadIdx.x == 0) {
+        const uint32_t b = blockIdx.x / p.kv.nkv;
+        p.new_lens[b] = min(min(p.lens[b], p.cap), p.budget);
+    }
+    const uint32_t per = ET / 2 / (p.kv.hd / (uint32_t)sizeof(W));
+    move_entries<W, IN_PLACE, ET / 2, SU>(p, blockIdx.x, threadIdx.x / (ET / 2), threadIdx.x % (ET / 2), 0, (uint64_t)SU * per);
 }
 
 template <class W>
@@ -327,11 +357,25 @@ extern "C" int bh_paged_kv_evict_i8(void* stream, const bh_kv8* kv, const uint32
     a.to_cols = a.in_place ? kv->max_blocks : out_max_blocks;
     a.cap = acc_stride, a.cap_out = acc_out_stride, a.budget = budget, a.sink = sink, a.recent = recent;
     const hipStream_t s = (hipStream_t)stream;
+    const bool wide = kv->head_dim % 16 == 0 && aligned_to(kv->k_pool, 16) && aligned_to(kv->v_pool, 16);
+    // One launch for few heads of few entries, where the host's two cost more than
+    // one workgroup's move (a sequence of 1111, 8 heads of 64, cut to 700: 12.1 us a
+    // call, 14.2 in two; kernel time 13.8 and 13.0. 128 heads of 512 by 128: kernel
+    // time 20 and 17.) Not where the new lengths may lie on the old ones, which other
+    // workgroups still read.
+    const bool apart = new_lens + batch <= seq_lens || seq_lens + batch <= new_lens;
+    if (acc_stride <= 4 * ET && heads <= 32 && (uint64_t)budget * kv->head_dim <= 65536 && apart) {
+        if (wide && a.in_place) kv_evict_small_kernel<uint4, true><<<(unsigned)heads, ET, 0, s>>>(a);
+        else if (wide) kv_evict_small_kernel<uint4, false><<<(unsigned)heads, ET, 0, s>>>(a);
+        else if (a.in_place) kv_evict_small_kernel<uint32_t, true><<<(unsigned)heads, ET, 0, s>>>(a);
+        else kv_evict_small_kernel<uint32_t, false><<<(unsigned)heads, ET, 0, s>>>(a);
+        const hipError_t e = hipGetLastError();
+        return e == hipSuccess ? BH_OK : fail(BH_ERR_HIP, "%s: %s", who, hipGetErrorString(e));
+    }
     if (acc_stride <= 4 * ET) kv_evict_select_kernel<4><<<(unsigned)heads, ET, 0, s>>>(a);
     else if (acc_stride <= 16 * ET) kv_evict_select_kernel<16><<<(unsigned)heads, ET, 0, s>>>(a);
     else kv_evict_select_long_kernel<<<(unsigned)heads, ET, 0, s>>>(a);
     hipError_t e = hipGetLastError();
-    const bool wide = kv->head_dim % 16 == 0 && aligned_to(kv->k_pool, 16) && aligned_to(kv->v_pool, 16);
     if (e == hipSuccess) e = wide ? go_move<uint4>(s, a, heads) : go_move<uint32_t>(s, a, heads);
     return e == hipSuccess ? BH_OK : fail(BH_ERR_HIP, "%s: %s", who, hipGetErrorString(e));
 }

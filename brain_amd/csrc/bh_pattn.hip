@@ -553,8 +553,8 @@ __global__ __launch_bounds__(SW * 64, (stream_waves<T, HD, NQ>())) void paged_at
 // a sequence's first, takes a step that looks at the scores and moves the
 // reference where one lies more than 2^SLACK above it.
 //
-// A prompt's last 2048 rows over 32768 keys, 32 heads over 8 of 128, bf16: 1.12
-// ms, 950 TFLOP/s, where a large library product reaches 1190 (the matrix unit is
+// A prompt's last 2048 rows over 32768 keys, 32 heads over 8 of 128, bf16: 1.10
+// ms, 970 TFLOP/s, where a large library product reaches 1190 (the matrix unit is
 // busy for 41 % of the cycles and the vector unit, with 32 exponentials a lane
 // and tile, for 65 %; 1.94 GHz under that load). f32, three products for one: 1000
 // rows over 8000 keys in 407 us, 900 TFLOP/s of products.

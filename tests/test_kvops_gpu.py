@@ -715,3 +715,23 @@ def test_weight_sums_long(gpu, rows, hd, dtype):
     for hints in ({}, dict(max_rows=max(rows), max_len=max(lens))):
         got = ops.paged_weight_sums_i8(q.to(gpu), lse.to(gpu), c.kv(ops, gpu), dl, acc.to(gpu), start.to(gpu), 0.1, **hints)
         near(got, want, bound, f"acc {hints}")
+
+
+@pytest.mark.parametrize("lens,budget,sink,recent,nkv,hd,bs", EVICT + [([900, 3, 1024, 700], 512, 4, 100, 3, 128, 16),
+                                                                       ([900, 3, 1024, 700], 513, 4, 100, 3, 128, 16)])
+def test_evict_lens_of_their_own(gpu, lens, budget, sink, recent, nkv, hd, bs):
+    """In place, the new lengths beside the old ones or in their place: the same cache, and the old lengths kept in the first case."""
+    g = gen(sum(lens), budget, hd, 5)
+    c = ref.Cache(g, len(lens), (max(lens) + bs - 1) // bs, bs, nkv, hd)
+    acc = torch.randn(len(lens), nkv, max(lens), generator=g).to(gpu)
+    dl = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    over, apart = c.kv(ops, gpu), c.kv(ops, gpu)
+    keep, new = ops.paged_kv_evict_i8(over, dl.clone(), acc, budget, sink, recent, new_lens=(same := dl.clone()))
+    ops.paged_kv_evict_i8(apart_ := c.kv(ops, gpu), same2 := dl.clone(), acc, budget, sink, recent, new_lens=same2)
+    keep2, new2 = ops.paged_kv_evict_i8(apart, dl, acc, budget, sink, recent)
+    want_keep, want_lens = ref.evict(lens, acc.cpu(), budget, sink, recent)
+    assert new is same and torch.equal(dl.cpu(), torch.tensor(lens, dtype=torch.int32))
+    for k, n in ((keep, new), (keep2, new2), (keep, same2)):
+        assert torch.equal(k.cpu(), want_keep) and torch.equal(n.cpu(), want_lens)
+    for t in ("k_pool", "v_pool", "k_scales", "v_scales"):
+        assert torch.equal(getattr(over, t), getattr(apart_, t)) and torch.equal(getattr(apart, t), getattr(apart_, t)), t
