@@ -47,7 +47,7 @@ __device__ __forceinline__ void select_entries(EvictArgs p) {
     constexpr int NW = ET / 64, BINS = 2048;
     __shared__ uint32_t hist[BINS], wtot[NW], pick[2];
     const uint32_t b = blockIdx.x / p.kv.nkv, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const uint32_t len = min(p.lens[b], p.cap);
+    const uint32_t len = min(kv_length(p.lens[b]), p.cap);
     const float* acc = p.acc + (uint64_t)blockIdx.x * p.cap;
     float* acc_out = p.acc_out ? p.acc_out + (uint64_t)blockIdx.x * p.cap_out : nullptr;
     int32_t* keep = p.keep + (uint64_t)blockIdx.x * p.budget;
@@ -156,7 +156,7 @@ __global__ __launch_bounds__(ET) void kv_evict_select_kernel(EvictArgs p) {
 __global__ __launch_bounds__(ET) void kv_evict_select_long_kernel(EvictArgs p) {
     __shared__ uint32_t hist[256], wtot[ET / 64], pick[2];
     const uint32_t b = blockIdx.x / p.kv.nkv, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const uint32_t len = min(p.lens[b], p.cap);
+    const uint32_t len = min(kv_length(p.lens[b]), p.cap);
     const float* acc = p.acc + (uint64_t)blockIdx.x * p.cap;
     float* acc_out = p.acc_out ? p.acc_out + (uint64_t)blockIdx.x * p.cap_out : nullptr;
     int32_t* keep = p.keep + (uint64_t)blockIdx.x * p.budget;
@@ -291,7 +291,7 @@ __global__ __launch_bounds__(MT) void kv_evict_move_kernel(EvictArgs p, uint32_t
     const uint32_t group = blockIdx.x / steps, bk = group >> 1;
     if (bk % p.kv.nkv == 0 && blockIdx.x % (2 * steps * p.kv.nkv) == 0 && threadIdx.x == 0) {
         const uint32_t b = bk / p.kv.nkv;
-        p.new_lens[b] = min(min(p.lens[b], p.cap), p.budget);
+        p.new_lens[b] = min(min(kv_length(p.lens[b]), p.cap), p.budget);
     }
     move_entries<W, IN_PLACE, MT, MU>(p, bk, group & 1, threadIdx.x, (uint64_t)(blockIdx.x % steps) * MU * per,
                                       (uint64_t)steps * MU * per);
@@ -305,7 +305,7 @@ __global__ __launch_bounds__(ET) void kv_evict_small_kernel(EvictArgs p) {
     __syncthreads();  // keep[] is written
     if (blockIdx.x % p.kv.nkv == 0 && threadIdx.x == 0) {
         const uint32_t b = blockIdx.x / p.kv.nkv;
-        p.new_lens[b] = min(min(p.lens[b], p.cap), p.budget);
+        p.new_lens[b] = min(min(kv_length(p.lens[b]), p.cap), p.budget);
     }
     const uint32_t per = ET / 2 / (p.kv.hd / (uint32_t)sizeof(W));
     move_entries<W, IN_PLACE, ET / 2, SU>(p, blockIdx.x, threadIdx.x / (ET / 2), threadIdx.x % (ET / 2), 0, (uint64_t)SU * per);

@@ -9,6 +9,7 @@
 
 #include "../../include/brain_hip.h"
 #include "bh_common.h"
+#include "bh_kvlen.h"
 
 namespace bh {
 
@@ -47,6 +48,7 @@ struct Kv8 {
         const uint64_t s = (uint64_t)tables[(uint64_t)b * cols + min(blk, cols - 1)] * bs + (j - blk * bs);
         return blk < cols && j < 0x80000000u && s < nslots ? (uint32_t)s : NO_SLOT;
     }
+    __device__ __forceinline__ uint32_t reach() const { return kv_reach(max_bt, bs); }
     __device__ __forceinline__ uint32_t slot(uint32_t b, uint32_t j) const { return slot_in(bt, max_bt, b, j); }
     __device__ __forceinline__ size_t row(uint32_t slot) const { return (size_t)slot * (nkv * hd); }  // bytes
 };
@@ -58,6 +60,7 @@ struct Kv8Rows {
     const uint32_t* lens;
     uint32_t batch, rows;
 
+    __device__ __forceinline__ uint32_t len(uint32_t b) const { return kv_length(lens[b]); }
     __device__ __forceinline__ uint32_t first(uint32_t b) const { return start ? min(start[b], rows) : min(b, rows); }
     __device__ __forceinline__ uint32_t end(uint32_t b) const { return start ? min(start[b + 1], rows) : min(b + 1, rows); }
 };

@@ -56,9 +56,9 @@ __global__ __launch_bounds__(64) void paged_attention_any_kernel(AttnArgs p) {
     uint32_t b = r;
     if (p.bt.start) b = wave_last(p.bt.batch, lane, [&](uint32_t i) { return p.bt.start[i] <= r; });
     if (b >= p.bt.batch) return;
-    const uint32_t e = p.bt.end(b), len = p.bt.lens[b];
+    const uint32_t r0 = p.bt.first(b), e = p.bt.end(b), len = p.bt.len(b);
     if (r >= e) return;
-    const uint32_t seen = len >= e - r ? len - (e - r) + 1 : 0;  // keys that the row sees
+    const uint32_t seen = min(kv_keys_seen(len, e - r0, r - r0), p.kv.reach());  // keys that the row sees
     for (uint32_t d = lane; d < hd; d += 64) qv[d] = T::get((const E*)p.q + r * p.qs + (uint64_t)h * hd + d);
     __syncthreads();
     const bool live = 4 * lane < hd;
@@ -107,7 +107,7 @@ __global__ __launch_bounds__(64) void paged_weight_sums_any_kernel(SumsArgs p, u
     typedef typename T::elem E;
     const uint32_t bk = blockIdx.x / nchunk, j = (blockIdx.x % nchunk) * 64 + threadIdx.x;
     const uint32_t b = bk / p.kv.nkv, kvh = bk % p.kv.nkv, hd = p.kv.hd;
-    const uint32_t len = p.bt.lens[b];
+    const uint32_t len = p.bt.len(b);
     if (j >= len || j >= p.cap) return;
     const uint32_t r0 = p.bt.first(b), r1 = p.bt.end(b), n = r1 > r0 ? r1 - r0 : 0u;
     const uint32_t slot = p.kv.slot(b, j);
@@ -214,7 +214,7 @@ template <int VB>
 __device__ __forceinline__ bool find_block(const Kv8Rows& bt, uint32_t group, uint32_t blk, uint32_t lane, Block& o) {
     uint32_t b, r0, r1;
     if (bt.start && bt.batch < 64) {  // one round trip: lane i has row_start[i] and sequence i's length
-        const uint32_t st = min(bt.start[min(lane, bt.batch)], bt.rows), ln = bt.lens[min(lane, bt.batch - 1)];
+        const uint32_t st = min(bt.start[min(lane, bt.batch)], bt.rows), ln = bt.len(min(lane, bt.batch - 1));
         asm volatile("" ::"v"(ln));  // both on their way before the branch
         const unsigned long long m = __ballot(lane < bt.batch && st * group / VB + lane <= blk);
         if (!m) return false;
@@ -227,7 +227,7 @@ __device__ __forceinline__ bool find_block(const Kv8Rows& bt, uint32_t group, ui
         else b = wave_last(bt.batch, lane, [&](uint32_t i) { return bt.first(i) * group / VB + i <= blk; });
         b = __builtin_amdgcn_readfirstlane((int)b);
         if (b >= bt.batch) return false;
-        r0 = bt.first(b), r1 = bt.end(b), o.len = bt.lens[b];
+        r0 = bt.first(b), r1 = bt.end(b), o.len = bt.len(b);
     }
     if (r1 <= r0) return false;
     o.b = b, o.r0 = r0, o.n = r1 - r0, o.nv = o.n * group;
@@ -236,7 +236,7 @@ __device__ __forceinline__ bool find_block(const Kv8Rows& bt, uint32_t group, ui
 }
 // The number of keys that row i of a block's sequence sees.
 __device__ __forceinline__ uint32_t keys_seen(const Block& o, uint32_t i) {
-    return o.len + i + 1 > o.n && o.len + i + 1 > i ? o.len + i + 1 - o.n : 0u;
+    return kv_keys_seen(o.len, o.n, i);
 }
 
 constexpr int SW = 4;  // waves
@@ -264,7 +264,7 @@ __global__ __launch_bounds__(SW * 64, (stream_waves<T, HD, NQ>())) void paged_at
     const uint32_t blk = p.by_nsplit.of(unit), split = unit - blk * p.nsplit;
     Block bl;
     if (!find_block<VB>(p.bt, p.group, blk, lane, bl)) return;
-    const uint32_t reach = (uint32_t)min((uint64_t)p.kv.max_bt * p.kv.bs, (uint64_t)0x7fff0000u);
+    const uint32_t reach = p.kv.reach();
     const uint32_t vend = min(bl.v0 + VB, bl.nv);
     const uint32_t kend = min(keys_seen(bl, p.by_group.of(vend - 1)), reach);  // keys that any of the vectors sees
     const uint32_t kall = min(keys_seen(bl, p.by_group.of(bl.v0)), reach);       // ... that all see
@@ -598,7 +598,7 @@ __global__ __launch_bounds__((tile_waves<T, HD>() * 64), (tile_waves<T, HD>() / 
     const uint32_t blk = p.by_nsplit.of(unit), split = unit - blk * p.nsplit;
     Block bl;
     if (!find_block<TVB>(p.bt, p.group, blk, lane, bl)) return;
-    const uint32_t reach = (uint32_t)min((uint64_t)p.kv.max_bt * p.kv.bs, (uint64_t)0x7fff0000u);
+    const uint32_t reach = p.kv.reach();
     const uint32_t vend = min(bl.v0 + TVB, bl.nv);
     const uint32_t kend = min(keys_seen(bl, p.by_group.of(vend - 1)), reach);
     const uint32_t k0 = split * p.span, k1 = split + 1 == p.nsplit ? kend : min(kend, k0 + p.span);
@@ -1082,9 +1082,9 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(AttnArgs p) {
     bl.b = b, bl.r0 = p.bt.first(b);
     const uint32_t r1 = p.bt.end(b);
     if (r >= r1) return;
-    bl.n = r1 - bl.r0, bl.nv = bl.n * p.group, bl.len = p.bt.lens[b];
+    bl.n = r1 - bl.r0, bl.nv = bl.n * p.group, bl.len = p.bt.len(b);
     const uint32_t v = (r - bl.r0) * p.group + h % p.group, blk = block_at<VB>(p.bt, p.group, b, bl.r0) + v / VB;
-    const uint32_t reach = (uint32_t)min((uint64_t)p.kv.max_bt * p.kv.bs, (uint64_t)0x7fff0000u);
+    const uint32_t reach = p.kv.reach();
     const uint32_t kend = min(keys_seen(bl, (min((v / VB + 1) * VB, bl.nv) - 1) / p.group), reach);  // of the vector's block
     const uint32_t live = max(1u, min(p.nsplit, (kend + p.span - 1) / p.span));                  // splits that had keys
     const uint64_t at = ((uint64_t)blk * p.nsplit * nkv + kvh) * VB + v % VB, far = (uint64_t)nkv * VB;
@@ -1144,7 +1144,7 @@ __global__ __launch_bounds__(256, 2) void paged_weight_sums_kernel(SumsArgs p) {
     const uint32_t r1 = p.bt.end(bl.b);
     bl.r0 = p.bt.first(bl.b);
     bl.n = r1 > bl.r0 ? r1 - bl.r0 : 0u;
-    bl.nv = bl.n * p.group, bl.v0 = 0, bl.len = p.bt.lens[bl.b];
+    bl.nv = bl.n * p.group, bl.v0 = 0, bl.len = p.bt.len(bl.b);
     const uint32_t end = min(bl.len, p.cap), kvs = nkv * HD;
     float* acc = p.acc + ((uint64_t)bl.b * nkv + kvh) * p.cap;
     auto kchunk = [&](int r, int ch) -> int { return r * (HD * 2) + ((HD == 128 ? ch ^ (r & 15) : ch ^ ((r >> 1) & 7)) << 4); };
@@ -1274,10 +1274,10 @@ __global__ __launch_bounds__(256, 2) void paged_weight_sums_stream_kernel(SumsAr
     Block bl;
     bl.b = p.by_nchunk.of(unit);
     const uint32_t r1 = p.bt.end(bl.b);
-    bl.r0 = p.bt.first(bl.b), bl.len = p.bt.lens[bl.b];
+    bl.r0 = p.bt.first(bl.b), bl.len = p.bt.len(bl.b);
     if (r1 <= bl.r0) return;
     bl.n = r1 - bl.r0, bl.nv = bl.n * p.group, bl.v0 = 0;
-    const uint32_t end = min(min(bl.len, p.cap), 0x7fff0000u), kvs = nkv * HD;
+    const uint32_t end = min(min(bl.len, p.cap), KV_REACH), kvs = nkv * HD;
     float* acc = p.acc + ((uint64_t)bl.b * nkv + kvh) * p.cap;
     auto kchunk = [&](int r, int ch) -> int { return r * (HD * 2) + ((HD == 128 ? ch ^ (r & 15) : ch ^ ((r >> 1) & 7)) << 4); };
     constexpr int QE = HD / 8;
@@ -1447,7 +1447,7 @@ Plan plan_attention(const Kv8& kv, const Kv8Rows& bt, const bh_kv8_batch* hint, 
     r.kind = vectors * kv.hd * (f32 ? 4 : 2) <= 40960 ? STREAM : TILE;
     r.vb = r.kind == TILE ? (f32 && kv.hd == 128 ? 32 * tile_waves<F32, 128>() : 256) : vectors <= 16 ? 16 : 32;
     r.blocks = !bt.start && group <= r.vb ? bt.batch : (uint32_t)(all / r.vb) + bt.batch;
-    const uint64_t reach = std::min<uint64_t>((uint64_t)kv.max_bt * kv.bs, 0x7fff0000u);
+    const uint64_t reach = kv_reach(kv.max_bt, kv.bs);
     const uint64_t len = std::max<uint64_t>(1, hint->max_len ? std::min<uint64_t>(hint->max_len, reach) : reach);
     // Splits of whole rounds: 32 keys for each wave, or two tiles.
     const uint32_t round = 128;
@@ -1585,7 +1585,7 @@ extern "C" int bh_paged_weight_sums_i8(void* stream, const void* q, uint64_t q_s
     SumsArgs a{};
     const int rc = check_call(who, kv, batch, n_heads, dtype, q_stride, &a.kv, &a.bt);
     if (rc) return rc;
-    if (acc_stride > 0x7fff0000u) return fail(BH_ERR_INVALID, "%s: acc_stride %u", who, acc_stride);
+    if (acc_stride > KV_REACH) return fail(BH_ERR_INVALID, "%s: acc_stride %u", who, acc_stride);
     if (batch->rows == 0 || batch->batch == 0 || acc_stride == 0) return BH_OK;
     if (!q || !lse || !acc) return fail(BH_ERR_INVALID, "%s: null buffer", who);
     a.q = q, a.qs = q_stride, a.lse = lse, a.acc = acc, a.cap = acc_stride;

@@ -41,7 +41,7 @@ __device__ __forceinline__ void turn(uint32_t pos, double freq, float& c, float&
 __device__ __forceinline__ bool row_slot(const Kv8& kv, const Kv8Rows& bt, uint32_t r, uint32_t lane, uint32_t& slot) {
     uint32_t b = r, e, len;
     if (bt.start && bt.batch < 64) {  // one round trip: lane i has row_start[i] and sequence i's length
-        const uint32_t st = min(bt.start[min(lane, bt.batch)], bt.rows), ln = bt.lens[min(lane, bt.batch - 1)];
+        const uint32_t st = min(bt.start[min(lane, bt.batch)], bt.rows), ln = bt.len(min(lane, bt.batch - 1));
         asm volatile("" ::"v"(ln));  // both on their way before the branch
         const unsigned long long m = __ballot(lane < bt.batch && st <= r);
         if (!m) return false;
@@ -51,7 +51,7 @@ __device__ __forceinline__ bool row_slot(const Kv8& kv, const Kv8Rows& bt, uint3
     } else {
         if (bt.start) b = wave_last(bt.batch, lane, [&](uint32_t i) { return bt.start[i] <= r; });
         if (b >= bt.batch) return false;
-        e = bt.end(b), len = bt.lens[b];
+        e = bt.end(b), len = bt.len(b);
     }
     if (r >= e) return false;
     slot = len < e - r ? NO_SLOT : kv.slot(b, len - (e - r));

@@ -253,7 +253,9 @@ typedef struct {
  * (ascending; none is fine; rows from row_start[batch] on are left as they
  * are), and they are the last of its seq_lens[b] positions: row i of n sits at
  * position seq_lens[b] - n + i. A row whose position that makes negative is
- * stored nowhere and sees no key. max_rows and max_len are the most rows and the longest length that the program knows
+ * stored nowhere and sees no key; a length below zero (as an int32) is one of 0,
+ * and positions that the table has no room for are keys that are not there.
+ * max_rows and max_len are the most rows and the longest length that the program knows
  * of: they choose how the work is split (0: not known), the results of a call
  * hold without them. */
 typedef struct {
@@ -323,7 +325,7 @@ int bh_paged_weight_sums_i8(void* stream, const void* q, uint64_t q_stride, int 
  * turned by its position stays so. Each block written to must belong to one
  * sequence, and, unless in place, be none that is read; out_tables has room for min(budget, acc_stride, the cache's
  * max_blocks * block_size) positions. seq_lens[b] past
- * acc_stride counts as acc_stride. new_lens may be seq_lens. An entry kept whose position has no slot (a table entry
+ * acc_stride counts as acc_stride, and one below zero (as an int32) as 0. new_lens may be seq_lens. An entry kept whose position has no slot (a table entry
  * outside the pool) does not move: its new place holds what it held. */
 int bh_paged_kv_evict_i8(void* stream, const bh_kv8* kv, const uint32_t* seq_lens, uint32_t batch, const float* acc,
                          uint32_t acc_stride, uint32_t budget, uint32_t sink, uint32_t recent,

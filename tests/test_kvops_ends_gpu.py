@@ -1,0 +1,53 @@
+"""The int8 paged cache's operators where their arguments end: lengths, sizes and values that programs do have, and that the
+parametrised cases of tests/test_kvops_gpu.py do not."""
+import math
+
+import pytest
+import torch
+
+import kvref as ref
+from brain_amd import ops
+from test_kvops_gpu import BF16, F32, gen, joined, near
+
+pytestmark = pytest.mark.gpu
+
+# rows, heads, kv heads, head_dim, block size: each kernel of attention and of the weight sums.
+KERNELS = [(1, 4, 2, 36, 8), (3, 4, 2, 64, 16), (60, 4, 2, 128, 16), (300, 4, 2, 64, 24), (3, 2, 1, 96, 5)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("n,nh,nkv,hd,bs", KERNELS)
+def test_lengths_below_zero_and_past_the_table(gpu, n, nh, nkv, hd, bs, dtype):
+    """Sequences that are off (-1 and other lengths below zero) see, store and keep nothing; one that is longer than its table
+    sees what the table has."""
+    g = gen(n, hd, bs, 31)
+    lens = [-1, 50, -5, 0x7FFFFFFF, -(1 << 31), 64]
+    c = ref.Cache(g, len(lens), -(-64 // bs), bs, nkv, hd, spare=6)
+    room = c.table.shape[1] * bs
+    start = ref.starts([1, n, n, n, 2, 1])
+    total = int(start[-1])
+    q = torch.randn(total, nh, hd, generator=g).to(dtype)
+    # The same for the plain forms: no length is 0, and the long one's rows all lie behind the table.
+    plain = [max(0, min(t, room + n)) for t in lens]
+    want, lse, ob, lb = ref.attention(c, q, start, plain, 0.1)
+    dl, ds = torch.tensor(lens, dtype=torch.int32, device=gpu), start.to(gpu)
+    acc = torch.rand(len(lens), nkv, room, generator=g)
+    new, bound = ref.weight_sums(c, q, lse.float(), start, plain, 0.1, acc)
+    for hints in ({}, dict(max_rows=n, max_len=room)):
+        kv = c.kv(ops, gpu)
+        out, got = ops.paged_attention_i8(q.to(gpu), kv, dl, ds, 0.1, **hints)
+        near(out, want, ob, f"out {hints}")
+        near(got, lse, lb, f"lse {hints}")
+        near(ops.paged_weight_sums_i8(q.to(gpu), lse.float().to(gpu), kv, dl, acc.to(gpu), ds, 0.1, **hints), new, bound, f"acc {hints}")
+    x, cut = joined(g, total, nh, nkv, hd, dtype)
+    dq, dk, dv = cut(x.to(gpu))
+    kv = c.kv(ops, gpu)
+    ops.qk_norm_rope_append_i8(dq, dk, dv, torch.zeros(total, dtype=torch.int32, device=gpu), ops.rope_frequencies(hd, 1e4), kv, dl, ds)
+    stored = sorted(s for b in (1, 5) for _, k in ref.chunk_rows(start, lens, b) if k > 0 and (s := c.slot(b, k - 1)) >= 0)
+    assert (kv.v_scales.cpu() != c.scales[1]).any(1).nonzero().view(-1).tolist() == stored
+    kv = c.kv(ops, gpu)
+    keep, new_lens = ops.paged_kv_evict_i8(kv, dl, acc.to(gpu), 20)
+    want_keep, want_lens = ref.evict(plain, acc, 20, 0, 0)
+    assert torch.equal(keep.cpu(), want_keep) and torch.equal(new_lens.cpu(), want_lens)
+    off = torch.tensor([c.slot(b, j) for b in (0, 2, 4) for j in range(room)])
+    assert torch.equal(kv.k_scales.cpu()[off], c.scales[0][off])
