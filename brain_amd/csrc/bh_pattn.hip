@@ -680,17 +680,24 @@ __global__ __launch_bounds__((tile_waves<T, HD>() * 64), (tile_waves<T, HD>() / 
     load(0, raw);
     load(1, second);
     __builtin_amdgcn_sched_barrier(0);
-    float qn = 0.0f;
+    float qn = 0.0f, qm = 0.0f;
     v4i qf[HD / 16][PARTS];
 #pragma unroll
     for (int t = 0; t < HD / 16; ++t) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) qn = qn + qx[t][e] * qx[t][e];
+        for (int e = 0; e < 8; ++e) {
+            qn = qn + qx[t][e] * qx[t][e];
+            qm = fmaxf(qm, fabsf(qx[t][e]));
+        }
         split8<PARTS>(qx[t], qf[t]);
     }
-    // Above |q|, whatever the roundings; infinite or NaN (no bound: a NaN here
-    // would be lost in the maximum) becomes infinite.
-    qn = sqrtf(qn + xor_lane<32>(qn)) * 1.001f;
+    // Above |q|, whatever the roundings: from 2^-100 on a sum of squares has lost
+    // less than a 2^-18th to those below f32's range; one below that (1e-25 each:
+    // all of it) gives way to HD times the largest. Infinite or NaN (no bound: a
+    // NaN here would be lost in the maximum) becomes infinite.
+    qn = qn + xor_lane<32>(qn);
+    qm = fmaxf(qm, xor_lane<32>(qm));
+    qn = (qn < 0x1p-100f ? qm * sqrtf((float)HD) : sqrtf(qn)) * 1.001f;
     qn = dead ? 0.0f : qn < INFINITY ? qn : INFINITY;
     // LDS images. K: chunk c (8 d) of key r. V^T: 32 keys at a time, lines of 256
     // bytes hold 4 d x 32 keys, 8 keys a chunk in the order of a lane's scores:

@@ -51,3 +51,24 @@ def test_lengths_below_zero_and_past_the_table(gpu, n, nh, nkv, hd, bs, dtype):
     assert torch.equal(keep.cpu(), want_keep) and torch.equal(new_lens.cpu(), want_lens)
     off = torch.tensor([c.slot(b, j) for b in (0, 2, 4) for j in range(room)])
     assert torch.equal(kv.k_scales.cpu()[off], c.scales[0][off])
+
+
+@pytest.mark.parametrize("n,nh,nkv,hd,dtype", [(60, 4, 2, 128, F32), (90, 4, 2, 64, F32), (100, 4, 2, 128, BF16), (300, 4, 2, 64, BF16)])
+def test_tiny_queries_over_large_key_scales(gpu, n, nh, nkv, hd, dtype):
+    """Queries whose squares are below f32's range, key scales that make up for it: scores of some hundred binades behind a
+    first part of small ones, over several tiles."""
+    g = gen(n, hd, 32)
+    bs, t = 16, 700
+    c = ref.Cache(g, 1, -(-t // bs), bs, nkv, hd)
+    # A score's deviation: 1e-25 * 73 * sqrt(hd) * scale.
+    for j in range(t):
+        c.scales[0][c.slot(0, j)] = (3.0 if j < 150 else 50.0) / (73 * hd ** 0.5) * 1e25
+    start, lens = ref.starts([n]), [t]
+    q = (torch.randn(n, nh, hd, generator=g) * 1e-25).to(dtype)
+    want, lse, ob, lb = ref.attention(c, q, start, lens, 1.0)
+    assert float(lse.min()) > 80 and float(ob.max()) < 0.1 * float(want.abs().max())
+    out, got = ops.paged_attention_i8(q.to(gpu), c.kv(ops, gpu), torch.tensor(lens, dtype=torch.int32, device=gpu), start.to(gpu), 1.0)
+    near(got, lse, lb, "lse")
+    # A weight of less than 2^-126 of its row's largest lies below f32's range and may be lost (the bounds count roundings
+    # only): at most that for each of the t keys, whose values are at most 127 * 1.2 / 60 (kvref.Cache's scales).
+    near(out, want, ob + t * 2.0 ** -126 * 127 * 1.2 / 60, "out")
