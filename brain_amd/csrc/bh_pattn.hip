@@ -25,8 +25,8 @@ struct AttnArgs {
     // The matrix kernels: blocks of query vectors, splits of the keys, what the
     // splits leave for the join.
     uint32_t blocks, nsplit, span;  // span: keys of a split
-    float* part;                    // [unit][kv head][vectors][hd], then
-    float2* ml;                     // [unit][kv head][vectors] maximum and sum
+    float* part;                    // [row][head][split][hd], then
+    float2* ml;                     // [row][head][split] maximum and sum
     uint32_t ovec;                  // outputs lie at multiples of 4 elements
 };
 struct SumsArgs {
@@ -516,15 +516,15 @@ __global__ __launch_bounds__(SW * 64, (stream_waves<T, HD, NQ>())) void paged_at
                 acc[i + 2] = acc[i + 2] + x.z * a, acc[i + 3] = acc[i + 3] + x.w * a;
             }
         }
+        const uint32_t iv = p.by_group.of(v);
+        const uint64_t row = (uint64_t)(bl.r0 + iv) * p.nh + kvh * p.group + (v - iv * p.group);
         if (p.nsplit > 1) {
-            const uint64_t at = ((uint64_t)unit * nkv + kvh) * VB + 16 * q + mv;
+            const uint64_t at = row * p.nsplit + split;
 #pragma unroll
             for (int i = 0; i < DT; i += 4)
                 *reinterpret_cast<float4*>(p.part + at * HD + d0 + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
             if (d0 == 0) p.ml[at] = make_float2(mm, ll);
         } else {
-            const uint32_t i = p.by_group.of(v);
-            const uint64_t row = (uint64_t)(bl.r0 + i) * p.nh + kvh * p.group + (v - i * p.group);
             E* dst = (E*)p.out + row * HD + d0;
 #pragma unroll
             for (int i = 0; i < DT; ++i) T::put(dst + i, ll == 0.0f ? 0.0f : acc[i] / ll);
@@ -1042,8 +1042,10 @@ __global__ __launch_bounds__((tile_waves<T, HD>() * 64), (tile_waves<T, HD>() / 
     const uint32_t v = wv0 + col;
     l = l + xor_lane<32>(l);
     if (v >= vend) return;
+    const uint32_t iv = p.by_group.of(v);
+    const uint64_t row = (uint64_t)(bl.r0 + iv) * p.nh + kvh * p.group + (v - iv * p.group);
     if (p.nsplit > 1) {
-        const uint64_t at = ((uint64_t)unit * nkv + kvh) * TVB + (v - bl.v0);
+        const uint64_t at = row * p.nsplit + split;
 #pragma unroll
         for (int j = 0; j < HD / 32; ++j)
 #pragma unroll
@@ -1053,8 +1055,6 @@ __global__ __launch_bounds__((tile_waves<T, HD>() * 64), (tile_waves<T, HD>() / 
         if (half == 0) p.ml[at] = make_float2(m, l);
         return;
     }
-    const uint32_t iv = p.by_group.of(v);
-    const uint64_t row = (uint64_t)(bl.r0 + iv) * p.nh + kvh * p.group + (v - iv * p.group);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     E* dst = (E*)p.out + row * HD;
 #pragma unroll
@@ -1077,9 +1077,9 @@ __global__ __launch_bounds__((tile_waves<T, HD>() * 64), (tile_waves<T, HD>() / 
 template <class T, int HD, int VB>
 __global__ __launch_bounds__(256) void paged_attention_join_kernel(AttnArgs p) {
     typedef typename T::elem E;
-    const uint32_t lane = threadIdx.x & 63, nkv = p.kv.nkv;
+    const uint32_t lane = threadIdx.x & 63;
     const uint32_t rh = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
-    const uint32_t r = rh / p.nh, h = rh % p.nh, kvh = h / p.group;
+    const uint32_t r = rh / p.nh, h = rh % p.nh;
     if (r >= p.bt.rows) return;
     uint32_t b = r;
     if (p.bt.start) b = wave_last(p.bt.batch, lane, [&](uint32_t i) { return p.bt.start[i] <= r; });
@@ -1090,12 +1090,12 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(AttnArgs p) {
     const uint32_t r1 = p.bt.end(b);
     if (r >= r1) return;
     bl.n = r1 - bl.r0, bl.nv = bl.n * p.group, bl.len = p.bt.len(b);
-    const uint32_t v = (r - bl.r0) * p.group + h % p.group, blk = block_at<VB>(p.bt, p.group, b, bl.r0) + v / VB;
+    const uint32_t v = (r - bl.r0) * p.group + h % p.group;
     const uint32_t reach = p.kv.reach();
     const uint32_t kend = min(keys_seen(bl, (min((v / VB + 1) * VB, bl.nv) - 1) / p.group), reach);  // of the vector's block
     const uint32_t live = max(1u, min(p.nsplit, (kend + p.span - 1) / p.span));                  // splits that had keys
-    const uint64_t at = ((uint64_t)blk * p.nsplit * nkv + kvh) * VB + v % VB, far = (uint64_t)nkv * VB;
-    const float2 ml = lane < live ? p.ml[at + lane * far] : make_float2(-INFINITY, 0.0f);
+    const uint64_t at = (uint64_t)rh * p.nsplit;
+    const float2 ml = lane < live ? p.ml[at + lane] : make_float2(-INFINITY, 0.0f);
     const float mm = xor_max<32>(ml.x), ref = mm == -INFINITY ? 0.0f : mm;
     const float a = __builtin_amdgcn_exp2f(ml.x - ref);
     const float ll = xor_sum<32>(lane < live ? ml.y * a : 0.0f);
@@ -1109,7 +1109,7 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(AttnArgs p) {
 #pragma unroll
         for (int u = 0; u < 8; ++u)
 #pragma unroll
-            for (int i = 0; i < DL; ++i) x[u][i] = src[min(s0 + u, live - 1) * far * HD + i];
+            for (int i = 0; i < DL; ++i) x[u][i] = src[min(s0 + u, live - 1) * HD + i];
         __builtin_amdgcn_sched_barrier(0);  // all on their way
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
@@ -1477,8 +1477,12 @@ Plan plan_attention(const Kv8& kv, const Kv8Rows& bt, const bh_kv8_batch* hint, 
     want = std::max<uint64_t>(1, want);
     r.span = (uint32_t)std::min<uint64_t>((rounds + want - 1) / want * round, 0x40000000u);
     r.nsplit = (uint32_t)((len + r.span - 1) / r.span);
+    // Partial sums have places by row and head, not by a block's vectors: a single
+    // token beside a long chunk, whose block is nearly empty, needs its own row only
+    // (63 single tokens and 256 rows of 32 heads of 128 over up to 8192 keys: 112
+    // MiB, by blocks 1519).
     if (r.nsplit > 1) {
-        r.ml_pairs = (uint64_t)r.blocks * r.nsplit * kv.nkv * r.vb;
+        r.ml_pairs = (uint64_t)bt.rows * nh * r.nsplit;
         r.part_floats = r.ml_pairs * kv.hd;
     }
     return r;

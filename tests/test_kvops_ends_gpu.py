@@ -1,12 +1,14 @@
 """The int8 paged cache's operators where their arguments end: lengths, sizes and values that programs do have, and that the
 parametrised cases of tests/test_kvops_gpu.py do not."""
+import ctypes as C
 import math
 
 import pytest
 import torch
 
 import kvref as ref
-from brain_amd import ops
+from brain_amd import load, ops
+from brain_amd._lib import Kv8BatchT, check
 from test_kvops_gpu import BF16, F32, gen, joined, near
 
 pytestmark = pytest.mark.gpu
@@ -72,3 +74,33 @@ def test_tiny_queries_over_large_key_scales(gpu, n, nh, nkv, hd, dtype):
     # A weight of less than 2^-126 of its row's largest lies below f32's range and may be lost (the bounds count roundings
     # only): at most that for each of the t keys, whose values are at most 127 * 1.2 / 60 (kvref.Cache's scales).
     near(out, want, ob + t * 2.0 ** -126 * 127 * 1.2 / 60, "out")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("many,n,hd", [(20, 70, 128), (70, 150, 64), (33, 300, 128)])
+def test_single_tokens_beside_a_chunk(gpu, many, n, hd, dtype):
+    """Dozens of single tokens and one prompt piece in a batch, keys split; with a workspace of exactly the size asked for."""
+    g = gen(many, n, hd)
+    nh, nkv, bs = 8, 4, 16
+    rows = [1] * many
+    rows.insert(many // 3, n)
+    rows.insert(2, 0)
+    lens = [max(r, int(torch.randint(1, 1400, (1,), generator=g))) for r in rows]
+    lens[many // 2] = 1400
+    c = ref.Cache(g, len(rows), -(-1400 // bs), bs, nkv, hd)
+    start = ref.starts(rows)
+    total = int(start[-1])
+    q = torch.randn(total, nh, hd, generator=g).to(dtype)
+    want, lse, ob, lb = ref.attention(c, q, start, lens, 0.1)
+    kv, dq, dl, ds = c.kv(ops, gpu), q.to(gpu), torch.tensor(lens, dtype=torch.int32, device=gpu), start.to(gpu)
+    for max_rows in (0, n, 1):
+        b, need = Kv8BatchT(ds.data_ptr(), dl.data_ptr(), len(rows), total, max_rows, 1400), C.c_uint64()
+        check(load().bh_paged_attention_i8_workspace(kv.ref, C.byref(b), nh, C.byref(need)))
+        assert need.value > 0
+        ws = torch.full((need.value // 4 + 64,), math.nan, device=gpu)
+        out, got = torch.full_like(dq, math.nan), torch.full((total, nh), math.nan, device=gpu)
+        check(load().bh_paged_attention_i8(torch.cuda.current_stream().cuda_stream, dq.data_ptr(), nh * hd, ops._ACT[dtype], nh,
+                                           kv.ref, C.byref(b), 0.1, out.data_ptr(), got.data_ptr(), ws.data_ptr(), need.value))
+        near(out, want, ob, f"out {max_rows}")
+        near(got, lse, lb, f"lse {max_rows}")
+        assert bool(torch.isnan(ws[need.value // 4:]).all()), "behind the workspace"
