@@ -284,7 +284,8 @@ class PagedKV8:
     n_kv * head_dim bytes a slot) and f32 scales [slots, n_kv] for keys and
     values, block_tables [batch, max_blocks] int32. Position j of sequence b is
     slot block_tables[b, j // block_size] * block_size + j % block_size. Holds
-    the tensors; make it once for a cache."""
+    the tensors and their addresses, so its attributes are fixed: make it once
+    for a cache, and another one for other tensors (a table that has grown)."""
 
     def __init__(self, k_pool, v_pool, k_scales, v_scales, block_tables, block_size, head_dim):
         if head_dim <= 0 or head_dim % 4 or head_dim > 256:
@@ -306,9 +307,14 @@ class PagedKV8:
         self.block_tables, self.block_size, self.head_dim, self.n_kv = block_tables, block_size, head_dim, n_kv
         self.desc = Kv8T(_ptr(k_pool), _ptr(v_pool), _ptr(k_scales), _ptr(v_scales), words, slots * n_kv,
                          _ptr(block_tables), block_tables.shape[1], block_size, n_kv, head_dim)
-        self.ref = C.byref(self.desc)
         self.sequences = block_tables.shape[0]
         self.needs = {}  # workspace bytes of paged_attention_i8, by the sizes of the call
+        self.ref = C.byref(self.desc)
+
+    def __setattr__(self, name, value):
+        if "ref" in self.__dict__:  # (the calls read desc: a tensor put here would not reach them)
+            raise AttributeError(f"PagedKV8.{name} is fixed; make another PagedKV8 for other tensors")
+        super().__setattr__(name, value)
 
 
 def _heads(t, dtype, hd, name):
