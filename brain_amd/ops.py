@@ -279,6 +279,11 @@ def _stream_of(dev):
     return _stream()
 
 
+# The C entries take sizes of 32 bits, and ctypes cuts what is longer without a
+# word: sizes that could be are checked here.
+_MOST = 0x7fffffff
+
+
 class PagedKV8:
     """An int8 paged KV cache (bh_kv8): pools of int32 words (4 codes each,
     n_kv * head_dim bytes a slot) and f32 scales [slots, n_kv] for keys and
@@ -290,11 +295,13 @@ class PagedKV8:
     def __init__(self, k_pool, v_pool, k_scales, v_scales, block_tables, block_size, head_dim):
         if head_dim <= 0 or head_dim % 4 or head_dim > 256:
             raise ValueError(f"PagedKV8: head_dim {head_dim}, a multiple of 4 up to 256")
-        if block_size <= 0:
+        if not 0 < block_size <= _MOST:
             raise ValueError(f"PagedKV8: block_size {block_size}")
         if k_scales.dim() != 2 or block_tables.dim() != 2:
             raise ValueError("PagedKV8: scales [slots, n_kv] and block_tables [batch, max_blocks] expected")
         slots, n_kv = k_scales.shape
+        if n_kv * head_dim > _MOST or block_tables.shape[1] > _MOST or block_tables.shape[0] > _MOST // 2:
+            raise ValueError(f"PagedKV8: {n_kv} kv heads, block_tables {tuple(block_tables.shape)}")
         words = slots * n_kv * head_dim // 4
         for name, t, dtype, numel in (("k_pool", k_pool, torch.int32, words), ("v_pool", v_pool, torch.int32, words),
                                       ("k_scales", k_scales, torch.float32, slots * n_kv),
@@ -325,6 +332,8 @@ def _heads(t, dtype, hd, name):
     if len(shape) != 3 or shape[2] != hd:
         raise ValueError(f"{name}: shape {tuple(shape)}, expected [rows, heads, {hd}]")
     rows, heads, _ = shape
+    if rows * heads > _MOST:
+        raise ValueError(f"{name}: {rows} rows of {heads} heads")
     rs, hs, es = t.stride()
     if es != 1 or (heads > 1 and hs != hd) or (rows > 1 and rs < heads * hd):
         raise ValueError(f"{name}: strides {t.stride()}; the heads of a row must lie side by side")
@@ -352,6 +361,8 @@ def _qk_rows(dev, q, k, v, positions, inv_freq, q_weight, k_weight, eps):
     if dtype not in _ACT:
         raise ValueError(f"q: dtype {dtype}, expected float32 or bfloat16")
     hd = q.shape[-1]
+    if hd > 256:
+        raise ValueError(f"q: head_dim {hd}, a multiple of 4 up to 256")
     rows, nh, qs = _heads(q, dtype, hd, "q")
     k_rows, nkv, ks = _heads(k, dtype, hd, "k")
     if k_rows != rows:
@@ -486,7 +497,7 @@ def paged_weight_sums_i8(q, lse, cache, seq_lens, acc, row_start=None, scale=Non
     from 0. Returns acc."""
     rows, nh, stride, batch = _queries(q, cache, seq_lens, row_start, max_rows, max_len)
     _need(lse, torch.float32, rows * nh, "lse")
-    if acc.dim() != 3 or acc.shape[0] < batch.batch or acc.shape[1] != cache.n_kv:
+    if acc.dim() != 3 or acc.shape[0] < batch.batch or acc.shape[1] != cache.n_kv or acc.shape[2] > _MOST:
         raise ValueError(f"acc: shape {tuple(acc.shape)}, expected [{batch.batch}, {cache.n_kv}, cap]")
     _need(acc, torch.float32, 0, "acc")
     _here(cache.dev, seq_lens, row_start, lse, acc)
@@ -510,19 +521,19 @@ def paged_kv_evict_i8(cache, seq_lens, acc, budget, sink=0, recent=0, out_tables
     _need(acc, torch.float32, 0, "acc")
     if batch > cache.sequences:
         raise ValueError(f"seq_lens: {batch} sequences, block_tables has {cache.sequences}")
-    if acc.dim() != 3 or acc.shape[0] < batch or acc.shape[1] != cache.n_kv:
+    if acc.dim() != 3 or acc.shape[0] < batch or acc.shape[1] != cache.n_kv or acc.shape[2] > _MOST:
         raise ValueError(f"acc: shape {tuple(acc.shape)}, expected [{batch}, {cache.n_kv}, cap]")
-    if budget <= 0 or sink < 0 or recent < 0 or sink + recent > budget:
+    if not 0 < budget <= _MOST or sink < 0 or recent < 0 or sink + recent > budget:
         raise ValueError(f"budget {budget} with sink {sink} and recent {recent}")
     to_ptr = to_cols = out_ptr = out_cap = 0
     if out_tables is not None:
         _need(out_tables, torch.int32, 0, "out_tables")
-        if out_tables.dim() != 2 or out_tables.shape[0] < batch:
+        if out_tables.dim() != 2 or out_tables.shape[0] < batch or out_tables.shape[1] > _MOST:
             raise ValueError(f"out_tables: shape {tuple(out_tables.shape)}, expected [{batch}, blocks]")
         to_ptr, to_cols = out_tables.data_ptr(), out_tables.shape[1]
     if acc_out is not None:
         _need(acc_out, torch.float32, 0, "acc_out")
-        if acc_out.dim() != 3 or acc_out.shape[0] < batch or acc_out.shape[1] != cache.n_kv:
+        if acc_out.dim() != 3 or acc_out.shape[0] < batch or acc_out.shape[1] != cache.n_kv or acc_out.shape[2] > _MOST:
             raise ValueError(f"acc_out: shape {tuple(acc_out.shape)}, expected [{batch}, {cache.n_kv}, >= {budget}]")
         out_ptr, out_cap = acc_out.data_ptr(), acc_out.shape[2]
     if keep is None:
