@@ -25,6 +25,7 @@ __device__ __forceinline__ uint32_t place(float v) {
 }
 
 constexpr uint32_t ET = 1024;
+constexpr uint32_t CUS = 256;  // compute units
 
 // A sequence within its budget keeps all.
 __device__ __forceinline__ void keep_all(const EvictArgs& p, uint32_t len, const float* acc, float* acc_out, int32_t* keep) {
@@ -358,13 +359,21 @@ extern "C" int bh_paged_kv_evict_i8(void* stream, const bh_kv8* kv, const uint32
     a.cap = acc_stride, a.cap_out = acc_out_stride, a.budget = budget, a.sink = sink, a.recent = recent;
     const hipStream_t s = (hipStream_t)stream;
     const bool wide = kv->head_dim % 16 == 0 && aligned_to(kv->k_pool, 16) && aligned_to(kv->v_pool, 16);
-    // One launch for few heads of few entries, where the host's two cost more than
-    // one workgroup's move (a sequence of 1111, 8 heads of 64, cut to 700: 12.1 us a
-    // call, 14.2 in two; kernel time 13.8 and 13.0. 128 heads of 512 by 128: kernel
-    // time 20 and 17.) Not where the new lengths may lie on the old ones, which other
-    // workgroups still read.
+    // One launch where it is no slower. In place a workgroup of its own walks each
+    // head's entries in two launches as well, with half the threads and a head's
+    // keys and values apart: one launch up to a head for each compute unit (time in
+    // a graph, us, one launch and two: 8 heads of 64, 1111 positions cut to 700, 14.0
+    // and 18.4; 256 heads of 128, 4000 cut to 2048, 69 and 81; 512 heads of 64, 1111
+    // cut to 700, 42 and 38). To other blocks two launches spread the move over the
+    // chip, so one is for few pieces of few heads, where the second launch costs more
+    // than it saves (the same, and between calls in a row: 32 heads of 64, 1111 cut
+    // to 512, 12.1 and 12.8, 12.3 and 14.9; to 704, at the limit, 13.1 and 13.0, 13.1
+    // and 14.9; to 896, 14.3 and 13.0, 14.4 and 15.3; 64 heads, 4000 cut to 640, 17.1
+    // and 15.4, 16.9 and 15.7). Not where the new lengths may lie on the old ones,
+    // which other workgroups still read.
     const bool apart = new_lens + batch <= seq_lens || seq_lens + batch <= new_lens;
-    if (acc_stride <= 4 * ET && heads <= 32 && (uint64_t)budget * kv->head_dim <= 65536 && apart) {
+    const uint64_t pieces = (uint64_t)budget * (kv->head_dim / (wide ? 16 : 4));
+    if (acc_stride <= 4 * ET && apart && (a.in_place ? heads <= CUS : heads <= 32 && pieces <= 2816)) {
         if (wide && a.in_place) kv_evict_small_kernel<uint4, true><<<(unsigned)heads, ET, 0, s>>>(a);
         else if (wide) kv_evict_small_kernel<uint4, false><<<(unsigned)heads, ET, 0, s>>>(a);
         else if (a.in_place) kv_evict_small_kernel<uint32_t, true><<<(unsigned)heads, ET, 0, s>>>(a);

@@ -104,3 +104,33 @@ def test_single_tokens_beside_a_chunk(gpu, many, n, hd, dtype):
         near(out, want, ob, f"out {max_rows}")
         near(got, lse, lb, f"lse {max_rows}")
         assert bool(torch.isnan(ws[need.value // 4:]).all()), "behind the workspace"
+
+
+@pytest.mark.parametrize("batch,nkv,hd,bs,cap,budget,in_place", [
+    (4, 8, 64, 16, 900, 704, False), (4, 8, 64, 16, 900, 705, False), (5, 7, 64, 8, 300, 100, False), (2, 3, 36, 7, 700, 312, False),
+    (2, 3, 36, 7, 700, 313, False), (1, 2, 128, 32, 4096, 3000, True), (1, 2, 128, 32, 4097, 3000, True), (32, 8, 16, 4, 90, 50, True),
+    (33, 8, 16, 4, 90, 50, True), (9, 2, 36, 5, 1100, 1000, True)])
+def test_evict_in_one_launch_or_two(gpu, batch, nkv, hd, bs, cap, budget, in_place):
+    """Either side of each limit that chooses how the eviction is launched; lengths around the budget among the long ones."""
+    g = gen(batch, nkv, hd, cap, budget)
+    c = ref.Cache(g, batch, -(-cap // bs), bs, nkv, hd, spare=batch * -(-budget // bs))
+    lens = torch.randint(budget, cap + 1, (batch,), generator=g).tolist()
+    lens[0] = cap
+    lens[-1] = [budget, budget - 1, cap][batch % 3]
+    acc = torch.randn(batch, nkv, cap, generator=g)
+    to = c.table if in_place else c.free.view(batch, -1).contiguous()
+    kv, dl = c.kv(ops, gpu), torch.tensor(lens, dtype=torch.int32, device=gpu)
+    out = torch.zeros(batch, nkv, budget, device=gpu)
+    keep, new = ops.paged_kv_evict_i8(kv, dl, acc.to(gpu), budget, 3, 20, None if in_place else to.to(gpu), out)
+    want, want_lens = ref.evict(lens, acc, budget, 3, 20)
+    assert torch.equal(keep.cpu(), want) and torch.equal(new.cpu(), want_lens)
+    assert torch.equal(dl.cpu(), torch.tensor(lens, dtype=torch.int32))
+    live, at = want >= 0, want.long().clamp_min(0)
+    assert torch.equal(out.cpu(), torch.where(live, acc.gather(2, at), torch.zeros(())))
+    slots = lambda t, j: t.long().gather(1, j.flatten(1) // bs).view(j.shape) * bs + j % bs  # noqa: E731
+    src, dst = slots(c.table, at), slots(to, torch.arange(budget).expand_as(at))
+    head = torch.arange(nkv)[None, :, None].expand_as(at)
+    for w, (pool, sc) in enumerate(((kv.k_pool, kv.k_scales), (kv.v_pool, kv.v_scales))):
+        codes, scales = c.codes[w].clone(), c.scales[w].clone()
+        codes[dst[live], head[live]], scales[dst[live], head[live]] = c.codes[w][src[live], head[live]], c.scales[w][src[live], head[live]]
+        assert torch.equal(pool.cpu().view(torch.int8).view(codes.shape), codes) and torch.equal(sc.cpu(), scales)
