@@ -134,3 +134,70 @@ def test_evict_in_one_launch_or_two(gpu, batch, nkv, hd, bs, cap, budget, in_pla
         codes, scales = c.codes[w].clone(), c.scales[w].clone()
         codes[dst[live], head[live]], scales[dst[live], head[live]] = c.codes[w][src[live], head[live]], c.scales[w][src[live], head[live]]
         assert torch.equal(pool.cpu().view(torch.int8).view(codes.shape), codes) and torch.equal(sc.cpu(), scales)
+
+
+@pytest.mark.parametrize("batch", [63, 64, 65])
+@pytest.mark.parametrize("hd,dtype", [(64, F32), (128, BF16), (36, F32)])
+def test_as_many_sequences_as_lanes(gpu, batch, hd, dtype):
+    """Batches at the wave's width, where the look-up of a row's sequence changes; empty sequences first, last and between."""
+    g = gen(batch, hd, 41)
+    nh, nkv, bs = 4, 2, 16
+    rows = torch.randint(0, 4, (batch,), generator=g).tolist()
+    rows[0] = rows[-1] = rows[-2] = 0
+    rows[batch // 2] = 9
+    lens = [max(r, int(torch.randint(0, 90, (1,), generator=g))) for r in rows]
+    c = ref.Cache(g, batch, 6, bs, nkv, hd)
+    start = ref.starts(rows)
+    total, pad = int(start[-1]), 3
+    dl, ds = torch.tensor(lens, dtype=torch.int32, device=gpu), start.to(gpu)
+    q = torch.randn(total + pad, nh, hd, generator=g).to(dtype)
+    want, lse, ob, lb = ref.attention(c, q, start, lens, 0.1)
+    acc = torch.rand(batch, nkv, 96, generator=g)
+    given = lse.float()
+    new, bound = ref.weight_sums(c, q, given, start, lens, 0.1, acc)
+    for hints in ({}, dict(max_rows=9, max_len=90)):
+        out = torch.full((total + pad, nh, hd), math.nan, dtype=dtype, device=gpu)
+        got = torch.full((total + pad, nh), math.nan, device=gpu)
+        kv = c.kv(ops, gpu)
+        ops.paged_attention_i8(q.to(gpu), kv, dl, ds, 0.1, out=out, lse=got, **hints)
+        near(out, want, ob, f"out {hints}")
+        near(got, lse, lb, f"lse {hints}")
+        near(ops.paged_weight_sums_i8(q.to(gpu), given.to(gpu), kv, dl, acc.to(gpu), ds, 0.1, **hints), new, bound, f"acc {hints}")
+    x, cut = joined(g, total + pad, nh, nkv, hd, dtype)
+    dq, dk, dv = cut(x.to(gpu))
+    kv = c.kv(ops, gpu)
+    q_out = torch.full((total + pad, nh, hd), 7.0, dtype=dtype, device=gpu)
+    ops.qk_norm_rope_append_i8(dq, dk, dv, torch.zeros(total + pad, dtype=torch.int32, device=gpu), ops.rope_frequencies(hd, 1e4), kv,
+                               dl, ds, q_out=q_out)
+    assert torch.equal(q_out[:total], dq[:total]) and bool((q_out[total:] == 7.0).all())  # no norm, no turn at position 0
+    where = [(r, c.slot(b, n - 1)) for b in range(batch) for r, n in ref.chunk_rows(start, lens, b)]
+    r, slots = torch.tensor([a for a, _ in where]), torch.tensor([s for _, s in where])
+    v = cut(x)[2][r].float()
+    # A code is within half a step of its scale, which is the largest element's 127th part.
+    scale = v.abs().amax(-1) / 127
+    got_scale = kv.v_scales.cpu()[slots]
+    assert bool(((got_scale - scale).abs() <= 2 * ref.EPS * scale).all())
+    codes = kv.v_pool.cpu().view(torch.int8).view(-1, nkv, hd)[slots].double()
+    assert bool(((codes - v.double() / got_scale.double()[..., None]).abs() <= 0.5 + 127 * 2 * ref.EPS).all())
+    rest = torch.ones(c.slots, dtype=torch.bool)
+    rest[slots] = False
+    assert torch.equal(kv.v_scales.cpu()[rest], c.scales[1][rest]) and torch.equal(kv.k_scales.cpu()[rest], c.scales[0][rest])
+
+
+@pytest.mark.parametrize("hd", [64, 128, 100])
+def test_norm_of_extremes_in_keys(gpu, hd):
+    """Zero, huge and non-finite heads among the keys: as the same values among the queries, each head for itself."""
+    q = torch.ones(4, 2, hd)
+    q[0, 0] = 0.0
+    q[1, 0] = 1e15
+    q[2, 0, 3] = math.inf
+    q[3, 1, 5] = math.nan
+    freq, pos, w = ops.rope_frequencies(hd, 1e4), torch.arange(4, dtype=torch.int32, device=gpu), torch.full((hd,), 0.5, device=gpu)
+    oq, ok = (t.cpu() for t in ops.qk_norm_rope(q.to(gpu), q.to(gpu), pos, freq, w, w))
+    assert torch.equal(torch.isnan(oq), torch.isnan(ok)) and torch.equal(oq.nan_to_num(9.0), ok.nan_to_num(9.0))
+    finite = torch.ones(4, 2, dtype=torch.bool)
+    finite[2, 0] = finite[3, 1] = False
+    want, bound = ref.turn(q, w.cpu(), 1e-6, pos.cpu(), freq.cpu())
+    for name, t in (("q", oq), ("k", ok)):
+        near(t[finite], want[finite], bound[finite] + ref.EPS * want[finite].abs(), name)
+        assert bool(torch.isnan(t[3, 1]).all()) and bool(torch.isnan(t[2, 0]).any())
