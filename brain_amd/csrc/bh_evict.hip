@@ -42,7 +42,8 @@ __device__ __forceinline__ void keep_all(const EvictArgs& p, uint32_t len, const
 // but exponents, a few bins for all weights to queue at); then a count of each
 // wave's kept entries says where it writes them. 1024 threads of 4 entries up to
 // 4096 positions (8 heads of 1111: 7.7 us), of 16 up to 16384 (16 sequences of up
-// to 8192, 128 workgroups: 12.6 us, histograms and barriers in turn).
+// to 8192, 128 workgroups, half the chip: 12.6 to 15.8 us from run to run,
+// histograms and barriers in turn).
 template <int VPT>
 __device__ __forceinline__ void select_entries(EvictArgs p) {
     constexpr int NW = ET / 64, BINS = 2048;
@@ -286,7 +287,9 @@ __device__ __forceinline__ void move_entries(const EvictArgs& p, uint32_t bk, ui
 }
 
 // To other blocks the passes are spread over `steps` workgroups. 16 sequences cut
-// to 2048 entries of 8 heads of 128: 138 MB in 26 us, 5.3 TB/s.
+// to 2048 entries of 8 heads of 128: 138 MB in 26 us, 5.3 TB/s. In place a head's
+// passes follow one another in one workgroup: the same eviction 72 us, 41 to other
+// blocks (calls in a row, with the selection).
 template <class W, bool IN_PLACE>
 __global__ __launch_bounds__(MT) void kv_evict_move_kernel(EvictArgs p, uint32_t steps, uint32_t per) {
     const uint32_t group = blockIdx.x / steps, bk = group >> 1;

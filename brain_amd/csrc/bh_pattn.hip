@@ -46,7 +46,9 @@ __device__ __forceinline__ float code_f(uint32_t w, int e) { return (float)(int8
 
 // Any head_dim: one wave for each row and query head. A lane takes a key for
 // the score and four elements of the context for the weighted sum, 64 keys at
-// a time, with a running maximum and sum.
+// a time, with a running maximum and sum. No matrix instructions, no split of the
+// keys, and each query head reads its keys anew: 32 rows of 16 heads over 8 of 96,
+// up to 4096 keys, bf16: 1.54 ms for traffic of 34 us; 256 rows 1.50 ms.
 template <class T>
 __global__ __launch_bounds__(64) void paged_attention_any_kernel(AttnArgs p) {
     typedef typename T::elem E;
@@ -101,7 +103,8 @@ __global__ __launch_bounds__(64) void paged_attention_any_kernel(AttnArgs p) {
     if (p.lse && lane == 0) p.lse[(uint64_t)r * p.nh + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
 }
 
-// Any head_dim: a thread for each (sequence, kv head, key).
+// Any head_dim: a thread for each (sequence, kv head, key), which goes through the
+// chunk's queries in order (the same batches: 200 us for 17 of traffic, 2.1 ms).
 template <class T>
 __global__ __launch_bounds__(64) void paged_weight_sums_any_kernel(SumsArgs p, uint32_t nchunk) {
     typedef typename T::elem E;
@@ -553,11 +556,14 @@ __global__ __launch_bounds__(SW * 64, (stream_waves<T, HD, NQ>())) void paged_at
 // a sequence's first, takes a step that looks at the scores and moves the
 // reference where one lies more than 2^SLACK above it.
 //
-// A prompt's last 2048 rows over 32768 keys, 32 heads over 8 of 128, bf16: 1.10
-// ms, 970 TFLOP/s, where a large library product reaches 1190 (the matrix unit is
-// busy for 41 % of the cycles and the vector unit, with 32 exponentials a lane
-// and tile, for 65 %; 1.94 GHz under that load). f32, three products for one: 1000
-// rows over 8000 keys in 407 us, 900 TFLOP/s of products.
+// A prompt's last 2048 rows over 32768 keys, 32 heads over 8 of 128, bf16: 1.10 to
+// 1.17 ms by the card, 910 to 970 TFLOP/s, where a large library product reaches
+// 1190 (the matrix unit is busy for 41 % of the cycles and the vector unit, with 32
+// exponentials a lane and tile, for 65 %; 1.94 GHz under that load). f32, three products for one: 1000
+// rows over 8000 keys in 407 us, 900 TFLOP/s of products. One kernel serves a call, chosen
+// for its longest chunk, so that single tokens beside a chunk take a block each
+// here: 63 of them and 256 rows over up to 8192 keys 550 us (bf16), where the
+// 256 rows alone take 97 and 64 single tokens, streaming, 197.
 constexpr int TK = 64;  // keys of a tile
 // 2^(ROOM + 7) (codes) times value scales below VMOST times 2^28 keys is finite.
 constexpr float SLACK = 6.0f, ROOM = 72.0f, VMOST = 1048576.0f;
@@ -1132,8 +1138,9 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(AttnArgs p) {
 // four queries' scores of one key, so a key's sum needs no exchange until the
 // end, and its order is that of the rows. A workgroup takes 64 KG keys of one
 // kv head, and more of them when the grid (made for max_len) does not reach.
-// 1024 rows over 16384 keys, 32 heads over 8 of 128, bf16: 168 us, 790 TFLOP/s,
-// with an exponential, an fma and a sum for every 128 multiply-adds.
+// 1024 rows over 16384 keys, 32 heads over 8 of 128, bf16: 170 us, 790 TFLOP/s,
+// with an exponential, an fma and a sum for every 128 multiply-adds: the matrix
+// unit's cycles and the vector unit's add up to the whole, one after the other.
 template <class T, int HD, int KG>
 __global__ __launch_bounds__(256, 2) void paged_weight_sums_kernel(SumsArgs p) {
     typedef typename T::elem E;
@@ -1264,8 +1271,8 @@ __global__ __launch_bounds__(256, 2) void paged_weight_sums_kernel(SumsArgs p) {
 // Few query vectors (rows x heads of a kv head up to 32, or 32 at a time): they
 // stay in LDS and the keys stream by, each wave with the next 64 in flight and no
 // barrier between. 32 sequences of up to 4096 keys, one row of 16 heads over 8 of
-// 128, f32: 113 MB in 39 us, 2.9 TB/s; a wave has few steps, so that the latency
-// of the first look-ups and codes shows. (Look-ups a step further ahead: 43 us.)
+// 128, f32: 113 MB in 39 us, 2.9 TB/s, with a table look-up before each step's
+// loads. (Look-ups a step further ahead: 43 us.)
 template <class T, int HD>
 __global__ __launch_bounds__(256, 2) void paged_weight_sums_stream_kernel(SumsArgs p) {
     typedef typename T::elem E;
