@@ -281,7 +281,7 @@ def _stream_of(dev):
 
 # The C entries take sizes of 32 bits, and ctypes cuts what is longer without a
 # word: sizes that could be are checked here.
-_MOST = 0x7fffffff
+_MOST, _U32 = 0x7fffffff, 0xffffffff
 
 
 class PagedKV8:
@@ -295,12 +295,12 @@ class PagedKV8:
     def __init__(self, k_pool, v_pool, k_scales, v_scales, block_tables, block_size, head_dim):
         if head_dim <= 0 or head_dim % 4 or head_dim > 256:
             raise ValueError(f"PagedKV8: head_dim {head_dim}, a multiple of 4 up to 256")
-        if not 0 < block_size <= _MOST:
+        if not 0 < block_size <= _U32:
             raise ValueError(f"PagedKV8: block_size {block_size}")
         if k_scales.dim() != 2 or block_tables.dim() != 2:
             raise ValueError("PagedKV8: scales [slots, n_kv] and block_tables [batch, max_blocks] expected")
         slots, n_kv = k_scales.shape
-        if n_kv * head_dim > _MOST or block_tables.shape[1] > _MOST or block_tables.shape[0] > _MOST // 2:
+        if n_kv * head_dim > _MOST or block_tables.shape[1] > _U32 or block_tables.shape[0] > _MOST // 2:
             raise ValueError(f"PagedKV8: {n_kv} kv heads, block_tables {tuple(block_tables.shape)}")
         words = slots * n_kv * head_dim // 4
         for name, t, dtype, numel in (("k_pool", k_pool, torch.int32, words), ("v_pool", v_pool, torch.int32, words),
@@ -528,12 +528,12 @@ def paged_kv_evict_i8(cache, seq_lens, acc, budget, sink=0, recent=0, out_tables
     to_ptr = to_cols = out_ptr = out_cap = 0
     if out_tables is not None:
         _need(out_tables, torch.int32, 0, "out_tables")
-        if out_tables.dim() != 2 or out_tables.shape[0] < batch or out_tables.shape[1] > _MOST:
+        if out_tables.dim() != 2 or out_tables.shape[0] < batch or out_tables.shape[1] > _U32:
             raise ValueError(f"out_tables: shape {tuple(out_tables.shape)}, expected [{batch}, blocks]")
         to_ptr, to_cols = out_tables.data_ptr(), out_tables.shape[1]
     if acc_out is not None:
         _need(acc_out, torch.float32, 0, "acc_out")
-        if acc_out.dim() != 3 or acc_out.shape[0] < batch or acc_out.shape[1] != cache.n_kv or acc_out.shape[2] > _MOST:
+        if acc_out.dim() != 3 or acc_out.shape[0] < batch or acc_out.shape[1] != cache.n_kv or acc_out.shape[2] > _U32:
             raise ValueError(f"acc_out: shape {tuple(acc_out.shape)}, expected [{batch}, {cache.n_kv}, >= {budget}]")
         out_ptr, out_cap = acc_out.data_ptr(), acc_out.shape[2]
     if keep is None:

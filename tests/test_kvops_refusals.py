@@ -49,3 +49,9 @@ def test_sizes_past_32_bits():
     no("budget", ops.paged_kv_evict_i8, c, lens, big(2, 2, 16), PAST)
     no("out_tables", ops.paged_kv_evict_i8, c, lens, big(2, 2, 16), 4, out_tables=big(2, PAST, dtype=torch.int32))
     no("acc_out", ops.paged_kv_evict_i8, c, lens, big(2, 2, 16), 4, acc_out=big(2, 2, PAST))
+
+
+def test_the_largest_sizes_are_taken():
+    """What fits in 32 bits is no error of the wrapper's: a block of up to 2^32 - 1 positions, tables as wide."""
+    assert cache(block_size=0xFFFFFFFF).desc.block_size == 0xFFFFFFFF
+    assert cache(block_tables=big(2, 0xFFFFFFFF, dtype=torch.int32)).desc.max_blocks == 0xFFFFFFFF
