@@ -11,6 +11,7 @@ LIB_PATH = os.path.join(HERE, "libbrain_hip.so")
 
 BH_OK, BH_ERR_INVALID, BH_ERR_HIP, BH_ERR_UNSUPPORTED, BH_ERR_NOMEM, BH_ERR_TIMEOUT = 0, -1, -2, -3, -4, -5
 BH_OUT_F32, BH_OUT_BF16, BH_OUT_I32 = 0, 1, 2
+BH_MOE_SOFTMAX, BH_MOE_SIGMOID = 0, 1
 BH_CREATE_LENIENT = 1
 BH_VARIANT_PACKED_INT8, BH_VARIANT_WORKGROUP_PER_OUTPUT = 1, 2
 
@@ -69,6 +70,22 @@ class QkRowsT(C.Structure):
                 ("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("eps", C.c_float)]
 
 
+class MoeRouterT(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("stride", C.c_uint64), ("dtype", C.c_int)] + \
+               [(n, C.c_uint32) for n in ("tokens", "n_experts", "top_k")] + \
+               [("mask", C.c_void_p), ("score", C.c_int), ("renormalize", C.c_int), ("scale", C.c_float)]
+
+
+class MoePlanT(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("offsets", "rows", "slots")]
+
+
+class GroupedI8T(C.Structure):
+    _fields_ = [("xq", C.c_void_p), ("sx", C.c_void_p), ("x_rows", C.c_uint32), ("rows", C.c_void_p), ("offsets", C.c_void_p),
+                ("places", C.c_uint32), ("n_experts", C.c_uint32), ("wq", C.c_void_p), ("sw", C.c_void_p),
+                ("bias", C.c_void_p), ("kg", C.c_uint32), ("n", C.c_uint32)]
+
+
 class CostT(C.Structure):
     _fields_ = [("flops", C.c_uint64), ("int_ops", C.c_uint64), ("bytes", C.c_uint64)]
 
@@ -97,6 +114,12 @@ SIGNATURES = {
     "bh_paged_attention_i8": (i32, [vp, vp, u64, i32, u32, P(Kv8T), P(Kv8BatchT), f32, vp, vp, vp, u64]),
     "bh_paged_weight_sums_i8": (i32, [vp, vp, u64, i32, u32, vp, P(Kv8T), P(Kv8BatchT), f32, vp, u32]),
     "bh_paged_kv_evict_i8": (i32, [vp, P(Kv8T), vp, u32, vp, u32, u32, u32, u32, vp, u32, vp, u32, vp, vp]),
+    "bh_moe_workspace": (i32, [u32, u32, u32, P(u64)]),
+    "bh_moe_route": (i32, [vp, P(MoeRouterT), vp, vp, P(MoePlanT), vp, u64]),
+    "bh_moe_plan_rows": (i32, [vp, vp, u32, u32, u32, u32, P(MoePlanT), vp, u64]),
+    "bh_matmul_i8_grouped": (i32, [vp, P(GroupedI8T), vp, i32]),
+    "bh_matmul_i8_grouped_glu": (i32, [vp, P(GroupedI8T), vp, i32]),
+    "bh_moe_combine": (i32, [vp, vp, i32, u32, vp, vp, u32, u32, u32, vp, vp, i32]),
     "bh_reserve_workspace": (i32, [vp, u32, u32, u32]),
     "bh_matmul_i8_static": (i32, [vp, vp, vp, f32, f32, vp, u32, u32, u32]),
     "bh_linear_i8": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, i32, u32, u32, u32]),

@@ -17,7 +17,8 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libbrain_hip.so")
 SOURCES = ["bh_api.hip", "bh_quant.hip", "bh_gemv.hip", "bh_gemm.hip", "bh_qwen3.hip", "bh_flash.hip", "bh_q4.hip", "bh_kv8.hip",
-           "bh_rope.hip", "bh_pattn.hip", "bh_evict.hip", "bh_st.cpp"]
+           "bh_rope.hip", "bh_pattn.hip", "bh_evict.hip", "bh_moe.hip",
+           "bh_grouped.hip", "bh_st.cpp"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",

@@ -1,0 +1,414 @@
+// The router of a sparse mixture of experts, the plan of which rows each
+// expert has, and the weighted sum of the experts' rows (bh_moe_route,
+// bh_moe_plan_rows, bh_moe_combine).
+//
+// Routing: a wave takes a token, its logits in registers (lane l holds experts l, l + 64,
+// ...), and finds the top_k largest one after another: the wave's maximum, then
+// the lowest index that has it (a ballot for each register, in order).
+//
+// Plan: a stable counting sort of the (token, choice) entries by expert. A wave takes
+// its entries 64 at a time; the lanes with the same expert are found with a
+// ballot for each bit of its index, so an entry's rank among them is a
+// popcount and the counts need no atomics: the plan is the same on every run.
+#include <cfloat>
+
+#include "bh_kvops.h"
+
+namespace bh {
+
+constexpr uint32_t MOE_MAX_EXPERTS = 1024, MOE_MAX_TOP = 64;
+constexpr uint32_t RT = 1024, RW = RT / 64;  // threads and waves of a routing workgroup
+
+struct RouteArgs {
+    const void* logits;
+    uint64_t stride;
+    const uint8_t* mask;
+    uint32_t items, e, k, first, div;  // k entries an item; entry i is of token i / div
+    int score, renormalize;
+    float scale;
+    float* weights;
+    int32_t* experts;
+    uint32_t *offsets, *rows;
+    int32_t* slots;
+    uint32_t* counts;  // [workgroups][e]: entries of each expert in each workgroup's tokens
+    uint32_t per;      // items of a workgroup
+};
+
+// The token's top k experts: lane j < k gets the j-th (-1: none) and its weight.
+template <class T, int NV>
+__device__ __forceinline__ void route_token(const RouteArgs& a, uint32_t t, uint32_t lane, int& expert, float& weight) {
+    const typename T::elem* l = reinterpret_cast<const typename T::elem*>(a.logits) + (uint64_t)t * a.stride;
+    expert = -1;
+    weight = 0.0f;
+    if (a.mask && !a.mask[t]) return;
+    float x[NV];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        const uint32_t i = v * 64 + lane;
+        const float f = T::get(l + min(i, a.e - 1));
+        x[v] = i < a.e && f == f ? f : -INFINITY;
+    }
+    float top = -INFINITY, logit = -INFINITY, total = 0.0f;
+    for (uint32_t j = 0; j < a.k; ++j) {
+        float m = x[0];
+#pragma unroll
+        for (int v = 1; v < NV; ++v) m = fmaxf(m, x[v]);
+        m = xor_max<32>(m);
+        if (m == -INFINITY) break;
+        if (j == 0) {
+            top = m;
+            // exp(l - top), where equal infinities are no distance apart
+            if (a.score == BH_MOE_SOFTMAX && !a.renormalize) {
+                float s = 0.0f;
+#pragma unroll
+                for (int v = 0; v < NV; ++v) s += x[v] == top ? 1.0f : expf(x[v] - top);
+                total = xor_sum<32>(s);
+            }
+        }
+        bool found = false;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const unsigned long long b = __ballot(x[v] == m);
+            if (!found && b) {
+                found = true;
+                const uint32_t at = (uint32_t)__builtin_ctzll(b);
+                if (lane == at) x[v] = -INFINITY;
+                if (lane == j) expert = v * 64 + (int)at;
+            }
+        }
+        if (lane == j) logit = m;
+    }
+    float s = 0.0f;
+    if (expert >= 0) {
+        if (a.score == BH_MOE_SOFTMAX) s = logit == top ? 1.0f : expf(logit - top);
+        // sigmoid; for a sum that is divided out, of far negative logits, exp(-top) times it
+        else if (a.renormalize && top < 0.0f) s = expf(logit - top) / (1.0f + expf(logit));
+        else s = 1.0f / (1.0f + expf(-logit));
+    }
+    if (a.renormalize) total = xor_sum<32>(s);
+    if (a.score == BH_MOE_SOFTMAX || a.renormalize) s = expert >= 0 ? s / total : 0.0f;
+    weight = s * a.scale;
+}
+
+// Inclusive sum over the lanes of a wave.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v, uint32_t lane) {
+#pragma unroll
+    for (int off = 1; off < 64; off *= 2) {
+        const uint32_t o = __shfl_up(v, off, 64);
+        if ((int)lane >= off) v += o;
+    }
+    return v;
+}
+
+// The lanes whose `key` is this lane's.
+__device__ __forceinline__ unsigned long long same_key(uint32_t key, uint32_t bits) {
+    unsigned long long same = ~0ull;
+    for (uint32_t b = 0; b < bits; ++b) {
+        const unsigned long long m = __ballot((key >> b) & 1);
+        same &= (key >> b) & 1 ? m : ~m;
+    }
+    return same;
+}
+
+// LDS accesses of a wave's lanes stay in this order.
+__device__ __forceinline__ void wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// A workgroup's tokens: their experts (routed here, ROUTE, or read), and of each entry
+// the rank among the entries of its expert in this workgroup. With one workgroup
+// (ONE) the plan is complete at the end; else `slots` holds the ranks and
+// `counts` the workgroup's counts, for moe_place_kernel. NV = 0: not routed here.
+template <class T, int NV, bool PLAN, bool ONE>
+__global__ __launch_bounds__(RT) void moe_route_kernel(RouteArgs a) {
+    extern __shared__ uint32_t off[];  // [e] offsets, then [RW][e] counts
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint32_t t0 = blockIdx.x * a.per, t1 = min(t0 + a.per, a.items);
+    // Wave w's tokens, in order: entries that follow each other.
+    const uint32_t share = (a.per + RW - 1) / RW, w0 = min(t0 + wave * share, t1), w1 = min(w0 + share, t1);
+    uint16_t *cnts = reinterpret_cast<uint16_t*>(off + a.e), *cnt = cnts + wave * a.e;
+    if constexpr (PLAN) {
+        for (uint32_t i = lane; i < a.e; i += 64) cnt[i] = 0;
+        wave_order();
+    }
+    if constexpr (NV > 0) {
+        for (uint32_t t = w0; t < w1; ++t) {
+            int expert;
+            float weight;
+            route_token<T, NV>(a, t, lane, expert, weight);
+            if (lane < a.k) {
+                a.experts[(uint64_t)t * a.k + lane] = expert;
+                a.weights[(uint64_t)t * a.k + lane] = weight;
+            }
+        }
+    }
+    if constexpr (!PLAN) return;
+    const uint32_t bits = 32 - (uint32_t)__builtin_clz(a.e);  // of a key, e itself (routed nowhere) included
+    const uint32_t i1 = w1 * a.k;
+    if (NV > 0) __threadfence_block();  // the wave reads the experts that its other lanes stored
+    auto key_of = [&](uint32_t i) -> uint32_t {
+        const uint32_t e = (uint32_t)a.experts[i] - a.first;
+        return e < a.e ? e : a.e;
+    };
+    for (uint32_t i0 = w0 * a.k; i0 < i1; i0 += 64) {
+        const uint32_t i = i0 + lane, key = i < i1 ? key_of(i) : a.e;
+        const unsigned long long same = same_key(key, bits), below = (1ull << lane) - 1;
+        if (key < a.e) {
+            const uint32_t before = cnt[key];
+            a.slots[i] = (int32_t)(before + (uint32_t)__popcll(same & below));
+            wave_order();
+            if (!(same & below)) cnt[key] = (uint16_t)(before + (uint32_t)__popcll(same));
+        } else if (i < i1) {
+            a.slots[i] = -1;
+        }
+        wave_order();
+    }
+    __syncthreads();
+    // Counts to where each wave's entries begin; the workgroup's counts.
+    for (uint32_t e = tid; e < a.e; e += RT) {
+        uint32_t sum = 0;
+        for (uint32_t w = 0; w < RW; ++w) {
+            const uint32_t c = cnts[w * a.e + e];
+            cnts[w * a.e + e] = (uint16_t)sum;
+            sum += c;
+        }
+        if constexpr (ONE) off[e] = sum;
+        else a.counts[(uint64_t)blockIdx.x * a.e + e] = sum;
+    }
+    __syncthreads();
+    if constexpr (ONE) {
+        if (wave == 0) {
+            uint32_t base = 0;
+            for (uint32_t e0 = 0; e0 < a.e; e0 += 64) {
+                const uint32_t e = e0 + lane, c = e < a.e ? off[e] : 0, upto = wave_scan(c, lane);
+                if (e < a.e) {
+                    off[e] = base + upto - c;
+                    a.offsets[e] = base + upto - c;
+                }
+                base += (uint32_t)__shfl((int)upto, 63, 64);
+            }
+            if (lane == 0) a.offsets[a.e] = base;
+        }
+        __syncthreads();
+    }
+    for (uint32_t i = w0 * a.k + lane; i < i1; i += 64) {
+        const uint32_t key = key_of(i);
+        if (key == a.e) continue;
+        const uint32_t at = (uint32_t)a.slots[i] + cnt[key] + (ONE ? off[key] : 0);
+        a.slots[i] = (int32_t)at;
+        if constexpr (ONE) a.rows[at] = i / a.div;
+    }
+}
+
+// Ranks to places: workgroup b's entries of an expert come behind those of the
+// workgroups before it.
+__global__ __launch_bounds__(RT) void moe_place_kernel(RouteArgs a) {
+    extern __shared__ uint32_t lds[];  // [e] all, [e] before
+    uint32_t *all = lds, *before = lds + a.e;
+    const uint32_t tid = threadIdx.x, lane = tid & 63;
+    for (uint32_t e = tid; e < a.e; e += RT) {
+        uint32_t sum = 0, mine = 0;
+        for (uint32_t b = 0; b < gridDim.x; ++b) {
+            if (b == blockIdx.x) mine = sum;
+            sum += a.counts[(uint64_t)b * a.e + e];
+        }
+        all[e] = sum;
+        before[e] = mine;
+    }
+    __syncthreads();
+    if (tid < 64) {
+        uint32_t base = 0;
+        for (uint32_t e0 = 0; e0 < a.e; e0 += 64) {
+            const uint32_t e = e0 + lane, c = e < a.e ? all[e] : 0, upto = wave_scan(c, lane);
+            if (e < a.e) {
+                before[e] += base + upto - c;
+                if (blockIdx.x == 0) a.offsets[e] = base + upto - c;
+            }
+            base += (uint32_t)__shfl((int)upto, 63, 64);
+        }
+        if (blockIdx.x == 0 && lane == 0) a.offsets[a.e] = base;
+    }
+    __syncthreads();
+    const uint32_t t0 = blockIdx.x * a.per, t1 = min(t0 + a.per, a.items);
+    for (uint32_t i = t0 * a.k + tid; i < t1 * a.k; i += RT) {
+        const uint32_t e = (uint32_t)a.experts[i] - a.first;
+        if (e >= a.e) continue;
+        const uint32_t at = (uint32_t)a.slots[i] + before[e];
+        a.slots[i] = (int32_t)at;
+        a.rows[at] = i / a.div;
+    }
+}
+
+// Tokens of a workgroup that routes: one workgroup up to 128 tokens. Entries of one
+// that only plans. (At most 64 * 128 entries: their counts fit 16 bits.)
+static uint32_t route_share(uint32_t tokens) { return tokens <= 128 ? std::max(tokens, 1u) : 64; }
+static uint32_t plan_share(uint32_t entries) { return entries <= 4096 ? std::max(entries, 1u) : 4096; }
+static uint32_t groups_of(uint32_t items, uint32_t per) { return std::max((items + per - 1) / per, 1u); }
+
+template <class T, int NV>
+static hipError_t launch_route(hipStream_t s, const RouteArgs& a, bool plan) {
+    const uint32_t wgs = groups_of(a.items, a.per);
+    if (!plan) {
+        moe_route_kernel<T, NV, false, false><<<wgs, RT, 0, s>>>(a);
+        return hipGetLastError();
+    }
+    const size_t lds = (size_t)a.e * 4 + (size_t)RW * a.e * 2;
+    if (wgs == 1) {
+        moe_route_kernel<T, NV, true, true><<<1, RT, lds, s>>>(a);
+        return hipGetLastError();
+    }
+    moe_route_kernel<T, NV, true, false><<<wgs, RT, lds, s>>>(a);
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return err;
+    moe_place_kernel<<<wgs, RT, (size_t)2 * a.e * 4, s>>>(a);
+    return hipGetLastError();
+}
+
+template <class T>
+static hipError_t launch_route_any(hipStream_t s, const RouteArgs& a, bool plan) {
+    if (a.e <= 64) return launch_route<T, 1>(s, a, plan);
+    if (a.e <= 128) return launch_route<T, 2>(s, a, plan);
+    if (a.e <= 256) return launch_route<T, 4>(s, a, plan);
+    if (a.e <= 512) return launch_route<T, 8>(s, a, plan);
+    return launch_route<T, 16>(s, a, plan);
+}
+
+static int check_plan(const char* who, uint32_t tokens, uint32_t top_k, uint32_t n_experts, const bh_moe_plan* plan,
+                      const void* ws, uint64_t ws_bytes, RouteArgs* a) {
+    if (n_experts == 0 || n_experts > MOE_MAX_EXPERTS)
+        return fail(BH_ERR_INVALID, "%s: %u experts (1 to %u)", who, n_experts, MOE_MAX_EXPERTS);
+    if ((uint64_t)tokens * top_k > 0x7fffffffu)
+        return fail(BH_ERR_INVALID, "%s: %u tokens of %u choices", who, tokens, top_k);
+    if (!plan) return BH_OK;
+    if (!plan->offsets || ((uint64_t)tokens * top_k && (!plan->rows || !plan->slots)))
+        return fail(BH_ERR_INVALID, "%s: null plan buffer", who);
+    uint64_t need = 0;
+    const int rc = bh_moe_workspace(tokens, top_k, n_experts, &need);
+    if (rc) return rc;
+    if (ws_bytes < need || (need && (!ws || !aligned_to(ws, 4))))
+        return fail(BH_ERR_INVALID, "%s: a workspace of %llu bytes, needs %llu", who, (unsigned long long)(ws ? ws_bytes : 0),
+                    (unsigned long long)need);
+    a->offsets = plan->offsets, a->rows = plan->rows, a->slots = plan->slots;
+    a->counts = static_cast<uint32_t*>(const_cast<void*>(ws));
+    return BH_OK;
+}
+
+// ---------------------------------------------------------------- the weighted sum
+struct CombineArgs {
+    const void* y;
+    const float* weights;
+    const int32_t* slots;
+    const void* add;
+    void* out;
+    uint32_t places, tokens, k, n, per;  // per: pieces of a token's row
+};
+
+// A thread sums W neighbouring columns of a token, its experts' rows one after another.
+template <class Y, class O, int W>
+__global__ __launch_bounds__(256) void moe_combine_kernel(CombineArgs a) {
+    const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (uint64_t)a.tokens * a.per) return;
+    const uint32_t t = (uint32_t)(i / a.per), c = (uint32_t)(i - (uint64_t)t * a.per) * W;
+    float s[W];
+#pragma unroll
+    for (int w = 0; w < W; ++w) s[w] = 0.0f;
+    for (uint32_t j = 0; j < a.k; ++j) {
+        const uint32_t slot = (uint32_t)a.slots[(uint64_t)t * a.k + j];
+        if (slot >= a.places) continue;
+        const float wt = a.weights[(uint64_t)t * a.k + j];
+        const typename Y::elem* y = reinterpret_cast<const typename Y::elem*>(a.y) + (uint64_t)slot * a.n + c;
+#pragma unroll
+        for (int w = 0; w < W; ++w) s[w] += wt * Y::get(y + w);
+    }
+    const uint64_t at = (uint64_t)t * a.n + c;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        float v = s[w];
+        if (a.add) v += O::get(reinterpret_cast<const typename O::elem*>(a.add) + at + w);
+        O::put(reinterpret_cast<typename O::elem*>(a.out) + at + w, v);
+    }
+}
+
+template <class Y, class O>
+static hipError_t launch_combine(hipStream_t s, CombineArgs a) {
+    a.per = a.n;
+    const uint64_t wgs = ((uint64_t)a.tokens * a.per + 255) / 256;
+    moe_combine_kernel<Y, O, 1><<<(unsigned)wgs, 256, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+}  // namespace bh
+
+using namespace bh;
+
+static int launched(hipError_t e, const char* who) {
+    return e == hipSuccess ? BH_OK : fail(BH_ERR_HIP, "%s: %s", who, hipGetErrorString(e));
+}
+
+extern "C" int bh_moe_workspace(uint32_t tokens, uint32_t top_k, uint32_t n_experts, uint64_t* bytes) {
+    if (!bytes) return fail(BH_ERR_INVALID, "bh_moe_workspace: null output");
+    if (n_experts == 0 || n_experts > MOE_MAX_EXPERTS || (uint64_t)tokens * top_k > 0x7fffffffu)
+        return fail(BH_ERR_INVALID, "bh_moe_workspace: %u tokens, %u choices, %u experts", tokens, top_k, n_experts);
+    const uint32_t entries = tokens * top_k;
+    const uint32_t wgs = std::max(groups_of(tokens, route_share(tokens)), groups_of(entries, plan_share(entries)));
+    *bytes = wgs > 1 ? (uint64_t)wgs * n_experts * 4 : 0;
+    return BH_OK;
+}
+
+extern "C" int bh_moe_route(void* stream, const bh_moe_router* r, float* weights, int32_t* experts,
+                            const bh_moe_plan* plan, void* ws, uint64_t ws_bytes) {
+    static const char* who = "bh_moe_route";
+    if (!r) return fail(BH_ERR_INVALID, "%s: null router", who);
+    RouteArgs a{};
+    const int rc = check_plan(who, r->tokens, r->top_k, r->n_experts, plan, ws, ws_bytes, &a);
+    if (rc) return rc;
+    if (r->top_k == 0 || r->top_k > MOE_MAX_TOP || r->top_k > r->n_experts)
+        return fail(BH_ERR_INVALID, "%s: the top %u of %u experts (at most %u)", who, r->top_k, r->n_experts, MOE_MAX_TOP);
+    if (r->dtype != BH_OUT_F32 && r->dtype != BH_OUT_BF16) return fail(BH_ERR_INVALID, "%s: dtype %d", who, r->dtype);
+    if (r->score != BH_MOE_SOFTMAX && r->score != BH_MOE_SIGMOID) return fail(BH_ERR_INVALID, "%s: score %d", who, r->score);
+    if (r->tokens > 1 && r->stride < r->n_experts)
+        return fail(BH_ERR_INVALID, "%s: stride %llu below %u experts", who, (unsigned long long)r->stride, r->n_experts);
+    if (r->tokens == 0 && !plan) return BH_OK;
+    if (r->tokens && (!r->logits || !weights || !experts)) return fail(BH_ERR_INVALID, "%s: null buffer", who);
+    a.logits = r->logits, a.stride = r->stride, a.mask = r->mask, a.items = r->tokens, a.e = r->n_experts;
+    a.k = a.div = r->top_k;
+    a.score = r->score, a.renormalize = r->renormalize, a.scale = r->scale, a.weights = weights, a.experts = experts;
+    a.per = route_share(r->tokens);
+    const hipStream_t s = (hipStream_t)stream;
+    const hipError_t e = r->dtype == BH_OUT_F32 ? launch_route_any<F32>(s, a, plan) : launch_route_any<Bf16>(s, a, plan);
+    return launched(e, who);
+}
+
+extern "C" int bh_moe_plan_rows(void* stream, const int32_t* experts, uint32_t tokens, uint32_t top_k, uint32_t first,
+                                uint32_t n_experts, const bh_moe_plan* plan, void* ws, uint64_t ws_bytes) {
+    static const char* who = "bh_moe_plan_rows";
+    if (!plan) return fail(BH_ERR_INVALID, "%s: null plan", who);
+    RouteArgs a{};
+    const int rc = check_plan(who, tokens, top_k, n_experts, plan, ws, ws_bytes, &a);
+    if (rc) return rc;
+    if ((uint64_t)tokens * top_k && !experts) return fail(BH_ERR_INVALID, "%s: null experts", who);
+    a.items = tokens * top_k, a.e = n_experts, a.k = 1, a.div = std::max(top_k, 1u), a.first = first;
+    a.experts = const_cast<int32_t*>(experts);
+    a.per = plan_share(a.items);
+    return launched(launch_route<F32, 0>((hipStream_t)stream, a, true), who);
+}
+
+extern "C" int bh_moe_combine(void* stream, const void* y, int y_dtype, uint32_t places, const float* weights,
+                              const int32_t* slots, uint32_t tokens, uint32_t top_k, uint32_t n, const void* add, void* out,
+                              int out_dtype) {
+    static const char* who = "bh_moe_combine";
+    if ((y_dtype != BH_OUT_F32 && y_dtype != BH_OUT_BF16) || (out_dtype != BH_OUT_F32 && out_dtype != BH_OUT_BF16))
+        return fail(BH_ERR_INVALID, "%s: dtypes %d and %d", who, y_dtype, out_dtype);
+    if (places > 0x7fffffffu || tokens > 0x7fffffffu || n > 0x7fffffffu || (uint64_t)tokens * top_k > 0x7fffffffu ||
+        (uint64_t)tokens * n > (uint64_t)0x7fffffff * 256)
+        return fail(BH_ERR_INVALID, "%s: %u places, %u tokens of %u choices, rows of %u", who, places, tokens, top_k, n);
+    if (tokens == 0 || n == 0) return BH_OK;
+    if (!out || (top_k && (!weights || !slots || (places && !y)))) return fail(BH_ERR_INVALID, "%s: null buffer", who);
+    const CombineArgs a{y, weights, slots, add, out, places, tokens, top_k, n, 0};
+    const hipStream_t s = (hipStream_t)stream;
+    hipError_t e;
+    if (y_dtype == BH_OUT_F32) e = out_dtype == BH_OUT_F32 ? launch_combine<F32, F32>(s, a) : launch_combine<F32, Bf16>(s, a);
+    else e = out_dtype == BH_OUT_F32 ? launch_combine<Bf16, F32>(s, a) : launch_combine<Bf16, Bf16>(s, a);
+    return launched(e, who);
+}

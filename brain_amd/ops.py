@@ -5,10 +5,12 @@ runs in the library's gfx950 kernels. Packed int8 tensors are torch.int32
 tensors holding the u32 words (4 int8 per word, little-endian along K).
 """
 import ctypes as C
+from typing import NamedTuple
 
 import torch
 
-from ._lib import BH_OUT_BF16, BH_OUT_F32, BH_OUT_I32, Kv8BatchT, Kv8T, QkRowsT, check, load
+from ._lib import (BH_MOE_SIGMOID, BH_MOE_SOFTMAX, BH_OUT_BF16, BH_OUT_F32, BH_OUT_I32, GroupedI8T, Kv8BatchT, Kv8T,
+                   MoePlanT, MoeRouterT, QkRowsT, check, load)
 
 _CODES = {torch.float32: BH_OUT_F32, torch.bfloat16: BH_OUT_BF16, torch.int32: BH_OUT_I32}
 
@@ -549,3 +551,192 @@ def paged_kv_evict_i8(cache, seq_lens, acc, budget, sink=0, recent=0, out_tables
                                       acc.shape[2], budget, sink, recent, to_ptr, to_cols, out_ptr, out_cap,
                                       keep.data_ptr(), new_lens.data_ptr()))
     return keep, new_lens
+
+
+# ---------------------------------------------------------------- a sparse mixture of experts
+
+class MoePlan(NamedTuple):
+    """Which rows each expert has, int32: the places of expert e are offsets[e]
+    .. offsets[e + 1] (offsets [n_experts + 1]), in the order of token and
+    choice; rows [tokens * top_k] is the token of a place, slots [tokens, top_k] the
+    place of a choice, -1 for none. rows behind offsets[-1] are not written."""
+    offsets: torch.Tensor
+    rows: torch.Tensor
+    slots: torch.Tensor
+
+
+_SCORES = {"softmax": BH_MOE_SOFTMAX, "sigmoid": BH_MOE_SIGMOID}
+_MOE_MAX_EXPERTS, _MOE_MAX_TOP = 1024, 64
+
+
+def _moe_sizes(who, tokens, top_k, n_experts):
+    if not 0 < n_experts <= _MOE_MAX_EXPERTS:
+        raise ValueError(f"{who}: {n_experts} experts, 1 to {_MOE_MAX_EXPERTS}")
+    if tokens * top_k > _MOST or tokens > _MOST:
+        raise ValueError(f"{who}: {tokens} tokens of {top_k} choices")
+
+
+def _moe_plan(dev, device, tokens, top_k, n_experts, plan):
+    """The plan's buffers and their workspace."""
+    entries = tokens * top_k
+    if plan is None:
+        plan = MoePlan(torch.empty(n_experts + 1, device=device, dtype=torch.int32),
+                       torch.empty(entries, device=device, dtype=torch.int32),
+                       torch.empty((tokens, top_k), device=device, dtype=torch.int32))
+    else:
+        _need(plan.offsets, torch.int32, n_experts + 1, "plan.offsets")
+        _need(plan.rows, torch.int32, entries, "plan.rows")
+        _need(plan.slots, torch.int32, entries, "plan.slots")
+        _here(dev, plan.offsets, plan.rows, plan.slots)
+    n = C.c_uint64()
+    check(load().bh_moe_workspace(tokens, top_k, n_experts, C.byref(n)))
+    ws = torch.empty(n.value, device=device, dtype=torch.uint8) if n.value else None
+    return plan, MoePlanT(plan.offsets.data_ptr(), plan.rows.data_ptr(), plan.slots.data_ptr()), ws, n.value
+
+
+def moe_route(logits, top_k, score="softmax", renormalize=True, scale=1.0, mask=None, plan=None, weights=None, experts=None):
+    """Each token's top_k experts of largest logit [tokens, n_experts] (f32 or
+    bf16; ties: the lower index), largest first, and their weights: the softmax
+    over all experts or the sigmoid of the logit, divided by the sum of the
+    token's own (renormalize) and times scale. mask [tokens] bool: false for
+    padding, which goes nowhere (-1, weight 0), as does a choice whose logit is NaN or
+    -inf. Returns (weights [tokens, top_k] f32, experts [tokens, top_k] int32,
+    MoePlan); plan=False: no plan is made (None)."""
+    if logits.dim() != 2 or logits.dtype not in _ACT:
+        raise ValueError(f"logits: {logits.dtype} {tuple(logits.shape)}, expected [tokens, n_experts] float32 or bfloat16")
+    tokens, n_experts = logits.shape
+    _moe_sizes("moe_route", tokens, top_k, n_experts)
+    if not 0 < top_k <= min(n_experts, _MOE_MAX_TOP):
+        raise ValueError(f"moe_route: the top {top_k} of {n_experts} experts (at most {_MOE_MAX_TOP})")
+    if score not in _SCORES:
+        raise ValueError(f"moe_route: score {score!r}, one of {sorted(_SCORES)}")
+    stride, one = logits.stride()
+    if (one != 1 and n_experts > 1) or (tokens > 1 and stride < n_experts):
+        raise ValueError(f"logits: strides {logits.stride()}; the experts of a token must lie side by side")
+    dev, device = logits.get_device(), logits.device
+    if mask is not None:
+        _need(mask, torch.bool, tokens, "mask")
+    if weights is None:
+        weights = torch.empty((tokens, top_k), device=device, dtype=torch.float32)
+    else:
+        _need(weights, torch.float32, tokens * top_k, "weights")
+    if experts is None:
+        experts = torch.empty((tokens, top_k), device=device, dtype=torch.int32)
+    else:
+        _need(experts, torch.int32, tokens * top_k, "experts")
+    _here(dev, mask, weights, experts)
+    stream = _stream_of(dev)
+    made = ref = ws = None
+    size = 0
+    if plan is not False:
+        made, desc, ws, size = _moe_plan(dev, device, tokens, top_k, n_experts, plan)
+        ref = C.byref(desc)
+    router = MoeRouterT(logits.data_ptr(), stride if tokens > 1 else n_experts, _ACT[logits.dtype], tokens, n_experts, top_k,
+                        _ptr(mask), _SCORES[score], 1 if renormalize else 0, scale)
+    check(load().bh_moe_route(stream, C.byref(router), weights.data_ptr(), experts.data_ptr(), ref, _ptr(ws), size))
+    return weights, experts, made
+
+
+def moe_plan(experts, n_experts, first=0, plan=None):
+    """The MoePlan of experts [tokens, top_k] int32 chosen elsewhere: of those in
+    [first, first + n_experts), which are an expert-parallel rank's own; others go
+    nowhere. An expert twice in a token is two places."""
+    if experts.dim() != 2:
+        raise ValueError(f"experts: shape {tuple(experts.shape)}, expected [tokens, top_k]")
+    tokens, top_k = experts.shape
+    _need(experts, torch.int32, 0, "experts")
+    _moe_sizes("moe_plan", tokens, top_k, n_experts)
+    if top_k > _MOST or not 0 <= first <= _MOST:
+        raise ValueError(f"moe_plan: {top_k} choices, first {first}")
+    dev = experts.get_device()
+    _here(dev, experts)
+    stream = _stream_of(dev)
+    plan, desc, ws, size = _moe_plan(dev, experts.device, tokens, top_k, n_experts, plan)
+    check(load().bh_moe_plan_rows(stream, experts.data_ptr(), tokens, top_k, first, n_experts, C.byref(desc), _ptr(ws), size))
+    return plan
+
+
+def _matmul_grouped(call, glu, xq, wq, sx, sw, offsets, rows, bias, out_dtype, out):
+    if xq.dim() != 2 or wq.dim() != 3 or wq.shape[2] != xq.shape[1]:
+        raise ValueError(f"{call}: xq {tuple(xq.shape)} and wq {tuple(wq.shape)}, expected [rows, K/4] and [experts, n, K/4]")
+    x_rows, kg = xq.shape
+    n_experts, n, _ = wq.shape
+    if glu and n % 2:
+        raise ValueError(f"{call}: {n} weight rows of gate and up")
+    places = x_rows if rows is None else rows.numel()
+    if max(x_rows, places, n_experts, n, 4 * kg) > _MOST:
+        raise ValueError(f"{call}: {places} places of {x_rows} rows, {n_experts} experts of {n} rows, K {4 * kg}")
+    cols = n // 2 if glu else n
+    _need(xq, torch.int32, 0, "xq")
+    _need(wq, torch.int32, 0, "wq")
+    _need(sx, torch.float32, x_rows, "sx")
+    _need(sw, torch.float32, n_experts * n, "sw")
+    _need(offsets, torch.int32, n_experts + 1, "offsets")
+    if rows is not None:
+        _need(rows, torch.int32, 0, "rows")
+    if bias is not None:
+        _need(bias, torch.float32, n_experts * n, "bias")
+    if out_dtype is None:
+        out_dtype = torch.float32 if out is None else out.dtype
+    if out_dtype not in (_ACT if glu else _CODES):
+        raise ValueError(f"{call}: out_dtype {out_dtype}")
+    if out is None:
+        out = torch.empty((places, cols), device=xq.device, dtype=out_dtype)
+    else:
+        _need(out, out_dtype, places * cols, "out")
+    dev = xq.get_device()
+    _here(dev, xq, wq, sx, sw, offsets, rows, bias, out)
+    g = GroupedI8T(xq.data_ptr(), sx.data_ptr(), x_rows, _ptr(rows), offsets.data_ptr(), places, n_experts, wq.data_ptr(),
+                   sw.data_ptr(), _ptr(bias), kg, n)
+    lib = load()
+    fn = lib.bh_matmul_i8_grouped_glu if glu else lib.bh_matmul_i8_grouped
+    check(fn(_stream_of(dev), C.byref(g), out.data_ptr(), _CODES[out_dtype]))
+    return out
+
+
+def matmul_i8_grouped(xq, wq, sx, sw, offsets, rows=None, bias=None, out_dtype=None, out=None):
+    """matmul_i8 grouped by expert: place p of offsets[e] .. offsets[e + 1]
+    multiplies row rows[p] (None: row p) of xq [x_rows, K/4] with wq[e] of
+    [n_experts, n, K/4], (f32(acc) * sx[row]) * sw[e] (+ bias[e]) -> out
+    [places, n], f32 (the default), bf16 or the raw int32 sums. Output rows of no group
+    are not written. A plan's offsets and rows (MoePlan), or any ascending
+    offsets of a program's own."""
+    return _matmul_grouped("matmul_i8_grouped", False, xq, wq, sx, sw, offsets, rows, bias, out_dtype, out)
+
+
+def matmul_i8_grouped_glu(xq, wq, sx, sw, offsets, rows=None, bias=None, out_dtype=None, out=None):
+    """matmul_i8_grouped of the gate and up projections in one, wq [n_experts,
+    2 f, K/4] with an expert's f gate rows first: out [places, f] = silu(gate) * up,
+    f32 (the default) or bf16."""
+    return _matmul_grouped("matmul_i8_grouped_glu", True, xq, wq, sx, sw, offsets, rows, bias, out_dtype, out)
+
+
+def moe_combine(y, weights, slots, add=None, out_dtype=None, out=None):
+    """out[t] = sum over j of weights[t, j] * y[slots[t, j]] (+ add[t]), f32 sums
+    in the order of j, over the experts' rows y [places, n] (f32 or bf16); a
+    slot outside y (-1: none) adds nothing. out [tokens, n] of out_dtype (y's
+    without one), as add is; out may be add."""
+    if y.dim() != 2 or slots.dim() != 2 or y.dtype not in _ACT:
+        raise ValueError(f"moe_combine: y {y.dtype} {tuple(y.shape)} and slots {tuple(slots.shape)}, expected [places, n] "
+                         "float32 or bfloat16 and [tokens, top_k]")
+    places, n = y.shape
+    tokens, top_k = slots.shape
+    if max(places, n, tokens, top_k, tokens * top_k) > _MOST:
+        raise ValueError(f"moe_combine: {places} places, {tokens} tokens of {top_k} choices, rows of {n}")
+    _need(slots, torch.int32, 0, "slots")
+    _need(weights, torch.float32, tokens * top_k, "weights")
+    if out_dtype is None:
+        out_dtype = y.dtype if out is None else out.dtype
+    if out_dtype not in _ACT:
+        raise ValueError(f"moe_combine: out_dtype {out_dtype}")
+    if out is None:
+        out = torch.empty((tokens, n), device=y.device, dtype=out_dtype)
+    else:
+        _need(out, out_dtype, tokens * n, "out")
+    if add is not None:
+        _need(add, out_dtype, tokens * n, "add")
+    dev = y.get_device()
+    _here(dev, y, weights, slots, add, out)
+    check(load().bh_moe_combine(_stream_of(dev), y.data_ptr(), _ACT[y.dtype], places, weights.data_ptr(), slots.data_ptr(),
+                                tokens, top_k, n, _ptr(add), out.data_ptr(), _ACT[out_dtype]))
+    return out

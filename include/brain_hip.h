@@ -332,6 +332,83 @@ int bh_paged_kv_evict_i8(void* stream, const bh_kv8* kv, const uint32_t* seq_len
                          const uint32_t* out_tables, uint32_t out_max_blocks, float* acc_out, uint32_t acc_out_stride,
                          int32_t* keep, uint32_t* new_lens);
 
+/* ----------------------------------------------------------------------
+ * A sparse mixture of experts with int8 weights, all experts in one call: the
+ * router's choice and its plan, the experts' products with as many rows as
+ * each has, and the weighted sum back. bh_moe_linear_gated_i8 above is the
+ * reference's kernel for one expert; these have no counterpart there.
+ * Nothing here allocates or synchronises, so all of it can be captured.
+ * ---------------------------------------------------------------------- */
+enum { BH_MOE_SOFTMAX = 0, BH_MOE_SIGMOID = 1 };
+typedef struct {
+    const void* logits; /* [tokens][n_experts], dtype BH_OUT_F32 or BH_OUT_BF16, `stride` elements from row to row */
+    uint64_t stride;
+    int dtype;
+    uint32_t tokens, n_experts, top_k; /* n_experts <= 1024, top_k <= 64 and <= n_experts */
+    const uint8_t* mask;               /* [tokens]: 0 for a token that is padding and goes nowhere; NULL: none is */
+    int score;                         /* a chosen expert's score: softmax over all experts, or the sigmoid of its logit */
+    int renormalize;                   /* 1: divided by the sum of the token's chosen scores */
+    float scale;                       /* times this */
+} bh_moe_router;
+
+/* Which rows each expert has. A place is one routed (token, choice); the places of
+ * expert e are offsets[e] .. offsets[e + 1], in the order of token and choice,
+ * rows[place] is the token and slots[token * top_k + choice] the place, or -1.
+ * rows behind offsets[n_experts] are left as they are. Room for tokens * top_k places. */
+typedef struct {
+    uint32_t* offsets; /* [n_experts + 1] */
+    uint32_t* rows;    /* [tokens * top_k] */
+    int32_t* slots;    /* [tokens][top_k] */
+} bh_moe_plan;
+
+/* Workspace of the two calls below (may be 0: then NULL will do). */
+int bh_moe_workspace(uint32_t tokens, uint32_t top_k, uint32_t n_experts, uint64_t* bytes);
+/* experts [tokens][top_k]: each token's top_k experts of largest logit, largest
+ * first (ties: the lower index), and weights [tokens][top_k] f32, their scores. A
+ * logit that is NaN or -inf is never chosen; a token with fewer than top_k
+ * others has -1 and weight 0 behind them, a masked one has nothing else.
+ * (Infinite logits share a softmax equally.) With `plan` (NULL: not wanted) also the
+ * plan of these experts. */
+int bh_moe_route(void* stream, const bh_moe_router* router, float* weights, int32_t* experts, const bh_moe_plan* plan,
+                 void* ws, uint64_t ws_bytes);
+/* The plan of experts [tokens][top_k] from elsewhere, of those in [first, first +
+ * n_experts) (an expert-parallel rank's own); others are routed nowhere. The
+ * same expert twice in a token is two places. n_experts <= 1024. */
+int bh_moe_plan_rows(void* stream, const int32_t* experts, uint32_t tokens, uint32_t top_k, uint32_t first,
+                     uint32_t n_experts, const bh_moe_plan* plan, void* ws, uint64_t ws_bytes);
+
+/* A product grouped by expert. Place p in [offsets[e], offsets[e + 1]) multiplies
+ * row rows[p] of x (NULL: row p) with the weights of expert e. Offsets count as at most
+ * `places`, a group that ends before it begins is empty, and output rows of
+ * no group are left as they are; a place whose row is outside x gets zeros (raw
+ * sums of 0 with BH_OUT_I32). */
+typedef struct {
+    const uint32_t* xq; /* [x_rows][kg] int8 codes, 4 per word */
+    const float* sx;    /* [x_rows] */
+    uint32_t x_rows;
+    const uint32_t* rows;    /* [places] or NULL */
+    const uint32_t* offsets; /* [n_experts + 1] */
+    uint32_t places, n_experts;
+    const uint32_t* wq; /* [n_experts][n][kg] */
+    const float* sw;    /* [n_experts][n] */
+    const float* bias;  /* [n_experts][n] or NULL */
+    uint32_t kg, n;
+} bh_grouped_i8;
+/* out [places][n] = (f32(acc) * sx[row]) * sw[e] (+ bias[e]), the arithmetic of
+ * bh_matmul_i8, as f32, bf16 or the raw i32 sums. */
+int bh_matmul_i8_grouped(void* stream, const bh_grouped_i8* g, void* out, int out_dtype);
+/* The gate and up projections of a gated expert in one call: the n weight rows of an expert are
+ * n / 2 of the gate, then n / 2 of the up projection (n even), and out [places][n / 2] =
+ * silu(gate) * up of the products above in f32, silu(v) = v / (1 + exp(-v)),
+ * stored as f32 or bf16. */
+int bh_matmul_i8_grouped_glu(void* stream, const bh_grouped_i8* g, void* out, int out_dtype);
+
+/* out [tokens][n] = sum over j of weights[t][j] * y[slots[t][j]] (+ add[t]) in f32, in
+ * the order of j; a slot outside [0, places) adds nothing. y [places][n] of dtype y_dtype,
+ * out and add [tokens][n] of out_dtype, each BH_OUT_F32 or BH_OUT_BF16. out may be add. */
+int bh_moe_combine(void* stream, const void* y, int y_dtype, uint32_t places, const float* weights, const int32_t* slots,
+                   uint32_t tokens, uint32_t top_k, uint32_t n, const void* add, void* out, int out_dtype);
+
 /* f32 -> bf16 bits, round to nearest even, NaN -> (bits >> 16) | 0x0040: the
  * conversion every bf16 output of this library goes through
  * (crates/model/src/half.rs:49-58, f32_to_bf16). x [n] f32 -> out [n] u16. */
