@@ -301,41 +301,111 @@ struct CombineArgs {
     const int32_t* slots;
     const void* add;
     void* out;
-    uint32_t places, tokens, k, n, per;  // per: pieces of a token's row
+    uint32_t places, tokens, k, n, per;  // per: waves of a token's row
 };
 
-// A thread sums W neighbouring columns of a token, its experts' rows one after another.
+// W neighbouring elements, in registers as f32.
+template <class T, int W>
+struct Piece {
+    static constexpr int BYTES = W * sizeof(typename T::elem), WORDS = BYTES >= 4 ? BYTES / 4 : 1;
+    typedef uint32_t Part __attribute__((ext_vector_type(WORDS < 4 ? WORDS : 4)));
+    static constexpr int PARTS = WORDS <= 4 ? 1 : WORDS / 4;
+    Part part[PARTS];
+    __device__ __forceinline__ void load(const typename T::elem* p) {
+        if constexpr (BYTES == 2) {
+            part[0] = *p;
+        } else {
+#pragma unroll
+            for (int i = 0; i < PARTS; ++i) part[i] = reinterpret_cast<const Part*>(p)[i];
+        }
+    }
+    __device__ __forceinline__ float get(int w) const {
+        if constexpr (sizeof(typename T::elem) == 4) {
+            return __builtin_bit_cast(float, (uint32_t)part[w / 4][w % 4]);
+        } else {
+            const uint32_t u = part[w / 8][w % 8 / 2];
+            return __builtin_bit_cast(float, w % 2 ? u & 0xffff0000u : u << 16);
+        }
+    }
+    __device__ __forceinline__ static void store(typename T::elem* p, const float (&v)[W]) {
+        if constexpr (BYTES == 2) {
+            T::put(p, v[0]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < PARTS; ++i) {
+                Part o;
+#pragma unroll
+                for (int q = 0; q < (WORDS < 4 ? WORDS : 4); ++q) {
+                    if constexpr (sizeof(typename T::elem) == 4) o[q] = __builtin_bit_cast(uint32_t, v[i * 4 + q]);
+                    else o[q] = pack_bf16x2(v[i * 8 + 2 * q], v[i * 8 + 2 * q + 1]);
+                }
+                reinterpret_cast<Part*>(p)[i] = o;
+            }
+        }
+    }
+};
+
+// A wave takes 64 W columns of a token; the slots and weights are in scalars, and the
+// pieces of up to 8 of the token's rows are on their way together. Bound by memory:
+// top_k rows read for one written.
 template <class Y, class O, int W>
 __global__ __launch_bounds__(256) void moe_combine_kernel(CombineArgs a) {
-    const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (uint64_t)a.tokens * a.per) return;
-    const uint32_t t = (uint32_t)(i / a.per), c = (uint32_t)(i - (uint64_t)t * a.per) * W;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
+    const uint32_t t = wave / a.per, c = (wave - t * a.per) * (64 * W) + (threadIdx.x & 63) * W;
+    if (t >= a.tokens || c >= a.n) return;
+    const typename Y::elem* y = reinterpret_cast<const typename Y::elem*>(a.y) + c;
+    const int32_t* slots = a.slots + (uint64_t)t * a.k;
+    const float* weights = a.weights + (uint64_t)t * a.k;
+    const uint64_t at = (uint64_t)t * a.n + c;
+    Piece<O, W> extra;
+    if (a.add) extra.load(reinterpret_cast<const typename O::elem*>(a.add) + at);
     float s[W];
 #pragma unroll
     for (int w = 0; w < W; ++w) s[w] = 0.0f;
-    for (uint32_t j = 0; j < a.k; ++j) {
-        const uint32_t slot = (uint32_t)a.slots[(uint64_t)t * a.k + j];
-        if (slot >= a.places) continue;
-        const float wt = a.weights[(uint64_t)t * a.k + j];
-        const typename Y::elem* y = reinterpret_cast<const typename Y::elem*>(a.y) + (uint64_t)slot * a.n + c;
+    for (uint32_t j0 = 0; j0 < a.k; j0 += 8) {
+        uint32_t slot[8];
+        Piece<Y, W> row[8];
 #pragma unroll
-        for (int w = 0; w < W; ++w) s[w] += wt * Y::get(y + w);
-    }
-    const uint64_t at = (uint64_t)t * a.n + c;
+        for (uint32_t j = 0; j < 8; ++j) slot[j] = j0 + j < a.k ? (uint32_t)slots[j0 + j] : ~0u;
+        // (A row for every choice, so that no load waits for a branch; k > 0 here, so places > 0.)
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-        float v = s[w];
-        if (a.add) v += O::get(reinterpret_cast<const typename O::elem*>(a.add) + at + w);
-        O::put(reinterpret_cast<typename O::elem*>(a.out) + at + w, v);
+        for (uint32_t j = 0; j < 8; ++j) row[j].load(y + (uint64_t)(slot[j] < a.places ? slot[j] : 0) * a.n);
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) {
+            if (slot[j] >= a.places) continue;
+            const float wt = weights[j0 + j];
+#pragma unroll
+            for (int w = 0; w < W; ++w) s[w] = fmaf(wt, row[j].get(w), s[w]);
+        }
     }
+    if (a.add) {
+#pragma unroll
+        for (int w = 0; w < W; ++w) s[w] += extra.get(w);
+    }
+    Piece<O, W>::store(reinterpret_cast<typename O::elem*>(a.out) + at, s);
 }
 
+template <class Y, class O, int W>
+static bool combine_fits(const CombineArgs& a) {
+    return a.n % W == 0 && aligned_to(a.y, std::min<size_t>(16, W * sizeof(typename Y::elem))) &&
+           aligned_to(a.out, std::min<size_t>(16, W * sizeof(typename O::elem))) &&
+           aligned_to(a.add, std::min<size_t>(16, W * sizeof(typename O::elem)));
+}
+template <class Y, class O, int W>
+static hipError_t launch_combine_as(hipStream_t s, CombineArgs a) {
+    a.per = (a.n + 64 * W - 1) / (64 * W);
+    const uint64_t wgs = ((uint64_t)a.tokens * a.per + 3) / 4;
+    if (wgs > 0x3fffffffu) return hipErrorInvalidConfiguration;
+    moe_combine_kernel<Y, O, W><<<(unsigned)wgs, 256, 0, s>>>(a);
+    return hipGetLastError();
+}
 template <class Y, class O>
 static hipError_t launch_combine(hipStream_t s, CombineArgs a) {
-    a.per = a.n;
-    const uint64_t wgs = ((uint64_t)a.tokens * a.per + 255) / 256;
-    moe_combine_kernel<Y, O, 1><<<(unsigned)wgs, 256, 0, s>>>(a);
-    return hipGetLastError();
+    if (a.places == 0) a.k = 0;
+    constexpr int most = sizeof(typename Y::elem) == 2 ? 8 : 4;  // 16 bytes of a row
+    if (combine_fits<Y, O, most>(a)) return launch_combine_as<Y, O, most>(s, a);
+    if (combine_fits<Y, O, 2>(a)) return launch_combine_as<Y, O, 2>(s, a);
+    return launch_combine_as<Y, O, 1>(s, a);
 }
 
 }  // namespace bh
@@ -400,8 +470,7 @@ extern "C" int bh_moe_combine(void* stream, const void* y, int y_dtype, uint32_t
     static const char* who = "bh_moe_combine";
     if ((y_dtype != BH_OUT_F32 && y_dtype != BH_OUT_BF16) || (out_dtype != BH_OUT_F32 && out_dtype != BH_OUT_BF16))
         return fail(BH_ERR_INVALID, "%s: dtypes %d and %d", who, y_dtype, out_dtype);
-    if (places > 0x7fffffffu || tokens > 0x7fffffffu || n > 0x7fffffffu || (uint64_t)tokens * top_k > 0x7fffffffu ||
-        (uint64_t)tokens * n > (uint64_t)0x7fffffff * 256)
+    if (places > 0x7fffffffu || tokens > 0x7fffffffu || n > 0x7fffffffu || (uint64_t)tokens * top_k > 0x7fffffffu)
         return fail(BH_ERR_INVALID, "%s: %u places, %u tokens of %u choices, rows of %u", who, places, tokens, top_k, n);
     if (tokens == 0 || n == 0) return BH_OK;
     if (!out || (top_k && (!weights || !slots || (places && !y)))) return fail(BH_ERR_INVALID, "%s: null buffer", who);
@@ -410,5 +479,6 @@ extern "C" int bh_moe_combine(void* stream, const void* y, int y_dtype, uint32_t
     hipError_t e;
     if (y_dtype == BH_OUT_F32) e = out_dtype == BH_OUT_F32 ? launch_combine<F32, F32>(s, a) : launch_combine<F32, Bf16>(s, a);
     else e = out_dtype == BH_OUT_F32 ? launch_combine<Bf16, F32>(s, a) : launch_combine<Bf16, Bf16>(s, a);
+    if (e == hipErrorInvalidConfiguration) return fail(BH_ERR_INVALID, "%s: grid too large", who);
     return launched(e, who);
 }
