@@ -2,9 +2,10 @@
 // expert has, and the weighted sum of the experts' rows (bh_moe_route,
 // bh_moe_plan_rows, bh_moe_combine).
 //
-// Routing: a wave takes a token, its logits in registers (lane l holds experts l, l + 64,
-// ...), and finds the top_k largest one after another: the wave's maximum, then
-// the lowest index that has it (a ballot for each register, in order).
+// Routing: a group of 16 lanes takes a token (the whole wave where there are more than 256 experts), its
+// logits in registers (lane l of G holds experts l, l + G, ...), and finds the
+// top_k largest one after another: the group's maximum, then the lowest index
+// that has it.
 //
 // Plan: a stable counting sort of the (token, choice) entries by expert. A wave takes
 // its entries 64 at a time; the lanes with the same expert are found with a
@@ -17,7 +18,8 @@
 namespace bh {
 
 constexpr uint32_t MOE_MAX_EXPERTS = 1024, MOE_MAX_TOP = 64;
-constexpr uint32_t RT = 1024, RW = RT / 64;  // threads and waves of a routing workgroup
+constexpr uint32_t RW = 16, RT = RW * 64;  // most waves and threads of a routing workgroup
+constexpr uint32_t MOE_ENTRIES = 4096;     // most entries of a workgroup (16 bits hold their ranks; LDS: 52 KB)
 
 struct RouteArgs {
     const void* logits;
@@ -30,31 +32,65 @@ struct RouteArgs {
     int32_t* experts;
     uint32_t *offsets, *rows;
     int32_t* slots;
-    uint32_t* counts;  // [workgroups][e]: entries of each expert in each workgroup's tokens
+    uint32_t* counts;  // [workgroups][e]: entries of each expert in each workgroup's items
     uint32_t per;      // items of a workgroup
 };
 
-// The token's top k experts: lane j < k gets the j-th (-1: none) and its weight.
-template <class T, int NV>
-__device__ __forceinline__ void route_token(const RouteArgs& a, uint32_t t, uint32_t lane, int& expert, float& weight) {
-    const typename T::elem* l = reinterpret_cast<const typename T::elem*>(a.logits) + (uint64_t)t * a.stride;
-    expert = -1;
-    weight = 0.0f;
-    if (a.mask && !a.mask[t]) return;
-    float x[NV];
+// Reductions over G = 16 or 64 neighbouring lanes; every lane gets the result.
+template <int CTRL>
+__device__ __forceinline__ uint32_t turned(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, false);
+}
+template <int G, class F>
+__device__ __forceinline__ uint32_t over_group(uint32_t v, F f) {
+    v = f(v, turned<0x128>(v));  // row_ror 8, 4, 2, 1: all 16 lanes of a row
+    v = f(v, turned<0x124>(v));
+    v = f(v, turned<0x122>(v));
+    v = f(v, turned<0x121>(v));
+    if constexpr (G == 64) {
+        v = f(v, xor_lane_u<16>(v));
+        v = f(v, xor_lane_u<32>(v));
+    }
+    return v;
+}
+template <int G>
+__device__ __forceinline__ float group_max(float v) {
+    return __builtin_bit_cast(float, over_group<G>(__builtin_bit_cast(uint32_t, v), [](uint32_t a, uint32_t b) {
+        return __builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)));
+    }));
+}
+template <int G>
+__device__ __forceinline__ float group_sum(float v) {
+    return __builtin_bit_cast(float, over_group<G>(__builtin_bit_cast(uint32_t, v), [](uint32_t a, uint32_t b) {
+        return __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b));
+    }));
+}
+template <int G>
+__device__ __forceinline__ uint32_t group_min(uint32_t v) {
+    return over_group<G>(v, [](uint32_t a, uint32_t b) { return min(a, b); });
+}
+
+// The top k experts of token t, of this lane's group (t >= items: of none): lane l of it gets choices l, l + G, ...
+// (-1: none) and their weights. For a whole wave.
+template <class T, int G, int NV, int NK>
+__device__ __forceinline__ void route_token(const RouteArgs& a, uint32_t t, uint32_t l, int (&expert)[NK], float (&weight)[NK]) {
+    const bool live = t < a.items && !(a.mask && !a.mask[min(t, a.items - 1)]);
+    const typename T::elem* row = reinterpret_cast<const typename T::elem*>(a.logits) + (uint64_t)min(t, a.items - 1) * a.stride;
+    float x[NV], logit[NK];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-        const uint32_t i = v * 64 + lane;
-        const float f = T::get(l + min(i, a.e - 1));
-        x[v] = i < a.e && f == f ? f : -INFINITY;
+        const uint32_t i = v * G + l;
+        const float f = T::get(row + min(i, a.e - 1));
+        x[v] = live && i < a.e && f == f ? f : -INFINITY;
     }
-    float top = -INFINITY, logit = -INFINITY, total = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NK; ++n) expert[n] = -1, logit[n] = -INFINITY;
+    float top = -INFINITY, total = 0.0f;
     for (uint32_t j = 0; j < a.k; ++j) {
         float m = x[0];
 #pragma unroll
         for (int v = 1; v < NV; ++v) m = fmaxf(m, x[v]);
-        m = xor_max<32>(m);
-        if (m == -INFINITY) break;
+        m = group_max<G>(m);
         if (j == 0) {
             top = m;
             // exp(l - top), where equal infinities are no distance apart
@@ -62,32 +98,39 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, uint32_t t, uint
                 float s = 0.0f;
 #pragma unroll
                 for (int v = 0; v < NV; ++v) s += x[v] == top ? 1.0f : expf(x[v] - top);
-                total = xor_sum<32>(s);
+                total = group_sum<G>(s);
             }
         }
-        bool found = false;
+        uint32_t at = ~0u;
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            const unsigned long long b = __ballot(x[v] == m);
-            if (!found && b) {
-                found = true;
-                const uint32_t at = (uint32_t)__builtin_ctzll(b);
-                if (lane == at) x[v] = -INFINITY;
-                if (lane == j) expert = v * 64 + (int)at;
-            }
+        for (int v = NV - 1; v >= 0; --v) at = x[v] == m ? v * G + l : at;
+        at = group_min<G>(at);
+        const bool found = m > -INFINITY;
+        if (!__any(found)) break;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) x[v] = at == v * G + l ? -INFINITY : x[v];
+#pragma unroll
+        for (int n = 0; n < NK; ++n)
+            if (found && j == n * G + l) expert[n] = (int)at, logit[n] = m;
+    }
+    float s[NK], sum = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NK; ++n) {
+        s[n] = 0.0f;
+        if (expert[n] >= 0) {
+            if (a.score == BH_MOE_SOFTMAX) s[n] = logit[n] == top ? 1.0f : expf(logit[n] - top);
+            // sigmoid; for a sum that is divided out, of far negative logits, exp(-top) times it
+            else if (a.renormalize && top < 0.0f) s[n] = expf(logit[n] - top) / (1.0f + expf(logit[n]));
+            else s[n] = 1.0f / (1.0f + expf(-logit[n]));
         }
-        if (lane == j) logit = m;
+        sum += s[n];
     }
-    float s = 0.0f;
-    if (expert >= 0) {
-        if (a.score == BH_MOE_SOFTMAX) s = logit == top ? 1.0f : expf(logit - top);
-        // sigmoid; for a sum that is divided out, of far negative logits, exp(-top) times it
-        else if (a.renormalize && top < 0.0f) s = expf(logit - top) / (1.0f + expf(logit));
-        else s = 1.0f / (1.0f + expf(-logit));
+    if (a.renormalize) total = group_sum<G>(sum);
+#pragma unroll
+    for (int n = 0; n < NK; ++n) {
+        if (a.score == BH_MOE_SOFTMAX || a.renormalize) s[n] = expert[n] >= 0 ? s[n] / total : 0.0f;
+        weight[n] = s[n] * a.scale;
     }
-    if (a.renormalize) total = xor_sum<32>(s);
-    if (a.score == BH_MOE_SOFTMAX || a.renormalize) s = expert >= 0 ? s / total : 0.0f;
-    weight = s * a.scale;
 }
 
 // Inclusive sum over the lanes of a wave.
@@ -116,59 +159,84 @@ __device__ __forceinline__ void wave_order() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// A workgroup's tokens: their experts (routed here, ROUTE, or read), and of each entry
+// Exclusive sums of n counts in LDS, by the first wave, to `to` (LDS; may be `from`) and, where given, `out`, the total behind them.
+__device__ __forceinline__ void place_experts(const uint32_t* from, uint32_t n, uint32_t lane, uint32_t* to, uint32_t* out) {
+    uint32_t base = 0;
+    for (uint32_t e0 = 0; e0 < n; e0 += 64) {
+        const uint32_t e = e0 + lane, c = e < n ? from[e] : 0, upto = wave_scan(c, lane);
+        if (e < n) {
+            to[e] = base + upto - c;
+            if (out) out[e] = base + upto - c;
+        }
+        base += (uint32_t)__shfl((int)upto, 63, 64);
+    }
+    if (out && lane == 0) out[n] = base;
+}
+
+// LDS of a workgroup that plans: offsets [e], counts [waves][e], key and rank of each entry.
+static size_t plan_lds(uint32_t e, uint32_t waves, uint32_t entries) {
+    return (size_t)e * 4 + ((size_t)waves * e + 1) / 2 * 4 + (size_t)entries * 4;
+}
+
+// A workgroup's items: their experts (routed here, or read: NV = 0), and of each entry
 // the rank among the entries of its expert in this workgroup. With one workgroup
 // (ONE) the plan is complete at the end; else `slots` holds the ranks and
-// `counts` the workgroup's counts, for moe_place_kernel. NV = 0: not routed here.
-template <class T, int NV, bool PLAN, bool ONE>
+// `counts` the workgroup's counts, for moe_place_kernel. Routing is bound by its
+// vector instructions, some 13 for each token and choice of 128 experts.
+template <class T, int G, int NV, int NK, bool PLAN, bool ONE>
 __global__ __launch_bounds__(RT) void moe_route_kernel(RouteArgs a) {
-    extern __shared__ uint32_t off[];  // [e] offsets, then [RW][e] counts
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const uint32_t t0 = blockIdx.x * a.per, t1 = min(t0 + a.per, a.items);
-    // Wave w's tokens, in order: entries that follow each other.
-    const uint32_t share = (a.per + RW - 1) / RW, w0 = min(t0 + wave * share, t1), w1 = min(w0 + share, t1);
+    extern __shared__ uint32_t lds[];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+    const uint32_t t0 = min(blockIdx.x * a.per, a.items), t1 = min(t0 + a.per, a.items);
+    // Wave w's items, in order: entries that follow each other. Whole groups of tokens.
+    constexpr uint32_t TOKENS = 64 / G;
+    uint32_t share = (t1 - t0 + waves - 1) / waves;
+    if constexpr (NV > 0) share = (share + TOKENS - 1) / TOKENS * TOKENS;
+    const uint32_t w0 = min(t0 + wave * share, t1), w1 = min(w0 + share, t1);
+    uint32_t* off = lds;
     uint16_t *cnts = reinterpret_cast<uint16_t*>(off + a.e), *cnt = cnts + wave * a.e;
+    // entry i of the workgroup: its key (low 16 bits) and its rank
+    uint32_t* entry = off + a.e + (waves * a.e + 1) / 2;
+    const uint32_t i0 = t0 * a.k;
     if constexpr (PLAN) {
         for (uint32_t i = lane; i < a.e; i += 64) cnt[i] = 0;
-        wave_order();
     }
     if constexpr (NV > 0) {
-        for (uint32_t t = w0; t < w1; ++t) {
-            int expert;
-            float weight;
-            route_token<T, NV>(a, t, lane, expert, weight);
-            if (lane < a.k) {
-                a.experts[(uint64_t)t * a.k + lane] = expert;
-                a.weights[(uint64_t)t * a.k + lane] = weight;
+        for (uint32_t t = w0; t < w1; t += TOKENS) {
+            const uint32_t mine = t + lane / G, l = lane % G;
+            int expert[NK];
+            float weight[NK];
+            route_token<T, G, NV, NK>(a, mine < w1 ? mine : a.items, l, expert, weight);
+#pragma unroll
+            for (int n = 0; n < NK; ++n) {
+                const uint32_t j = n * G + l;
+                if (j < a.k && mine < w1) {
+                    a.experts[(uint64_t)mine * a.k + j] = expert[n];
+                    a.weights[(uint64_t)mine * a.k + j] = weight[n];
+                    if constexpr (PLAN) entry[mine * a.k + j - i0] = min((uint32_t)expert[n], a.e);
+                }
             }
         }
     }
     if constexpr (!PLAN) return;
+    wave_order();
     const uint32_t bits = 32 - (uint32_t)__builtin_clz(a.e);  // of a key, e itself (routed nowhere) included
-    const uint32_t i1 = w1 * a.k;
-    if (NV > 0) __threadfence_block();  // the wave reads the experts that its other lanes stored
-    auto key_of = [&](uint32_t i) -> uint32_t {
-        const uint32_t e = (uint32_t)a.experts[i] - a.first;
-        return e < a.e ? e : a.e;
-    };
-    for (uint32_t i0 = w0 * a.k; i0 < i1; i0 += 64) {
-        const uint32_t i = i0 + lane, key = i < i1 ? key_of(i) : a.e;
+    const uint32_t from = w0 * a.k, to = w1 * a.k;
+    for (uint32_t i = from + lane; i - lane < to; i += 64) {
+        uint32_t key = a.e;
+        if (i < to) key = NV > 0 ? entry[i - i0] : min((uint32_t)a.experts[i] - a.first, a.e);
         const unsigned long long same = same_key(key, bits), below = (1ull << lane) - 1;
-        if (key < a.e) {
-            const uint32_t before = cnt[key];
-            a.slots[i] = (int32_t)(before + (uint32_t)__popcll(same & below));
-            wave_order();
-            if (!(same & below)) cnt[key] = (uint16_t)(before + (uint32_t)__popcll(same));
-        } else if (i < i1) {
-            a.slots[i] = -1;
-        }
+        const uint32_t before = key < a.e ? cnt[key] : 0;
+        wave_order();
+        if (key < a.e && !(same & below)) cnt[key] = (uint16_t)(before + (uint32_t)__popcll(same));
+        if (i < to) entry[i - i0] = key | (before + (uint32_t)__popcll(same & below)) << 16;
         wave_order();
     }
     __syncthreads();
     // Counts to where each wave's entries begin; the workgroup's counts.
-    for (uint32_t e = tid; e < a.e; e += RT) {
+    for (uint32_t e = tid; e < a.e; e += blockDim.x) {
         uint32_t sum = 0;
-        for (uint32_t w = 0; w < RW; ++w) {
+        for (uint32_t w = 0; w < waves; ++w) {
             const uint32_t c = cnts[w * a.e + e];
             cnts[w * a.e + e] = (uint16_t)sum;
             sum += c;
@@ -178,100 +246,139 @@ __global__ __launch_bounds__(RT) void moe_route_kernel(RouteArgs a) {
     }
     __syncthreads();
     if constexpr (ONE) {
-        if (wave == 0) {
-            uint32_t base = 0;
-            for (uint32_t e0 = 0; e0 < a.e; e0 += 64) {
-                const uint32_t e = e0 + lane, c = e < a.e ? off[e] : 0, upto = wave_scan(c, lane);
-                if (e < a.e) {
-                    off[e] = base + upto - c;
-                    a.offsets[e] = base + upto - c;
-                }
-                base += (uint32_t)__shfl((int)upto, 63, 64);
-            }
-            if (lane == 0) a.offsets[a.e] = base;
-        }
+        if (wave == 0) place_experts(off, a.e, lane, off, a.offsets);
         __syncthreads();
     }
-    for (uint32_t i = w0 * a.k + lane; i < i1; i += 64) {
-        const uint32_t key = key_of(i);
-        if (key == a.e) continue;
-        const uint32_t at = (uint32_t)a.slots[i] + cnt[key] + (ONE ? off[key] : 0);
+    for (uint32_t i = from + lane; i < to; i += 64) {
+        const uint32_t key = entry[i - i0] & 0xffff;
+        if (key == a.e) {
+            a.slots[i] = -1;
+            continue;
+        }
+        const uint32_t at = (entry[i - i0] >> 16) + cnt[key] + (ONE ? off[key] : 0);
         a.slots[i] = (int32_t)at;
         if constexpr (ONE) a.rows[at] = i / a.div;
     }
 }
 
+// The counts of a call of many workgroups become the sums before each, and those of all go behind the last:
+// a workgroup takes an expert.
+__global__ __launch_bounds__(256) void moe_scan_kernel(RouteArgs a, uint32_t wgs) {
+    __shared__ uint32_t part[4];
+    const uint32_t e = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    uint32_t base = 0;
+    for (uint32_t b0 = 0; b0 < wgs; b0 += 256) {
+        const uint32_t b = b0 + tid, c = b < wgs ? a.counts[(uint64_t)b * a.e + e] : 0;
+        const uint32_t upto = wave_scan(c, lane);
+        __syncthreads();
+        if (lane == 63) part[wave] = upto;
+        __syncthreads();
+        uint32_t before = base;
+        for (uint32_t w = 0; w < wave; ++w) before += part[w];
+        if (b < wgs) a.counts[(uint64_t)b * a.e + e] = before + upto - c;
+        base += part[0] + part[1] + part[2] + part[3];
+    }
+    if (tid == 0) a.counts[(uint64_t)wgs * a.e + e] = base;
+}
+
 // Ranks to places: workgroup b's entries of an expert come behind those of the
-// workgroups before it.
+// workgroups before it. SUMMED: moe_scan_kernel has added them up; else every workgroup does.
+template <bool SUMMED>
 __global__ __launch_bounds__(RT) void moe_place_kernel(RouteArgs a) {
     extern __shared__ uint32_t lds[];  // [e] all, [e] before
     uint32_t *all = lds, *before = lds + a.e;
-    const uint32_t tid = threadIdx.x, lane = tid & 63;
-    for (uint32_t e = tid; e < a.e; e += RT) {
-        uint32_t sum = 0, mine = 0;
-        for (uint32_t b = 0; b < gridDim.x; ++b) {
-            if (b == blockIdx.x) mine = sum;
-            sum += a.counts[(uint64_t)b * a.e + e];
+    const uint32_t tid = threadIdx.x, wgs = gridDim.x;
+    if constexpr (SUMMED) {
+        for (uint32_t e = tid; e < a.e; e += RT) {
+            all[e] = a.counts[(uint64_t)wgs * a.e + e];
+            before[e] = a.counts[(uint64_t)blockIdx.x * a.e + e];
         }
-        all[e] = sum;
-        before[e] = mine;
-    }
-    __syncthreads();
-    if (tid < 64) {
-        uint32_t base = 0;
-        for (uint32_t e0 = 0; e0 < a.e; e0 += 64) {
-            const uint32_t e = e0 + lane, c = e < a.e ? all[e] : 0, upto = wave_scan(c, lane);
-            if (e < a.e) {
-                before[e] += base + upto - c;
-                if (blockIdx.x == 0) a.offsets[e] = base + upto - c;
+    } else {
+        for (uint32_t e = tid; e < 2 * a.e; e += RT) lds[e] = 0;
+        __syncthreads();
+        // A thread adds up an expert's counts in every parts-th workgroup. (Sums of integers: any order.)
+        const uint32_t parts = a.e < RT ? RT / a.e : 1, part = tid / a.e, e = tid - part * a.e;
+        if (part < parts) {
+            uint32_t sum = 0, mine = 0;
+#pragma unroll 8
+            for (uint32_t b = part; b < wgs; b += parts) {
+                const uint32_t c = a.counts[(uint64_t)b * a.e + e];
+                sum += c;
+                mine += b < blockIdx.x ? c : 0;
             }
-            base += (uint32_t)__shfl((int)upto, 63, 64);
+            atomicAdd(&all[e], sum);
+            atomicAdd(&before[e], mine);
         }
-        if (blockIdx.x == 0 && lane == 0) a.offsets[a.e] = base;
     }
     __syncthreads();
-    const uint32_t t0 = blockIdx.x * a.per, t1 = min(t0 + a.per, a.items);
+    if (tid < 64) place_experts(all, a.e, tid, all, blockIdx.x == 0 ? a.offsets : nullptr);
+    __syncthreads();
+    const uint32_t t0 = min(blockIdx.x * a.per, a.items), t1 = min(t0 + a.per, a.items);
     for (uint32_t i = t0 * a.k + tid; i < t1 * a.k; i += RT) {
         const uint32_t e = (uint32_t)a.experts[i] - a.first;
         if (e >= a.e) continue;
-        const uint32_t at = (uint32_t)a.slots[i] + before[e];
+        const uint32_t at = (uint32_t)a.slots[i] + before[e] + all[e];
         a.slots[i] = (int32_t)at;
         a.rows[at] = i / a.div;
     }
 }
 
-// Tokens of a workgroup that routes: one workgroup up to 128 tokens. Entries of one
-// that only plans. (At most 64 * 128 entries: their counts fit 16 bits.)
-static uint32_t route_share(uint32_t tokens) { return tokens <= 128 ? std::max(tokens, 1u) : 64; }
-static uint32_t plan_share(uint32_t entries) { return entries <= 4096 ? std::max(entries, 1u) : 4096; }
+// Items of a workgroup: one workgroup up to 128 tokens or 4096 entries, else 256 or as
+// many as it takes.
+static uint32_t share_of(uint32_t items, uint32_t k, uint32_t one) {
+    const uint32_t most = std::max(MOE_ENTRIES / std::max(k, 1u), 1u);
+    if (items <= std::min(one, most)) return std::max(items, 1u);
+    return std::min(most, std::max((items + 255) / 256, one / 4));
+}
+static uint32_t route_share(uint32_t tokens, uint32_t k) { return share_of(tokens, k, 128); }
+static uint32_t plan_share(uint32_t entries) { return share_of(entries, 1, 4096); }
 static uint32_t groups_of(uint32_t items, uint32_t per) { return std::max((items + per - 1) / per, 1u); }
+// From this many workgroups on their counts are summed in a launch of its own.
+constexpr uint32_t SCAN_GROUPS = 512;
 
-template <class T, int NV>
-static hipError_t launch_route(hipStream_t s, const RouteArgs& a, bool plan) {
+template <class T, int G, int NV, int NK>
+static hipError_t launch_route_as(hipStream_t s, const RouteArgs& a, bool plan) {
     const uint32_t wgs = groups_of(a.items, a.per);
+    // (Four tokens of a wave at a time, or an entry a lane.)
+    const uint32_t per_wave = NV > 0 ? 64 / G : 64;
+    const uint32_t waves = std::min(RW, std::max(1u, (std::min(a.per, a.items) + per_wave - 1) / per_wave));
     if (!plan) {
-        moe_route_kernel<T, NV, false, false><<<wgs, RT, 0, s>>>(a);
+        moe_route_kernel<T, G, NV, NK, false, false><<<wgs, waves * 64, 0, s>>>(a);
         return hipGetLastError();
     }
-    const size_t lds = (size_t)a.e * 4 + (size_t)RW * a.e * 2;
+    const size_t lds = plan_lds(a.e, waves, a.per * a.k);
     if (wgs == 1) {
-        moe_route_kernel<T, NV, true, true><<<1, RT, lds, s>>>(a);
+        moe_route_kernel<T, G, NV, NK, true, true><<<1, waves * 64, lds, s>>>(a);
         return hipGetLastError();
     }
-    moe_route_kernel<T, NV, true, false><<<wgs, RT, lds, s>>>(a);
-    const hipError_t err = hipGetLastError();
+    moe_route_kernel<T, G, NV, NK, true, false><<<wgs, waves * 64, lds, s>>>(a);
+    hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
-    moe_place_kernel<<<wgs, RT, (size_t)2 * a.e * 4, s>>>(a);
+    if (wgs < SCAN_GROUPS) {
+        moe_place_kernel<false><<<wgs, RT, (size_t)2 * a.e * 4, s>>>(a);
+        return hipGetLastError();
+    }
+    moe_scan_kernel<<<a.e, 256, 0, s>>>(a, wgs);
+    if ((err = hipGetLastError()) != hipSuccess) return err;
+    moe_place_kernel<true><<<wgs, RT, (size_t)2 * a.e * 4, s>>>(a);
     return hipGetLastError();
+}
+
+template <class T, int G, int NV>
+static hipError_t launch_route(hipStream_t s, const RouteArgs& a, bool plan) {
+    if (a.k <= G) return launch_route_as<T, G, NV, 1>(s, a, plan);
+    return launch_route_as<T, G, NV, 64 / G>(s, a, plan);
 }
 
 template <class T>
 static hipError_t launch_route_any(hipStream_t s, const RouteArgs& a, bool plan) {
-    if (a.e <= 64) return launch_route<T, 1>(s, a, plan);
-    if (a.e <= 128) return launch_route<T, 2>(s, a, plan);
-    if (a.e <= 256) return launch_route<T, 4>(s, a, plan);
-    if (a.e <= 512) return launch_route<T, 8>(s, a, plan);
-    return launch_route<T, 16>(s, a, plan);
+    if (a.e <= 16) return launch_route<T, 16, 1>(s, a, plan);
+    if (a.e <= 32) return launch_route<T, 16, 2>(s, a, plan);
+    if (a.e <= 64) return launch_route<T, 16, 4>(s, a, plan);
+    if (a.e <= 128) return launch_route<T, 16, 8>(s, a, plan);
+    if (a.e <= 256) return launch_route<T, 16, 16>(s, a, plan);
+    if (a.e <= 512) return launch_route<T, 64, 8>(s, a, plan);
+    return launch_route<T, 64, 16>(s, a, plan);
 }
 
 static int check_plan(const char* who, uint32_t tokens, uint32_t top_k, uint32_t n_experts, const bh_moe_plan* plan,
@@ -421,8 +528,8 @@ extern "C" int bh_moe_workspace(uint32_t tokens, uint32_t top_k, uint32_t n_expe
     if (n_experts == 0 || n_experts > MOE_MAX_EXPERTS || (uint64_t)tokens * top_k > 0x7fffffffu)
         return fail(BH_ERR_INVALID, "bh_moe_workspace: %u tokens, %u choices, %u experts", tokens, top_k, n_experts);
     const uint32_t entries = tokens * top_k;
-    const uint32_t wgs = std::max(groups_of(tokens, route_share(tokens)), groups_of(entries, plan_share(entries)));
-    *bytes = wgs > 1 ? (uint64_t)wgs * n_experts * 4 : 0;
+    const uint32_t wgs = std::max(groups_of(tokens, route_share(tokens, top_k)), groups_of(entries, plan_share(entries)));
+    *bytes = wgs > 1 ? (uint64_t)(wgs + 1) * n_experts * 4 : 0;
     return BH_OK;
 }
 
@@ -444,7 +551,7 @@ extern "C" int bh_moe_route(void* stream, const bh_moe_router* r, float* weights
     a.logits = r->logits, a.stride = r->stride, a.mask = r->mask, a.items = r->tokens, a.e = r->n_experts;
     a.k = a.div = r->top_k;
     a.score = r->score, a.renormalize = r->renormalize, a.scale = r->scale, a.weights = weights, a.experts = experts;
-    a.per = route_share(r->tokens);
+    a.per = route_share(r->tokens, r->top_k);
     const hipStream_t s = (hipStream_t)stream;
     const hipError_t e = r->dtype == BH_OUT_F32 ? launch_route_any<F32>(s, a, plan) : launch_route_any<Bf16>(s, a, plan);
     return launched(e, who);
@@ -461,7 +568,7 @@ extern "C" int bh_moe_plan_rows(void* stream, const int32_t* experts, uint32_t t
     a.items = tokens * top_k, a.e = n_experts, a.k = 1, a.div = std::max(top_k, 1u), a.first = first;
     a.experts = const_cast<int32_t*>(experts);
     a.per = plan_share(a.items);
-    return launched(launch_route<F32, 0>((hipStream_t)stream, a, true), who);
+    return launched(launch_route_as<F32, 64, 0, 1>((hipStream_t)stream, a, true), who);
 }
 
 extern "C" int bh_moe_combine(void* stream, const void* y, int y_dtype, uint32_t places, const float* weights,

@@ -32,7 +32,7 @@ def check_plan(plan, experts, n_experts, first=0):
 # ---------------------------------------------------------------- routing
 
 SIZES = [(1, 1, 1), (1, 8, 2), (1, 128, 8), (3, 7, 7), (5, 60, 4), (64, 64, 8), (65, 65, 6), (128, 128, 8), (129, 128, 8),
-         (130, 256, 8), (300, 512, 16), (200, 1024, 64), (1000, 3, 2), (777, 16, 1), (2049, 130, 5)]
+         (130, 256, 8), (128, 1024, 64), (2, 17, 17), (6, 33, 20), (300, 512, 16), (200, 1024, 64), (1000, 3, 2), (777, 16, 1), (2049, 130, 5)]
 
 
 def logits_of(tokens, n, dtype, seed):
@@ -86,6 +86,24 @@ def test_route_values_without_order(gpu, dtype, score, renormalize):
     assert n == (experts >= 0).sum()
 
 
+def test_route_many_tokens(gpu):
+    """Enough workgroups that their counts are summed in a launch of its own; every entry checked."""
+    tokens, n, top_k = 600000, 16, 4
+    x = torch.randn(tokens, n, generator=gen(1)).to(gpu)
+    mask = (torch.arange(tokens) % 7 != 0).to(gpu)
+    w, e, plan = ops.moe_route(x, top_k, mask=mask)
+    want = x.double().sort(dim=1, descending=True, stable=True)
+    assert torch.equal(e, torch.where(mask[:, None], want.indices[:, :top_k], -1).int())
+    same_ints(plan.offsets, moeref.plan(e.cpu().numpy(), n)[0])
+    flat = e.flatten().long()
+    order = torch.where(flat >= 0, flat, n).sort(stable=True).indices
+    live = int(plan.offsets[-1])
+    assert torch.equal(plan.rows[:live], (order[:live] // top_k).int())
+    place = torch.full_like(flat, -1)
+    place[order[:live]] = torch.arange(live, device=gpu)
+    assert torch.equal(plan.slots.flatten().long(), place)
+
+
 def test_route_rows_of_a_wider_matrix(gpu):
     """A stride, and rows that do not begin at aligned addresses."""
     wide = logits_of(50, 77, F32, 1).to(gpu)
@@ -119,7 +137,8 @@ def test_no_tokens(gpu):
 
 
 @pytest.mark.parametrize("tokens,top_k,n,first", [(1, 1, 1, 0), (1, 70, 3, 0), (7, 3, 4, 2), (100, 8, 1024, 0), (1000, 5, 11, 4),
-                                                  (5000, 3, 64, 0), (4097, 1, 300, 10), (20000, 8, 128, 0), (1, 30000, 2, 0)])
+                                                  (5000, 3, 64, 0), (4097, 1, 300, 10), (20000, 8, 128, 0), (1, 30000, 2, 0),
+                                                  (1000000, 3, 5, 0)])
 def test_plan(gpu, tokens, top_k, n, first):
     """Experts from elsewhere: the same one twice in a token, and ones outside the range."""
     e = torch.randint(-2, n + first + 3, (tokens, top_k), generator=gen(tokens), dtype=torch.int32)
