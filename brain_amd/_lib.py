@@ -115,10 +115,10 @@ SIGNATURES = {
     "bh_paged_weight_sums_i8": (i32, [vp, vp, u64, i32, u32, vp, P(Kv8T), P(Kv8BatchT), f32, vp, u32]),
     "bh_paged_kv_evict_i8": (i32, [vp, P(Kv8T), vp, u32, vp, u32, u32, u32, u32, vp, u32, vp, u32, vp, vp]),
     "bh_moe_workspace": (i32, [u32, u32, u32, P(u64)]),
-    "bh_moe_route": (i32, [vp, P(MoeRouterT), vp, vp, P(MoePlanT), vp, u64]),
-    "bh_moe_plan_rows": (i32, [vp, vp, u32, u32, u32, u32, P(MoePlanT), vp, u64]),
-    "bh_matmul_i8_grouped": (i32, [vp, P(GroupedI8T), vp, i32]),
-    "bh_matmul_i8_grouped_glu": (i32, [vp, P(GroupedI8T), vp, i32]),
+    "bh_moe_route": (i32, [vp, vp, vp, vp, vp, vp, u64]),
+    "bh_moe_plan_rows": (i32, [vp, vp, u32, u32, u32, u32, vp, vp, u64]),
+    "bh_matmul_i8_grouped": (i32, [vp, vp, vp, i32]),
+    "bh_matmul_i8_grouped_glu": (i32, [vp, vp, vp, i32]),
     "bh_moe_combine": (i32, [vp, vp, i32, u32, vp, vp, u32, u32, u32, vp, vp, i32]),
     "bh_reserve_workspace": (i32, [vp, u32, u32, u32]),
     "bh_matmul_i8_static": (i32, [vp, vp, vp, f32, f32, vp, u32, u32, u32]),

@@ -5,12 +5,13 @@ runs in the library's gfx950 kernels. Packed int8 tensors are torch.int32
 tensors holding the u32 words (4 int8 per word, little-endian along K).
 """
 import ctypes as C
+import struct
 from typing import NamedTuple
 
 import torch
 
-from ._lib import (BH_MOE_SIGMOID, BH_MOE_SOFTMAX, BH_OUT_BF16, BH_OUT_F32, BH_OUT_I32, GroupedI8T, Kv8BatchT, Kv8T,
-                   MoePlanT, MoeRouterT, QkRowsT, check, load)
+from ._lib import (BH_MOE_SIGMOID, BH_MOE_SOFTMAX, BH_OUT_BF16, BH_OUT_F32, BH_OUT_I32, Kv8BatchT, Kv8T, QkRowsT, check,
+                   load)
 
 _CODES = {torch.float32: BH_OUT_F32, torch.bfloat16: BH_OUT_BF16, torch.int32: BH_OUT_I32}
 
@@ -19,9 +20,14 @@ _CODES = {torch.float32: BH_OUT_F32, torch.bfloat16: BH_OUT_BF16, torch.int32: B
 # Stream object on the way (3.4 us, a third of a decode linear's host time;
 # this one 0.1 us).
 if hasattr(torch._C, "_cuda_getCurrentRawStream"):
+    _raw_stream = torch._C._cuda_getCurrentRawStream
+
     def _stream():
-        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+        return _raw_stream(torch.cuda.current_device())
 else:
+    def _raw_stream(dev):
+        return torch.cuda.current_stream(dev).cuda_stream
+
     def _stream():
         return torch.cuda.current_stream().cuda_stream
 
@@ -278,7 +284,15 @@ def _stream_of(dev):
         raise ValueError("brain_amd.ops: tensors must live on the GPU")
     if dev != _current():
         raise ValueError(f"brain_amd.ops: the tensors are on GPU {dev}, the current device is {_current()}")
-    return _stream()
+    return _raw_stream(dev)
+
+
+# Descriptions for the C entries are packed (0.3 us) instead of ctypes structures
+# made for a call (1 us); _fits is _need and _here in one.
+def _fits(t, dtype, numel, dev, name):
+    if t.dtype is not dtype or t.numel() < numel or t.get_device() != dev or not t.is_contiguous():
+        _need(t, dtype, numel, name)
+        _here(dev, t)
 
 
 # The C entries take sizes of 32 bits, and ctypes cuts what is longer without a
@@ -576,6 +590,12 @@ def _moe_sizes(who, tokens, top_k, n_experts):
         raise ValueError(f"{who}: {tokens} tokens of {top_k} choices")
 
 
+_route_pack = struct.Struct("PQiIIIPiif4x").pack  # bh_moe_router
+_plan_pack = struct.Struct("PPP").pack                # bh_moe_plan
+_group_pack = struct.Struct("PPI4xPPIIPPPII").pack    # bh_grouped_i8
+_ws_needs = {}  # workspace bytes of moe_route and moe_plan, by the sizes of the call
+
+
 def _moe_plan(dev, device, tokens, top_k, n_experts, plan):
     """The plan's buffers and their workspace."""
     entries = tokens * top_k
@@ -584,14 +604,19 @@ def _moe_plan(dev, device, tokens, top_k, n_experts, plan):
                        torch.empty(entries, device=device, dtype=torch.int32),
                        torch.empty((tokens, top_k), device=device, dtype=torch.int32))
     else:
-        _need(plan.offsets, torch.int32, n_experts + 1, "plan.offsets")
-        _need(plan.rows, torch.int32, entries, "plan.rows")
-        _need(plan.slots, torch.int32, entries, "plan.slots")
-        _here(dev, plan.offsets, plan.rows, plan.slots)
-    n = C.c_uint64()
-    check(load().bh_moe_workspace(tokens, top_k, n_experts, C.byref(n)))
-    ws = torch.empty(n.value, device=device, dtype=torch.uint8) if n.value else None
-    return plan, MoePlanT(plan.offsets.data_ptr(), plan.rows.data_ptr(), plan.slots.data_ptr()), ws, n.value
+        _fits(plan.offsets, torch.int32, n_experts + 1, dev, "plan.offsets")
+        _fits(plan.rows, torch.int32, entries, dev, "plan.rows")
+        _fits(plan.slots, torch.int32, entries, dev, "plan.slots")
+    sizes = (tokens, top_k, n_experts)
+    need = _ws_needs.get(sizes)
+    if need is None:
+        n = C.c_uint64()
+        check(load().bh_moe_workspace(tokens, top_k, n_experts, C.byref(n)))
+        if len(_ws_needs) > 4096:
+            _ws_needs.clear()
+        need = _ws_needs[sizes] = n.value
+    ws = torch.empty(need, device=device, dtype=torch.uint8) if need else None
+    return plan, _plan_pack(plan.offsets.data_ptr(), plan.rows.data_ptr(), plan.slots.data_ptr()), ws, need
 
 
 def moe_route(logits, top_k, score="softmax", renormalize=True, scale=1.0, mask=None, plan=None, weights=None, experts=None):
@@ -602,11 +627,12 @@ def moe_route(logits, top_k, score="softmax", renormalize=True, scale=1.0, mask=
     padding, which goes nowhere (-1, weight 0), as does a choice whose logit is NaN or
     -inf. Returns (weights [tokens, top_k] f32, experts [tokens, top_k] int32,
     MoePlan); plan=False: no plan is made (None)."""
-    if logits.dim() != 2 or logits.dtype not in _ACT:
-        raise ValueError(f"logits: {logits.dtype} {tuple(logits.shape)}, expected [tokens, n_experts] float32 or bfloat16")
-    tokens, n_experts = logits.shape
+    dtype, shape = logits.dtype, logits.shape
+    if len(shape) != 2 or dtype not in _ACT:
+        raise ValueError(f"logits: {dtype} {tuple(shape)}, expected [tokens, n_experts] float32 or bfloat16")
+    tokens, n_experts = shape
     _moe_sizes("moe_route", tokens, top_k, n_experts)
-    if not 0 < top_k <= min(n_experts, _MOE_MAX_TOP):
+    if not 0 < top_k <= n_experts or top_k > _MOE_MAX_TOP:
         raise ValueError(f"moe_route: the top {top_k} of {n_experts} experts (at most {_MOE_MAX_TOP})")
     if score not in _SCORES:
         raise ValueError(f"moe_route: score {score!r}, one of {sorted(_SCORES)}")
@@ -615,25 +641,23 @@ def moe_route(logits, top_k, score="softmax", renormalize=True, scale=1.0, mask=
         raise ValueError(f"logits: strides {logits.stride()}; the experts of a token must lie side by side")
     dev, device = logits.get_device(), logits.device
     if mask is not None:
-        _need(mask, torch.bool, tokens, "mask")
+        _fits(mask, torch.bool, tokens, dev, "mask")
     if weights is None:
         weights = torch.empty((tokens, top_k), device=device, dtype=torch.float32)
     else:
-        _need(weights, torch.float32, tokens * top_k, "weights")
+        _fits(weights, torch.float32, tokens * top_k, dev, "weights")
     if experts is None:
         experts = torch.empty((tokens, top_k), device=device, dtype=torch.int32)
     else:
-        _need(experts, torch.int32, tokens * top_k, "experts")
-    _here(dev, mask, weights, experts)
+        _fits(experts, torch.int32, tokens * top_k, dev, "experts")
     stream = _stream_of(dev)
-    made = ref = ws = None
+    made = desc = ws = None
     size = 0
     if plan is not False:
         made, desc, ws, size = _moe_plan(dev, device, tokens, top_k, n_experts, plan)
-        ref = C.byref(desc)
-    router = MoeRouterT(logits.data_ptr(), stride if tokens > 1 else n_experts, _ACT[logits.dtype], tokens, n_experts, top_k,
-                        _ptr(mask), _SCORES[score], 1 if renormalize else 0, scale)
-    check(load().bh_moe_route(stream, C.byref(router), weights.data_ptr(), experts.data_ptr(), ref, _ptr(ws), size))
+    router = _route_pack(logits.data_ptr(), stride if tokens > 1 else n_experts, _ACT[dtype], tokens, n_experts, top_k,
+                         0 if mask is None else mask.data_ptr(), _SCORES[score], 1 if renormalize else 0, scale)
+    check(load().bh_moe_route(stream, router, weights.data_ptr(), experts.data_ptr(), desc, _ptr(ws), size))
     return weights, experts, made
 
 
@@ -644,38 +668,41 @@ def moe_plan(experts, n_experts, first=0, plan=None):
     if experts.dim() != 2:
         raise ValueError(f"experts: shape {tuple(experts.shape)}, expected [tokens, top_k]")
     tokens, top_k = experts.shape
-    _need(experts, torch.int32, 0, "experts")
+    dev = experts.get_device()
     _moe_sizes("moe_plan", tokens, top_k, n_experts)
     if top_k > _MOST or not 0 <= first <= _MOST:
         raise ValueError(f"moe_plan: {top_k} choices, first {first}")
-    dev = experts.get_device()
-    _here(dev, experts)
+    _fits(experts, torch.int32, 0, dev, "experts")
     stream = _stream_of(dev)
     plan, desc, ws, size = _moe_plan(dev, experts.device, tokens, top_k, n_experts, plan)
-    check(load().bh_moe_plan_rows(stream, experts.data_ptr(), tokens, top_k, first, n_experts, C.byref(desc), _ptr(ws), size))
+    check(load().bh_moe_plan_rows(stream, experts.data_ptr(), tokens, top_k, first, n_experts, desc, _ptr(ws), size))
     return plan
 
 
 def _matmul_grouped(call, glu, xq, wq, sx, sw, offsets, rows, bias, out_dtype, out):
-    if xq.dim() != 2 or wq.dim() != 3 or wq.shape[2] != xq.shape[1]:
-        raise ValueError(f"{call}: xq {tuple(xq.shape)} and wq {tuple(wq.shape)}, expected [rows, K/4] and [experts, n, K/4]")
-    x_rows, kg = xq.shape
-    n_experts, n, _ = wq.shape
-    if glu and n % 2:
-        raise ValueError(f"{call}: {n} weight rows of gate and up")
+    x_shape, w_shape = xq.shape, wq.shape
+    if len(x_shape) != 2 or len(w_shape) != 3 or w_shape[2] != x_shape[1]:
+        raise ValueError(f"{call}: xq {tuple(x_shape)} and wq {tuple(w_shape)}, expected [rows, K/4] and [experts, n, K/4]")
+    x_rows, kg = x_shape
+    n_experts, n, _ = w_shape
+    cols = n
+    if glu:
+        if n % 2:
+            raise ValueError(f"{call}: {n} weight rows of gate and up")
+        cols = n // 2
     places = x_rows if rows is None else rows.numel()
-    if max(x_rows, places, n_experts, n, 4 * kg) > _MOST:
+    if x_rows > _MOST or places > _MOST or n_experts > _MOST or n > _MOST or 4 * kg > _MOST:
         raise ValueError(f"{call}: {places} places of {x_rows} rows, {n_experts} experts of {n} rows, K {4 * kg}")
-    cols = n // 2 if glu else n
-    _need(xq, torch.int32, 0, "xq")
-    _need(wq, torch.int32, 0, "wq")
-    _need(sx, torch.float32, x_rows, "sx")
-    _need(sw, torch.float32, n_experts * n, "sw")
-    _need(offsets, torch.int32, n_experts + 1, "offsets")
+    dev = xq.get_device()
+    _fits(xq, torch.int32, 0, dev, "xq")
+    _fits(wq, torch.int32, 0, dev, "wq")
+    _fits(sx, torch.float32, x_rows, dev, "sx")
+    _fits(sw, torch.float32, n_experts * n, dev, "sw")
+    _fits(offsets, torch.int32, n_experts + 1, dev, "offsets")
     if rows is not None:
-        _need(rows, torch.int32, 0, "rows")
+        _fits(rows, torch.int32, 0, dev, "rows")
     if bias is not None:
-        _need(bias, torch.float32, n_experts * n, "bias")
+        _fits(bias, torch.float32, n_experts * n, dev, "bias")
     if out_dtype is None:
         out_dtype = torch.float32 if out is None else out.dtype
     if out_dtype not in (_ACT if glu else _CODES):
@@ -683,14 +710,12 @@ def _matmul_grouped(call, glu, xq, wq, sx, sw, offsets, rows, bias, out_dtype, o
     if out is None:
         out = torch.empty((places, cols), device=xq.device, dtype=out_dtype)
     else:
-        _need(out, out_dtype, places * cols, "out")
-    dev = xq.get_device()
-    _here(dev, xq, wq, sx, sw, offsets, rows, bias, out)
-    g = GroupedI8T(xq.data_ptr(), sx.data_ptr(), x_rows, _ptr(rows), offsets.data_ptr(), places, n_experts, wq.data_ptr(),
-                   sw.data_ptr(), _ptr(bias), kg, n)
+        _fits(out, out_dtype, places * cols, dev, "out")
+    g = _group_pack(xq.data_ptr(), sx.data_ptr(), x_rows, 0 if rows is None else rows.data_ptr(), offsets.data_ptr(), places,
+                    n_experts, wq.data_ptr(), sw.data_ptr(), 0 if bias is None else bias.data_ptr(), kg, n)
     lib = load()
     fn = lib.bh_matmul_i8_grouped_glu if glu else lib.bh_matmul_i8_grouped
-    check(fn(_stream_of(dev), C.byref(g), out.data_ptr(), _CODES[out_dtype]))
+    check(fn(_stream_of(dev), g, out.data_ptr(), _CODES[out_dtype]))
     return out
 
 
@@ -716,27 +741,28 @@ def moe_combine(y, weights, slots, add=None, out_dtype=None, out=None):
     in the order of j, over the experts' rows y [places, n] (f32 or bf16); a
     slot outside y (-1: none) adds nothing. out [tokens, n] of out_dtype (y's
     without one), as add is; out may be add."""
-    if y.dim() != 2 or slots.dim() != 2 or y.dtype not in _ACT:
-        raise ValueError(f"moe_combine: y {y.dtype} {tuple(y.shape)} and slots {tuple(slots.shape)}, expected [places, n] "
+    y_shape, s_shape, y_dtype = y.shape, slots.shape, y.dtype
+    if len(y_shape) != 2 or len(s_shape) != 2 or y_dtype not in _ACT:
+        raise ValueError(f"moe_combine: y {y_dtype} {tuple(y_shape)} and slots {tuple(s_shape)}, expected [places, n] "
                          "float32 or bfloat16 and [tokens, top_k]")
-    places, n = y.shape
-    tokens, top_k = slots.shape
-    if max(places, n, tokens, top_k, tokens * top_k) > _MOST:
+    places, n = y_shape
+    tokens, top_k = s_shape
+    if places > _MOST or n > _MOST or tokens > _MOST or top_k > _MOST or tokens * top_k > _MOST:
         raise ValueError(f"moe_combine: {places} places, {tokens} tokens of {top_k} choices, rows of {n}")
-    _need(slots, torch.int32, 0, "slots")
-    _need(weights, torch.float32, tokens * top_k, "weights")
+    dev = y.get_device()
+    _fits(y, y_dtype, 0, dev, "y")
+    _fits(slots, torch.int32, 0, dev, "slots")
+    _fits(weights, torch.float32, tokens * top_k, dev, "weights")
     if out_dtype is None:
-        out_dtype = y.dtype if out is None else out.dtype
+        out_dtype = y_dtype if out is None else out.dtype
     if out_dtype not in _ACT:
         raise ValueError(f"moe_combine: out_dtype {out_dtype}")
     if out is None:
         out = torch.empty((tokens, n), device=y.device, dtype=out_dtype)
     else:
-        _need(out, out_dtype, tokens * n, "out")
+        _fits(out, out_dtype, tokens * n, dev, "out")
     if add is not None:
-        _need(add, out_dtype, tokens * n, "add")
-    dev = y.get_device()
-    _here(dev, y, weights, slots, add, out)
-    check(load().bh_moe_combine(_stream_of(dev), y.data_ptr(), _ACT[y.dtype], places, weights.data_ptr(), slots.data_ptr(),
+        _fits(add, out_dtype, tokens * n, dev, "add")
+    check(load().bh_moe_combine(_stream_of(dev), y.data_ptr(), _ACT[y_dtype], places, weights.data_ptr(), slots.data_ptr(),
                                 tokens, top_k, n, _ptr(add), out.data_ptr(), _ACT[out_dtype]))
     return out

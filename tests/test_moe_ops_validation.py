@@ -238,3 +238,10 @@ def test_reference_plan():
     assert offsets.tolist() == [0, 2, 2, 4] and rows.tolist() == [0, 1, 0, 2] and slots.tolist() == [[2, 0], [1, -1], [-1, 3]]
     w, e = moeref.route(torch.tensor([[0.0, 3.0, 3.0, float("nan")]]), 2)
     assert e.tolist() == [[1, 2]] and np.allclose(w, 0.5)
+
+
+def test_packed_descriptions():
+    """What brain_amd.ops packs by hand is the C structure."""
+    assert ops._route_pack(1, 2, 3, 4, 5, 6, 7, 8, 9, 1.5) == bytes(MoeRouterT(1, 2, 3, 4, 5, 6, 7, 8, 9, 1.5))
+    assert ops._plan_pack(1, 2, 3) == bytes(MoePlanT(1, 2, 3))
+    assert ops._group_pack(*range(1, 13)) == bytes(GroupedI8T(*range(1, 13)))
