@@ -138,14 +138,16 @@ struct Tiles {
 };
 
 // v / (1 + exp(-v)) to 7 half steps: exp(-v) is 2^p, p = -v log2(e) rounded, by v_exp_f32 (1 ulp), times 1 + what p
-// lost, to first order (2^-23 |p|: below 2^-16); the reciprocal is v_rcp_f32 (1 ulp).
+// lost, to first order (2^-23 |p|: below 2^-16); the reciprocal is v_rcp_f32 (1 ulp). That is for |v| up
+// to 87.3, where the reciprocal leaves the normal numbers; beyond 88 exp is held there (less than v 2^-126 is left of
+// far negative ones).
 // ROUGH, for a result of 8 bits: without that correction (p <= 126 is off by 2^-17 then).
 template <bool ROUGH = false>
 __device__ __forceinline__ float silu(float v) {
     constexpr float L = 1.44269502f, LO = 1.92596299e-8f, LN2 = 0.693147182f;  // log2(e) = L + LO
-    const float p = -v * L;
-    if constexpr (ROUGH) return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(p));
-    const float lost = fmaf(-v, LO, fmaf(-v, L, -p));
+    if constexpr (ROUGH) return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-v * L));
+    const float w = __builtin_amdgcn_fmed3f(v, -88.0f, 88.0f), p = -w * L;
+    const float lost = fmaf(-w, LO, fmaf(-w, L, -p));
     const float x = __builtin_amdgcn_exp2f(p);
     return v * __builtin_amdgcn_rcpf(1.0f + fmaf(x, lost * LN2, x));
 }
@@ -161,90 +163,90 @@ __device__ __forceinline__ v4i load_piece(const uint8_t* row, uint32_t kb, uint3
     return r;
 }
 
-// ---------------------------------------------------------------- the plain kernel
-// A workgroup takes up to 64 rows of an expert and 16 columns (of gate and up both)
-// a wave, straight from memory: v_mfma_i32_16x16x64_i8 with rows of x as its
-// first operand and weight rows as its second. Lane l feeds 16 bytes of row l % 16 at
-// K piece l / 16 and gets column l % 16 of rows 4 (l / 16) .. + 3.
-constexpr uint32_t GS_ROWS = 64;
-template <int OUT, bool GLU, int NF>
-__device__ __forceinline__ void stream_rows(const GroupedArgs& a, const Tile& tile, uint32_t col0) {
-    constexpr int C = GLU ? 2 : 1;
+// ---------------------------------------------------------------- few rows
+// A workgroup takes up to 16 rows of an expert and 16 columns (of gate and up both),
+// straight from memory: v_mfma_i32_16x16x64_i8 with rows of x as its first operand
+// and weight rows as its second. Lane l feeds 16 bytes of row l % 16 at K piece l / 16
+// and gets column l % 16 of rows 4 (l / 16) .. + 3. Its waves share K, 128 bytes (a line
+// of each weight row) at a time in turn, and their sums meet in LDS. What counts is how many bytes are
+// on their way: a wave asks for 256 bytes of every row before it multiplies. WHOLE: K is a multiple of 64.
+constexpr uint32_t GS_ROWS = 16, GS_WAVES = 8;
+template <int OUT, bool GLU, bool WHOLE>
+__global__ __launch_bounds__(GS_WAVES * 64) void grouped_step_kernel(GroupedArgs a, uint32_t tiles_n) {
+    constexpr int C = GLU ? 2 : 1, U = 4;
+    typedef int v4iu __attribute__((ext_vector_type(4), aligned(4)));
+    __shared__ v4i sums[GS_WAVES][C][64];
     const uint32_t lane = threadIdx.x & 63, r16 = lane & 15, piece = lane >> 4;
-    const uint32_t kbytes = a.kg * 4, rows = min(tile.rows, GS_ROWS);
-    const uint8_t *xp[NF], *wp[C];
-#pragma unroll
-    for (int f = 0; f < NF; ++f) {
-        const uint32_t p = tile.first + min(f * 16 + r16, rows - 1);
-        const uint32_t row = min(a.rows ? a.rows[p] : p, a.x_rows - 1);
-        xp[f] = reinterpret_cast<const uint8_t*>(a.xq) + (uint64_t)row * kbytes;
-    }
-    const uint32_t col = min(col0 + r16, a.f - 1);
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), waves = blockDim.x >> 6;
+    const uint32_t kbytes = a.kg * 4, col0 = blockIdx.x % tiles_n * 16;
+    Tile tile;
+    if (!find_tile<GS_ROWS>(a, blockIdx.x / tiles_n, tile)) return;
+    const uint32_t rows = min(tile.rows, GS_ROWS), col = min(col0 + r16, a.f - 1);
+    const uint8_t* wp[C];
 #pragma unroll
     for (int c = 0; c < C; ++c)
         wp[c] = reinterpret_cast<const uint8_t*>(a.wq) + ((uint64_t)tile.e * a.n + (uint64_t)c * a.f + col) * kbytes;
-    v4i acc[NF][C];
+    const uint32_t p = tile.first + min(r16, rows - 1);
+    const uint8_t* xp = reinterpret_cast<const uint8_t*>(a.xq) + (uint64_t)min(a.rows ? a.rows[p] : p, a.x_rows - 1) * kbytes;
+    v4i acc[C];
 #pragma unroll
-    for (int f = 0; f < NF; ++f)
+    for (int c = 0; c < C; ++c) acc[c] = v4i{0, 0, 0, 0};
+    for (uint32_t k0 = wave * 128; k0 < kbytes; k0 += waves * 128 * (U / 2)) {
+        v4i w[U][C], x[U];
 #pragma unroll
-        for (int c = 0; c < C; ++c) acc[f][c] = v4i{0, 0, 0, 0};
-    for (uint32_t k0 = 0; k0 < kbytes; k0 += 64) {
-        const uint32_t kb = k0 + piece * 16;
-        v4i w[C];
+        for (int u = 0; u < U; ++u) {
+            const uint32_t kb = k0 + (u / 2) * waves * 128 + (u % 2) * 64 + piece * 16;
+            if constexpr (WHOLE) {
+                // (Behind the row's end its last piece again, times zeros.)
+                const uint32_t at = min(kb, kbytes - 64 + piece * 16);
 #pragma unroll
-        for (int c = 0; c < C; ++c) w[c] = load_piece(wp[c], kb, kbytes);
-#pragma unroll
-        for (int f = 0; f < NF; ++f) {
-            const v4i x = load_piece(xp[f], kb, kbytes);
-#pragma unroll
-            for (int c = 0; c < C; ++c) acc[f][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x, w[c], acc[f][c], 0, 0, 0);
-        }
-    }
-    if (col0 + r16 >= a.f) return;
-    float sw[C] = {}, bias[C] = {};
-    if constexpr (OUT != OUT_I32) {
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const uint64_t at = (uint64_t)tile.e * a.n + (uint64_t)c * a.f + col;
-            sw[c] = a.sw[at];
-            if (a.bias) bias[c] = a.bias[at];
-        }
-    }
-#pragma unroll
-    for (int f = 0; f < NF; ++f)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t r = f * 16 + piece * 4 + i;
-            if (r >= rows) continue;
-            const uint32_t p = tile.first + r, row = a.rows ? a.rows[p] : p;
-            const bool there = row < a.x_rows;
-            const uint64_t at = (uint64_t)p * a.f + col;
-            if constexpr (OUT == OUT_I32) {
-                reinterpret_cast<int*>(a.out)[at] = there ? acc[f][0][i] : 0;
+                for (int c = 0; c < C; ++c) w[u][c] = *reinterpret_cast<const v4iu*>(wp[c] + at);
+                x[u] = *reinterpret_cast<const v4iu*>(xp + at);
             } else {
-                const float sx = a.sx[there ? row : 0];
-                float v = dequant(acc[f][0][i], sx, sw[0]);
-                if (a.bias) v = v + bias[0];
-                if constexpr (GLU) {
-                    float u = dequant(acc[f][C - 1][i], sx, sw[C - 1]);
-                    if (a.bias) u = u + bias[C - 1];
-                    v = silu(v) * u;
-                }
-                store_out<OUT>(a.out, (int64_t)at, there ? v : 0.0f);
+#pragma unroll
+                for (int c = 0; c < C; ++c) w[u][c] = load_piece(wp[c], kb, kbytes);
+                x[u] = load_piece(xp, kb, kbytes);
             }
         }
-}
-
-template <int OUT, bool GLU>
-__global__ __launch_bounds__(256) void grouped_stream_kernel(GroupedArgs a, uint32_t tiles_n) {
-    const uint32_t wave = threadIdx.x >> 6, tn = blockIdx.x % tiles_n;
-    Tile tile;
-    if (!find_tile<GS_ROWS>(a, blockIdx.x / tiles_n, tile)) return;
-    const uint32_t col0 = (tn * 4 + wave) * 16;
-    if (col0 >= a.f) return;
-    if (tile.rows <= 16) stream_rows<OUT, GLU, 1>(a, tile, col0);
-    else if (tile.rows <= 32) stream_rows<OUT, GLU, 2>(a, tile, col0);
-    else stream_rows<OUT, GLU, 4>(a, tile, col0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t kb = k0 + (u / 2) * waves * 128 + (u % 2) * 64;
+            if (WHOLE && kb >= kbytes) x[u] = v4i{0, 0, 0, 0};
+#pragma unroll
+            for (int c = 0; c < C; ++c) acc[c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[u], w[u][c], acc[c], 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) sums[wave][c][lane] = acc[c];
+    __syncthreads();
+    // Thread t finishes register t / 64 of lane t % 64.
+    for (uint32_t q = threadIdx.x; q < 256; q += blockDim.x) {
+        const uint32_t i = q >> 6, l = q & 63, r = 4 * (l >> 4) + i, c16 = col0 + (l & 15);
+        if (r >= rows || c16 >= a.f) continue;
+        int y[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            y[c] = 0;
+            for (uint32_t w = 0; w < waves; ++w) y[c] += reinterpret_cast<const int*>(&sums[w][c][l])[i];
+        }
+        const uint32_t place = tile.first + r, row = a.rows ? a.rows[place] : place;
+        const bool there = row < a.x_rows;
+        const uint64_t at = (uint64_t)place * a.f + c16;
+        if constexpr (OUT == OUT_I32) {
+            reinterpret_cast<int*>(a.out)[at] = there ? y[0] : 0;
+        } else {
+            const float sx = a.sx[there ? row : 0];
+            float v[C];
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const uint64_t n = (uint64_t)tile.e * a.n + (uint64_t)c * a.f + c16;
+                v[c] = dequant(y[c], sx, a.sw[n]);
+                if (a.bias) v[c] = v[c] + a.bias[n];
+            }
+            if constexpr (GLU) v[0] = silu<OUT == OUT_BF16>(v[0]) * v[C - 1];
+            store_out<OUT>(a.out, (int64_t)at, there ? v[0] : 0.0f);
+        }
+    }
 }
 
 // ---------------------------------------------------------------- tiles through LDS
@@ -737,20 +739,33 @@ static hipError_t launch_grouped(hipStream_t s, const GroupedArgs& a) {
     // Copies to LDS: whole stages, aligned rows, 32-bit offsets.
     const uint64_t row = (uint64_t)a.kg * 4, per = a.places / a.experts;
     const bool copies = row % 128 == 0 && aligned_to(a.xq, 16) && aligned_to(a.wq, 16) &&
-                        std::max(a.x_rows, a.n) * row < (1ull << 32);
-    if (copies && a.f < (1u << 29)) {
-        if (per < 40) return launch_tiles<TileCfg<64, 128, 2, 2, 3, 128, 2, false, true>, OUT, GLU, false>(s, a);
-        if (per < 192) return launch_tiles<TileCfg<128, 128, 2, 2, 4, 64, 2, false, false>, OUT, GLU, false>(s, a);
+                        std::max(a.x_rows, a.n) * row < (1ull << 32) && a.f < (1u << 29);
+    // How many tiles of 64 and of 128 rows there may be, for the compute units.
+    constexpr uint32_t cols = GLU ? 64 : 128;
+    const uint64_t wide = (a.f + cols - 1) / cols;
+    const uint64_t t64 = most_tiles(a.places, a.experts, 64) * wide, t128 = most_tiles(a.places, a.experts, 128) * wide;
+    if (copies && !(per < 8 && t64 <= 128)) {
+        if (per < 40 || t64 <= CUS) {
+            if (t64 <= CUS) return launch_tiles<TileCfg<64, 128, 2, 2, 6, 128, 1, false, true>, OUT, GLU, false>(s, a);
+            return launch_tiles<TileCfg<64, 128, 2, 2, 3, 128, 2, false, true>, OUT, GLU, false>(s, a);
+        }
+        if (per < 192) {
+            if (t128 <= CUS) return launch_tiles<TileCfg<128, 128, 2, 2, 4, 128, 1, false, false>, OUT, GLU, false>(s, a);
+            return launch_tiles<TileCfg<128, 128, 2, 2, 4, 64, 2, false, false>, OUT, GLU, false>(s, a);
+        }
         return launch_tiles<TileCfg<256, 256, 4, 2, 4, 64, 1, true, false>, OUT, GLU, false>(s, a);
     }
-    if (per >= 8 && a.f < (1u << 29)) {
+    if (!copies && per >= 8 && a.f < (1u << 29)) {
         if (per < 128) return launch_tiles<TileCfg<64, 128, 2, 2, 3, 64, 2, false, false>, OUT, GLU, true>(s, a);
         return launch_tiles<TileCfg<128, 128, 2, 2, 3, 64, 2, false, false>, OUT, GLU, true>(s, a);
     }
-    const uint32_t tiles_n = (a.f + 63) / 64;
+    const uint32_t tiles_n = (a.f + 15) / 16;
     const uint64_t wgs = most_tiles(a.places, a.experts, GS_ROWS) * tiles_n;
     if (wgs > 0x7fffffffu) return hipErrorInvalidConfiguration;
-    grouped_stream_kernel<OUT, GLU><<<(unsigned)wgs, 256, 0, s>>>(a, tiles_n);
+    // A wave for each 256 bytes of K, up to 8.
+    const unsigned threads = 64 * (unsigned)std::min<uint64_t>(GS_WAVES, std::max<uint64_t>(1, (row + 255) / 256));
+    if (row && row % 64 == 0) grouped_step_kernel<OUT, GLU, true><<<(unsigned)wgs, threads, 0, s>>>(a, tiles_n);
+    else grouped_step_kernel<OUT, GLU, false><<<(unsigned)wgs, threads, 0, s>>>(a, tiles_n);
     return hipGetLastError();
 }
 

@@ -76,12 +76,19 @@ def product(xq, wq, sx, sw, offsets, rows=None, bias=None):
     return torch.where(there[:, None], v, torch.zeros(())), used
 
 
-def glu(v):
-    """silu(gate) * up in 64 bits of f32 products [places, 2 f], and how far 32 bits may be from it: exp's 2 ulp (4 half steps), the sum, the
-    quotient and the product a half step each; below exp's range (|gate| > 87) less than |gate * up| 2^-126 is left."""
+def glu(v, dtype=torch.float32):
+    """silu(gate) * up in 64 bits of f32 products [places, 2 f], and how far an output of `dtype` may be from it: exp's 2 ulp (4 half steps),
+    the sum, the quotient and the product a half step each; below exp's range (|gate| > 87) less than |gate * up| 2^-126 is left.
+    For bf16, exp(-gate) may be 2^p of a p = -gate log2(e) of 32 bits, log2(e) too: p is then off by a half step for each of the two,
+    |p| 2^-24 (1 + 1 / 4) (log2(e) in 32 bits is off by 1.93e-8, under a quarter of 2^-24 of it), which moves 2^p by ln(2) times as
+    much, relatively: |gate| 2^-24 (5 / 4). And the result is rounded to bf16."""
     gate, up = v.double().split(v.shape[1] // 2, 1)
     h = gate / (1.0 + torch.exp(-gate)) * up
-    return h, 7 * 2.0 ** -24 * h.abs() + (gate * up).abs() * 2.0 ** -126
+    tol = 7 * 2.0 ** -24 * h.abs() + (gate * up).abs() * 2.0 ** -126
+    if dtype == torch.bfloat16:
+        tol = tol + 1.25 * 2.0 ** -24 * gate.abs() * h.abs()
+        tol = tol + HALF[dtype] * (h.abs() + tol)
+    return h, tol
 
 
 def combine(y, weights, slots, add=None):

@@ -212,9 +212,7 @@ def check_products(gpu, xq, wq, sx, sw, bias, offsets, rows, glu_too=True, word=
         if n % 2 or not glu_too:
             continue
         for b, v in ((None, want), (bias, biased)):
-            h, tol = moeref.glu(v)
-            if dtype == BF16:
-                tol = tol + HALF[BF16] * (h.abs() + tol)
+            h, tol = moeref.glu(v, dtype)
             out = ops.matmul_i8_grouped_glu(xq, wq, sx, sw, offsets, rows, bias=b, out=empty(dtype, n // 2))
             assert bool((out[~used] == 99).all())
             off = (out.cpu().double() - h).abs() - tol
@@ -237,11 +235,33 @@ def test_grouped(gpu, counts, k, n):
     check_products(gpu, xq, wq, sx, sw, bias, offsets_of(counts, gpu), rows)
 
 
+@pytest.mark.parametrize("counts,n", [([20] * 40, 1100), ([100, 3, 200] * 4, 1500), ([100] * 28 + [0, 199], 1500), ([300, 0, 500, 1], 700),
+                                      ([1, 0, 2], 400), ([9, 30, 0, 11], 300)])
+@pytest.mark.parametrize("k", [128, 384, 1152, 1156])
+def test_grouped_tiles(gpu, counts, n, k):
+    """Few and many tiles of every height, and K of one stage, of a few and of many, and one that is not whole."""
+    places = sum(counts) + 2
+    xq, wq, sx, sw, bias = operands(90, len(counts), n, k, k + n, gpu)
+    rows = torch.randint(0, 90, (places,), generator=gen(n), dtype=torch.int32).to(gpu)
+    check_products(gpu, xq, wq, sx, sw, bias, offsets_of(counts, gpu), rows)
+
+
 @pytest.mark.parametrize("k,n", [(128, 130), (500, 34), (1024, 256)])
 def test_grouped_without_rows(gpu, k, n):
     counts = [3, 70, 0, 200]
     xq, wq, sx, sw, bias = operands(280, 4, n, k, 3, gpu)
     check_products(gpu, xq, wq, sx, sw, bias, offsets_of(counts, gpu), None)
+
+
+@pytest.mark.parametrize("counts", [[3, 20], [300, 500]])
+@pytest.mark.parametrize("size", [0.1, 10.0, 1e3, 1e8, 1e30])
+def test_glu_far_gates(gpu, counts, size):
+    """Gates far outside exp's range, of both signs: no NaN, nothing where the up product is not."""
+    xq, wq, sx, sw, bias = operands(80, 2, 64, 128, 11, gpu)
+    sx = sx * (size / 0.005 / 0.002 / 5e4)
+    rows = torch.randint(0, 80, (sum(counts),), generator=gen(11), dtype=torch.int32).to(gpu)
+    sw[:, 32:] = 1e-3 / size  # up products of about 1
+    check_products(gpu, xq, wq, sx, sw, bias, offsets_of(counts, gpu), rows)
 
 
 @pytest.mark.parametrize("word", [1, 2, 3])
