@@ -21,17 +21,6 @@ struct GroupedArgs {
     uint32_t n, f;  // weight rows of an expert, columns of an output row (n, or n / 2: GLU)
 };
 
-// Inclusive sum over the lanes of a wave, by DPP row shifts and broadcasts.
-__device__ __forceinline__ uint32_t lane_scan(uint32_t v) {
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);  // row_shr:1
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);  // row_shr:2
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);  // row_shr:4
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);  // row_shr:8
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1, 3
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2, 3
-    return v;
-}
-
 struct Tile {
     uint32_t e, first, rows;  // expert, first place, rows from there to the group's end
 };
@@ -176,6 +165,8 @@ __global__ __launch_bounds__(GS_WAVES * 64) void grouped_step_kernel(GroupedArgs
     constexpr int C = GLU ? 2 : 1, U = 4;
     typedef int v4iu __attribute__((ext_vector_type(4), aligned(4)));
     __shared__ v4i sums[GS_WAVES][C][64];
+    __shared__ uint32_t place_row[16];
+    __shared__ float row_sx[16];
     const uint32_t lane = threadIdx.x & 63, r16 = lane & 15, piece = lane >> 4;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), waves = blockDim.x >> 6;
     const uint32_t kbytes = a.kg * 4, col0 = blockIdx.x % tiles_n * 16;
@@ -186,28 +177,36 @@ __global__ __launch_bounds__(GS_WAVES * 64) void grouped_step_kernel(GroupedArgs
 #pragma unroll
     for (int c = 0; c < C; ++c)
         wp[c] = reinterpret_cast<const uint8_t*>(a.wq) + ((uint64_t)tile.e * a.n + (uint64_t)c * a.f + col) * kbytes;
-    const uint32_t p = tile.first + min(r16, rows - 1);
-    const uint8_t* xp = reinterpret_cast<const uint8_t*>(a.xq) + (uint64_t)min(a.rows ? a.rows[p] : p, a.x_rows - 1) * kbytes;
+    const uint32_t p = tile.first + min(r16, rows - 1), x_row = a.rows ? a.rows[p] : p;
+    const uint8_t* xp = reinterpret_cast<const uint8_t*>(a.xq) + (uint64_t)min(x_row, a.x_rows - 1) * kbytes;
+    // Scales and bias, on their way beside the operands: a thread's results are all of column l % 16.
+    float sx = 0.0f, sw[C], bias[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const uint64_t n = (uint64_t)tile.e * a.n + (uint64_t)c * a.f + col;
+        sw[c] = OUT != OUT_I32 ? a.sw[n] : 0.0f;
+        bias[c] = OUT != OUT_I32 && a.bias ? a.bias[n] : 0.0f;
+    }
     v4i acc[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) acc[c] = v4i{0, 0, 0, 0};
     for (uint32_t k0 = wave * 128; k0 < kbytes; k0 += waves * 128 * (U / 2)) {
         v4i w[U][C], x[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
+        auto load = [&](const uint8_t* row, int u) -> v4i {
             const uint32_t kb = k0 + (u / 2) * waves * 128 + (u % 2) * 64 + piece * 16;
-            if constexpr (WHOLE) {
-                // (Behind the row's end its last piece again, times zeros.)
-                const uint32_t at = min(kb, kbytes - 64 + piece * 16);
+            // (WHOLE: behind the row's end its last piece again, times zeros.)
+            if constexpr (WHOLE) return *reinterpret_cast<const v4iu*>(row + min(kb, kbytes - 64 + piece * 16));
+            else return load_piece(row, kb, kbytes);
+        };
+        // The weights first: where x lies is still being looked up.
 #pragma unroll
-                for (int c = 0; c < C; ++c) w[u][c] = *reinterpret_cast<const v4iu*>(wp[c] + at);
-                x[u] = *reinterpret_cast<const v4iu*>(xp + at);
-            } else {
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int c = 0; c < C; ++c) w[u][c] = load_piece(wp[c], kb, kbytes);
-                x[u] = load_piece(xp, kb, kbytes);
-            }
-        }
+            for (int c = 0; c < C; ++c) w[u][c] = load(wp[c], u);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u] = load(xp, u);
+        if (OUT != OUT_I32 && k0 == 0) sx = a.sx[min(x_row, a.x_rows - 1)];  // (wave 0)
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const uint32_t kb = k0 + (u / 2) * waves * 128 + (u % 2) * 64;
@@ -218,30 +217,30 @@ __global__ __launch_bounds__(GS_WAVES * 64) void grouped_step_kernel(GroupedArgs
     }
 #pragma unroll
     for (int c = 0; c < C; ++c) sums[wave][c][lane] = acc[c];
+    if (OUT != OUT_I32 && kbytes == 0) sx = a.sx[min(x_row, a.x_rows - 1)];
+    if (wave == 0) place_row[r16] = x_row, row_sx[r16] = sx;
     __syncthreads();
     // Thread t finishes register t / 64 of lane t % 64.
     for (uint32_t q = threadIdx.x; q < 256; q += blockDim.x) {
-        const uint32_t i = q >> 6, l = q & 63, r = 4 * (l >> 4) + i, c16 = col0 + (l & 15);
-        if (r >= rows || c16 >= a.f) continue;
+        const uint32_t i = q >> 6, l = q & 63, r = 4 * (l >> 4) + i;
+        if (r >= rows || col0 + r16 >= a.f) continue;
         int y[C];
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             y[c] = 0;
             for (uint32_t w = 0; w < waves; ++w) y[c] += reinterpret_cast<const int*>(&sums[w][c][l])[i];
         }
-        const uint32_t place = tile.first + r, row = a.rows ? a.rows[place] : place;
-        const bool there = row < a.x_rows;
-        const uint64_t at = (uint64_t)place * a.f + c16;
+        const bool there = place_row[r] < a.x_rows;
+        const uint64_t at = (uint64_t)(tile.first + r) * a.f + col;
         if constexpr (OUT == OUT_I32) {
             reinterpret_cast<int*>(a.out)[at] = there ? y[0] : 0;
         } else {
-            const float sx = a.sx[there ? row : 0];
+            const float sx = row_sx[r];
             float v[C];
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                const uint64_t n = (uint64_t)tile.e * a.n + (uint64_t)c * a.f + c16;
-                v[c] = dequant(y[c], sx, a.sw[n]);
-                if (a.bias) v[c] = v[c] + a.bias[n];
+                v[c] = dequant(y[c], sx, sw[c]);
+                if (a.bias) v[c] = v[c] + bias[c];
             }
             if constexpr (GLU) v[0] = silu<OUT == OUT_BF16>(v[0]) * v[C - 1];
             store_out<OUT>(a.out, (int64_t)at, there ? v[0] : 0.0f);

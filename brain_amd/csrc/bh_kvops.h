@@ -85,6 +85,17 @@ __device__ __forceinline__ uint32_t wave_last(uint32_t n, uint32_t lane, F below
     return NO_SLOT;
 }
 
+// Inclusive sum over the lanes of a wave, by DPP row shifts and broadcasts.
+__device__ __forceinline__ uint32_t lane_scan(uint32_t v) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);  // row_shr:1
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);  // row_shr:2
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);  // row_shr:4
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);  // row_shr:8
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1, 3
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2, 3
+    return v;
+}
+
 // Host checks: BH_OK, or the error of `who`.
 int check_kv8(const char* who, const bh_kv8* kv, Kv8* out);
 int check_kv8_batch(const char* who, const bh_kv8_batch* bt, Kv8Rows* out);

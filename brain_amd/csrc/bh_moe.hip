@@ -133,16 +133,6 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, uint32_t t, uint
     }
 }
 
-// Inclusive sum over the lanes of a wave.
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v, uint32_t lane) {
-#pragma unroll
-    for (int off = 1; off < 64; off *= 2) {
-        const uint32_t o = __shfl_up(v, off, 64);
-        if ((int)lane >= off) v += o;
-    }
-    return v;
-}
-
 // The lanes whose `key` is this lane's.
 __device__ __forceinline__ unsigned long long same_key(uint32_t key, uint32_t bits) {
     unsigned long long same = ~0ull;
@@ -163,12 +153,12 @@ __device__ __forceinline__ void wave_order() {
 __device__ __forceinline__ void place_experts(const uint32_t* from, uint32_t n, uint32_t lane, uint32_t* to, uint32_t* out) {
     uint32_t base = 0;
     for (uint32_t e0 = 0; e0 < n; e0 += 64) {
-        const uint32_t e = e0 + lane, c = e < n ? from[e] : 0, upto = wave_scan(c, lane);
+        const uint32_t e = e0 + lane, c = e < n ? from[e] : 0, upto = lane_scan(c);
         if (e < n) {
             to[e] = base + upto - c;
             if (out) out[e] = base + upto - c;
         }
-        base += (uint32_t)__shfl((int)upto, 63, 64);
+        base += (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
     }
     if (out && lane == 0) out[n] = base;
 }
@@ -269,7 +259,7 @@ __global__ __launch_bounds__(256) void moe_scan_kernel(RouteArgs a, uint32_t wgs
     uint32_t base = 0;
     for (uint32_t b0 = 0; b0 < wgs; b0 += 256) {
         const uint32_t b = b0 + tid, c = b < wgs ? a.counts[(uint64_t)b * a.e + e] : 0;
-        const uint32_t upto = wave_scan(c, lane);
+        const uint32_t upto = lane_scan(c);
         __syncthreads();
         if (lane == 63) part[wave] = upto;
         __syncthreads();
@@ -288,6 +278,13 @@ __global__ __launch_bounds__(RT) void moe_place_kernel(RouteArgs a) {
     extern __shared__ uint32_t lds[];  // [e] all, [e] before
     uint32_t *all = lds, *before = lds + a.e;
     const uint32_t tid = threadIdx.x, wgs = gridDim.x;
+    // The thread's first entry is on its way beside the counts.
+    const uint32_t t0 = min(blockIdx.x * a.per, a.items), t1 = min(t0 + a.per, a.items), end = t1 * a.k;
+    uint32_t i = t0 * a.k + tid, e0 = ~0u, rank = 0;
+    if (i < end) {
+        e0 = (uint32_t)a.experts[i] - a.first;
+        rank = (uint32_t)a.slots[i];
+    }
     if constexpr (SUMMED) {
         for (uint32_t e = tid; e < a.e; e += RT) {
             all[e] = a.counts[(uint64_t)wgs * a.e + e];
@@ -300,7 +297,7 @@ __global__ __launch_bounds__(RT) void moe_place_kernel(RouteArgs a) {
         const uint32_t parts = a.e < RT ? RT / a.e : 1, part = tid / a.e, e = tid - part * a.e;
         if (part < parts) {
             uint32_t sum = 0, mine = 0;
-#pragma unroll 8
+#pragma unroll 16
             for (uint32_t b = part; b < wgs; b += parts) {
                 const uint32_t c = a.counts[(uint64_t)b * a.e + e];
                 sum += c;
@@ -313,13 +310,17 @@ __global__ __launch_bounds__(RT) void moe_place_kernel(RouteArgs a) {
     __syncthreads();
     if (tid < 64) place_experts(all, a.e, tid, all, blockIdx.x == 0 ? a.offsets : nullptr);
     __syncthreads();
-    const uint32_t t0 = min(blockIdx.x * a.per, a.items), t1 = min(t0 + a.per, a.items);
-    for (uint32_t i = t0 * a.k + tid; i < t1 * a.k; i += RT) {
-        const uint32_t e = (uint32_t)a.experts[i] - a.first;
-        if (e >= a.e) continue;
-        const uint32_t at = (uint32_t)a.slots[i] + before[e] + all[e];
-        a.slots[i] = (int32_t)at;
-        a.rows[at] = i / a.div;
+    while (i < end) {
+        if (e0 < a.e) {
+            const uint32_t at = rank + before[e0] + all[e0];
+            a.slots[i] = (int32_t)at;
+            a.rows[at] = i / a.div;
+        }
+        i += RT;
+        if (i < end) {
+            e0 = (uint32_t)a.experts[i] - a.first;
+            rank = (uint32_t)a.slots[i];
+        }
     }
 }
 
@@ -333,8 +334,9 @@ static uint32_t share_of(uint32_t items, uint32_t k, uint32_t one) {
 static uint32_t route_share(uint32_t tokens, uint32_t k) { return share_of(tokens, k, 128); }
 static uint32_t plan_share(uint32_t entries) { return share_of(entries, 1, 4096); }
 static uint32_t groups_of(uint32_t items, uint32_t per) { return std::max((items + per - 1) / per, 1u); }
-// From this many workgroups on their counts are summed in a launch of its own.
-constexpr uint32_t SCAN_GROUPS = 512;
+// From this many workgroups on their counts are summed in a launch of its own (256 of them, 128 experts: 11.8 us
+// of every workgroup adding up all, 3.8 + 3.5 us apart; 25 of them, 60 experts: 3.3 us in one).
+constexpr uint32_t SCAN_GROUPS = 64;
 
 template <class T, int G, int NV, int NK>
 static hipError_t launch_route_as(hipStream_t s, const RouteArgs& a, bool plan) {
