@@ -5,6 +5,7 @@
 // How many rows an expert has is known on the device only, so a launch has as many
 // workgroups as any offsets could need and each finds its rows itself (find_tile); the
 // ones too many end at once.
+#include <cmath>
 #include <type_traits>
 
 #include "bh_kvops.h"
@@ -746,6 +747,11 @@ static hipError_t launch_grouped(hipStream_t s, const GroupedArgs& a) {
     if (copies && !(per < 8 && t64 <= 128)) {
         if (per < 40 || t64 <= CUS) {
             if (t64 <= CUS) return launch_tiles<TileCfg<64, 128, 2, 2, 6, 128, 1, false, true>, OUT, GLU, false>(s, a);
+            // Two workgroups of a unit with tiles of 128 columns, or three of one wave each with half of them: what
+            // leaves less idle in the last round, where as many experts have rows as even chances give.
+            const double e = a.experts, busy = e * (1.0 - std::pow(1.0 - 1.0 / e, (double)a.places));
+            const double w2 = 2 * CUS * std::ceil(busy * wide / (2 * CUS)), w3 = 1.5 * CUS * std::ceil(2 * busy * wide / (3 * CUS));
+            if (per < 12 && row >= 1024 && w3 <= w2) return launch_tiles<TileCfg<32, 64, 1, 1, 4, 128, 3, false, true>, OUT, GLU, false>(s, a);
             return launch_tiles<TileCfg<64, 128, 2, 2, 3, 128, 2, false, true>, OUT, GLU, false>(s, a);
         }
         if (per < 192) {

@@ -236,7 +236,7 @@ def test_grouped(gpu, counts, k, n):
 
 
 @pytest.mark.parametrize("counts,n", [([20] * 40, 1100), ([100, 3, 200] * 4, 1500), ([100] * 28 + [0, 199], 1500), ([300, 0, 500, 1], 700),
-                                      ([1, 0, 2], 400), ([9, 30, 0, 11], 300)])
+                                      ([1, 0, 2], 400), ([9, 30, 0, 11], 300), ([3, 5, 0, 40, 1, 2] * 10, 800), ([1, 0, 33, 2] * 8, 1700)])
 @pytest.mark.parametrize("k", [128, 384, 1152, 1156])
 def test_grouped_tiles(gpu, counts, n, k):
     """Few and many tiles of every height, and K of one stage, of a few and of many, and one that is not whole."""
@@ -278,6 +278,44 @@ def test_grouped_without_depth(gpu):
     xq, wq, sx, sw, bias = operands(5, 2, 6, 0, 5, gpu)
     rows = torch.tensor([0, 1, 2, 3, 4, 0], dtype=torch.int32, device=gpu)
     check_products(gpu, xq, wq, sx, sw, bias, offsets_of([2, 3], gpu), rows)
+
+
+@pytest.mark.parametrize("counts", [[20, 0, 30], [100, 150, 90], [300, 500]])
+def test_grouped_without_depth_many_rows(gpu, counts):
+    xq, wq, sx, sw, bias = operands(7, len(counts), 900, 0, 5, gpu)
+    rows = torch.randint(0, 7, (sum(counts) + 1,), generator=gen(5), dtype=torch.int32).to(gpu)
+    check_products(gpu, xq, wq, sx, sw, bias, offsets_of(counts, gpu), rows)
+
+
+@pytest.mark.parametrize("counts", [[3, 2], [90, 30], [400, 300]])
+def test_grouped_far_rows_of_x(gpu, counts):
+    """Rows whose bytes pass 32 bits: 4.3 GB of activations, the first and the last ones read."""
+    k, x_rows, n = 1024, (1 << 22) + 37, 300
+    xq = torch.zeros(x_rows, k // 4, dtype=torch.int32, device=gpu)
+    near, far = torch.arange(40), torch.arange(x_rows - 40, x_rows)
+    pick = torch.cat([near, far])
+    small, wq, _, sw, _ = operands(80, 2, n, k, 12, gpu)
+    xq[pick.to(gpu)] = small
+    sx = torch.rand(x_rows, device=gpu)
+    at = torch.randint(0, 80, (sum(counts),), generator=gen(12))
+    out = ops.matmul_i8_grouped(xq, wq, sx, sw, offsets_of(counts, gpu), pick[at].int().to(gpu))
+    want, _ = moeref.product(small, wq, sx[pick.to(gpu)], sw, [0, counts[0], sum(counts)], at.int())
+    same_bits(out, want)
+
+
+@pytest.mark.parametrize("experts", [1, 1000])
+def test_grouped_far_outputs(gpu, experts):
+    """More than 2^31 results: the rows at both ends and around every 2^30th of them."""
+    places, n, k = 140000, 16384, 128
+    g = gen(13)
+    wq = torch.randint(-128, 128, (experts, n, k), device=gpu, dtype=torch.int8).view(torch.int32)
+    xq = torch.randint(-128, 128, (places, k), generator=g, dtype=torch.int8).view(torch.int32).to(gpu)
+    sx, sw = torch.rand(places, device=gpu), torch.rand(experts, n, device=gpu)
+    out = ops.matmul_i8_grouped(xq, wq, sx, sw, offsets_of([places // experts] * experts, gpu), out_dtype=BF16)
+    for r in sorted({r for c in (0, 65535, 131071, places - 1) for r in range(max(0, c - 2), min(places, c + 3))}):
+        e = r // (places // experts)
+        want, _ = moeref.product(xq[r:r + 1], wq[e:e + 1], sx[r:r + 1], sw[e:e + 1], [0, 1])
+        same_bits(out[r:r + 1], want)
 
 
 @pytest.mark.parametrize("k,n", [(64, 32), (256, 256)])
