@@ -3,8 +3,12 @@
 // for the places p of expert e, and silu(gate) * up of two such products.
 //
 // How many rows an expert has is known on the device only, so a launch has as many
-// workgroups as any offsets could need and each finds its rows itself (find_tile); the
-// ones too many end at once.
+// workgroups as any offsets could need, or as the chip holds, and each finds its rows itself
+// (find_tile, Tiles); the ones too many end at once.
+//
+// Few rows are bound by the weights' way from memory, which every kernel here asks for once: 48 tokens
+// through 126 of 128 experts (355 MB) 55 us, 6.5 TB/s, where a plain read of 1 GiB reaches 6.8. Many
+// rows are bound by LDS and the matrix cores (1.9 POPS).
 #include <cmath>
 #include <type_traits>
 
@@ -256,10 +260,13 @@ __global__ __launch_bounds__(GS_WAVES * 64) void grouped_step_kernel(GroupedArgs
 // word-aligned into registers and stored, zeros behind K. 16-byte piece c of row r lies at place
 // c ^ swizzle(r) of the row, so that the 16 lanes that LDS serves at a time, 16
 // rows of one piece, find 16 different places of its 256-byte lines.
-//   v_mfma_i32_32x32x32_i8 takes weight rows as its first operand: lane l gets row
-// l % 32 of x and columns 8 (v / 4) + 4 (l / 32) + v % 4 in register v. With GLU every other
-// 32 weight rows of the tile are the up projection's, so a wave's fragments 2 j and 2 j + 1
-// are the gate and the up products of the same 32 columns.
+//   v_mfma_i32_32x32x32_i8 takes rows of x as its first operand: lane l gets column l % 32 and rows 8 (v / 4)
+// + 4 (l / 32) + v % 4 in register v. Which weight row a column stands for is chosen so (`weight_row`) that a lane
+// has the gate and the up product of the same column, and, with enough fragments, of two neighbouring
+// columns: results leave as whole lines straight from the registers (through LDS, turned around, that
+// took 65 us of 8192 tokens' 319, this way 27 of 292).
+//   A workgroup stays for the next tile: its rows are looked up beside the products, and its first stages are
+// copied while the results of the tile before leave (4096 tokens, 128 experts: 187 us a workgroup a tile, 174 so).
 //   The group's last tile has fewer than BM rows: waves leave out the 32-row
 // fragments that hold none.
 template <int BM_, int BN_, int WM_, int WN_, int STAGES_, int DK_, int WGS_, bool PP_, bool ONCE_>
@@ -744,26 +751,44 @@ static hipError_t launch_grouped(hipStream_t s, const GroupedArgs& a) {
     constexpr uint32_t cols = GLU ? 64 : 128;
     const uint64_t wide = (a.f + cols - 1) / cols;
     const uint64_t t64 = most_tiles(a.places, a.experts, 64) * wide, t128 = most_tiles(a.places, a.experts, 128) * wide;
+    // Which kernel, by the rows an expert has on average and by how many tiles there are. Both sides of each line in
+    // us, weights from memory (several sets in turn), bf16 out; "128 experts": 8 of 128 a token, gate and up 2048 x
+    // (2 x 768), down 768 x 2048; "8 experts": 2 of 8, 2048 x (2 x 4096), 4096 x 2048; "64 experts": 6 of 64,
+    // 2048 x (2 x 1408), 1408 x 2048.
     if (copies && !(per < 8 && t64 <= 128)) {
-        if (per < 40 || t64 <= CUS) {
+        if (per < 56 || t64 <= CUS) {
+            // 64 rows, weights once and around the caches (per 48, 64 experts: 79.5 and 43.7, of 128 rows 87.2 and 53.9;
+            // per 64, 128 experts: 104.7 and 60.2, 100.7 and 59.3). 128-byte stages, whole lines, so that the hint helps: 128 tokens,
+            // 128 experts, 62 with it and 72 without; with 64-byte stages, which fetch a line twice, 91 and 76.
+            // A tile a unit: six stages deep instead of two workgroups of three (64 tokens, 8 experts, down: 19.0 and 29.7).
             if (t64 <= CUS) return launch_tiles<TileCfg<64, 128, 2, 2, 6, 128, 1, false, true>, OUT, GLU, false>(s, a);
             // Two workgroups of a unit with tiles of 128 columns, or three of one wave each with half of them: what
-            // leaves less idle in the last round, where as many experts have rows as even chances give.
+            // leaves less idle in the last round, where as many experts have rows as even chances give (8 tokens, 128
+            // experts: 36.0 and 28.4; 16 tokens, 8 experts: 24.5 and 27.6). Short K has too little for so small a tile (256 experts of 512
+            // x 1024, 48 tokens: 21.6 and 24.1).
             const double e = a.experts, busy = e * (1.0 - std::pow(1.0 - 1.0 / e, (double)a.places));
             const double w2 = 2 * CUS * std::ceil(busy * wide / (2 * CUS)), w3 = 1.5 * CUS * std::ceil(2 * busy * wide / (3 * CUS));
             if (per < 12 && row >= 1024 && w3 <= w2) return launch_tiles<TileCfg<32, 64, 1, 1, 4, 128, 3, false, true>, OUT, GLU, false>(s, a);
             return launch_tiles<TileCfg<64, 128, 2, 2, 3, 128, 2, false, true>, OUT, GLU, false>(s, a);
         }
         if (per < 192) {
+            // 512 tokens, 8 experts, down: 27.0 four wide stages deep, 33.1 two workgroups of four narrow ones.
             if (t128 <= CUS) return launch_tiles<TileCfg<128, 128, 2, 2, 4, 128, 1, false, false>, OUT, GLU, false>(s, a);
             return launch_tiles<TileCfg<128, 128, 2, 2, 4, 64, 2, false, false>, OUT, GLU, false>(s, a);
         }
+        // Per 128, 128 experts: 122 with 128 rows, 126 with 256; per 256: 182 and 155. 8192 tokens, 8 experts: 291 (1.9
+        // POPS; a dense product of that size, bh_matmul_i8_dyn, takes 342), 254 without the results' way out, 183 the copies alone,
+        // 205 the products alone: LDS carries 128 KB for the 1024 cycles of a stage's products.
         return launch_tiles<TileCfg<256, 256, 4, 2, 4, 64, 1, true, false>, OUT, GLU, false>(s, a);
     }
+    // Other operands through registers (8 experts of 2044 x (2 x 4092), per 16: 41.0 and the step kernel 51.1; per 4: 38.8
+    // and 38.1; per 64 and 256: 70.1 and 156.8 with 64 rows, 49.3 and 116.0 with 128; 7 of 500 x 332, per 292: 7.8 and 8.2).
     if (!copies && per >= 8 && a.f < (1u << 29)) {
-        if (per < 128) return launch_tiles<TileCfg<64, 128, 2, 2, 3, 64, 2, false, false>, OUT, GLU, true>(s, a);
+        if (per < 48 || t64 <= CUS) return launch_tiles<TileCfg<64, 128, 2, 2, 3, 64, 2, false, false>, OUT, GLU, true>(s, a);
         return launch_tiles<TileCfg<128, 128, 2, 2, 3, 64, 2, false, false>, OUT, GLU, true>(s, a);
     }
+    // Few tiles of few rows: one token, 128 experts 8.8 (deep tiles of 64 rows 10.6), down 6.9 (7.3); one token of 8 experts, down
+    // 6.8 (14.8); 16 tokens 18.7 (18.0).
     const uint32_t tiles_n = (a.f + 15) / 16;
     const uint64_t wgs = most_tiles(a.places, a.experts, GS_ROWS) * tiles_n;
     if (wgs > 0x7fffffffu) return hipErrorInvalidConfiguration;
