@@ -378,10 +378,10 @@ int bh_moe_plan_rows(void* stream, const int32_t* experts, uint32_t tokens, uint
                      uint32_t n_experts, const bh_moe_plan* plan, void* ws, uint64_t ws_bytes);
 
 /* A product grouped by expert. Place p in [offsets[e], offsets[e + 1]) multiplies
- * row rows[p] of x (NULL: row p) with the weights of expert e. Offsets count as at most
- * `places`, a group that ends before it begins is empty, and output rows of
- * no group are left as they are; a place whose row is outside x gets zeros (raw
- * sums of 0 with BH_OUT_I32). */
+ * row rows[p] of x (NULL: row p) with the weights of expert e. Offsets ascend; they count as at
+ * most `places`, a group that ends before it begins is empty, a place of several groups holds the
+ * result of any of them, and output rows of no group are left as they are. A place whose row is
+ * outside x gets zeros (raw sums of 0 with BH_OUT_I32, which needs no sx, sw and bias). */
 typedef struct {
     const uint32_t* xq; /* [x_rows][kg] int8 codes, 4 per word */
     const float* sx;    /* [x_rows] */
@@ -405,7 +405,8 @@ int bh_matmul_i8_grouped_glu(void* stream, const bh_grouped_i8* g, void* out, in
 
 /* out [tokens][n] = sum over j of weights[t][j] * y[slots[t][j]] (+ add[t]) in f32, in
  * the order of j; a slot outside [0, places) adds nothing. y [places][n] of dtype y_dtype,
- * out and add [tokens][n] of out_dtype, each BH_OUT_F32 or BH_OUT_BF16. out may be add. */
+ * out and add [tokens][n] of out_dtype, each BH_OUT_F32 or BH_OUT_BF16. out may be add, and
+ * overlaps nothing else. */
 int bh_moe_combine(void* stream, const void* y, int y_dtype, uint32_t places, const float* weights, const int32_t* slots,
                    uint32_t tokens, uint32_t top_k, uint32_t n, const void* add, void* out, int out_dtype);
 

@@ -163,3 +163,11 @@ def test_runs_repeat(gpu):
     for _ in range(5):
         assert torch.equal(layer(x, logits).view(torch.int16), first.view(torch.int16))
         assert all(torch.equal(a, b) for a, b in zip(ops.moe_route(logits, 4)[2], plan))
+
+
+def test_layer_without_tokens(gpu):
+    layer = make(gpu, 4, 64, 32, 2)
+    assert layer(torch.empty(0, 64, device=gpu), torch.empty(0, 4, device=gpu)).shape == (0, 64)
+    x, logits = inputs(gpu, layer, 9, F32, 1)
+    none = layer(x, logits, mask=torch.zeros(9, dtype=torch.bool, device=gpu), add=x)
+    assert torch.equal(none, x)

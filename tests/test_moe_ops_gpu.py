@@ -400,3 +400,87 @@ def test_combine_skips_what_is_not_there(gpu):
     assert bool((out[0] == 3).all()) and bool((out[1] == 0).all())
     out = ops.moe_combine(y[:0], w, slots)
     assert bool((out == 0).all())
+
+
+def test_combine_far_rows(gpu):
+    """Rows whose bytes pass 32 bits: 4.3 GB of bf16, the first and the last."""
+    places, n = (1 << 20) + 5, 2056
+    y = torch.zeros(places, n, dtype=BF16, device=gpu)
+    pick = torch.tensor([0, 1, places - 2, places - 1])
+    y[pick.to(gpu)] = torch.randn(4, n, generator=gen(20)).to(BF16).to(gpu)
+    slots = torch.tensor([[places - 1, 0], [1, places - 2], [places, places - 1]], dtype=torch.int32)
+    w = torch.rand(3, 2, generator=gen(21))
+    small = torch.tensor([[3, 0], [1, 2], [4, 3]], dtype=torch.int32)
+    want, size = moeref.combine(y[pick.to(gpu)], w, small)
+    out = ops.moe_combine(y, w.to(gpu), slots.to(gpu), out_dtype=F32)
+    assert bool(((out.cpu().double() - want).abs() <= 4 * HALF[F32] * size).all())
+
+
+def test_route_far_rows(gpu):
+    """Rows of logits 2^31 elements apart."""
+    base = torch.empty(2 * 2 ** 31 + 64, dtype=BF16, device=gpu)
+    x = base.as_strided((3, 60), (2 ** 31, 1))
+    logits = logits_of(3, 60, BF16, 22)
+    x.copy_(logits)
+    want, experts = moeref.route(logits, 5)
+    w, e, plan = ops.moe_route(x, 5)
+    same_ints(e, experts)
+    check_weights(w, want, 5)
+    check_plan(plan, experts, 60)
+
+
+def test_grouped_sums_need_no_scales(gpu):
+    """The C entry's raw sums, without scales."""
+    import ctypes as C
+
+    from brain_amd import _lib
+
+    for counts in ([2, 3], [90, 200]):
+        xq, wq, sx, sw, _ = operands(50, 2, 130, 128, 23, gpu)
+        rows = torch.randint(0, 50, (sum(counts),), generator=gen(23), dtype=torch.int32).to(gpu)
+        offsets = offsets_of(counts, gpu)
+        out = torch.zeros(sum(counts), 130, dtype=torch.int32, device=gpu)
+        g = _lib.GroupedI8T(xq.data_ptr(), None, 50, rows.data_ptr(), offsets.data_ptr(), sum(counts), 2, wq.data_ptr(), None, None, 32, 130)
+        _lib.check(_lib.load().bh_matmul_i8_grouped(torch.cuda.current_stream().cuda_stream, C.byref(g), out.data_ptr(), _lib.BH_OUT_I32))
+        acc = moeref.sums(xq, wq, offsets.tolist(), rows, sum(counts))[0]
+        assert torch.equal(out.cpu().double(), acc)
+
+
+@pytest.mark.parametrize("tokens", [3, 3000])
+def test_route_on_two_streams(gpu, tokens):
+    """Calls at once, each with its own buffers: the bits of the calls one after another."""
+    data = [logits_of(tokens, 128, F32, s).to(gpu) for s in range(4)]
+    want = [ops.moe_route(x, 8) for x in data]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in data]
+    for _ in range(5):
+        got = []
+        for s, x in zip(streams, data):
+            with torch.cuda.stream(s):
+                got.append(ops.moe_route(x, 8))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and all(torch.equal(p, q) for p, q in zip(a[2], b[2]))
+
+
+def test_route_many_tokens_in_a_graph(gpu):
+    """Many tokens (three launches and a workspace), captured; replays on other logits equal eager calls."""
+    tokens, n, top_k = 9000, 64, 4
+    x = logits_of(tokens, n, F32, 30).to(gpu)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.moe_route(x, top_k)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        w, e, plan = ops.moe_route(x, top_k)
+    for rep in range(4):
+        x.copy_(logits_of(tokens, n, F32, 31 + rep))
+        want = ops.moe_route(x, top_k)
+        for t in (w, e, *plan):
+            t.fill_(-7)
+        torch.randn(1000, device=gpu).sum()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(w, want[0]) and torch.equal(e, want[1]) and all(torch.equal(p, q) for p, q in zip(plan, want[2]))
