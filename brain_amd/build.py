@@ -30,7 +30,7 @@ FLAGS = [
 
 # Sources whose code decides the GEMV/tile crossover: the tune store keys its
 # tables by a fingerprint of these and of FLAGS (bh_tune_save / bh_tune_load).
-FP_SOURCES = ["bh_gemv.hip", "bh_gemm.hip", "bh_common.h"]
+FP_SOURCES = ["bh_gemv.hip", "bh_gemm.hip", "bh_common.h", "bh_pingpong.h"]
 
 
 def kernel_fingerprint():

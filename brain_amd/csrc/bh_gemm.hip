@@ -29,6 +29,7 @@
 #include <type_traits>
 
 #include "bh_common.h"
+#include "bh_pingpong.h"
 #include "bh_ws.h"
 
 namespace bh {
@@ -579,66 +580,43 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_i8_dma_kernel(GemmArgs a) {
     };
 
     if constexpr (PP) {
-        // Ping-pong: the 8 waves form two groups of 4 (one wave of each per
-        // SIMD) that run one phase apart, so on every SIMD one wave multiplies
-        // while the other reads LDS and issues DMA. Each stage takes two
-        // phases per wave, L (wait for the stage, read all its fragments into
-        // registers, issue the DMA of stage +3 into the buffer the stage
-        // before freed) and C (the stage's MFMAs), each closed by a
-        // workgroup barrier. Group 1 starts one barrier late and group 0 ends
-        // one barrier later, so both pass the same number of barriers.
-        //   Stage s is needed by group 0 at its L(s): its own DMA waits there;
-        // group 1 waits for its share of stage s during L(s-1), which ends
-        // before group 0's L(s); for stage 0 every wave waits before a common
-        // first barrier.
-        //   The DMA of L(s) overwrites stage s-1's buffer: group 0 read it in
-        // L(s-1), two phases earlier, group 1 in the phase just before.
+        // The 8 waves in two groups of 4 that run one phase apart, in the order
+        // of ping_pong: on every SIMD one wave multiplies while the other reads
+        // LDS and issues DMA.
         static_assert(WM * WN == 8 && STAGES == 4, "ping-pong: 8 waves, 4 stages");
         // Wave-uniform in a scalar register, so the group branches are real
         // branches: a barrier under an exec mask would still execute.
         const int grp = __builtin_amdgcn_readfirstlane(wave) >> 2;
         v4i pa[C::KSTEPS][C::FM], pb[C::KSTEPS][C::FN];
         FragB praw[C::KSTEPS][C::FN];
-        // Stage 0 complete (every wave's share) before group 0's first L.
-        if (nk > 0) wait_ahead<C::LOADS, STAGES - 2>(min(nk - 1, STAGES - 2));
-        __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
-        if (grp == 1) {
-            __builtin_amdgcn_s_barrier();
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        for (int it = 0; it < nk; ++it) {
-            if (grp == 0) wait_ahead<C::LOADS, STAGES - 2>(min(nk - 1 - it, STAGES - 2));
-            else wait_ahead<C::LOADS, STAGES - 3>(min(nk - 2 - it, STAGES - 3));
-            const uint8_t* A = lds + (it % STAGES) * C::STAGE;
+        ping_pong<STAGES>(
+            grp, nk, [&](auto most, int ahead) { wait_ahead<C::LOADS, decltype(most)::value>(ahead); },
+            [&]() {
+                __builtin_amdgcn_sched_barrier(0);
+                __builtin_amdgcn_s_barrier();
+                __builtin_amdgcn_sched_barrier(0);
+            },
+            [&](int it) {
+                const uint8_t* A = lds + (it % STAGES) * C::STAGE;
 #pragma unroll
-            for (int ks = 0; ks < C::KSTEPS; ++ks) read_frags(A, ks, pa[ks], praw[ks]);
-            if (it + STAGES - 1 < nk) issue(kt0 + it + STAGES - 1, (it + STAGES - 1) % STAGES);
-            __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the fragments are in registers
+                for (int ks = 0; ks < C::KSTEPS; ++ks) read_frags(A, ks, pa[ks], praw[ks]);
+                if (it + STAGES - 1 < nk) issue(kt0 + it + STAGES - 1, (it + STAGES - 1) % STAGES);
+                __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the fragments are in registers
 #pragma unroll
-            for (int ks = 0; ks < C::KSTEPS; ++ks)
+                for (int ks = 0; ks < C::KSTEPS; ++ks)
 #pragma unroll
-                for (int j = 0; j < C::FN; ++j) pb[ks][j] = whole(praw[ks][j]);
-            __builtin_amdgcn_sched_barrier(0);
-            __builtin_amdgcn_s_barrier();
-            __builtin_amdgcn_sched_barrier(0);
+                    for (int j = 0; j < C::FN; ++j) pb[ks][j] = whole(praw[ks][j]);
+            },
+            [&]() {
 #pragma unroll
-            for (int ks = 0; ks < C::KSTEPS; ++ks)
+                for (int ks = 0; ks < C::KSTEPS; ++ks)
 #pragma unroll
-                for (int i = 0; i < C::FM; ++i)
+                    for (int i = 0; i < C::FM; ++i)
 #pragma unroll
-                    for (int j = 0; j < C::FN; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(pb[ks][j], pa[ks][i], acc[i][j], 0, 0, 0);
-            __builtin_amdgcn_sched_barrier(0);
-            __builtin_amdgcn_s_barrier();
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        if (grp == 0) {
-            __builtin_amdgcn_sched_barrier(0);
-            __builtin_amdgcn_s_barrier();
-            __builtin_amdgcn_sched_barrier(0);
-        }
+                        for (int j = 0; j < C::FN; ++j)
+                            acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(pb[ks][j], pa[ks][i], acc[i][j], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            });
     } else {
     v4i fa[2][C::FM];
     FragB fb[2][C::FN];

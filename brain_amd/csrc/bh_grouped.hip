@@ -13,6 +13,7 @@
 #include <type_traits>
 
 #include "bh_kvops.h"
+#include "bh_pingpong.h"
 
 namespace bh {
 
@@ -477,34 +478,25 @@ __global__ __launch_bounds__(C::NT, C::WGS * C::NT / 256 > 1 ? C::WGS * C::NT / 
                 __syncthreads();
             }
         } else if constexpr (C::PP) {
-            // Two groups of four waves, one of each on every SIMD, run a phase apart: one
-            // multiplies a stage while the other reads the next one's fragments and issues
-            // copies. Group 1 starts a barrier late and group 0 ends one later. Group 0 needs
-            // stage s at its read of it; group 1 waits for its share of s one read earlier,
-            // which ends before that. The copies issued at read s go to the
-            // buffer of stage s - 1, which both groups have read by then.
+            // Two groups of four waves a phase apart, in the order of ping_pong.
             static_assert(C::WM * C::WN == 8 && C::STAGES == 4, "two groups of four waves, four stages");
             const int group = __builtin_amdgcn_readfirstlane(wave) >> 2;
             v4i pa[C::KSTEPS][C::FM], pb[C::KSTEPS][C::FN];
-            wait_stages<C::LOADS, C::STAGES - 2>(min(nk - 1, C::STAGES - 2));
-            barrier_here();
-            if (group == 1) barrier_here();
-            for (int it = 0; it < nk; ++it) {
-                if (group == 0) wait_stages<C::LOADS, C::STAGES - 2>(min(nk - 1 - it, C::STAGES - 2));
-                else wait_stages<C::LOADS, C::STAGES - 3>(min(nk - 2 - it, C::STAGES - 3));
-                const uint8_t* A = lds + (it % C::STAGES) * C::STAGE;
+            ping_pong<C::STAGES>(
+                group, nk, [&](auto most, int ahead) { wait_stages<C::LOADS, decltype(most)::value>(ahead); }, [&]() { barrier_here(); },
+                [&](int it) {
+                    const uint8_t* A = lds + (it % C::STAGES) * C::STAGE;
 #pragma unroll
-                for (int ks = 0; ks < C::KSTEPS; ++ks) read_frags(live, A, ks, pa[ks], pb[ks]);
-                const bool more = it + C::STAGES - 1 < nk;
-                const int to = (it + C::STAGES - 1) % C::STAGES;
-                if (more) issue(it + C::STAGES - 1, to);
-                wait_lds();
-                barrier_here();
+                    for (int ks = 0; ks < C::KSTEPS; ++ks) read_frags(live, A, ks, pa[ks], pb[ks]);
+                    const int next = it + C::STAGES - 1;
+                    if (next < nk) issue(next, next % C::STAGES);
+                    wait_lds();
+                },
+                [&]() {
 #pragma unroll
-                for (int ks = 0; ks < C::KSTEPS; ++ks) multiply(live, pa[ks], pb[ks], 0, L * C::FN);
-                barrier_here();
-            }
-            if (group == 0) barrier_here();
+                    for (int ks = 0; ks < C::KSTEPS; ++ks) multiply(live, pa[ks], pb[ks], 0, L * C::FN);
+                    __builtin_amdgcn_sched_barrier(0);
+                });
         } else {
             // The fragments of a k step are read while the step before is multiplied, those
             // of a stage's first step at the end of the stage before: stages it and
