@@ -568,6 +568,9 @@ extern "C" int bh_moe_plan_rows(void* stream, const int32_t* experts, uint32_t t
     RouteArgs a{};
     const int rc = check_plan(who, tokens, top_k, n_experts, plan, ws, ws_bytes, &a);
     if (rc) return rc;
+    // (The kernels take expert - first as an unsigned number: a negative expert, of none, stays outside up to here.)
+    if ((uint64_t)first + n_experts > 1ull << 31)
+        return fail(BH_ERR_INVALID, "%s: %u experts from first %u on pass 2^31", who, n_experts, first);
     if ((uint64_t)tokens * top_k && !experts) return fail(BH_ERR_INVALID, "%s: null experts", who);
     a.items = tokens * top_k, a.e = n_experts, a.k = 1, a.div = std::max(top_k, 1u), a.first = first;
     a.experts = const_cast<int32_t*>(experts);

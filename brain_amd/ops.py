@@ -664,14 +664,14 @@ def moe_route(logits, top_k, score="softmax", renormalize=True, scale=1.0, mask=
 def moe_plan(experts, n_experts, first=0, plan=None):
     """The MoePlan of experts [tokens, top_k] int32 chosen elsewhere: of those in
     [first, first + n_experts), which are an expert-parallel rank's own; others go
-    nowhere. An expert twice in a token is two places."""
+    nowhere. An expert twice in a token is two places. first + n_experts <= 2^31."""
     if experts.dim() != 2:
         raise ValueError(f"experts: shape {tuple(experts.shape)}, expected [tokens, top_k]")
     tokens, top_k = experts.shape
     dev = experts.get_device()
     _moe_sizes("moe_plan", tokens, top_k, n_experts)
-    if top_k > _MOST or not 0 <= first <= _MOST:
-        raise ValueError(f"moe_plan: {top_k} choices, first {first}")
+    if top_k > _MOST or not 0 <= first <= _MOST + 1 - n_experts:
+        raise ValueError(f"moe_plan: {top_k} choices, first {first} of {n_experts} experts")
     _fits(experts, torch.int32, 0, dev, "experts")
     stream = _stream_of(dev)
     plan, desc, ws, size = _moe_plan(dev, experts.device, tokens, top_k, n_experts, plan)

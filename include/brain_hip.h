@@ -372,8 +372,8 @@ int bh_moe_workspace(uint32_t tokens, uint32_t top_k, uint32_t n_experts, uint64
 int bh_moe_route(void* stream, const bh_moe_router* router, float* weights, int32_t* experts, const bh_moe_plan* plan,
                  void* ws, uint64_t ws_bytes);
 /* The plan of experts [tokens][top_k] from elsewhere, of those in [first, first +
- * n_experts) (an expert-parallel rank's own); others are routed nowhere. The
- * same expert twice in a token is two places. n_experts <= 1024. */
+ * n_experts) (an expert-parallel rank's own); others, negative ones among them, are routed nowhere. The
+ * same expert twice in a token is two places. n_experts <= 1024, first + n_experts <= 2^31. */
 int bh_moe_plan_rows(void* stream, const int32_t* experts, uint32_t tokens, uint32_t top_k, uint32_t first,
                      uint32_t n_experts, const bh_moe_plan* plan, void* ws, uint64_t ws_bytes);
 
