@@ -14,6 +14,7 @@
 
 #include "bh_kvops.h"
 #include "bh_pingpong.h"
+#include "bh_tilespan.h"
 
 namespace bh {
 
@@ -67,12 +68,12 @@ __device__ __forceinline__ bool find_tile(const GroupedArgs& a, uint32_t tile, T
 
 // The tiles of a launch over row tiles of TR rows and tiles_n column tiles, in an order in which neighbours
 // share what they read: an expert's row tiles (8 at most) of one column tile, then the next
-// columns. Workgroups go to the 8 XCDs in turn, each with an L2 of its own: XCD i gets the i-th
-// eighth of the tiles that there are, its workgroups tile by tile in turn.
+// columns. Each XCD has an L2 of its own, and gets an eighth of the tiles that follow each other (tile_span).
 template <uint32_t TR>
 struct Tiles {
     uint32_t o[5], upto;  // lane l: offsets of experts e0 + 4 l .. + 3; the tiles up to them
-    uint32_t e0, tiles_n, at, end, step;
+    uint32_t e0, tiles_n;
+    TileSpan span;
 
     __device__ __forceinline__ void load(const GroupedArgs& a, uint32_t base) {
         const uint32_t lane = threadIdx.x & 63;
@@ -81,7 +82,7 @@ struct Tiles {
         upto = base + lane_scan(tiles_of(0) + tiles_of(1) + tiles_of(2) + tiles_of(3));
     }
     __device__ __forceinline__ uint32_t tiles_of(int j) const { return o[j + 1] > o[j] ? (o[j + 1] - o[j] + TR - 1) / TR : 0; }
-    __device__ __forceinline__ void begin(const GroupedArgs& a, uint32_t columns) {
+    __device__ __forceinline__ void begin(const GroupedArgs& a, uint32_t columns, uint32_t most) {
         tiles_n = columns;
         uint32_t total = 0;
         for (e0 = 0;; e0 += 256) {
@@ -89,16 +90,13 @@ struct Tiles {
             total = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
             if (e0 + 256 >= a.experts) break;
         }
-        const uint64_t all = (uint64_t)total * tiles_n, share = (all + 7) / 8, from = (blockIdx.x & 7) * share;
-        at = (uint32_t)(from + (blockIdx.x >> 3));
-        end = (uint32_t)min(from + share, all);
-        step = gridDim.x >> 3;
+        span = tile_span(total, tiles_n, most, blockIdx.x, gridDim.x);
     }
     // The workgroup's next tile (for a whole wave); false: there is none.
     __device__ __forceinline__ bool next(const GroupedArgs& a, Tile& out, uint32_t& tn) {
-        if (at >= end) return false;
-        const uint32_t id = at, lane = threadIdx.x & 63;
-        at += step;
+        if (span.at >= span.end) return false;
+        const uint32_t id = span.at, lane = threadIdx.x & 63;
+        span.at += span.step;
         if (a.experts > 256) {
             uint32_t base = 0;
             for (e0 = 0;; e0 += 256) {
@@ -315,7 +313,7 @@ __device__ __forceinline__ void barrier_here() {
 }
 
 template <class C, int OUT, bool GLU, bool BIAS, bool REG>
-__global__ __launch_bounds__(C::NT, C::WGS * C::NT / 256 > 1 ? C::WGS * C::NT / 256 : 1) void grouped_tile_kernel(GroupedArgs a, uint32_t tiles_n) {
+__global__ __launch_bounds__(C::NT, C::WGS * C::NT / 256 > 1 ? C::WGS * C::NT / 256 : 1) void grouped_tile_kernel(GroupedArgs a, uint32_t tiles_n, uint32_t most) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int BNF = GLU ? C::BN / 2 : C::BN;  // output columns of a tile
     constexpr int DK = C::DK, JS = GLU ? 2 : 1;   // fragments of an output column
@@ -334,7 +332,7 @@ __global__ __launch_bounds__(C::NT, C::WGS * C::NT / 256 > 1 ? C::WGS * C::NT / 
     Tiles<C::BM> tiles;
     Tile tile;
     uint32_t tn;
-    tiles.begin(a, tiles_n);
+    tiles.begin(a, tiles_n, most);
     if (!tiles.next(a, tile, tn)) return;
 
     // Weight row, of the expert's, of tile row r. Lane c of a wave's fragments holds P neighbouring output
@@ -711,7 +709,8 @@ __global__ __launch_bounds__(256) void grouped_zero_kernel(GroupedArgs a) {
 
 constexpr unsigned CUS = 256;  // compute units of the MI355X
 
-// The most tiles of TR rows that `places` rows in up to `experts` groups can be.
+// The most tiles of TR rows that `places` rows in up to `experts` groups without common places can be. No call takes
+// more: where offsets give places to several groups, tiles behind them are left out.
 static uint64_t most_tiles(uint64_t places, uint64_t experts, uint64_t tr) {
     return std::min(places, (places + std::min(experts, places) * (tr - 1)) / tr);
 }
@@ -724,8 +723,8 @@ static hipError_t launch_tiles(hipStream_t s, const GroupedArgs& a) {
     const uint64_t tiles = most_tiles(a.places, a.experts, C::BM) * tiles_n;
     if (tiles > 0x7fffffffu) return hipErrorInvalidConfiguration;
     const unsigned wgs = (unsigned)std::min<uint64_t>((tiles + 7) / 8 * 8, CUS * C::WGS);
-    if (scaled && a.bias) grouped_tile_kernel<C, OUT, GLU, scaled, REG><<<wgs, C::NT, 0, s>>>(a, tiles_n);
-    else grouped_tile_kernel<C, OUT, GLU, false, REG><<<wgs, C::NT, 0, s>>>(a, tiles_n);
+    if (scaled && a.bias) grouped_tile_kernel<C, OUT, GLU, scaled, REG><<<wgs, C::NT, 0, s>>>(a, tiles_n, (uint32_t)tiles);
+    else grouped_tile_kernel<C, OUT, GLU, false, REG><<<wgs, C::NT, 0, s>>>(a, tiles_n, (uint32_t)tiles);
     return hipGetLastError();
 }
 

@@ -725,7 +725,7 @@ def matmul_i8_grouped(xq, wq, sx, sw, offsets, rows=None, bias=None, out_dtype=N
     [n_experts, n, K/4], (f32(acc) * sx[row]) * sw[e] (+ bias[e]) -> out
     [places, n], f32 (the default), bf16 or the raw int32 sums. Output rows of no group
     are not written. A plan's offsets and rows (MoePlan), or any ascending
-    offsets of a program's own."""
+    offsets of a program's own: where groups share places, results are left out."""
     return _matmul_grouped("matmul_i8_grouped", False, xq, wq, sx, sw, offsets, rows, bias, out_dtype, out)
 
 

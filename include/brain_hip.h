@@ -378,10 +378,12 @@ int bh_moe_plan_rows(void* stream, const int32_t* experts, uint32_t tokens, uint
                      uint32_t n_experts, const bh_moe_plan* plan, void* ws, uint64_t ws_bytes);
 
 /* A product grouped by expert. Place p in [offsets[e], offsets[e + 1]) multiplies
- * row rows[p] of x (NULL: row p) with the weights of expert e. Offsets ascend; they count as at
- * most `places`, a group that ends before it begins is empty, a place of several groups holds the
- * result of any of them, and output rows of no group are left as they are. A place whose row is
- * outside x gets zeros (raw sums of 0 with BH_OUT_I32, which needs no sx, sw and bias). */
+ * row rows[p] of x (NULL: row p) with the weights of expert e. Offsets ascend, as a plan's do; they count as at
+ * most `places`, a group that ends before it begins is empty, and output rows of no group are left as
+ * they are. A place whose row is outside x gets zeros (raw sums of 0 with BH_OUT_I32, which needs no sx,
+ * sw and bias). No place is of two groups: where offsets that do not ascend give one to two, results of
+ * groups are left out, and which ones is not defined (nothing but the groups' rows is written then
+ * either). */
 typedef struct {
     const uint32_t* xq; /* [x_rows][kg] int8 codes, 4 per word */
     const float* sx;    /* [x_rows] */
