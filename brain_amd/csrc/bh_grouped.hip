@@ -265,7 +265,8 @@ __global__ __launch_bounds__(GS_WAVES * 64) void grouped_step_kernel(GroupedArgs
 // columns: results leave as whole lines straight from the registers (through LDS, turned around, that
 // took 65 us of 8192 tokens' 319, this way 27 of 292).
 //   A workgroup stays for the next tile: its rows are looked up beside the products, and its first stages are
-// copied while the results of the tile before leave (4096 tokens, 128 experts: 187 us a workgroup a tile, 174 so).
+// asked for before the results of the tile before leave (4096 tokens, 128 experts: 187 us a workgroup a tile, 174 so). The
+// first wait for a stage waits for those stores too: loads and stores are counted as one, in order, and the stores came later.
 //   The group's last tile has fewer than BM rows: waves leave out the 32-row
 // fragments that hold none.
 template <int BM_, int BN_, int WM_, int WN_, int STAGES_, int DK_, int WGS_, bool PP_, bool ONCE_>
@@ -742,7 +743,8 @@ static hipError_t launch_grouped(hipStream_t s, const GroupedArgs& a) {
     constexpr uint32_t cols = GLU ? 64 : 128;
     const uint64_t wide = (a.f + cols - 1) / cols;
     const uint64_t t64 = most_tiles(a.places, a.experts, 64) * wide, t128 = most_tiles(a.places, a.experts, 128) * wide;
-    // Which kernel, by the rows an expert has on average and by how many tiles there are. Both sides of each line in
+    // Which kernel, by the rows an expert has on average and by how many tiles there are, if every place is of a group: the
+    // host knows the room only, so a rank's share of a plan is treated as all of it. Both sides of each line, of whole plans, in
     // us, weights from memory (several sets in turn), bf16 out; "128 experts": 8 of 128 a token, gate and up 2048 x
     // (2 x 768), down 768 x 2048; "8 experts": 2 of 8, 2048 x (2 x 4096), 4096 x 2048; "64 experts": 6 of 64,
     // 2048 x (2 x 1408), 1408 x 2048.

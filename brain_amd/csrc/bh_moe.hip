@@ -173,8 +173,9 @@ static size_t plan_lds(uint32_t e, uint32_t waves, uint32_t entries) {
 // A workgroup's items: their experts (routed here, or read: NV = 0), and of each entry
 // the rank among the entries of its expert in this workgroup. With one workgroup
 // (ONE) the plan is complete at the end; else `slots` holds the ranks and
-// `counts` the workgroup's counts, for moe_place_kernel. Routing is bound by its
-// vector instructions, some 13 for each token and choice of 128 experts.
+// `counts` the workgroup's counts, for moe_place_kernel. Some 13 vector instructions for each token and choice of 128
+// experts are 2.8 us of the 9.6 that 16384 tokens take (8 choices); the rest is latency: the logits' way in, four tokens of
+// a wave one choice after another, 16 waves' counts summed in turn between barriers, the results' way out.
 template <class T, int G, int NV, int NK, bool PLAN, bool ONE>
 __global__ __launch_bounds__(RT) void moe_route_kernel(RouteArgs a) {
     extern __shared__ uint32_t lds[];

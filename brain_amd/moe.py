@@ -1,7 +1,7 @@
 """The int8 mixture-of-experts feed-forward of a decoder layer: router choice, gated experts, weighted sum.
 
-Six launches for any number of tokens and experts, with no host synchronisation
-between them, so a decode step can be captured:
+Six calls for any number of tokens and experts (the route is one to three launches),
+with no host synchronisation between them, so a decode step can be captured:
 
     sx, xq       = quant(x)                          ops.quantize_rows[_bf16]
     weights, plan = route(logits)                     ops.moe_route
