@@ -25,19 +25,20 @@ namespace bh {
 // integral constant). Stages 0 .. STAGES - 2 have been asked for, as far as there are so many. group: of this wave, 0 or 1.
 template <int STAGES, class Wait, class Barrier, class Read, class Multiply>
 __attribute__((always_inline)) constexpr void ping_pong(int group, int nk, Wait wait, Barrier barrier, Read read, Multiply multiply) {
-    static_assert(STAGES >= 4, "group 1 waits for a stage while two later ones may be on their way");
-    constexpr std::integral_constant<int, STAGES - 2> two{};
-    constexpr std::integral_constant<int, STAGES - 3> one{};
+    static_assert(STAGES >= 3, "a stage that is read, one waited for, one asked for");
+    // Stages behind the one waited for that may be on their way: group 1 waits before it asks for the last of them.
+    constexpr std::integral_constant<int, STAGES - 2> asked{};
+    constexpr std::integral_constant<int, STAGES - 3> unasked{};
     auto least = [](int a, int b) { return a < b ? a : b; };
-    wait(two, least(nk - 1, STAGES - 2));
+    wait(asked, least(nk - 1, STAGES - 2));
     barrier();
     if (group == 1) barrier();
     for (int it = 0; it < nk; ++it) {
-        if (group == 1) wait(one, least(nk - 2 - it, STAGES - 3));
+        if (group == 1) wait(unasked, least(nk - 2 - it, STAGES - 3));
         read(it);
         barrier();
         multiply();
-        if (group == 0) wait(two, least(nk - 2 - it, STAGES - 2));
+        if (group == 0) wait(asked, least(nk - 2 - it, STAGES - 2));
         barrier();
     }
     if (group == 0) barrier();

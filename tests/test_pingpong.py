@@ -65,6 +65,7 @@ static void check() {
     }
 }
 int main() {
+    check<3>();
     check<4>();
     check<5>();
     check<6>();
